@@ -8,26 +8,10 @@
 //   * sparse optimizers: SGD and Adagrad applied to exactly the rows a batch touched, from the one-row-per-distinct-id
 //     gradients the segmented reduction produces.  The reference stops at un-aggregated per-triple gradient pieces
 //     (apps/kge/kge.py:393-515) and has no update step.
+#include "philox.cuh"
 #include "rows.cuh"
 
 namespace kge {
-
-// ---- Philox4x32-10 (Salmon et al., "Parallel random numbers: as easy as 1, 2, 3", SC'11) ----------------------------
-struct Philox4 { uint32_t x[4]; };
-__host__ __device__ inline Philox4 philox4x32_10(uint32_t c0, uint32_t c1, uint32_t c2, uint32_t c3, uint32_t k0, uint32_t k1) {
-    const uint32_t M0 = 0xD2511F53u, M1 = 0xCD9E8D57u, W0 = 0x9E3779B9u, W1 = 0xBB67AE85u;
-    for (int round = 0; round < 10; ++round) {
-        const uint64_t p0 = static_cast<uint64_t>(M0) * c0, p1 = static_cast<uint64_t>(M1) * c2;
-        const uint32_t hi0 = static_cast<uint32_t>(p0 >> 32), lo0 = static_cast<uint32_t>(p0);
-        const uint32_t hi1 = static_cast<uint32_t>(p1 >> 32), lo1 = static_cast<uint32_t>(p1);
-        const uint32_t n0 = hi1 ^ c1 ^ k0, n1 = lo1, n2 = hi0 ^ c3 ^ k1, n3 = lo0;
-        c0 = n0; c1 = n1; c2 = n2; c3 = n3;
-        k0 += W0; k1 += W1;
-    }
-    Philox4 r;
-    r.x[0] = c0; r.x[1] = c1; r.x[2] = c2; r.x[3] = c3;
-    return r;
-}
 
 // Element i of stream `stream`: counter (i low, i high, stream, 0), key (seed low, seed high); words 0 and 1 are used.
 __device__ __forceinline__ void draw2(unsigned long long seed, uint32_t stream, long long i, uint32_t& a, uint32_t& b) {

@@ -383,6 +383,69 @@ KGE_API int kge_apply_sgd(void* table, int32_t dtype, int32_t dim, const int64_t
 KGE_API int kge_apply_adagrad(void* table, int32_t dtype, float* state, int32_t dim, const int64_t* ids, int64_t n,
                               const int64_t* n_dev, int64_t first_row, const float* grad, float lr, float eps, kge_stream_t stream);
 
+/* ---- losses over scores ------------------------------------------------------------------------------------------
+ * Preference loss: every positive against its n negatives, relative to a frozen reference scorer, with gradients.
+ *   z = beta ((pos[b] - ref_pos[b]) - (neg[b][j] - ref_neg[b][j])) - margin
+ *   KGE_PREF_LOGISTIC  l = (1 - smoothing) softplus(-z) + smoothing softplus(z)     (paired log-ratio loss; without a reference
+ *                      and with beta = 1 the Bayesian personalised ranking loss)
+ *   KGE_PREF_SQUARE    l = z^2                                                       (smoothing must be 0)
+ *   loss = scale * sum_b weight[b] / c_b * sum_{j valid} l;  dpos, dneg = its derivatives with respect to pos, neg.
+ * c_b = number of valid negatives of row b: n, or the number of nonzero bytes of mask[b][0..n).  Nothing of a masked pair is
+ * read into the result (it may hold infinities or NaN), its dneg is 0; a row without valid negatives, or of weight 0, adds
+ * nothing and gets zero gradients.  pos, ref_pos, weight, dpos (rows); neg, ref_neg, mask, dneg (rows, n) with row pitches in
+ * elements; ref_pos and ref_neg are both given or both NULL; mask, weight may be NULL (all valid, weight 1).  All fp32 (the
+ * scorers' output type), aligned to 4 bytes; sums in a fixed order.  dneg may be neg itself (same pitch).  loss (1,).
+ * Chunk-shared scores (batch/chunk, chunk, n) are the same rows.  n <= 2^30.  No reference counterpart. */
+#define KGE_PREF_LOGISTIC 0
+#define KGE_PREF_SQUARE 1
+KGE_API size_t kge_preference_workspace_bytes(int64_t rows, int64_t n);
+KGE_API int kge_preference_loss(const float* pos, const float* ref_pos, const float* neg, int64_t ld_neg, const float* ref_neg,
+                        int64_t ld_ref, const uint8_t* mask, int64_t ld_mask, const float* weight, int64_t rows, int64_t n,
+                        int32_t kind, float beta, float margin, float smoothing, float scale, float* loss, float* dpos,
+                        float* dneg, int64_t ld_dneg, void* workspace, size_t workspace_bytes, kge_stream_t stream);
+
+/* Score rows as distributions over candidates: scores (rows, n) fp32 or bf16 with row pitch ld in elements; row r has the
+ * candidates [0, n_cand[r]) (n_cand clamped to [0, n]; NULL: all n); action[r] is the chosen one (id_bits wide).
+ *   kge_log_prob           logp[r] = log softmax(scores[r] / temperature)[action[r]];  stats (rows, 3): what the gradient needs
+ *   kge_log_prob_backward  dscores[r][j] = dlogp[r] / temperature * (1[j = action[r]] - softmax_j), zeros at [n_cand[r], n)
+ *   kge_policy_loss        ratio = exp(logp - old_logp);
+ *                          l = -min(ratio A, clip(ratio, 1 - clip_low, 1 + clip_high) A)
+ *                              + kl_coef * kl,   kl = exp(ref_logp - logp) - (ref_logp - logp) - 1  (0 without ref_logp)
+ *                          loss = scale * sum_r weight[r] l_r and dscores = d(loss) / d(scores), in one call; logp and kl
+ *                          (rows) are written too.  weight NULL: 1.  A clipped row's policy part has zero gradient.
+ * action[r] = -1: nothing was chosen; any other id outside [0, n_cand[r]) is reported as KGE_ERR_ID_RANGE (kge_check) and taken
+ * as -1.  Such a row, a row without candidates and a row whose scores are all -infinity has logp = kl = 0, adds nothing and
+ * gets zero gradients; a row of weight 0 adds nothing and gets zero gradients.  A score of -infinity has probability 0; NaN or
+ * +infinity make the row's outputs NaN.  dscores has the dtype of scores, pitch ldd, may be scores itself (same pitch); columns
+ * past n are not touched.  Statistics and sums are fp32 / fp64 in a fixed order.  old_logp, ref_logp, advantage, weight, dlogp,
+ * logp, kl are fp32 (rows), loss (1,).  n <= 2^30.  workspace from kge_candidates_workspace_bytes.  No reference counterpart. */
+KGE_API size_t kge_candidates_workspace_bytes(int64_t rows, int64_t n);
+KGE_API int kge_log_prob(const void* scores, int32_t dtype, int64_t ld, int64_t rows, int64_t n, const int32_t* n_cand,
+                         const void* action, int32_t id_bits, float temperature, float* logp, float* stats, void* workspace,
+                         size_t workspace_bytes, kge_stream_t stream);
+KGE_API int kge_log_prob_backward(const void* scores, int32_t dtype, int64_t ld, int64_t rows, int64_t n, const int32_t* n_cand,
+                         const void* action, int32_t id_bits, float temperature, const float* stats, const float* dlogp,
+                         void* dscores, int64_t ldd, kge_stream_t stream);
+KGE_API int kge_policy_loss(const void* scores, int32_t dtype, int64_t ld, int64_t rows, int64_t n, const int32_t* n_cand,
+                         const void* action, int32_t id_bits, float temperature, const float* old_logp, const float* ref_logp,
+                         const float* advantage, const float* weight, float clip_low, float clip_high, float kl_coef, float scale,
+                         float* loss, float* logp, float* kl, void* dscores, int64_t ldd, void* workspace,
+                         size_t workspace_bytes, kge_stream_t stream);
+
+/* ---- rows from features: dropout ------------------------------------------------------------------------------
+ * out[i][j] = x[i][j] / (1 - p) where element e = i * dim + j is kept, 0 where it is dropped, + residual[i][j] if residual is
+ * not NULL.  The mask is never stored: e is kept iff word e % 4 of Philox4x32-10 is >= floor(p * 2^32), counter words
+ * (e / 4 low, e / 4 high, stream_id, 2^31 | (step mod 2^31)), key words (seed low, seed high).  The gradient with respect to x
+ * is the same call on d(out) (without residual) under the same seed, stream_id and step; d(residual) = d(out).
+ * step_dev: NULL, or a device int64 that is added to `step` when the kernel runs, so that a captured and replayed call draws
+ * a new mask each time its caller advances that counter.  (The id samplers use counter word 3 = 0: no words are shared.)
+ * x, residual, out: (rows, dim) of one dtype with row pitches ldx, ldr, ldo in elements, aligned to the element size; out may
+ * be x or residual itself (same pitch), not overlap them otherwise.  0 <= p < 1.  A dropped element is 0 whatever x held.
+ * fp32 arithmetic, one rounding to the dtype.  No reference counterpart. */
+KGE_API int kge_dropout(const void* x, int32_t dtype, int64_t rows, int32_t dim, int64_t ldx, const void* residual, int64_t ldr,
+                        void* out, int64_t ldo, double p, uint64_t seed, uint32_t stream_id, int64_t step, const int64_t* step_dev,
+                        kge_stream_t stream);
+
 /* ---- measurement aid -----------------------------------------------------------------------------------
  * Launches `blocks` x 256 threads of independent fp32 FMA chains (iters x 128 FMAs per thread) and returns the
  * flop count (2 per FMA) in *flops_out; time it with CUDA events to get this GPU's attainable fp32 FMA rate,
