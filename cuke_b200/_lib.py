@@ -16,6 +16,7 @@ MODELS = {"TransE": 0, "TransH": 1, "TransR": 2, "TransF": 3, "DistMult": 4, "RE
 DTYPES = {"f32": 0, "bf16": 1}
 NEG_MODES = {"none": 0, "per_triple": 1, "chunk_shared": 2}
 PRECISIONS = {"fp32": 0, "tensor": 1, "tensor_tf32": 2}
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
 PREFERENCE_KINDS = {"logistic": 0, "square": 1}
 FLAG_CHECK_IDS = 1            # kge_problem.reserved
 ERR_WAIT_TIMEOUT, ERR_ID_RANGE = 2, 8     # values of the device error word (kge_check)
@@ -104,6 +105,9 @@ SIGNATURES = {
     "kge_log_prob_backward": (C.c_int, [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _i32, _f32, _vp, _vp, _vp, _i64, _vp]),
     "kge_policy_loss": (C.c_int, [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _i32, _f32, _vp, _vp, _vp, _vp, _f32, _f32, _f32, _f32, _vp, _vp,
                                   _vp, _vp, _i64, _vp, _sz, _vp]),
+    "kge_linear_workspace_bytes": (_sz, [_i64, _i64, _i64, _i32, _i32]),
+    "kge_linear_forward": (C.c_int, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _i32, _vp, _i64, _vp, _vp, _sz, _vp]),
+    "kge_linear_backward": (C.c_int, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i32, _vp, _i64, _vp, _vp, _vp, _sz, _vp]),
     "kge_apply_sgd": (C.c_int, [_vp, _i32, _i32, _vp, _i64, _vp, _i64, _vp, _f32, _vp]),
     "kge_apply_adagrad": (C.c_int, [_vp, _i32, _vp, _i32, _vp, _i64, _vp, _i64, _vp, _f32, _f32, _vp]),
 }

@@ -1,0 +1,614 @@
+// Rows from features: out = act(x w + b) (+ residual) and its gradient, bf16 with fp32 accumulation.
+//
+//   forward   z = x w + b        x (M, K), w (K, N) in the framework's matrix orientation out[j] = sum_i x[i] w[i][j]
+//             out = act(z) + residual, and for training slope = act'(z) in fp16 (2^-12 relative: an eighth of a bf16 rounding)
+//   backward  dz = dout * slope (bf16),  dx = dz w^T,  dw = x^T dz,  db = sum over rows of dz,  d(residual) = dout
+//
+// The three products run on one persistent tcgen05 kernel over CTA pairs (256-row tiles, cta_group::2): operands are
+// used as they lie in memory, K-major or MN-major, so nothing is transposed; two accumulators in tensor memory let a
+// tile's epilogue overlap the next tile's main loop.  Bias, activation, residual and slope are applied to the fp32
+// accumulator in the epilogue, with one rounding to bf16.
+#include <string.h>
+#include <atomic>
+#include <cuda_fp16.h>
+#include "umma.cuh"
+
+namespace kge {
+
+enum { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3 };
+enum { LE_FORWARD = 0, LE_STORE = 1, LE_PARTIAL = 2 };
+
+constexpr int LG_BM = 128;                        // rows of a tile per CTA (a pair: 256)
+constexpr int LG_BK = 64;                         // contraction per stage: one 128-byte swizzle row of bf16
+constexpr int LG_A_BYTES = LG_BM * LG_BK * 2;
+constexpr int LG_SLAB = LG_BK * 128;              // MN-major slab: 64 k-rows x 128 bytes
+constexpr int LG_THREADS = 320;                   // warp 0: TMA, warp 1: MMA and tensor memory, warps 2..9: epilogue
+constexpr int LG_EPI_WARPS = 8;
+constexpr int LG_MAX_SMEM = 227 * 1024;
+constexpr int LG_ACC_COLS = 256;
+
+struct LinEpilogue {
+    const __nv_bfloat16* bias; const __nv_bfloat16* res; long long ldr;
+    __nv_bfloat16* out; long long ldo;
+    __half* slope;                                // (M, N) packed, or NULL
+    float* part;                                  // LE_PARTIAL: (splits, M, N)
+    int act;
+    int wide, wide_slope;                         // rows of out / slope start on 32-byte boundaries
+};
+struct LinGemm {
+    int m, n;                                     // output rows and columns
+    int kb;                                       // stages of the whole contraction
+    int bn, a_mn, b_mn, stages, splits, tiles_m, tiles_n;
+    LinEpilogue e;
+    int32_t* err;
+};
+
+// ---- elementwise pieces -------------------------------------------------------------------------------------------
+__device__ __forceinline__ float lin_ex2(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
+__device__ __forceinline__ float lin_rcp(float x) { float r; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
+// 1 / (1 + exp(-x)): exp overflows to +inf for very negative x and the reciprocal is then 0
+__device__ __forceinline__ float lin_sigmoid(float x) { return lin_rcp(1.f + lin_ex2(-1.4426950408889634f * x)); }
+
+// (act(z), act'(z)); gelu is the tanh form, 0.5 z (1 + tanh u) = z sigmoid(2 u), u = sqrt(2 / pi) (z + 0.044715 z^3)
+template <int ACT>
+__device__ __forceinline__ float2 lin_act(float z) {
+    if (ACT == ACT_NONE) return make_float2(z, 1.f);
+    if (ACT == ACT_RELU) return make_float2(z > 0.f ? z : (z != z ? z : 0.f), z > 0.f ? 1.f : 0.f);
+    // s rounds to 0 or 1 far from the origin: z s and s (1 - s) are then taken as the limits they have, so that neither an
+    // infinite z nor the polynomial's overflow turns into NaN (a NaN z stays one)
+    if (ACT == ACT_SILU) {
+        const float s = lin_sigmoid(z), y = s == 0.f ? 0.f : z * s, om = 1.f - s;
+        return make_float2(y, om > 0.f ? fmaf(y, om, s) : s);
+    }
+    const float c = 1.5957691216057308f;          // 2 sqrt(2 / pi)
+    const float z2 = z * z;
+    const float s = lin_sigmoid(c * z * fmaf(0.044715f, z2, 1.f));
+    const float y = s == 0.f ? 0.f : z * s, om = 1.f - s;
+    return make_float2(y, om > 0.f && s != 0.f ? fmaf(y * om, c * fmaf(3.f * 0.044715f, z2, 1.f), s) : s);
+}
+__device__ __forceinline__ uint32_t lin_bf2(float a, float b) {
+    __nv_bfloat162 p = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&p);
+}
+__device__ __forceinline__ uint32_t lin_h2(float a, float b) {
+    __half2 p = __floats2half2_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&p);
+}
+__device__ __forceinline__ float lin_lo(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float lin_hi(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
+
+__device__ __forceinline__ void lin_st8(void* p, const uint32_t* w) {      // 32 bytes, 32-byte aligned
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 :: "l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+}
+// 16 packed words (32 16-bit elements) of one row, `lim` of them valid (a multiple of 8 elements)
+__device__ __forceinline__ void lin_store16(void* p, const uint32_t (&w)[16], int lim, bool wide) {
+    uint4* q = static_cast<uint4*>(p);
+    if (wide && lim == 32) { lin_st8(p, w); lin_st8(q + 2, w + 8); return; }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (8 * i < lim) q[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+}
+
+template <int ACT>
+__device__ __forceinline__ void lin_apply(float (&v)[32], const uint32_t (&bias)[16], const uint32_t (&res)[16], uint32_t (&slope)[16]) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const float2 a = lin_act<ACT>(v[2 * i] + lin_lo(bias[i])), b = lin_act<ACT>(v[2 * i + 1] + lin_hi(bias[i]));
+        v[2 * i] = a.x + lin_lo(res[i]);
+        v[2 * i + 1] = b.x + lin_hi(res[i]);
+        slope[i] = lin_h2(a.y, b.y);
+    }
+}
+
+// 32 consecutive columns of one output row: fp32 sums in v -> bias, activation, residual -> bf16 row and fp16 slope
+__device__ __forceinline__ void lin_finish(const LinEpilogue& e, float (&v)[32], const uint32_t (&res)[16], long long row, int col, int lim, int n) {
+    uint32_t bias[16], slope[16];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint4 b = make_uint4(0u, 0u, 0u, 0u);
+        if (e.bias && 8 * i < lim) b = __ldg(reinterpret_cast<const uint4*>(e.bias + col) + i);
+        bias[4 * i] = b.x; bias[4 * i + 1] = b.y; bias[4 * i + 2] = b.z; bias[4 * i + 3] = b.w;
+    }
+    switch (e.act) {
+        case ACT_NONE: lin_apply<ACT_NONE>(v, bias, res, slope); break;
+        case ACT_RELU: lin_apply<ACT_RELU>(v, bias, res, slope); break;
+        case ACT_SILU: lin_apply<ACT_SILU>(v, bias, res, slope); break;
+        default: lin_apply<ACT_GELU>(v, bias, res, slope); break;
+    }
+    uint32_t w[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) w[i] = lin_bf2(v[2 * i], v[2 * i + 1]);
+    lin_store16(e.out + row * e.ldo + col, w, lim, e.wide);
+    if (e.slope) lin_store16(e.slope + row * n + col, slope, lim, e.wide_slope);
+}
+__device__ __forceinline__ void lin_residual(const LinEpilogue& e, uint32_t (&res)[16], long long row, int col, int lim) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint4 r = make_uint4(0u, 0u, 0u, 0u);
+        if (e.res && 8 * i < lim) r = *(reinterpret_cast<const uint4*>(e.res + row * e.ldr + col) + i);
+        res[4 * i] = r.x; res[4 * i + 1] = r.y; res[4 * i + 2] = r.z; res[4 * i + 3] = r.w;
+    }
+}
+
+// ---- the product ----------------------------------------------------------------------------------------------------
+// Work item = (output tile, share of the contraction); items of the same share run over the column tiles first, so the
+// pairs working at one time read the same rows of A.  Pair p takes items p, p + pairs, ...
+template <int EPI>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LG_THREADS, 1)
+linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, LinGemm p) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    const int half_n = p.bn / 2;                                   // B columns staged by each CTA
+    const int b_slabs = (half_n + 63) / 64;
+    const int b_bytes = p.b_mn ? b_slabs * LG_SLAB : half_n * 128;
+    const int b_room = (b_bytes + 1023) & ~1023;                   // swizzle atoms start on 1024-byte boundaries
+    const int stage_bytes = LG_A_BYTES + b_room;
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + p.stages * stage_bytes);
+    uint64_t* empty = full + p.stages;
+    uint64_t* acc_full = empty + p.stages;
+    uint64_t* acc_empty = acc_full + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = umma::cluster_ctarank();
+    const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
+    const int tiles = p.tiles_m * p.tiles_n, items = tiles * p.splits;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < p.stages; ++s) { umma::mbar_init(&full[s], 1); umma::mbar_init(&empty[s], 1); }
+        for (int s = 0; s < 2; ++s) { umma::mbar_init(&acc_full[s], 1); umma::mbar_init(&acc_empty[s], 2 * LG_EPI_WARPS); }
+        umma::fence_barrier_init();
+    }
+    if (warp == 1) { umma::tmem_alloc_pair(tmem_slot, 2 * LG_ACC_COLS); umma::tmem_relinquish_pair(); }
+    umma::tc_fence_before();
+    __syncthreads();
+    umma::cluster_sync();
+    umma::tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            umma::prefetch_tensormap(&map_a); umma::prefetch_tensormap(&map_b);
+            int s = 0; uint32_t ph = 0;
+            bool ok = true;
+            const uint32_t tx_pair = 2u * (LG_A_BYTES + b_bytes);
+            for (int item = pair; item < items && ok; item += n_pairs) {
+                const int split = item / tiles, tile = item - split * tiles;
+                const int tm = tile / p.tiles_n;
+                const int m0 = tm * 2 * LG_BM + static_cast<int>(rank) * LG_BM;
+                const int nb0 = (tile - tm * p.tiles_n) * p.bn + static_cast<int>(rank) * half_n;
+                const int kb0 = static_cast<int>(static_cast<long long>(p.kb) * split / p.splits);
+                const int kb1 = static_cast<int>(static_cast<long long>(p.kb) * (split + 1) / p.splits);
+                for (int kb = kb0; kb < kb1; ++kb) {
+                    if (!umma::mbar_wait(&empty[s], ph ^ 1)) { atomicOr(p.err, KGE_ERR_WAIT_TIMEOUT); ok = false; break; }
+                    uint8_t* a = smem + s * stage_bytes;
+                    uint8_t* b = a + LG_A_BYTES;
+                    const uint32_t lead = umma::map_to_cta(umma::smem_u32(&full[s]), 0);
+                    if (rank == 0) umma::mbar_expect_tx(&full[s], tx_pair);
+                    const int k0 = kb * LG_BK;
+                    if (!p.a_mn) {
+                        umma::tma_load_3d_pair(a, &map_a, k0, m0, 0, lead);
+                    } else {
+                        umma::tma_load_3d_pair(a, &map_a, m0, k0, 0, lead);
+                        umma::tma_load_3d_pair(a + LG_SLAB, &map_a, m0 + 64, k0, 0, lead);
+                    }
+                    if (!p.b_mn) {
+                        umma::tma_load_3d_pair(b, &map_b, k0, nb0, 0, lead);
+                    } else {
+                        for (int sl = 0; sl < b_slabs; ++sl) umma::tma_load_3d_pair(b + sl * LG_SLAB, &map_b, nb0 + 64 * sl, k0, 0, lead);
+                    }
+                    if (++s == p.stages) { s = 0; ph ^= 1; }
+                }
+            }
+            for (int i = 0; i < p.stages && ok; ++i) {         // every commit aimed at this CTA has landed before it may exit
+                if (!umma::mbar_wait(&empty[s], ph ^ 1)) { atomicOr(p.err, KGE_ERR_WAIT_TIMEOUT); ok = false; }
+                if (++s == p.stages) { s = 0; ph ^= 1; }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            const uint64_t a_tmpl = p.a_mn ? umma::smem_desc_mn(0, LG_SLAB, 1024u, 2u) : umma::smem_desc_k_sw128(0);
+            const uint64_t b_tmpl = p.b_mn ? umma::smem_desc_mn(0, LG_SLAB, 1024u, 2u) : umma::smem_desc_k_sw128(0);
+            const uint32_t a_step = (p.a_mn ? 2048u : 32u) >> 4, b_step = (p.b_mn ? 2048u : 32u) >> 4;
+            const uint32_t idesc = umma::instr_desc(1u, 2 * LG_BM, static_cast<uint32_t>(p.bn), static_cast<uint32_t>(p.a_mn), static_cast<uint32_t>(p.b_mn));
+            int s = 0, lt = 0; uint32_t ph = 0;
+            bool ok = true;
+            for (int item = pair; item < items && ok; item += n_pairs, ++lt) {
+                const int split = item / tiles;
+                const int nkb = static_cast<int>(static_cast<long long>(p.kb) * (split + 1) / p.splits) -
+                                static_cast<int>(static_cast<long long>(p.kb) * split / p.splits);
+                const int buf = lt & 1;
+                if (!umma::mbar_wait(&acc_empty[buf], (static_cast<uint32_t>(lt >> 1) & 1) ^ 1)) { atomicOr(p.err, KGE_ERR_WAIT_TIMEOUT); ok = false; break; }
+                umma::tc_fence_after();
+                const uint32_t tmem_d = tmem_base + buf * LG_ACC_COLS;
+                for (int kb = 0; kb < nkb; ++kb) {
+                    if (!umma::mbar_wait(&full[s], ph)) { atomicOr(p.err, KGE_ERR_WAIT_TIMEOUT); ok = false; break; }
+                    umma::tc_fence_after();
+                    const uint32_t st = (umma::smem_u32(smem + s * stage_bytes) & 0x3FFFFu) >> 4;
+                    uint64_t da = a_tmpl | st, db = b_tmpl | (st + (LG_A_BYTES >> 4));
+#pragma unroll
+                    for (int k = 0; k < 4; ++k, da += a_step, db += b_step) umma::mma_f16_pair(tmem_d, da, db, idesc, (kb > 0 || k > 0) ? 1u : 0u);
+                    const uint32_t e0 = umma::smem_u32(&empty[s]);
+                    umma::mma_commit_pair(e0);
+                    umma::mma_commit_pair(umma::map_to_cta(e0, 1));
+                    if (++s == p.stages) { s = 0; ph ^= 1; }
+                }
+                const uint32_t f0 = umma::smem_u32(&acc_full[buf]);
+                umma::mma_commit_pair(f0);
+                umma::mma_commit_pair(umma::map_to_cta(f0, 1));
+            }
+        }
+    } else {
+        // thread = row of the tile; the two warps of a lane quarter take alternate 32-column chunks
+        const int q = warp & 3, half = (warp - 2) >> 2;
+        const int chunks = (p.bn + 31) / 32;
+        int lt = 0;
+        for (int item = pair; item < items; item += n_pairs, ++lt) {
+            const int split = item / tiles, tile = item - split * tiles;
+            const int tm = tile / p.tiles_n;
+            const int row = tm * 2 * LG_BM + static_cast<int>(rank) * LG_BM + q * 32 + lane;
+            const int n0 = (tile - tm * p.tiles_n) * p.bn;
+            const int buf = lt & 1;
+            const bool row_ok = row < p.m;
+            const uint32_t taddr = tmem_base + buf * LG_ACC_COLS + (static_cast<uint32_t>(q * 32) << 16);
+            bool ready = false;
+            // one vote per wait: the whole warp goes on, or the whole warp gives up
+            auto wait_full = [&]() { return __all_sync(kFull, umma::mbar_wait(&acc_full[buf], static_cast<uint32_t>(lt >> 1) & 1)) != 0; };
+#pragma unroll 1
+            for (int c = half; c < chunks; c += 2) {
+                const int col = n0 + c * 32;
+                const int lim = min(32, min(p.bn - c * 32, p.n - col));
+                const bool live = row_ok && lim > 0;
+                uint32_t res[16];
+                if (EPI == LE_FORWARD) lin_residual(p.e, res, row, col, live ? lim : 0);
+                if (!ready) {
+                    ready = wait_full();
+                    if (!ready) break;
+                    umma::tc_fence_after();
+                }
+                float v[32];
+                __syncwarp();                     // tensor-memory reads are warp-collective
+                umma::tmem_ld32(taddr + c * 32, v);
+                if (live) {
+                    if (EPI == LE_FORWARD) {
+                        lin_finish(p.e, v, res, row, col, lim, p.n);
+                    } else if (EPI == LE_STORE) {
+                        uint32_t w[16];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) w[i] = lin_bf2(v[2 * i], v[2 * i + 1]);
+                        lin_store16(p.e.out + row * p.e.ldo + col, w, lim, p.e.wide);
+                    } else {
+                        float* d = p.e.part + (static_cast<long long>(split) * p.m + row) * p.n + col;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (8 * i < lim) lin_st8(d + 8 * i, reinterpret_cast<const uint32_t*>(v) + 8 * i);
+                    }
+                }
+                __syncwarp();
+            }
+            if (!ready && (half < chunks || !wait_full())) {      // (a warp without a chunk only keeps step)
+                if (lane == 0) atomicOr(p.err, KGE_ERR_WAIT_TIMEOUT);
+                break;
+            }
+            umma::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) umma::mbar_arrive_cluster(umma::map_to_cta(umma::smem_u32(&acc_empty[buf]), 0));
+        }
+    }
+    umma::tc_fence_before();
+    __syncthreads();
+    umma::cluster_sync();
+    if (warp == 1) { umma::tc_fence_after(); umma::tmem_dealloc_pair(tmem_base, 2 * LG_ACC_COLS); }
+}
+
+// Sum of the shares of a split contraction in share order, then the epilogue; one thread per 8 columns.
+template <int EPI>
+__global__ void __launch_bounds__(256) linear_join_kernel(LinEpilogue e, long long m, int n, int splits) {
+    const int per_row = n / 8;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < m * per_row; i += (long long)gridDim.x * 256) {
+        const long long row = i / per_row;
+        const int col = static_cast<int>(i - row * per_row) * 8;
+        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        for (int s = 0; s < splits; ++s) {
+            const float4* d = reinterpret_cast<const float4*>(e.part + (static_cast<long long>(s) * m + row) * n + col);
+            const float4 a = __ldcs(d), b = __ldcs(d + 1);
+            v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w; v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+        }
+        if (EPI == LE_FORWARD) {
+            uint4 bias = make_uint4(0u, 0u, 0u, 0u), res = bias;
+            if (e.bias) bias = __ldg(reinterpret_cast<const uint4*>(e.bias + col));
+            if (e.res) res = *reinterpret_cast<const uint4*>(e.res + row * e.ldr + col);
+            const uint32_t bw[4] = {bias.x, bias.y, bias.z, bias.w}, rw[4] = {res.x, res.y, res.z, res.w};
+            uint32_t sl[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                float2 lo, hi;
+                const float z0 = v[2 * k] + lin_lo(bw[k]), z1 = v[2 * k + 1] + lin_hi(bw[k]);
+                switch (e.act) {
+                    case ACT_NONE: lo = lin_act<ACT_NONE>(z0); hi = lin_act<ACT_NONE>(z1); break;
+                    case ACT_RELU: lo = lin_act<ACT_RELU>(z0); hi = lin_act<ACT_RELU>(z1); break;
+                    case ACT_SILU: lo = lin_act<ACT_SILU>(z0); hi = lin_act<ACT_SILU>(z1); break;
+                    default: lo = lin_act<ACT_GELU>(z0); hi = lin_act<ACT_GELU>(z1); break;
+                }
+                v[2 * k] = lo.x + lin_lo(rw[k]); v[2 * k + 1] = hi.x + lin_hi(rw[k]);
+                sl[k] = lin_h2(lo.y, hi.y);
+            }
+            if (e.slope) *reinterpret_cast<uint4*>(e.slope + row * n + col) = make_uint4(sl[0], sl[1], sl[2], sl[3]);
+        }
+        *reinterpret_cast<uint4*>(e.out + row * e.ldo + col) =
+            make_uint4(lin_bf2(v[0], v[1]), lin_bf2(v[2], v[3]), lin_bf2(v[4], v[5]), lin_bf2(v[6], v[7]));
+    }
+}
+
+// dz = dout * slope (skipped when slope is NULL: dz is dout itself) and the column sums of dz per block of LZ_ROWS rows.
+// A warp covers 256 columns of a row (8 per lane), the 8 warps of a CTA take rows in turn.
+constexpr int LZ_ROWS = 256;
+__global__ void __launch_bounds__(256) linear_dz_kernel(const __nv_bfloat16* __restrict__ dout, long long ldd, const __half* __restrict__ slope,
+                                                        __nv_bfloat16* __restrict__ dz, float* __restrict__ colpart, long long m, int n) {
+    __shared__ float red[8][256];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int col = blockIdx.y * 256 + lane * 8;
+    const long long r0 = static_cast<long long>(blockIdx.x) * LZ_ROWS, r1 = min(m, r0 + LZ_ROWS);
+    float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (col < n) {
+#pragma unroll 4
+        for (long long r = r0 + warp; r < r1; r += 8) {
+            const uint4 d = __ldcs(reinterpret_cast<const uint4*>(dout + r * ldd + col));
+            const uint32_t dw[4] = {d.x, d.y, d.z, d.w};
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) { v[2 * k] = lin_lo(dw[k]); v[2 * k + 1] = lin_hi(dw[k]); }
+            if (slope) {
+                const uint4 s = __ldcs(reinterpret_cast<const uint4*>(slope + r * n + col));
+                const uint32_t sw[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&sw[k]));
+                    v[2 * k] *= f.x; v[2 * k + 1] *= f.y;
+                }
+                *reinterpret_cast<uint4*>(dz + r * n + col) =
+                    make_uint4(lin_bf2(v[0], v[1]), lin_bf2(v[2], v[3]), lin_bf2(v[4], v[5]), lin_bf2(v[6], v[7]));
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) sum[k] += v[k];
+        }
+    }
+    if (!colpart) return;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) red[warp][lane * 8 + k] = sum[k];
+    __syncthreads();
+    const int c = blockIdx.y * 256 + threadIdx.x;
+    if (c < n) {
+        float t = 0.f;
+        for (int w = 0; w < 8; ++w) t += red[w][threadIdx.x];
+        colpart[static_cast<long long>(blockIdx.x) * n + c] = t;
+    }
+}
+// db[c] = sum over row blocks, in fp32 and in a fixed order (8 interleaved partial sums per column)
+__global__ void __launch_bounds__(256) linear_db_kernel(const float* colpart, long long blocks, int n, __nv_bfloat16* db) {
+    __shared__ float red[8][33];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int c = blockIdx.x * 32 + lane;
+    float t = 0.f;
+    if (c < n)
+        for (long long b = warp; b < blocks; b += 8) t += colpart[b * n + c];
+    red[warp][lane] = t;
+    __syncthreads();
+    if (warp == 0 && c < n) {
+        for (int w = 1; w < 8; ++w) t += red[w][lane];
+        db[c] = __float2bfloat16_rn(t);
+    }
+}
+
+// ---- host -----------------------------------------------------------------------------------------------------------
+static int lin_sms() {
+    int dev = 0, sms = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms < 2) {
+        cudaGetLastError();
+        return 148;
+    }
+    return sms;
+}
+static int lin_bn(long long n) {          // equal tiles of at most 256 columns, multiples of 16
+    const long long tiles = (n + 255) / 256;
+    return static_cast<int>(((n + tiles - 1) / tiles + 15) / 16 * 16);
+}
+// Shares of the contraction: the count with the least (rounds of work items x stages per item + cost of the join).
+static int lin_splits(long long m, long long n, long long k, int sms) {
+    const int bn = lin_bn(n);
+    const long long tiles = ((m + 255) / 256) * ((n + bn - 1) / bn), kb = (k + 63) / 64, slots = sms / 2;
+    if (tiles >= slots) return 1;
+    double best = 0.0;
+    int pick = 1;
+    for (int s = 1; s <= 32 && s <= kb; ++s) {
+        const double rounds = static_cast<double>((tiles * s + slots - 1) / slots);
+        double t = rounds * (0.3 * bn / 256 * ((kb + s - 1) / s) + 1.0);             // us
+        if (s > 1) t += 2.5 + 8.0 * s * m * n / 6.0e6;
+        if (s == 1 || t < best) { best = t; pick = s; }
+    }
+    return pick;
+}
+
+template <int EPI>
+static int lin_launch(const CUtensorMap& a, const CUtensorMap& b, const LinGemm& p, unsigned ctas, size_t smem, cudaStream_t s) {
+    static std::atomic<bool> attr_set[128];          // the shared-memory opt-in is per device and kernel
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return cuda_status(cudaGetLastError(), "cudaGetDevice");
+    if (dev < 0 || dev >= 128 || !attr_set[dev].load(std::memory_order_acquire)) {
+        cudaError_t e = cudaFuncSetAttribute(linear_pair_kernel<EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, LG_MAX_SMEM);
+        if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(linear_pair_kernel)");
+        if (dev >= 0 && dev < 128) attr_set[dev].store(true, std::memory_order_release);
+    }
+    linear_pair_kernel<EPI><<<ctas, LG_THREADS, smem, s>>>(a, b, p);
+    KGE_LAUNCH_CHECK("linear_pair_kernel");
+    return 0;
+}
+
+// out[m][n] (+ epilogue) = sum_k A[m][k] B[n][k].  a_mn / b_mn: the operand lies as (k rows, m or n columns).
+static int lin_gemm(const void* a, long long lda, int a_mn, const void* b, long long ldb, int b_mn, long long m, long long n, long long k,
+                    LinEpilogue e, bool forward, float* part, size_t part_bytes, cudaStream_t s) {
+    const int sms = lin_sms();
+    LinGemm p;
+    memset(&p, 0, sizeof(p));
+    p.m = static_cast<int>(m); p.n = static_cast<int>(n); p.kb = static_cast<int>((k + LG_BK - 1) / LG_BK);
+    p.bn = lin_bn(n); p.a_mn = a_mn; p.b_mn = b_mn;
+    p.tiles_m = static_cast<int>((m + 2 * LG_BM - 1) / (2 * LG_BM));
+    p.tiles_n = static_cast<int>((n + p.bn - 1) / p.bn);
+    p.splits = lin_splits(m, n, k, sms);
+    if (p.splits > 1 && (!part || part_bytes < sizeof(float) * static_cast<size_t>(p.splits) * m * n)) p.splits = 1;
+    e.wide = (e.ldo & 15) == 0 && (reinterpret_cast<uintptr_t>(e.out) & 31) == 0;
+    e.wide_slope = (n & 15) == 0 && (reinterpret_cast<uintptr_t>(e.slope) & 31) == 0;
+    e.part = part;
+    p.e = e;
+    p.err = device_error_word();
+    if (!p.err) { set_error("linear: no usable device"); return KGE_E_DEVICE; }
+    CUtensorMap ma, mb;
+    int rc;
+    if (a_mn) rc = make_tensor_map_2d(&ma, a, 2, k, m, lda * 2, LG_BK, 64);
+    else rc = make_tensor_map_2d(&ma, a, 2, m, k, lda * 2, LG_BM, LG_BK);
+    if (rc) return rc;
+    if (b_mn) rc = make_tensor_map_2d(&mb, b, 2, k, n, ldb * 2, LG_BK, 64);
+    else rc = make_tensor_map_2d(&mb, b, 2, n, k, ldb * 2, static_cast<uint32_t>(p.bn / 2), LG_BK);
+    if (rc) return rc;
+    const int half_n = p.bn / 2;
+    const int b_room = ((b_mn ? (half_n + 63) / 64 * LG_SLAB : half_n * 128) + 1023) & ~1023;
+    const int stage = LG_A_BYTES + b_room;
+    p.stages = (LG_MAX_SMEM - 1024 - 256) / stage;
+    if (p.stages > 8) p.stages = 8;
+    const size_t smem = static_cast<size_t>(p.stages) * stage + 1024 + 256;
+    const long long items = static_cast<long long>(p.tiles_m) * p.tiles_n * p.splits;
+    if (items >= (1LL << 30)) { set_error("linear: %lld tiles exceed the tile index", items); return KGE_E_RANGE; }
+    const unsigned ctas = 2u * static_cast<unsigned>(items < sms / 2 ? items : sms / 2);
+    if (p.splits == 1) return forward ? lin_launch<LE_FORWARD>(ma, mb, p, ctas, smem, s) : lin_launch<LE_STORE>(ma, mb, p, ctas, smem, s);
+    if ((rc = lin_launch<LE_PARTIAL>(ma, mb, p, ctas, smem, s))) return rc;
+    const long long groups = (m * (n / 8) + 255) / 256;
+    const unsigned blocks = static_cast<unsigned>(groups < 148 * 8 ? groups : 148 * 8);
+    if (forward) linear_join_kernel<LE_FORWARD><<<blocks, 256, 0, s>>>(e, m, p.n, p.splits);
+    else linear_join_kernel<LE_STORE><<<blocks, 256, 0, s>>>(e, m, p.n, p.splits);
+    KGE_LAUNCH_CHECK("linear_join_kernel");
+    return 0;
+}
+
+static size_t lin_up(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
+static size_t lin_part_bytes(long long m, long long n, long long k, int sms) {
+    const int s = lin_splits(m, n, k, sms);
+    return s > 1 ? lin_up(sizeof(float) * static_cast<size_t>(s) * m * n) : 0;
+}
+
+}  // namespace kge
+
+using namespace kge;
+
+static int check_linear(const char* fn, int64_t m, int64_t k, int64_t n, int32_t act) {
+    if (act < ACT_NONE || act > ACT_GELU) { set_error("%s: unknown activation %d", fn, act); return KGE_E_UNSUPPORTED; }
+    if (m < 0 || k < 1 || n < 1) { set_error("%s: sizes m = %lld, k = %lld, n = %lld", fn, (long long)m, (long long)k, (long long)n); return KGE_E_SHAPE; }
+    if ((k & 7) || (n & 7)) { set_error("%s: bf16 rows need k %% 8 == 0 and n %% 8 == 0 (16-byte rows), got k = %lld, n = %lld", fn, (long long)k, (long long)n); return KGE_E_UNSUPPORTED; }
+    if (m > (1LL << 30) || k > (1LL << 20) || n > (1LL << 20)) { set_error("%s: m above 2^30 or k, n above 2^20", fn); return KGE_E_RANGE; }
+    return 0;
+}
+static int check_rows(const char* fn, const char* name, const void* p, int64_t ld, int64_t rows, int64_t cols, bool required) {
+    if (!p) {
+        if (!required) return 0;
+        set_error("%s: %s is NULL", fn, name); return KGE_E_NULL;
+    }
+    if (!aligned16(p)) { set_error("%s: %s is not 16-byte aligned", fn, name); return KGE_E_ALIGN; }
+    if (rows > 1 && ld < cols) { set_error("%s: row pitch %lld of %s is below %lld", fn, (long long)ld, name, (long long)cols); return KGE_E_SHAPE; }
+    if (rows > 1 && (ld & 7)) { set_error("%s: row pitch %lld of %s is not a multiple of 8 (16-byte rows)", fn, (long long)ld, name); return KGE_E_ALIGN; }
+    if (ld > (1LL << 32)) { set_error("%s: row pitch of %s above 2^32", fn, name); return KGE_E_RANGE; }
+    return 0;
+}
+static int check_workspace(const char* fn, const void* p) {
+    if (!p) { set_error("%s: workspace is NULL", fn); return KGE_E_NULL; }
+    if (reinterpret_cast<uintptr_t>(p) & 255) { set_error("%s: workspace is not 256-byte aligned", fn); return KGE_E_ALIGN; }
+    return 0;
+}
+// a single row is read through its own length, whatever pitch came with it
+static long long pitch_of(int64_t ld, int64_t rows, int64_t cols) { return rows > 1 ? ld : cols; }
+
+extern "C" {
+
+size_t kge_linear_workspace_bytes(int64_t m, int64_t k, int64_t n, int32_t act, int32_t backward) {
+    if (m <= 0 || k <= 0 || n <= 0 || check_linear("kge_linear_workspace_bytes", m, k, n, act)) return 0;
+    const int sms = lin_sms();
+    if (!backward) return lin_part_bytes(m, n, k, sms);
+    const size_t dx = lin_part_bytes(m, k, n, sms), dw = lin_part_bytes(k, n, m, sms);
+    return (act != ACT_NONE ? lin_up(2 * static_cast<size_t>(m) * n) : 0) + lin_up(sizeof(float) * ((m + LZ_ROWS - 1) / LZ_ROWS) * n) + (dx > dw ? dx : dw);
+}
+
+int kge_linear_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* residual, int64_t ldr,
+                       int64_t m, int64_t k, int64_t n, int32_t act, void* out, int64_t ldo, void* slope, void* workspace,
+                       size_t workspace_bytes, kge_stream_t stream) {
+    const char* fn = "kge_linear_forward";
+    int rc = check_linear(fn, m, k, n, act);
+    if (rc || m == 0) return rc;
+    if ((rc = check_rows(fn, "x", x, ldx, m, k, true)) || (rc = check_rows(fn, "w", w, ldw, k, n, true)) ||
+        (rc = check_rows(fn, "bias", bias, n, 1, n, false)) || (rc = check_rows(fn, "residual", residual, ldr, m, n, false)) ||
+        (rc = check_rows(fn, "out", out, ldo, m, n, true)) || (rc = check_rows(fn, "slope", slope, n, m, n, false))) return rc;
+    const size_t need = kge_linear_workspace_bytes(m, k, n, act, 0);
+    if (workspace_bytes < need) { set_error("%s: workspace needs %zu bytes, got %zu", fn, need, workspace_bytes); return KGE_E_WORKSPACE; }
+    if (need && (rc = check_workspace(fn, workspace))) return rc;
+    LinEpilogue e;
+    memset(&e, 0, sizeof(e));
+    e.bias = static_cast<const __nv_bfloat16*>(bias);
+    e.res = static_cast<const __nv_bfloat16*>(residual); e.ldr = pitch_of(ldr, m, n);
+    e.out = static_cast<__nv_bfloat16*>(out); e.ldo = pitch_of(ldo, m, n);
+    e.slope = act == ACT_NONE ? nullptr : static_cast<__half*>(slope);
+    e.act = act;
+    return lin_gemm(x, pitch_of(ldx, m, k), 0, w, pitch_of(ldw, k, n), 1, m, n, k, e, true, static_cast<float*>(workspace), workspace_bytes,
+                    reinterpret_cast<cudaStream_t>(stream));
+}
+
+int kge_linear_backward(const void* dout, int64_t ldd, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* slope,
+                        int64_t m, int64_t k, int64_t n, int32_t act, void* dx, int64_t lddx, void* dw, void* dbias, void* workspace,
+                        size_t workspace_bytes, kge_stream_t stream) {
+    const char* fn = "kge_linear_backward";
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    int rc = check_linear(fn, m, k, n, act);
+    if (rc) return rc;
+    if ((rc = check_rows(fn, "dw", dw, n, k, n, false)) || (rc = check_rows(fn, "dbias", dbias, n, 1, n, false))) return rc;
+    if (m == 0) {                           // no rows: the sums over them are zero
+        cudaError_t e = dw ? cudaMemsetAsync(dw, 0, 2 * static_cast<size_t>(k) * n, s) : cudaSuccess;
+        if (e == cudaSuccess && dbias) e = cudaMemsetAsync(dbias, 0, 2 * static_cast<size_t>(n), s);
+        return cuda_status(e, "kge_linear_backward: cudaMemsetAsync");
+    }
+    if ((rc = check_rows(fn, "dout", dout, ldd, m, n, true)) || (rc = check_rows(fn, "x", x, ldx, m, k, dw != nullptr)) ||
+        (rc = check_rows(fn, "w", w, ldw, k, n, dx != nullptr)) || (rc = check_rows(fn, "slope", slope, n, m, n, act != ACT_NONE)) ||
+        (rc = check_rows(fn, "dx", dx, lddx, m, k, false))) return rc;
+    const size_t need = kge_linear_workspace_bytes(m, k, n, act, 1);
+    if (workspace_bytes < need) { set_error("%s: workspace needs %zu bytes, got %zu", fn, need, workspace_bytes); return KGE_E_WORKSPACE; }
+    if ((rc = check_workspace(fn, workspace))) return rc;
+    char* ws = static_cast<char*>(workspace);
+    __nv_bfloat16* dz = nullptr;
+    if (act != ACT_NONE) { dz = reinterpret_cast<__nv_bfloat16*>(ws); ws += lin_up(2 * static_cast<size_t>(m) * n); }
+    const long long blocks = (m + LZ_ROWS - 1) / LZ_ROWS;
+    float* colpart = reinterpret_cast<float*>(ws);
+    ws += lin_up(sizeof(float) * blocks * n);
+    const size_t part_bytes = workspace_bytes - static_cast<size_t>(ws - static_cast<char*>(workspace));
+    ldd = pitch_of(ldd, m, n);
+    if (dz || dbias) {
+        linear_dz_kernel<<<dim3(static_cast<unsigned>(blocks), static_cast<unsigned>((n + 255) / 256)), 256, 0, s>>>(
+            static_cast<const __nv_bfloat16*>(dout), ldd, dz ? static_cast<const __half*>(slope) : nullptr, dz, dbias ? colpart : nullptr, m,
+            static_cast<int>(n));
+        KGE_LAUNCH_CHECK("linear_dz_kernel");
+    }
+    if (dbias) {
+        linear_db_kernel<<<static_cast<unsigned>((n + 31) / 32), 256, 0, s>>>(colpart, blocks, static_cast<int>(n), static_cast<__nv_bfloat16*>(dbias));
+        KGE_LAUNCH_CHECK("linear_db_kernel");
+    }
+    const void* g = dz ? static_cast<const void*>(dz) : dout;
+    const long long ldg = dz ? n : ldd;
+    LinEpilogue e;
+    memset(&e, 0, sizeof(e));
+    if (dx) {
+        e.out = static_cast<__nv_bfloat16*>(dx); e.ldo = pitch_of(lddx, m, k);
+        if ((rc = lin_gemm(g, ldg, 0, w, pitch_of(ldw, k, n), 0, m, k, n, e, false, reinterpret_cast<float*>(ws), part_bytes, s))) return rc;
+    }
+    if (dw) {
+        e.out = static_cast<__nv_bfloat16*>(dw); e.ldo = n;
+        if ((rc = lin_gemm(x, pitch_of(ldx, m, k), 1, g, ldg, 1, k, n, m, e, false, reinterpret_cast<float*>(ws), part_bytes, s))) return rc;
+    }
+    return 0;
+}
+
+}  // extern "C"

@@ -1,4 +1,4 @@
-"""Entity rows from features: dropout with a counter-based mask.
+"""Entity rows from features: a matrix product with bias, activation and residual, and dropout with a counter-based mask.
 
 The framework's scorers read rows of a table; here rows are computed.  Everything is a kernel of the library on the
 current CUDA stream.  Gradients are explicit calls, as in cuke_b200.scoring.  No counterpart in the reference, whose
@@ -6,12 +6,12 @@ entities are table rows only (apps/kge/data/data_init.py:6-15).
 """
 from __future__ import annotations
 
-from typing import Optional, Union
+from typing import Optional, Tuple, Union
 
 import torch
 
 from . import _lib
-from ._lib import DTYPES, check
+from ._lib import ACTIVATIONS, DTYPES, check
 from .scoring import _dtype_of, _ptr, _stream
 
 
@@ -77,3 +77,74 @@ def dropout(x: torch.Tensor, p: float, seed: int, stream_id: int = 0, step: Unio
     check(_lib.lib().kge_dropout(_ptr(x), dt, rows, dim, ldx, _ptr(residual), ldr, _ptr(out), ldo, float(p),
                                  int(seed) & 0xFFFFFFFFFFFFFFFF, int(stream_id) & 0xFFFFFFFF, int(step) & 0x7FFFFFFF, _ptr(step_dev), _stream()))
     return out
+
+
+def _matrix(t: torch.Tensor, name: str, rows: int, cols: int) -> int:
+    """Row pitch of a (rows, cols) bfloat16 matrix."""
+    if t.dtype != torch.bfloat16:
+        raise TypeError(f"{name} must be bfloat16, got {t.dtype}")
+    if t.shape != (rows, cols):
+        raise ValueError(f"{name} must be ({rows}, {cols}), got {tuple(t.shape)}")
+    return pitch(t, name)
+
+
+def _act(act: str) -> int:
+    if act not in ACTIVATIONS:
+        raise ValueError(f"act is one of {sorted(ACTIVATIONS)}")
+    return ACTIVATIONS[act]
+
+
+def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None, act: str = "none",
+           residual: Optional[torch.Tensor] = None, save_preact: bool = False, out: Optional[torch.Tensor] = None):
+    """act(x w + bias) + residual: entity rows computed from features (kge_linear_forward in include/kge_b200.h).
+
+    x (M, K), w (K, N) - out[j] = sum_i x[i] w[i][j], as for the relation matrices -, bias (N,) and residual (M, N) are
+    bfloat16, accumulation is fp32 with one rounding at the end; K and N are multiples of 8, rows start on 16-byte
+    boundaries.  act: "none", "relu", "silu" or "gelu" (tanh form).  With save_preact=True returns (out, preact), preact
+    being what linear_backward needs of the pre-activation: act'(x w + bias) in float16, or None for act="none"."""
+    need_here(x, w, bias, residual, out)
+    if x.dim() != 2 or w.dim() != 2:
+        raise ValueError("x and w must be matrices")
+    m, k, n = x.shape[0], x.shape[1], w.shape[1]
+    code = _act(act)
+    ldx, ldw = _matrix(x, "x", m, k), _matrix(w, "w", k, n)
+    ldr = 0 if residual is None else _matrix(residual, "residual", m, n)
+    if bias is not None and (bias.dtype != torch.bfloat16 or bias.shape != (n,) or not bias.is_contiguous()):
+        raise ValueError(f"bias must be a contiguous bfloat16 vector of {n}")
+    if out is None:
+        out = torch.empty((m, n), dtype=torch.bfloat16, device=x.device)
+    ldo = _matrix(out, "out", m, n)
+    if residual is not None and residual.data_ptr() == out.data_ptr() and ldr != ldo:
+        raise ValueError("out may be residual only with the same row pitch")
+    preact = torch.empty((m, n), dtype=torch.float16, device=x.device) if save_preact and code else None
+    L = _lib.lib()
+    need = L.kge_linear_workspace_bytes(m, k, n, code, 0)
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    check(L.kge_linear_forward(_ptr(x), ldx, _ptr(w), ldw, _ptr(bias), _ptr(residual), ldr, m, k, n, code, _ptr(out), ldo, _ptr(preact),
+                               _ptr(ws), need, _stream()))
+    return (out, preact) if save_preact else out
+
+
+def linear_backward(dout: torch.Tensor, x: torch.Tensor, w: torch.Tensor, preact: Optional[torch.Tensor] = None, act: str = "none",
+                    need_dx: bool = True, need_dw: bool = True,
+                    need_dbias: bool = True) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor], Optional[torch.Tensor]]:
+    """(dx, dw, dbias) of linear, bfloat16, from d(out) (M, N) and the preact it saved; None where not needed.  The gradient
+    of `residual` is dout itself."""
+    need_here(dout, x, w, preact)
+    if x.dim() != 2 or w.dim() != 2:
+        raise ValueError("x and w must be matrices")
+    m, k, n = x.shape[0], x.shape[1], w.shape[1]
+    code = _act(act)
+    ldd, ldx, ldw = _matrix(dout, "dout", m, n), _matrix(x, "x", m, k), _matrix(w, "w", k, n)
+    if code and (preact is None or preact.dtype != torch.float16 or preact.shape != (m, n) or not preact.is_contiguous()):
+        raise ValueError("preact must be what linear(..., save_preact=True) returned")
+    dev = x.device
+    dx = torch.empty((m, k), dtype=torch.bfloat16, device=dev) if need_dx else None
+    dw = torch.empty((k, n), dtype=torch.bfloat16, device=dev) if need_dw else None
+    db = torch.empty(n, dtype=torch.bfloat16, device=dev) if need_dbias else None
+    L = _lib.lib()
+    need = L.kge_linear_workspace_bytes(m, k, n, code, 1)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    check(L.kge_linear_backward(_ptr(dout), ldd, _ptr(x), ldx, _ptr(w), ldw, _ptr(preact) if code else None, m, k, n, code, _ptr(dx), k, _ptr(dw),
+                                _ptr(db), _ptr(ws), need, _stream()))
+    return dx, dw, db

@@ -432,6 +432,29 @@ KGE_API int kge_policy_loss(const void* scores, int32_t dtype, int64_t ld, int64
                          float* loss, float* logp, float* kl, void* dscores, int64_t ldd, void* workspace,
                          size_t workspace_bytes, kge_stream_t stream);
 
+/* ---- rows from features: matrix product with bias, activation and residual ---------------------------------------------
+ * out = act(x w + bias) + residual over bf16 operands with fp32 accumulation and one rounding to bf16, on the tensor cores:
+ * entity rows computed from feature vectors instead of being read from a table.  w (k, n) has the orientation of the relation
+ * matrices: out[j] = sum_i x[i] w[i][j].  act: none, relu, silu z s(z), gelu (tanh form) z s(2 sqrt(2/pi) (z + 0.044715 z^3)),
+ * s the logistic function.  bias (n), residual (m, n) may be NULL.  slope: NULL, or (m, n) fp16 packed, receives act'(z) for the
+ * backward call (not written for KGE_ACT_NONE).  residual may be out itself (same pitch).
+ *   kge_linear_backward  dz = dout * slope (bf16);  dx = dz w^T (m, k);  dw = x^T dz (k, n) packed;  dbias = sum of dz over the rows
+ *   (fp32 sums of the unrounded dz).  dx, dw, dbias may each be NULL (not computed); the gradient of residual is dout itself.
+ * All operands are bf16 with 16-byte aligned bases and row pitches that are multiples of 8 elements; k, n multiples of 8; any m.
+ * workspace (kge_linear_workspace_bytes; may be 0 bytes for the forward call) is 256-byte aligned.  The sums are taken in a fixed
+ * order: the same call gives the same bits.  No reference counterpart. */
+#define KGE_ACT_NONE 0
+#define KGE_ACT_RELU 1
+#define KGE_ACT_SILU 2
+#define KGE_ACT_GELU 3
+KGE_API size_t kge_linear_workspace_bytes(int64_t m, int64_t k, int64_t n, int32_t act, int32_t backward);
+KGE_API int kge_linear_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* residual,
+                       int64_t ldr, int64_t m, int64_t k, int64_t n, int32_t act, void* out, int64_t ldo, void* slope,
+                       void* workspace, size_t workspace_bytes, kge_stream_t stream);
+KGE_API int kge_linear_backward(const void* dout, int64_t ldd, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* slope,
+                       int64_t m, int64_t k, int64_t n, int32_t act, void* dx, int64_t lddx, void* dw, void* dbias,
+                       void* workspace, size_t workspace_bytes, kge_stream_t stream);
+
 /* ---- rows from features: dropout ------------------------------------------------------------------------------
  * out[i][j] = x[i][j] / (1 - p) where element e = i * dim + j is kept, 0 where it is dropped, + residual[i][j] if residual is
  * not NULL.  The mask is never stored: e is kept iff word e % 4 of Philox4x32-10 is >= floor(p * 2^32), counter words
