@@ -28,7 +28,7 @@ struct CandArgs {
     int32_t* err;
 };
 
-enum { CM_LOGP = 0, CM_POLICY = 1, CM_GRAD = 2 };
+enum { CM_LOGP = 0, CM_POLICY = 1 };
 
 __device__ __forceinline__ float cand_get(const float* p) { return *p; }
 __device__ __forceinline__ float cand_get(const __nv_bfloat16* p) { return __bfloat162float(*p); }
@@ -47,13 +47,8 @@ __device__ __forceinline__ int cand_action(const CandArgs& a, long long row, int
     return -1;
 }
 
-// Logarithm of the chosen candidate's probability from x = (s_a - m) / T and S' (S = e_a + S').
-__device__ __forceinline__ double cand_logp(double x, float rest) {
-    return x == 0.0 ? -log1p(static_cast<double>(rest)) : x - log(exp(x) + static_cast<double>(rest));
-}
-
 // Loss term of one row and, in *g, d(loss) / d(logp); logp and kl are stored by the caller's thread.
-__device__ __forceinline__ double policy_term(const CandArgs& a, long long row, double logp, double* g) {
+__device__ __forceinline__ double policy_term(const CandArgs& a, long long row, double logp, double* g, bool write) {
     const double w = a.weight ? a.weight[row] : 1.0;
     const double A = a.adv[row], ratio = exp(logp - static_cast<double>(a.old_logp[row]));
     const double lo = 1.0 - static_cast<double>(a.clip_lo), hi = 1.0 + static_cast<double>(a.clip_hi);
@@ -65,83 +60,455 @@ __device__ __forceinline__ double policy_term(const CandArgs& a, long long row, 
         l += a.kl_coef * kl;
         dl -= a.kl_coef * e;
     }
-    a.logp[row] = static_cast<float>(logp);
-    a.kl[row] = static_cast<float>(kl);
+    if (write) { a.logp[row] = static_cast<float>(logp); a.kl[row] = static_cast<float>(kl); }
     if (w == 0.0) { *g = 0.0; return 0.0; }
     *g = w * a.scale * dl;
     return w * a.scale * l;
 }
 
-// One CTA per row: maximum, sum, gradient in three passes over the row.
-template <typename T, int MODE>
-__global__ void __launch_bounds__(256) cand_row_kernel(CandArgs a) {
-    __shared__ float red[8];
-    __shared__ float bc[2];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+// What follows from a row's statistics: logp, kl, loss term (returned), and the factor ga of the gradient,
+// ds_j = ga (rest [j = a] - e_j [j != a]) with e_j = exp((s_j - m) / T).  One thread of a row calls it.
+template <int MODE>
+__device__ __forceinline__ double cand_finish(const CandArgs& a, long long row, int act, float sa, float m, float rest, bool write, float* ga) {
+    const double x = act >= 0 ? static_cast<double>(sa - m) * static_cast<double>(a.inv_temp) : 0.0;
+    const bool live = act >= 0 && !(sa == -INFINITY && rest == 0.f);
+    const double ea = x == 0.0 ? 1.0 : exp(x);
+    const double S = ea + static_cast<double>(rest);
+    const double lp = !live ? 0.0 : x == 0.0 ? -log1p(static_cast<double>(rest)) : x - log(S);
+    const float inv = live ? static_cast<float>(1.0 / S) : 0.f;
+    *ga = 0.f;
+    if (MODE == CM_LOGP) {
+        if (write) {
+            a.logp[row] = static_cast<float>(lp);
+            a.stats[3 * row] = m; a.stats[3 * row + 1] = rest; a.stats[3 * row + 2] = inv;
+        }
+        return 0.0;
+    }
+    if (!live) {
+        if (write) { a.logp[row] = 0.f; a.kl[row] = 0.f; }
+        return 0.0;
+    }
+    double g;
+    const double l = policy_term(a, row, lp, &g, write);
+    if (g != 0.0) *ga = static_cast<float>(g * a.inv_temp) * inv;         // (a row of weight 0 may hold NaN)
+    return l;
+}
+
+// ---- 16-byte vectors of a row --------------------------------------------------------------------------------------
+// A row is cut into a head of fewer than V elements up to the first 16-byte boundary, whole vectors, and a tail; head and
+// tail elements are one extra element each of 16 threads.  Vector v holds the elements head + v V, ...
+template <typename T> struct Vec;
+template <> struct Vec<float> {
+    static constexpr int V = 4;
+    static constexpr uint32_t kLow = 0xFF800000u;          // a word of -infinity
+    __device__ static __forceinline__ float max(uint4 r) {
+        return fmaxf(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)), fmaxf(__uint_as_float(r.z), __uint_as_float(r.w)));
+    }
+    __device__ static __forceinline__ void open(uint4 r, float (&f)[4]) {
+        f[0] = __uint_as_float(r.x); f[1] = __uint_as_float(r.y); f[2] = __uint_as_float(r.z); f[3] = __uint_as_float(r.w);
+    }
+    __device__ static __forceinline__ uint4 close(const float (&f)[4]) {
+        return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+    }
+};
+template <> struct Vec<__nv_bfloat16> {
+    static constexpr int V = 8;
+    static constexpr uint32_t kLow = 0xFF80FF80u;
+    __device__ static __forceinline__ float max(uint4 r) {
+        const __nv_bfloat162 a = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&r.x), *reinterpret_cast<__nv_bfloat162*>(&r.y));
+        const __nv_bfloat162 b = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&r.z), *reinterpret_cast<__nv_bfloat162*>(&r.w));
+        const float2 f = __bfloat1622float2(__hmax2(a, b));
+        return fmaxf(f.x, f.y);
+    }
+    __device__ static __forceinline__ void open(uint4 r, float (&f)[8]) {
+        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(w[i] << 16); f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u); }
+    }
+    __device__ static __forceinline__ uint4 close(const float (&f)[8]) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            __nv_bfloat162 p = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+            w[i] = *reinterpret_cast<uint32_t*>(&p);
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+};
+__device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY ? 0.f : m; }
+template <typename T>
+__device__ __forceinline__ int head_of(const T* p, int n) {
+    const int to = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / static_cast<int>(sizeof(T));
+    return to < n ? to : n;
+}
+// Elements from `cnt` on read as -infinity.
+template <typename T>
+__device__ __forceinline__ uint4 mask_past(uint4 r, int first, int cnt) {
+    float f[Vec<T>::V];
+    Vec<T>::open(r, f);
+#pragma unroll
+    for (int k = 0; k < Vec<T>::V; ++k) if (first + k >= cnt) f[k] = -INFINITY;
+    return Vec<T>::close(f);
+}
+// (m, rest) of two disjoint parts of a row
+__device__ __forceinline__ void merge_parts(float& m, float& rest, float m2, float r2, float c) {
+    const float top = finite_or_zero(fmaxf(m, m2));
+    rest = rest * cand_ex2((m - top) * c) + r2 * cand_ex2((m2 - top) * c);
+    m = fmaxf(m, m2);
+}
+
+// ---- rows kept in registers -------------------------------------------------------------------------------------------
+// A group of 32 lanes (one warp a row), or of THREADS x cluster size, reads its row once, as I vectors a thread, and keeps it
+// until the gradient is written: 8 bytes of traffic per fp32 score, 4 per bf16.  Each warp takes its own maximum and sum; the
+// (m, rest) pairs of a row's warps are merged after one barrier.  fp32 scores are replaced by their exponentials in place, so
+// the gradient costs one multiplication each; bf16 scores stay packed and are exponentiated a second time.
+constexpr int kMaxCluster = 8;
+template <typename T, int THREADS, int I, int MODE>
+__global__ void __launch_bounds__(THREADS == 32 ? 256 : THREADS, THREADS == 32 ? (I == 8 ? 3 : 4) : 1024 / THREADS)
+cand_cached_kernel(CandArgs a) {
+    constexpr int V = Vec<T>::V;
+    constexpr bool kWarp32 = THREADS == 32;
+    constexpr bool kKeepExp = sizeof(T) == 4;
+    constexpr int kWarps = THREADS / 32;
+    __shared__ float2 parts[2][kWarp32 ? 1 : kWarps];
+    __shared__ float bcast[2];
+    __shared__ double red[8];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int tid = kWarp32 ? lane : threadIdx.x;
+    uint32_t rank = 0, csize = 1;
+    if (!kWarp32) {
+        asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+        asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(csize));
+    }
+    const long long groups = kWarp32 ? (long long)gridDim.x * (blockDim.x >> 5) : gridDim.x / csize;
+    const long long first_row = kWarp32 ? (long long)blockIdx.x * (blockDim.x >> 5) + warp : blockIdx.x / csize;
+    const float c = a.inv_temp * 1.4426950408889634f;
     double total = 0.0;
-    for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    int flip = 0;
+    for (long long row = first_row; row < a.rows; row += groups, flip ^= 1) {
         const T* s = static_cast<const T*>(a.scores) + row * a.ld;
         const int cnt = cand_count(a, row);
-        const int act = cand_action(a, row, cnt, tid == 0 && MODE != CM_GRAD);
-        float m, rest;
-        if (MODE == CM_GRAD) {
-            m = a.stats[3 * row]; rest = a.stats[3 * row + 1];
-        } else {
-            m = -INFINITY;
-            for (int j = tid; j < cnt; j += 256) m = fmaxf(m, cand_get(s + j));
+        const int act = cand_action(a, row, cnt, tid == 0 && rank == 0);
+        const float sa = act >= 0 ? cand_get(s + act) : 0.f;
+        const int head = head_of(s, a.n), nv = (a.n - head) / V;
+        const int share = (nv + static_cast<int>(csize) - 1) / static_cast<int>(csize);       // this CTA's vectors: [v0, v1)
+        const int v0 = static_cast<int>(rank) * share, v1 = min(nv, v0 + share);
+        // the extra element of this thread, if any
+        int xi = -1;
+        if (rank == 0 && tid < 16) {
+            if (tid < 8) { if (tid < head) xi = tid; }
+            else if (head + nv * V + tid - 8 < a.n) xi = head + nv * V + tid - 8;
+        }
+        const uint4* sv = reinterpret_cast<const uint4*>(s + head);
+        uint4 r[I];
 #pragma unroll
-            for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, o));
-            if (lane == 0) red[warp] = m;
-            __syncthreads();
-            m = red[0];
-            for (int i = 1; i < 8; ++i) m = fmaxf(m, red[i]);
-            __syncthreads();
-            if (m == -INFINITY) m = 0.f;         // no candidate, or none with a finite score: the sum below says which
+        for (int i = 0; i < I; ++i) {
+            const int v = v0 + tid + i * THREADS;
+            r[i] = make_uint4(Vec<T>::kLow, Vec<T>::kLow, Vec<T>::kLow, Vec<T>::kLow);
+            if (v < v1 && head + v * V < cnt) r[i] = __ldcs(sv + v);
         }
-        const float c = a.inv_temp * 1.4426950408889634f;
-        if (MODE != CM_GRAD) {
-            rest = 0.f;
-            for (int j = tid; j < cnt; j += 256) if (j != act) rest += cand_ex2((cand_get(s + j) - m) * c);
-            rest = warp_sum(rest);
-            if (lane == 0) red[warp] = rest;
-            __syncthreads();
-            rest = 0.f;
-            for (int i = 0; i < 8; ++i) rest += red[i];
-        }
-        if (tid == 0) {
-            double g = 0.0;
-            float inv = 0.f;
-            if (MODE == CM_GRAD) {
-                g = a.dlogp[row]; inv = act >= 0 ? a.stats[3 * row + 2] : 0.f;
-            } else {
-                const float sa = act >= 0 ? cand_get(s + act) : 0.f;
-                const double x = act >= 0 ? static_cast<double>(sa - m) * static_cast<double>(a.inv_temp) : 0.0;
-                const bool live = act >= 0 && !(sa == -INFINITY && rest == 0.f);
-                const double lp = live ? cand_logp(x, rest) : 0.0;
-                if (live) inv = static_cast<float>(1.0 / (exp(x) + rest));
-                if (MODE == CM_POLICY) {
-                    if (live) total += policy_term(a, row, lp, &g);
-                    else { a.logp[row] = 0.f; a.kl[row] = 0.f; }
-                } else {
-                    a.logp[row] = static_cast<float>(lp);
-                    a.stats[3 * row] = m; a.stats[3 * row + 1] = rest; a.stats[3 * row + 2] = inv;
-                }
+        float xe = xi >= 0 && xi < cnt ? cand_get(s + xi) : -INFINITY;
+        if (a.n_cand) {
+#pragma unroll
+            for (int i = 0; i < I; ++i) {
+                const int at = head + (v0 + tid + i * THREADS) * V;
+                if (at < cnt && at + V > cnt) r[i] = mask_past<T>(r[i], at, cnt);
             }
-            bc[0] = static_cast<float>(g * a.inv_temp); bc[1] = inv;
+        }
+        float mw = xe;
+#pragma unroll
+        for (int i = 0; i < I; ++i) mw = fmaxf(mw, Vec<T>::max(r[i]));
+#pragma unroll
+        for (int o = 16; o; o >>= 1) mw = fmaxf(mw, __shfl_xor_sync(kFull, mw, o));
+        const float mz = finite_or_zero(mw);
+        // the vector (register index) of this thread that holds the chosen candidate
+        int own = -1;
+        if (act >= head && act < head + nv * V) {
+            const int v = (act - head) / V - v0;
+            if (v >= 0 && v % THREADS == tid && v0 + v < v1) own = v / THREADS;
+        }
+        float rest = 0.f;
+        {
+            const float e = cand_ex2((xe - mz) * c);
+            if (xi != act) rest = e;
+            if (kKeepExp) xe = e;
+        }
+#pragma unroll
+        for (int i = 0; i < I; ++i) {
+            float f[V];
+            Vec<T>::open(r[i], f);
+#pragma unroll
+            for (int k = 0; k < V; ++k) f[k] = cand_ex2((f[k] - mz) * c);
+            if (kKeepExp) r[i] = Vec<T>::close(f);
+            if (i == own) {
+#pragma unroll
+                for (int k = 0; k < V; ++k) if ((act - head) % V == k) f[k] = 0.f;
+            }
+            float t = 0.f;
+#pragma unroll
+            for (int k = 0; k < V; k += 4) t += (f[k] + f[k + 1]) + (f[k + 2] + f[k + 3]);
+            rest += t;
+        }
+        rest = warp_sum(rest);
+        float m = mw, ga = 0.f;
+        if (kWarp32) {
+            if (lane == 0) total += cand_finish<MODE>(a, row, act, sa, finite_or_zero(m), rest, true, &ga);
+            if (MODE != CM_LOGP) ga = __shfl_sync(kFull, ga, 0);
+        } else {
+            if (lane == 0) parts[flip][warp] = make_float2(mw, rest);
+            if (csize == 1) {
+                __syncthreads();
+            } else {
+                asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+            }
+            // every warp merges all parts of the row, in the same order
+            m = -INFINITY; rest = 0.f;
+            const int n_parts = kWarps * static_cast<int>(csize);
+            for (int j = lane; j < n_parts; j += 32) {
+                float2 q;
+                const uint32_t addr = static_cast<uint32_t>(__cvta_generic_to_shared(&parts[flip][j % kWarps]));
+                uint32_t remote;
+                asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(static_cast<uint32_t>(j / kWarps)));
+                asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(q.x), "=f"(q.y) : "r"(remote) : "memory");
+                merge_parts(m, rest, q.x, q.y, c);
+            }
+#pragma unroll
+            for (int o = 16; o; o >>= 1) {
+                const float m2 = __shfl_xor_sync(kFull, m, o), r2 = __shfl_xor_sync(kFull, rest, o);
+                merge_parts(m, rest, m2, r2, c);
+            }
+            if (MODE == CM_LOGP) {
+                if (threadIdx.x == 0 && rank == 0) cand_finish<MODE>(a, row, act, sa, finite_or_zero(m), rest, true, &ga);
+            } else {
+                if (threadIdx.x == 0) {
+                    const double l = cand_finish<MODE>(a, row, act, sa, finite_or_zero(m), rest, rank == 0, &ga);
+                    if (rank == 0) total += l;
+                    bcast[flip] = ga;
+                }
+                __syncthreads();
+                ga = bcast[flip];
+            }
         }
         if (MODE != CM_LOGP) {
-            __syncthreads();
-            const float ga = bc[0] == 0.f ? 0.f : bc[0] * bc[1];      // (a row of weight 0 may hold NaN)
             T* d = static_cast<T*>(a.dscores) + row * a.ldd;
-            for (int j = tid; j < a.n; j += 256) {
-                float v = 0.f;
-                if (j < cnt && ga != 0.f) v = j == act ? ga * rest : -ga * cand_ex2((cand_get(s + j) - m) * c);
-                cand_put(d + j, v);
+            uint4* dv = reinterpret_cast<uint4*>(d + head);
+            const float mall = finite_or_zero(m);
+            // (a warp without a finite score has only zeros to scale: mz = 0 stands for nothing there)
+            const float f0 = ga == 0.f || (kKeepExp && mw == -INFINITY) ? 0.f : kKeepExp ? -ga * cand_ex2((mz - mall) * c) : -ga;
+            const float fa = ga == 0.f ? 0.f : ga * rest;
+#pragma unroll
+            for (int i = 0; i < I; ++i) {
+                const int v = v0 + tid + i * THREADS;
+                if (v < v1) {
+                    const int at = head + v * V;
+                    float f[V];
+                    if (at >= cnt || ga == 0.f) {
+#pragma unroll
+                        for (int k = 0; k < V; ++k) f[k] = 0.f;
+                    } else {
+                        Vec<T>::open(r[i], f);
+#pragma unroll
+                        for (int k = 0; k < V; ++k) f[k] = f0 * (kKeepExp ? f[k] : cand_ex2((f[k] - mall) * c));
+                        if (i == own) {
+#pragma unroll
+                            for (int k = 0; k < V; ++k) if (at + k == act) f[k] = fa;
+                        }
+                        if (at + V > cnt) {
+#pragma unroll
+                            for (int k = 0; k < V; ++k) if (at + k >= cnt) f[k] = 0.f;
+                        }
+                    }
+                    __stcs(dv + v, Vec<T>::close(f));
+                }
             }
+            if (xi >= 0) {
+                float v = 0.f;
+                if (xi < cnt && ga != 0.f) v = xi == act ? fa : f0 * (kKeepExp ? xe : cand_ex2((xe - mall) * c));
+                cand_put(d + xi, v);
+            }
+        }
+    }
+    if (!kWarp32 && csize > 1)            // no CTA leaves while another may still read its parts
+        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (MODE == CM_POLICY) {
+        if (kWarp32) {
+            if (lane == 0) red[warp] = total;
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                for (int w = 1; w < 8; ++w) total += red[w];
+                a.partial[blockIdx.x] = total;
+            }
+        } else if (threadIdx.x == 0 && rank == 0) {
+            a.partial[blockIdx.x / csize] = total;
+        }
+    }
+}
+
+// ---- rows cut over several CTAs, in passes ----------------------------------------------------------------------------
+// For a few long rows (every SM reads), rows that no cluster can hold, and rows whose gradient lies at another alignment.
+// Pass 1: (m, rest) of every chunk of a row; pass 2: a warp per row joins them; pass 3 (policy): the gradient, elementwise.
+template <typename T>
+__global__ void __launch_bounds__(256) cand_stats_kernel(CandArgs a, float2* parts, int chunk, int chunks) {
+    constexpr int V = Vec<T>::V;
+    __shared__ float2 red[8];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const float c = a.inv_temp * 1.4426950408889634f;
+    for (long long u = blockIdx.x; u < a.rows * chunks; u += gridDim.x) {
+        const long long row = u / chunks;
+        const int k = static_cast<int>(u - row * chunks);
+        const int cnt = cand_count(a, row), act = cand_action(a, row, cnt, tid == 0 && k == 0);
+        const int j0 = k * chunk, n = min(chunk, cnt - j0);                // (may be <= 0)
+        float m = -INFINITY, rest = 0.f;
+        if (n > 0) {
+            const T* s = static_cast<const T*>(a.scores) + row * a.ld + j0;
+            const int head = head_of(s, n), nv = (n - head) / V, la = act - j0;
+            const uint4* sv = reinterpret_cast<const uint4*>(s + head);
+            if (tid < 16) {
+                const int xi = tid < 8 ? (tid < head ? tid : -1) : (head + nv * V + tid - 8 < n ? head + nv * V + tid - 8 : -1);
+                if (xi >= 0) {
+                    m = cand_get(s + xi);
+                    rest = xi == la ? 0.f : cand_ex2((m - finite_or_zero(m)) * c);
+                }
+            }
+            const int av = la >= head && la < head + nv * V ? (la - head) / V : -1;
+            for (int base = tid; base < nv; base += 4 * 256) {
+                uint4 r[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    r[i] = make_uint4(Vec<T>::kLow, Vec<T>::kLow, Vec<T>::kLow, Vec<T>::kLow);
+                    if (base + i * 256 < nv) r[i] = __ldcs(sv + base + i * 256);
+                }
+                const float bm = fmaxf(fmaxf(Vec<T>::max(r[0]), Vec<T>::max(r[1])), fmaxf(Vec<T>::max(r[2]), Vec<T>::max(r[3])));
+                const float top = fmaxf(m, bm), mz = finite_or_zero(top);
+                if (bm > m) { rest *= cand_ex2((m - mz) * c); m = top; }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float f[V];
+                    Vec<T>::open(r[i], f);
+#pragma unroll
+                    for (int q = 0; q < V; ++q) f[q] = cand_ex2((f[q] - mz) * c);
+                    if (base + i * 256 == av) {
+#pragma unroll
+                        for (int q = 0; q < V; ++q) if ((la - head) % V == q) f[q] = 0.f;
+                    }
+                    float t = 0.f;
+#pragma unroll
+                    for (int q = 0; q < V; q += 4) t += (f[q] + f[q + 1]) + (f[q + 2] + f[q + 3]);
+                    rest += t;
+                }
+            }
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) {
+            const float m2 = __shfl_xor_sync(kFull, m, o), r2 = __shfl_xor_sync(kFull, rest, o);
+            merge_parts(m, rest, m2, r2, c);
+        }
+        if (lane == 0) red[warp] = make_float2(m, rest);
+        __syncthreads();
+        if (tid == 0) {
+            for (int w = 1; w < 8; ++w) merge_parts(m, rest, red[w].x, red[w].y, c);
+            parts[u] = make_float2(m, rest);
         }
         __syncthreads();
     }
-    if (MODE == CM_POLICY && tid == 0) a.partial[blockIdx.x] = total;
+}
+
+template <typename T, int MODE>
+__global__ void __launch_bounds__(256) cand_join_kernel(CandArgs a, const float2* parts, int chunks, float* coef) {
+    __shared__ double red[8];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const float c = a.inv_temp * 1.4426950408889634f;
+    double total = 0.0;
+    for (long long row = (long long)blockIdx.x * 8 + warp; row < a.rows; row += (long long)gridDim.x * 8) {
+        float m = -INFINITY, rest = 0.f;
+        for (int k = lane; k < chunks; k += 32) {
+            const float2 q = parts[row * chunks + k];
+            merge_parts(m, rest, q.x, q.y, c);
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) {
+            const float m2 = __shfl_xor_sync(kFull, m, o), r2 = __shfl_xor_sync(kFull, rest, o);
+            merge_parts(m, rest, m2, r2, c);
+        }
+        if (lane == 0) {
+            const int act = cand_action(a, row, cand_count(a, row), false);
+            const float sa = act >= 0 ? cand_get(static_cast<const T*>(a.scores) + row * a.ld + act) : 0.f;
+            float ga;
+            total += cand_finish<MODE>(a, row, act, sa, finite_or_zero(m), rest, true, &ga);
+            if (MODE == CM_POLICY) { coef[3 * row] = finite_or_zero(m); coef[3 * row + 1] = rest; coef[3 * row + 2] = ga; }
+        }
+    }
+    if (MODE == CM_POLICY) {
+        if (lane == 0) red[warp] = total;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            for (int w = 1; w < 8; ++w) total += red[w];
+            a.partial[blockIdx.x] = total;
+        }
+    }
+}
+
+// ds from (m, rest, ga) per row, or, with dlogp, from the stats of log_prob: ga = dlogp / T / S.  A warp takes pieces of
+// 32 x 4 vectors (ALIGNED: scores and gradient rows at the same 16-byte phase) or of 32 x 4 elements.
+template <typename T, bool ALIGNED>
+__global__ void __launch_bounds__(256) cand_grad_kernel(CandArgs a, const float* coef, long long pieces) {
+    constexpr int V = ALIGNED ? Vec<T>::V : 1;
+    const int lane = threadIdx.x & 31;
+    const float c = a.inv_temp * 1.4426950408889634f;
+    const long long units = a.rows * pieces;
+    for (long long u = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); u < units; u += (long long)gridDim.x * 8) {
+        const long long row = u / pieces;
+        const int piece = static_cast<int>(u - row * pieces);
+        const T* s = static_cast<const T*>(a.scores) + row * a.ld;
+        T* d = static_cast<T*>(a.dscores) + row * a.ldd;
+        const int cnt = cand_count(a, row), act = cand_action(a, row, cnt, false);
+        const float m = __ldg(coef + 3 * row), rest = __ldg(coef + 3 * row + 1);
+        float ga = __ldg(coef + 3 * row + 2);
+        if (a.dlogp) { const float g = __ldg(a.dlogp + row) * a.inv_temp; ga = g == 0.f || act < 0 ? 0.f : g * ga; }
+        const float fa = ga == 0.f ? 0.f : ga * rest;
+        auto one = [&](int j, float x) { return j >= cnt || ga == 0.f ? 0.f : j == act ? fa : -ga * cand_ex2((x - m) * c); };
+        if constexpr (ALIGNED) {
+            const int head = head_of(s, a.n), nv = (a.n - head) / V;
+            const uint4* sv = reinterpret_cast<const uint4*>(s + head);
+            uint4* dv = reinterpret_cast<uint4*>(d + head);
+            uint4 r[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int v = piece * 128 + i * 32 + lane;
+                if (v < nv && head + v * V < cnt) r[i] = __ldcs(sv + v);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int v = piece * 128 + i * 32 + lane, at = head + v * V;
+                if (v >= nv) continue;
+                float f[V];
+                if (at >= cnt || ga == 0.f) {
+#pragma unroll
+                    for (int k = 0; k < V; ++k) f[k] = 0.f;
+                } else {
+                    Vec<T>::open(r[i], f);
+                    if (at + V > cnt || (act >= at && act < at + V)) {
+#pragma unroll
+                        for (int k = 0; k < V; ++k) f[k] = one(at + k, f[k]);
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < V; ++k) f[k] = -ga * cand_ex2((f[k] - m) * c);
+                    }
+                }
+                __stcs(dv + v, Vec<T>::close(f));
+            }
+            if (piece == 0 && lane < 16) {
+                const int xi = lane < 8 ? (lane < head ? lane : -1) : (head + nv * V + lane - 8 < a.n ? head + nv * V + lane - 8 : -1);
+                if (xi >= 0) cand_put(d + xi, one(xi, xi < cnt ? cand_get(s + xi) : 0.f));
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int j = piece * 128 + i * 32 + lane;
+                if (j < a.n) cand_put(d + j, one(j, j < cnt ? cand_get(s + j) : 0.f));
+            }
+        }
+    }
 }
 
 __global__ void __launch_bounds__(256) sum_partials_kernel(const double* partial, int n, float* out) {
@@ -163,19 +530,94 @@ int launch_sum_partials(const double* partial, int n, float* out, cudaStream_t s
     return 0;
 }
 
-constexpr int kCandMaxBlocks = 148 * 8;
+constexpr int kCandMaxBlocks = 148 * 8;            // CTAs that leave a partial sum of the loss
 
-static int launch_candidates(const CandArgs& a, int dtype, int mode, cudaStream_t s) {
-    if (a.rows == 0) return 0;
-    const unsigned blocks = static_cast<unsigned>(a.rows < kCandMaxBlocks ? a.rows : kCandMaxBlocks);
-#define KGE_CAND(M) do { if (dtype == KGE_F32) cand_row_kernel<float, M><<<blocks, 256, 0, s>>>(a); \
-                         else cand_row_kernel<__nv_bfloat16, M><<<blocks, 256, 0, s>>>(a); } while (0)
-    if (mode == CM_LOGP) KGE_CAND(CM_LOGP);
-    else if (mode == CM_POLICY) KGE_CAND(CM_POLICY);
-    else KGE_CAND(CM_GRAD);
-#undef KGE_CAND
-    KGE_LAUNCH_CHECK("cand_row_kernel");
+// Workspace: partial sums of the loss, then per-chunk (m, rest) and per-row coefficients of the multi-pass form.
+struct CandLayout { int chunk, chunks; size_t off_parts, off_coef, total; };
+static CandLayout cand_layout(long long rows, long long n) {
+    CandLayout L;
+    // chunks of at least 8192 scores (32 KB of fp32: enough loads in flight per CTA), about 16 CTAs' worth of them per SM
+    long long per = (rows * n + 148 * 16 - 1) / (148 * 16);
+    per = per < 8192 ? 8192 : (per + 1023) / 1024 * 1024;
+    if (per > n) per = n > 0 ? n : 1;
+    L.chunk = static_cast<int>(per);
+    L.chunks = static_cast<int>((n + per - 1) / per);
+    if (L.chunks < 1) L.chunks = 1;
+    L.off_parts = kCandMaxBlocks * sizeof(double);
+    L.off_coef = L.off_parts + sizeof(float2) * static_cast<size_t>(rows) * L.chunks;
+    L.total = L.off_coef + 3 * sizeof(float) * static_cast<size_t>(rows);
+    return L;
+}
+
+template <typename T, int THREADS, int I, int MODE>
+static int cand_cached(const CandArgs& a, int cluster, int* n_partial, cudaStream_t s) {
+    const int wpb = THREADS == 32 ? 8 : 1;
+    const long long want = THREADS == 32 ? (a.rows + wpb - 1) / wpb : a.rows;
+    const long long cap = THREADS == 32 ? kCandMaxBlocks : 148 * (1024 / THREADS) / cluster;
+    const long long groups = want < cap ? want : cap;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(groups * cluster));
+    cfg.blockDim = dim3(THREADS == 32 ? 256 : THREADS);
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = cluster; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+    cfg.attrs = at; cfg.numAttrs = cluster > 1 ? 1 : 0;
+    *n_partial = static_cast<int>(groups);
+    cudaError_t e = cudaLaunchKernelEx(&cfg, cand_cached_kernel<T, THREADS, I, MODE>, a);
+    if (e != cudaSuccess) return cuda_status(e, "cand_cached_kernel");
+    KGE_LAUNCH_CHECK("cand_cached_kernel");
     return 0;
+}
+
+template <typename T>
+static int cand_gradient(const CandArgs& a, const float* coef, bool aligned, cudaStream_t s) {
+    const int per = 128 * (aligned ? Vec<T>::V : 1);
+    const long long pieces = a.n > 0 ? (a.n + per - 1) / per : 1, want = (a.rows * pieces + 7) / 8;
+    const unsigned blocks = static_cast<unsigned>(want < 148 * 64 ? want : 148 * 64);
+    if (aligned) cand_grad_kernel<T, true><<<blocks, 256, 0, s>>>(a, coef, pieces);
+    else cand_grad_kernel<T, false><<<blocks, 256, 0, s>>>(a, coef, pieces);
+    KGE_LAUNCH_CHECK("cand_grad_kernel");
+    return 0;
+}
+
+template <typename T>
+static bool same_phase(const CandArgs& a) {
+    const uintptr_t d = reinterpret_cast<uintptr_t>(a.scores) - reinterpret_cast<uintptr_t>(a.dscores);
+    return ((d & 15) == 0) && (a.rows == 1 || (((a.ld - a.ldd) * static_cast<long long>(sizeof(T))) & 15) == 0);
+}
+
+template <typename T, int MODE>
+static int cand_passes(const CandArgs& a, void* ws, int* n_partial, cudaStream_t s) {
+    const CandLayout L = cand_layout(a.rows, a.n);
+    float2* parts = reinterpret_cast<float2*>(static_cast<char*>(ws) + L.off_parts);
+    float* coef = reinterpret_cast<float*>(static_cast<char*>(ws) + L.off_coef);
+    const long long units = a.rows * L.chunks;
+    cand_stats_kernel<T><<<static_cast<unsigned>(units < 148 * 64 ? units : 148 * 64), 256, 0, s>>>(a, parts, L.chunk, L.chunks);
+    KGE_LAUNCH_CHECK("cand_stats_kernel");
+    const long long jb = (a.rows + 7) / 8;
+    *n_partial = static_cast<int>(jb < kCandMaxBlocks ? jb : kCandMaxBlocks);
+    cand_join_kernel<T, MODE><<<*n_partial, 256, 0, s>>>(a, parts, L.chunks, coef);
+    KGE_LAUNCH_CHECK("cand_join_kernel");
+    return MODE == CM_POLICY ? cand_gradient<T>(a, coef, same_phase<T>(a), s) : 0;
+}
+
+// Which form: the smallest group that holds a row in registers; passes where the rows are too long for a cluster, where the
+// groups of all rows would leave most SMs idle, or where the gradient's alignment differs.
+template <typename T, int MODE>
+static int cand_go(const CandArgs& a, void* ws, int* n_partial, cudaStream_t s) {
+    const long long nv = a.n / Vec<T>::V;              // vectors of a row, at most
+    if (MODE == CM_POLICY && !same_phase<T>(a)) return cand_passes<T, MODE>(a, ws, n_partial, s);
+    if (nv <= 32) return cand_cached<T, 32, 1, MODE>(a, 1, n_partial, s);
+    if (nv <= 64) return cand_cached<T, 32, 2, MODE>(a, 1, n_partial, s);
+    if (nv <= 128) return cand_cached<T, 32, 4, MODE>(a, 1, n_partial, s);
+    if (nv <= 256) return cand_cached<T, 32, 8, MODE>(a, 1, n_partial, s);
+    if (nv <= 128 * 8) return cand_cached<T, 128, 8, MODE>(a, 1, n_partial, s);
+    if (nv <= 256 * 8) return cand_cached<T, 256, 8, MODE>(a, 1, n_partial, s);
+    int cluster = 1;
+    while (cluster <= kMaxCluster && nv > cluster * 512LL * 8) cluster *= 2;
+    if (cluster > kMaxCluster || a.rows * cluster < 32) return cand_passes<T, MODE>(a, ws, n_partial, s);
+    return cand_cached<T, 512, 8, MODE>(a, cluster, n_partial, s);
 }
 
 }  // namespace kge
@@ -189,6 +631,7 @@ static int check_candidates(const char* fn, const void* scores, int32_t dtype, i
     if (!(temperature > 0.f) || !(1.f / temperature > 0.f) || isinf(1.f / temperature)) { set_error("%s: temperature %g is not a positive number", fn, temperature); return KGE_E_RANGE; }
     if (rows < 0 || n < 0) { set_error("%s: negative size", fn); return KGE_E_SHAPE; }
     if (n > (1LL << 30) || rows > (1LL << 40)) { set_error("%s: more than 2^30 candidates or 2^40 rows", fn); return KGE_E_RANGE; }
+    if (n > 0 && rows > (1LL << 46) / n) { set_error("%s: more than 2^46 scores", fn); return KGE_E_RANGE; }
     if (rows > 1 && ld < n) { set_error("%s: row pitch %lld is below n", fn, (long long)ld); return KGE_E_SHAPE; }
     if (ld > (1LL << 40)) { set_error("%s: row pitch above 2^40", fn); return KGE_E_RANGE; }
     if (rows == 0) return 0;
@@ -218,8 +661,8 @@ static int check_gradient(const char* fn, void* dscores, int32_t dtype, int64_t 
 extern "C" {
 
 size_t kge_candidates_workspace_bytes(int64_t rows, int64_t n) {
-    (void)rows; (void)n;
-    return kCandMaxBlocks * sizeof(double);
+    if (rows <= 0 || n < 0 || n > (1LL << 30) || rows > (1LL << 40) || (n > 0 && rows > (1LL << 46) / n)) return 0;
+    return cand_layout(rows, n).total;
 }
 
 int kge_log_prob(const void* scores, int32_t dtype, int64_t ld, int64_t rows, int64_t n, const int32_t* n_cand, const void* action,
@@ -234,7 +677,9 @@ int kge_log_prob(const void* scores, int32_t dtype, int64_t ld, int64_t rows, in
     if (!workspace) { set_error("%s: workspace is NULL", fn); return KGE_E_NULL; }
     if (!aligned16(workspace)) { set_error("%s: workspace is not 16-byte aligned", fn); return KGE_E_ALIGN; }
     a.logp = logp; a.stats = stats;
-    return launch_candidates(a, dtype, CM_LOGP, reinterpret_cast<cudaStream_t>(stream));
+    int parts;
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    return dtype == KGE_F32 ? cand_go<float, CM_LOGP>(a, workspace, &parts, s) : cand_go<__nv_bfloat16, CM_LOGP>(a, workspace, &parts, s);
 }
 
 int kge_log_prob_backward(const void* scores, int32_t dtype, int64_t ld, int64_t rows, int64_t n, const int32_t* n_cand, const void* action,
@@ -247,7 +692,8 @@ int kge_log_prob_backward(const void* scores, int32_t dtype, int64_t ld, int64_t
     if ((rc = check_floats(fn, "stats", stats, true)) || (rc = check_floats(fn, "dlogp", dlogp, true)) ||
         (rc = check_gradient(fn, dscores, dtype, ldd, rows, n))) return rc;
     a.stats = const_cast<float*>(stats); a.dlogp = dlogp; a.dscores = dscores; a.ldd = ldd;
-    return launch_candidates(a, dtype, CM_GRAD, reinterpret_cast<cudaStream_t>(stream));
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    return dtype == KGE_F32 ? cand_gradient<float>(a, stats, same_phase<float>(a), s) : cand_gradient<__nv_bfloat16>(a, stats, same_phase<__nv_bfloat16>(a), s);
 }
 
 int kge_policy_loss(const void* scores, int32_t dtype, int64_t ld, int64_t rows, int64_t n, const int32_t* n_cand, const void* action,
@@ -273,8 +719,9 @@ int kge_policy_loss(const void* scores, int32_t dtype, int64_t ld, int64_t rows,
     a.old_logp = old_logp; a.ref_logp = ref_logp; a.adv = advantage; a.weight = weight;
     a.clip_lo = clip_low; a.clip_hi = clip_high; a.kl_coef = kl_coef; a.scale = scale;
     a.partial = static_cast<double*>(workspace);
-    if ((rc = launch_candidates(a, dtype, CM_POLICY, s))) return rc;
-    return launch_sum_partials(a.partial, static_cast<int>(rows < kCandMaxBlocks ? rows : kCandMaxBlocks), loss, s);
+    int parts = 0;
+    rc = dtype == KGE_F32 ? cand_go<float, CM_POLICY>(a, workspace, &parts, s) : cand_go<__nv_bfloat16, CM_POLICY>(a, workspace, &parts, s);
+    return rc ? rc : launch_sum_partials(a.partial, parts, loss, s);
 }
 
 }  // extern "C"
