@@ -7,8 +7,7 @@
 //
 // The sum is kept as S = e_a + S', S' over the other candidates: 1 - p_a = S' / S and (where a is the maximum)
 // logp = -log1p(S') then keep their digits when the chosen candidate has nearly all the mass.
-// Row statistics are fp32; what is left per row (one logarithm, two exponentials) is done in 64 bits, because the ratio
-// and the KL term subtract numbers that are nearly equal.
+// Row statistics are fp32, the loss is summed over rows in 64 bits.
 #include "common.cuh"
 
 namespace kge {
@@ -47,51 +46,59 @@ __device__ __forceinline__ int cand_action(const CandArgs& a, long long row, int
     return -1;
 }
 
-// Loss term of one row and, in *g, d(loss) / d(logp); logp and kl are stored by the caller's thread.
-__device__ __forceinline__ double policy_term(const CandArgs& a, long long row, double logp, double* g, bool write) {
-    const double w = a.weight ? a.weight[row] : 1.0;
-    const double A = a.adv[row], ratio = exp(logp - static_cast<double>(a.old_logp[row]));
-    const double lo = 1.0 - static_cast<double>(a.clip_lo), hi = 1.0 + static_cast<double>(a.clip_hi);
-    const bool held = (A > 0.0 && ratio > hi) || (A < 0.0 && ratio < lo);
-    double l = -(held ? (A > 0.0 ? hi : lo) : ratio) * A, dl = held ? 0.0 : -ratio * A, kl = 0.0;
-    if (a.ref_logp) {
-        const double d = static_cast<double>(a.ref_logp[row]) - logp, e = expm1(d);
-        kl = e - d;
-        l += a.kl_coef * kl;
-        dl -= a.kl_coef * e;
-    }
-    if (write) { a.logp[row] = static_cast<float>(logp); a.kl[row] = static_cast<float>(kl); }
-    if (w == 0.0) { *g = 0.0; return 0.0; }
-    *g = w * a.scale * dl;
-    return w * a.scale * l;
+// The scalars of a row.  Differences of logarithms are subtracted in 64 bits; the functions themselves are fp32, because
+// 64-bit ones are a chain of some thousand cycles that a whole row waits for.  log S is one fp32 logarithm y plus the residual
+// S exp(-y) - 1 (exact product inside the fma, so what remains is the error of one expf: ~6e-8 absolute whatever log S is).
+__device__ __forceinline__ double cand_log_sum(double S) {
+    const float s = static_cast<float>(S), y = logf(s);
+    const float r = fmaf(s, expf(-y), -1.f) + static_cast<float>(S - static_cast<double>(s)) / s;
+    return static_cast<double>(y) + static_cast<double>(r);
+}
+// e^d - 1 - d: its power series near 0, where the three terms cancel (next term below 2^-24 of the sum for |d| <= 1)
+__device__ __forceinline__ float exp_minus_line(float d) {
+    if (fabsf(d) > 1.f) return expm1f(d) - d;
+    float t = 1.f / 479001600.f;
+    t = fmaf(t, d, 1.f / 39916800.f); t = fmaf(t, d, 1.f / 3628800.f); t = fmaf(t, d, 1.f / 362880.f); t = fmaf(t, d, 1.f / 40320.f);
+    t = fmaf(t, d, 1.f / 5040.f); t = fmaf(t, d, 1.f / 720.f); t = fmaf(t, d, 1.f / 120.f); t = fmaf(t, d, 1.f / 24.f);
+    t = fmaf(t, d, 1.f / 6.f); t = fmaf(t, d, 0.5f);
+    return d * d * t;
 }
 
 // What follows from a row's statistics: logp, kl, loss term (returned), and the factor ga of the gradient,
 // ds_j = ga (rest [j = a] - e_j [j != a]) with e_j = exp((s_j - m) / T).  One thread of a row calls it.
 template <int MODE>
 __device__ __forceinline__ double cand_finish(const CandArgs& a, long long row, int act, float sa, float m, float rest, bool write, float* ga) {
-    const double x = act >= 0 ? static_cast<double>(sa - m) * static_cast<double>(a.inv_temp) : 0.0;
+    const double x = act >= 0 ? (static_cast<double>(sa) - static_cast<double>(m)) * static_cast<double>(a.inv_temp) : 0.0;
     const bool live = act >= 0 && !(sa == -INFINITY && rest == 0.f);
-    const double ea = x == 0.0 ? 1.0 : exp(x);
-    const double S = ea + static_cast<double>(rest);
-    const double lp = !live ? 0.0 : x == 0.0 ? -log1p(static_cast<double>(rest)) : x - log(S);
-    const float inv = live ? static_cast<float>(1.0 / S) : 0.f;
+    const double S = static_cast<double>(expf(static_cast<float>(x))) + static_cast<double>(rest);
+    const double lp = !live ? 0.0 : x == 0.0 && rest < 0.5f ? -static_cast<double>(log1pf(rest)) : x - cand_log_sum(S);
+    const float inv = live ? 1.f / static_cast<float>(S) : 0.f;
     *ga = 0.f;
+    if (write) a.logp[row] = static_cast<float>(lp);
     if (MODE == CM_LOGP) {
-        if (write) {
-            a.logp[row] = static_cast<float>(lp);
-            a.stats[3 * row] = m; a.stats[3 * row + 1] = rest; a.stats[3 * row + 2] = inv;
-        }
+        if (write) { a.stats[3 * row] = m; a.stats[3 * row + 1] = rest; a.stats[3 * row + 2] = inv; }
         return 0.0;
     }
     if (!live) {
-        if (write) { a.logp[row] = 0.f; a.kl[row] = 0.f; }
+        if (write) a.kl[row] = 0.f;
         return 0.0;
     }
-    double g;
-    const double l = policy_term(a, row, lp, &g, write);
-    if (g != 0.0) *ga = static_cast<float>(g * a.inv_temp) * inv;         // (a row of weight 0 may hold NaN)
-    return l;
+    const float w = (a.weight ? a.weight[row] : 1.f) * a.scale, A = a.adv[row];
+    const float ratio = expf(static_cast<float>(lp - static_cast<double>(a.old_logp[row])));
+    const float lo = 1.f - a.clip_lo, hi = 1.f + a.clip_hi;
+    const bool held = (A > 0.f && ratio > hi) || (A < 0.f && ratio < lo);
+    float l = -(held ? (A > 0.f ? hi : lo) : ratio) * A, dl = held ? 0.f : -ratio * A, kl = 0.f;
+    if (a.ref_logp) {
+        const float d = static_cast<float>(static_cast<double>(a.ref_logp[row]) - lp);
+        kl = exp_minus_line(d);
+        l = fmaf(a.kl_coef, kl, l);
+        dl = fmaf(-a.kl_coef, kl + d, dl);               // e^d - 1 = kl + d
+    }
+    if (write) a.kl[row] = kl;
+    if (w == 0.f) return 0.0;                            // (a row of weight 0 may hold NaN)
+    const float g = w * dl * a.inv_temp;
+    if (g != 0.f) *ga = g * inv;
+    return static_cast<double>(w) * static_cast<double>(l);
 }
 
 // ---- 16-byte vectors of a row --------------------------------------------------------------------------------------
@@ -135,6 +142,11 @@ template <> struct Vec<__nv_bfloat16> {
         return make_uint4(w[0], w[1], w[2], w[3]);
     }
 };
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kFull, v, o));
+    return v;
+}
 __device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY ? 0.f : m; }
 template <typename T>
 __device__ __forceinline__ int head_of(const T* p, int n) {
@@ -170,8 +182,8 @@ cand_cached_kernel(CandArgs a) {
     constexpr bool kWarp32 = THREADS == 32;
     constexpr bool kKeepExp = sizeof(T) == 4;
     constexpr int kWarps = THREADS / 32;
-    __shared__ float2 parts[2][kWarp32 ? 1 : kWarps];
-    __shared__ float bcast[2];
+    __shared__ float2 parts[kWarp32 ? 1 : kWarps];
+    __shared__ float bcast;
     __shared__ double red[8];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int tid = kWarp32 ? lane : threadIdx.x;
@@ -180,18 +192,19 @@ cand_cached_kernel(CandArgs a) {
         asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
         asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(csize));
     }
-    const long long groups = kWarp32 ? (long long)gridDim.x * (blockDim.x >> 5) : gridDim.x / csize;
-    const long long first_row = kWarp32 ? (long long)blockIdx.x * (blockDim.x >> 5) + warp : blockIdx.x / csize;
+    const int cshift = 31 - __clz(static_cast<int>(csize));        // cluster sizes are powers of two
+    const long long groups = kWarp32 ? (long long)gridDim.x * 8 : 1;
+    const long long first_row = kWarp32 ? (long long)blockIdx.x * 8 + warp : blockIdx.x >> cshift;
+    const long long rows = kWarp32 ? a.rows : first_row + 1;        // a CTA or cluster has one row, a warp goes on
     const float c = a.inv_temp * 1.4426950408889634f;
     double total = 0.0;
-    int flip = 0;
-    for (long long row = first_row; row < a.rows; row += groups, flip ^= 1) {
+    for (long long row = first_row; row < rows; row += groups) {
         const T* s = static_cast<const T*>(a.scores) + row * a.ld;
         const int cnt = cand_count(a, row);
         const int act = cand_action(a, row, cnt, tid == 0 && rank == 0);
         const float sa = act >= 0 ? cand_get(s + act) : 0.f;
         const int head = head_of(s, a.n), nv = (a.n - head) / V;
-        const int share = (nv + static_cast<int>(csize) - 1) / static_cast<int>(csize);       // this CTA's vectors: [v0, v1)
+        const int share = (nv + static_cast<int>(csize) - 1) >> cshift;       // this CTA's vectors: [v0, v1)
         const int v0 = static_cast<int>(rank) * share, v1 = min(nv, v0 + share);
         // the extra element of this thread, if any
         int xi = -1;
@@ -218,8 +231,7 @@ cand_cached_kernel(CandArgs a) {
         float mw = xe;
 #pragma unroll
         for (int i = 0; i < I; ++i) mw = fmaxf(mw, Vec<T>::max(r[i]));
-#pragma unroll
-        for (int o = 16; o; o >>= 1) mw = fmaxf(mw, __shfl_xor_sync(kFull, mw, o));
+        mw = warp_max(mw);
         const float mz = finite_or_zero(mw);
         // the vector (register index) of this thread that holds the chosen candidate
         int own = -1;
@@ -250,12 +262,16 @@ cand_cached_kernel(CandArgs a) {
             rest += t;
         }
         rest = warp_sum(rest);
+        if (!kKeepExp) {          // keep the packed words, not their unpacked values, in registers until the gradient
+#pragma unroll
+            for (int i = 0; i < I; ++i) asm volatile("" : "+r"(r[i].x), "+r"(r[i].y), "+r"(r[i].z), "+r"(r[i].w));
+        }
         float m = mw, ga = 0.f;
         if (kWarp32) {
             if (lane == 0) total += cand_finish<MODE>(a, row, act, sa, finite_or_zero(m), rest, true, &ga);
             if (MODE != CM_LOGP) ga = __shfl_sync(kFull, ga, 0);
         } else {
-            if (lane == 0) parts[flip][warp] = make_float2(mw, rest);
+            if (lane == 0) parts[warp] = make_float2(mw, rest);
             if (csize == 1) {
                 __syncthreads();
             } else {
@@ -263,30 +279,33 @@ cand_cached_kernel(CandArgs a) {
             }
             // every warp merges all parts of the row, in the same order
             m = -INFINITY; rest = 0.f;
-            const int n_parts = kWarps * static_cast<int>(csize);
-            for (int j = lane; j < n_parts; j += 32) {
-                float2 q;
-                const uint32_t addr = static_cast<uint32_t>(__cvta_generic_to_shared(&parts[flip][j % kWarps]));
-                uint32_t remote;
-                asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(static_cast<uint32_t>(j / kWarps)));
-                asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(q.x), "=f"(q.y) : "r"(remote) : "memory");
-                merge_parts(m, rest, q.x, q.y, c);
+            if (csize == 1) {
+                if (lane < kWarps) { m = parts[lane].x; rest = parts[lane].y; }
+            } else {
+                for (int j = lane; j < kWarps * static_cast<int>(csize); j += 32) {
+                    float2 q;
+                    const uint32_t addr = static_cast<uint32_t>(__cvta_generic_to_shared(&parts[j % kWarps]));
+                    uint32_t remote;
+                    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(static_cast<uint32_t>(j / kWarps)));
+                    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(q.x), "=f"(q.y) : "r"(remote) : "memory");
+                    merge_parts(m, rest, q.x, q.y, c);
+                }
+                // the parts have been read: no CTA of the cluster leaves before the others have got here
+                asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
             }
-#pragma unroll
-            for (int o = 16; o; o >>= 1) {
-                const float m2 = __shfl_xor_sync(kFull, m, o), r2 = __shfl_xor_sync(kFull, rest, o);
-                merge_parts(m, rest, m2, r2, c);
-            }
+            const float mine = m;
+            m = warp_max(m);
+            rest = warp_sum(rest * cand_ex2((mine - finite_or_zero(m)) * c));
             if (MODE == CM_LOGP) {
                 if (threadIdx.x == 0 && rank == 0) cand_finish<MODE>(a, row, act, sa, finite_or_zero(m), rest, true, &ga);
             } else {
                 if (threadIdx.x == 0) {
                     const double l = cand_finish<MODE>(a, row, act, sa, finite_or_zero(m), rest, rank == 0, &ga);
                     if (rank == 0) total += l;
-                    bcast[flip] = ga;
+                    bcast = ga;
                 }
                 __syncthreads();
-                ga = bcast[flip];
+                ga = bcast;
             }
         }
         if (MODE != CM_LOGP) {
@@ -328,8 +347,7 @@ cand_cached_kernel(CandArgs a) {
             }
         }
     }
-    if (!kWarp32 && csize > 1)            // no CTA leaves while another may still read its parts
-        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (!kWarp32 && csize > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     if (MODE == CM_POLICY) {
         if (kWarp32) {
             if (lane == 0) red[warp] = total;
@@ -339,7 +357,7 @@ cand_cached_kernel(CandArgs a) {
                 a.partial[blockIdx.x] = total;
             }
         } else if (threadIdx.x == 0 && rank == 0) {
-            a.partial[blockIdx.x / csize] = total;
+            a.partial[blockIdx.x >> cshift] = total;
         }
     }
 }
@@ -511,26 +529,30 @@ __global__ void __launch_bounds__(256) cand_grad_kernel(CandArgs a, const float*
     }
 }
 
-__global__ void __launch_bounds__(256) sum_partials_kernel(const double* partial, int n, float* out) {
-    __shared__ double red[256];
+__global__ void __launch_bounds__(1024) sum_partials_kernel(const double* partial, int n, float* out) {
+    __shared__ double red[32];
     double v = 0.0;
-    for (int i = threadIdx.x; i < n; i += 256) v += partial[i];
-    red[threadIdx.x] = v;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < n; i += 1024) v += partial[i];
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
     __syncthreads();
-    for (int o = 128; o; o >>= 1) {
-        if (threadIdx.x < o) red[threadIdx.x] += red[threadIdx.x + o];
-        __syncthreads();
+    if (threadIdx.x < 32) {
+        v = red[threadIdx.x];
+#pragma unroll
+        for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+        if (threadIdx.x == 0) *out = static_cast<float>(v);
     }
-    if (threadIdx.x == 0) *out = static_cast<float>(red[0]);
 }
 
 int launch_sum_partials(const double* partial, int n, float* out, cudaStream_t s) {
-    sum_partials_kernel<<<1, 256, 0, s>>>(partial, n, out);
+    sum_partials_kernel<<<1, 1024, 0, s>>>(partial, n, out);
     KGE_LAUNCH_CHECK("sum_partials_kernel");
     return 0;
 }
 
-constexpr int kCandMaxBlocks = 148 * 8;            // CTAs that leave a partial sum of the loss
+constexpr int kCandMaxBlocks = 148 * 8;            // CTAs that leave a partial sum of the loss, where they take rows in turn
 
 // Workspace: partial sums of the loss, then per-chunk (m, rest) and per-row coefficients of the multi-pass form.
 struct CandLayout { int chunk, chunks; size_t off_parts, off_coef, total; };
@@ -543,7 +565,7 @@ static CandLayout cand_layout(long long rows, long long n) {
     L.chunk = static_cast<int>(per);
     L.chunks = static_cast<int>((n + per - 1) / per);
     if (L.chunks < 1) L.chunks = 1;
-    L.off_parts = kCandMaxBlocks * sizeof(double);
+    L.off_parts = sizeof(double) * static_cast<size_t>(rows > kCandMaxBlocks ? rows : kCandMaxBlocks);
     L.off_coef = L.off_parts + sizeof(float2) * static_cast<size_t>(rows) * L.chunks;
     L.total = L.off_coef + 3 * sizeof(float) * static_cast<size_t>(rows);
     return L;
@@ -551,10 +573,9 @@ static CandLayout cand_layout(long long rows, long long n) {
 
 template <typename T, int THREADS, int I, int MODE>
 static int cand_cached(const CandArgs& a, int cluster, int* n_partial, cudaStream_t s) {
-    const int wpb = THREADS == 32 ? 8 : 1;
-    const long long want = THREADS == 32 ? (a.rows + wpb - 1) / wpb : a.rows;
-    const long long cap = THREADS == 32 ? kCandMaxBlocks : 148 * (1024 / THREADS) / cluster;
-    const long long groups = want < cap ? want : cap;
+    // warps take rows in turn; a CTA or cluster has one row, so that its loads start while others write
+    const long long want = THREADS == 32 ? (a.rows + 7) / 8 : a.rows;
+    const long long groups = THREADS == 32 && want > kCandMaxBlocks ? kCandMaxBlocks : want;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(groups * cluster));
     cfg.blockDim = dim3(THREADS == 32 ? 256 : THREADS);
@@ -612,11 +633,12 @@ static int cand_go(const CandArgs& a, void* ws, int* n_partial, cudaStream_t s) 
     if (nv <= 64) return cand_cached<T, 32, 2, MODE>(a, 1, n_partial, s);
     if (nv <= 128) return cand_cached<T, 32, 4, MODE>(a, 1, n_partial, s);
     if (nv <= 256) return cand_cached<T, 32, 8, MODE>(a, 1, n_partial, s);
+    if (a.rows >= (1LL << 31)) return cand_passes<T, MODE>(a, ws, n_partial, s);      // (beyond a grid of one CTA a row)
     if (nv <= 128 * 8) return cand_cached<T, 128, 8, MODE>(a, 1, n_partial, s);
     if (nv <= 256 * 8) return cand_cached<T, 256, 8, MODE>(a, 1, n_partial, s);
     int cluster = 1;
     while (cluster <= kMaxCluster && nv > cluster * 512LL * 8) cluster *= 2;
-    if (cluster > kMaxCluster || a.rows * cluster < 32) return cand_passes<T, MODE>(a, ws, n_partial, s);
+    if (cluster > kMaxCluster || a.rows * cluster < 32 || a.rows >= (1LL << 31) / kMaxCluster) return cand_passes<T, MODE>(a, ws, n_partial, s);
     return cand_cached<T, 512, 8, MODE>(a, cluster, n_partial, s);
 }
 

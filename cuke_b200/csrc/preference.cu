@@ -24,67 +24,199 @@ struct PrefArgs {
 };
 enum { PREF_LOGISTIC = 0, PREF_SQUARE = 1 };
 
+__device__ __forceinline__ float pref_ex2(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
+__device__ __forceinline__ float pref_rcp(float x) { float r; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
+
+// Loss and slope of one pair.  With t = exp(-|z|): sigmoid(|z|) = 1 / (1 + t), sigmoid(-|z|) = t / (1 + t), and
+// softplus(-|z|) = log1p(t) = 2 atanh(w), w = t / (2 + t) in [0, 1/3]: atanh(w) / w as a polynomial in w^2 (Chebyshev
+// interpolation of degree 4 on [0, 1/9], 4e-9 relative), so small terms keep their digits at the cost of one reciprocal and six
+// fused multiply-adds: the loss is bound by memory only if a pair stays below some 40 instructions.
+template <bool SQUARE>
 __device__ __forceinline__ void pref_pair(const PrefArgs& a, float z, float& l, float& d) {
-    if (a.kind == PREF_SQUARE) { l = z * z; d = 2.f * z; return; }
-    const float t = __expf(-fabsf(z)), inv = __frcp_rn(1.f + t);
-    const float up = z >= 0.f ? inv : t * inv, down = z >= 0.f ? t * inv : inv;      // sigmoid(z), sigmoid(-z)
+    if (SQUARE) { l = z * z; d = 2.f * z; return; }
+    const float t = pref_ex2(fabsf(z) * -1.4426950408889634f);
+    const float inv = pref_rcp(1.f + t), w = t * pref_rcp(2.f + t), x = w * w;
+    const float q = fmaf(fmaf(fmaf(fmaf(0.14078890f, x, 0.13982579f), x, 0.20012298f), x, 0.33333161f), x, 1.f);
+    const float small = t * inv, down = z >= 0.f ? small : inv;                      // sigmoid(-z)
     const float keep = 1.f - a.smooth;
-    l = log1pf(t) + keep * fmaxf(-z, 0.f);
+    l = fmaf(w + w, q, keep * fmaxf(-z, 0.f));
     d = -keep * down;
-    if (a.smooth > 0.f) { l += a.smooth * fmaxf(z, 0.f); d += a.smooth * up; }        // (0 x inf without the test)
+    if (a.smooth > 0.f) {                                                            // (0 x inf without the test)
+        l = fmaf(a.smooth, fmaxf(z, 0.f), l);
+        d = fmaf(a.smooth, z >= 0.f ? inv : small, d);
+    }
 }
 
-// One warp per row.
-__global__ void __launch_bounds__(256) pref_kernel(PrefArgs a) {
-    __shared__ double red[8];
+__device__ __forceinline__ int nonzero_bytes(uint32_t w) { return __popc(__vcmpne4(w, 0u)) >> 3; }
+
+template <int G>
+__device__ __forceinline__ float pref_group_sum(float v) {
+#pragma unroll
+    for (int o = (G < 32 ? G : 32) / 2; o; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+    return v;
+}
+template <int G>
+__device__ __forceinline__ int pref_group_sum(int v) {
+#pragma unroll
+    for (int o = (G < 32 ? G : 32) / 2; o; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+    return v;
+}
+
+// A group of G threads per row: one thread for a handful of negatives, a quarter warp, a warp, or a whole CTA.  VEC: four
+// negatives per access (all rows of neg, ref_neg, dneg on 16-byte and of mask on 4-byte boundaries).  The valid negatives of
+// a row are counted first - the mask is a thirteenth of the traffic and comes from L1 the second time - so that the main pass
+// writes final gradients; it requests U accesses of each array before it uses the first.  Without VEC a thread has the same four
+// negatives, read one by one: the order of the additions, and so every bit of the result, does not depend on alignment.
+template <int G, bool VEC, bool SQUARE>
+__global__ void __launch_bounds__(G > 256 ? G : 256) pref_kernel(PrefArgs a) {
+    constexpr int BLOCK = G > 256 ? G : 256;
+    constexpr int W = 4;                           // consecutive negatives of a thread
+    constexpr int U = G == 1 ? 1 : 2;
+    __shared__ double red[32];
+    __shared__ float rl[32], rd[32];
+    __shared__ int rc[32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int gl = threadIdx.x % G;
     double total = 0.0;
-    for (long long row = (long long)blockIdx.x * 8 + warp; row < a.rows; row += (long long)gridDim.x * 8) {
-        const float* neg = a.neg + row * a.ldn;
-        const float* rneg = a.rneg ? a.rneg + row * a.ldr : nullptr;
-        const unsigned char* mask = a.mask ? a.mask + row * a.ldm : nullptr;
-        int cnt = a.n;
+    const long long step = (long long)gridDim.x * (BLOCK / G);
+    // every lane of a warp makes the same number of turns: the shuffles below need all of them
+    const long long first = (long long)blockIdx.x * (BLOCK / G) + (G > 32 ? 0 : warp * (32 / G));
+    for (long long base_row = first; base_row < a.rows; base_row += step) {
+        const long long row = base_row + (G < 32 ? lane / G : 0);
+        const bool live = row < a.rows;
+        const long long rr = live ? row : a.rows - 1;
+        const int n = live ? a.n : 0;
+        const float* neg = a.neg + rr * a.ldn;
+        const float* rneg = a.rneg ? a.rneg + rr * a.ldr : nullptr;
+        const unsigned char* mask = a.mask ? a.mask + rr * a.ldm : nullptr;
+        float* dneg = a.dneg + rr * a.ldd;
+        int cnt = n;
         if (mask) {
             cnt = 0;
-            for (int j = lane; j < a.n; j += 32) cnt += mask[j] != 0;
-            cnt = __reduce_add_sync(kFull, cnt);
-        }
-        const float base = a.pos[row] - (a.rpos ? a.rpos[row] : 0.f);
-        const float w = a.weight ? a.weight[row] : 1.f;
-        const float cw = cnt > 0 ? a.scale * w / static_cast<float>(cnt) : 0.f;
-        float ls = 0.f, ds = 0.f;
-        for (int j = lane; j < a.n; j += 32) {
-            float l = 0.f, d = 0.f;
-            if (!mask || mask[j]) {
-                const float h = base - (neg[j] - (rneg ? rneg[j] : 0.f));
-                pref_pair(a, a.beta * h - a.margin, l, d);
-                d *= a.beta;
-                ls += l; ds += d;
+            for (int j = gl * W; j < n; j += G * W) {
+                if (VEC) {
+                    cnt += nonzero_bytes(*reinterpret_cast<const uint32_t*>(mask + j));
+                } else {
+#pragma unroll
+                    for (int k = 0; k < W; ++k) cnt += j + k < n && mask[j + k] != 0;
+                }
             }
-            a.dneg[row * a.ldd + j] = cw != 0.f ? -cw * d : 0.f;
+            cnt = pref_group_sum<G>(cnt);
+            if (G > 32) {
+                if (lane == 0) rc[warp] = cnt;
+                __syncthreads();
+                cnt = 0;
+                for (int w = 0; w < G / 32; ++w) cnt += rc[w];
+            }
         }
-        ls = warp_sum(ls); ds = warp_sum(ds);
-        if (lane == 0) {
-            a.dpos[row] = cw != 0.f ? cw * ds : 0.f;
+        const float base = a.pos[rr] - (a.rpos ? a.rpos[rr] : 0.f);
+        const float weight = a.weight ? a.weight[rr] : 1.f;
+        const float cw = cnt > 0 ? a.scale * weight / static_cast<float>(cnt) : 0.f;
+        const float dscale = -cw * a.beta;
+        float ls = 0.f, ds = 0.f;
+        for (int j0 = gl * W; j0 < n; j0 += G * W * U) {
+            float x[U][W], y[U][W];
+            uint32_t m[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int j = j0 + u * G * W;
+                m[u] = 0;
+                if (j < n) {
+                    if (VEC) {
+                        const float4 f = __ldcs(reinterpret_cast<const float4*>(neg + j));
+                        float4 g = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (rneg) g = __ldcs(reinterpret_cast<const float4*>(rneg + j));
+                        m[u] = mask ? __vcmpne4(*reinterpret_cast<const uint32_t*>(mask + j), 0u) : 0xFFFFFFFFu;
+                        x[u][0] = f.x; x[u][1] = f.y; x[u][2] = f.z; x[u][3] = f.w;
+                        y[u][0] = g.x; y[u][1] = g.y; y[u][2] = g.z; y[u][3] = g.w;
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < W; ++k) {
+                            x[u][k] = y[u][k] = 0.f;
+                            if (j + k < n) {
+                                x[u][k] = neg[j + k];
+                                if (rneg) y[u][k] = rneg[j + k];
+                                if (!mask || mask[j + k]) m[u] |= 0xFFu << (8 * k);
+                            }
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int j = j0 + u * G * W;
+                if (j < n) {
+                    float o[W];
+#pragma unroll
+                    for (int k = 0; k < W; ++k) {
+                        float l, d;
+                        pref_pair<SQUARE>(a, fmaf(a.beta, base - (x[u][k] - y[u][k]), -a.margin), l, d);
+                        const bool on = (m[u] >> (8 * k)) & 1u;
+                        ls += on ? l : 0.f;
+                        ds += on ? d : 0.f;
+                        o[k] = on && cw != 0.f ? dscale * d : 0.f;
+                    }
+                    if (VEC) {
+                        __stcs(reinterpret_cast<float4*>(dneg + j), make_float4(o[0], o[1], o[2], o[3]));
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < W; ++k) if (j + k < n) dneg[j + k] = o[k];
+                    }
+                }
+            }
+        }
+        ls = pref_group_sum<G>(ls); ds = pref_group_sum<G>(ds);
+        if (G > 32) {
+            if (lane == 0) { rl[warp] = ls; rd[warp] = ds; }
+            __syncthreads();
+            if (threadIdx.x == 0)
+                for (int w = 1; w < G / 32; ++w) { ls += rl[w]; ds += rd[w]; }
+        }
+        if (gl == 0 && live) {
+            a.dpos[row] = cw != 0.f ? -dscale * ds : 0.f;
             if (cw != 0.f) total += static_cast<double>(cw) * ls;
         }
+        if (G > 32) __syncthreads();               // rc, rl, rd are free for the next row
     }
-    if (lane == 0) red[warp] = total;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int i = 1; i < 8; ++i) total += red[i];
-        a.partial[blockIdx.x] = total;
+    if (G > 32) {
+        if (threadIdx.x == 0) a.partial[blockIdx.x] = total;
+    } else {
+#pragma unroll
+        for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(kFull, total, o);
+        if (lane == 0) red[warp] = total;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            for (int w = 1; w < 8; ++w) total += red[w];
+            a.partial[blockIdx.x] = total;
+        }
     }
 }
 
 constexpr int kPrefMaxBlocks = 148 * 8;
 
-static int launch_preference(const PrefArgs& a, float* loss, cudaStream_t s) {
-    const long long want = (a.rows + 7) / 8;
+template <int G, bool VEC, bool SQUARE>
+static int pref_go(const PrefArgs& a, float* loss, cudaStream_t s) {
+    constexpr int per = G > 256 ? 1 : 256 / G;
+    const long long want = (a.rows + per - 1) / per;
     const unsigned blocks = static_cast<unsigned>(want < kPrefMaxBlocks ? want : kPrefMaxBlocks);
-    pref_kernel<<<blocks, 256, 0, s>>>(a);
+    pref_kernel<G, VEC, SQUARE><<<blocks, G > 256 ? G : 256, 0, s>>>(a);
     KGE_LAUNCH_CHECK("pref_kernel");
     return launch_sum_partials(a.partial, static_cast<int>(blocks), loss, s);
+}
+template <bool VEC, bool SQUARE>
+static int pref_pick(const PrefArgs& a, float* loss, cudaStream_t s) {
+    if (a.n <= 4) return pref_go<1, false, SQUARE>(a, loss, s);
+    if (a.n <= 64) return pref_go<8, VEC, SQUARE>(a, loss, s);
+    // a CTA per row where a warp per row would leave SMs without work
+    if (a.n > 2048 && a.rows < 148 * 16) return pref_go<1024, VEC, SQUARE>(a, loss, s);
+    return pref_go<32, VEC, SQUARE>(a, loss, s);
+}
+
+static int launch_preference(const PrefArgs& a, float* loss, cudaStream_t s) {
+    const bool vec = a.n % 4 == 0 && aligned16(a.neg) && aligned16(a.dneg) && aligned16(a.rneg) && (reinterpret_cast<uintptr_t>(a.mask) & 3) == 0 &&
+                     (a.rows == 1 || ((a.ldn | a.ldd | (a.rneg ? a.ldr : 0) | (a.mask ? a.ldm : 0)) & 3) == 0);
+    if (a.kind == PREF_SQUARE) return vec ? pref_pick<true, true>(a, loss, s) : pref_pick<false, true>(a, loss, s);
+    return vec ? pref_pick<true, false>(a, loss, s) : pref_pick<false, false>(a, loss, s);
 }
 
 }  // namespace kge
