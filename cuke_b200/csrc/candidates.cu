@@ -66,8 +66,14 @@ __device__ __forceinline__ float exp_minus_line(float d) {
 
 // What follows from a row's statistics: logp, kl, loss term (returned), and the factor ga of the gradient,
 // ds_j = ga (rest [j = a] - e_j [j != a]) with e_j = exp((s_j - m) / T).  One thread of a row calls it.
+struct RowSide { float w, adv, old, ref; };            // a row's operands of the policy loss
+__device__ __forceinline__ float cand_side(const CandArgs& a, long long row, int which) {
+    const float* p = which == 0 ? a.weight : which == 1 ? a.adv : which == 2 ? a.old_logp : a.ref_logp;
+    return p ? __ldg(p + row) : which == 0 ? 1.f : 0.f;
+}
 template <int MODE>
-__device__ __forceinline__ double cand_finish(const CandArgs& a, long long row, int act, float sa, float m, float rest, bool write, float* ga) {
+__device__ __forceinline__ double cand_finish(const CandArgs& a, long long row, int act, float sa, float m, float rest, bool write,
+                                              const RowSide& o, float* ga) {
     const double x = act >= 0 ? (static_cast<double>(sa) - static_cast<double>(m)) * static_cast<double>(a.inv_temp) : 0.0;
     const bool live = act >= 0 && !(sa == -INFINITY && rest == 0.f);
     const double S = static_cast<double>(expf(static_cast<float>(x))) + static_cast<double>(rest);
@@ -83,13 +89,13 @@ __device__ __forceinline__ double cand_finish(const CandArgs& a, long long row, 
         if (write) a.kl[row] = 0.f;
         return 0.0;
     }
-    const float w = (a.weight ? a.weight[row] : 1.f) * a.scale, A = a.adv[row];
-    const float ratio = expf(static_cast<float>(lp - static_cast<double>(a.old_logp[row])));
+    const float w = o.w * a.scale, A = o.adv;
+    const float ratio = expf(static_cast<float>(lp - static_cast<double>(o.old)));
     const float lo = 1.f - a.clip_lo, hi = 1.f + a.clip_hi;
     const bool held = (A > 0.f && ratio > hi) || (A < 0.f && ratio < lo);
     float l = -(held ? (A > 0.f ? hi : lo) : ratio) * A, dl = held ? 0.f : -ratio * A, kl = 0.f;
     if (a.ref_logp) {
-        const float d = static_cast<float>(static_cast<double>(a.ref_logp[row]) - lp);
+        const float d = static_cast<float>(static_cast<double>(o.ref) - lp);
         kl = exp_minus_line(d);
         l = fmaf(a.kl_coef, kl, l);
         dl = fmaf(-a.kl_coef, kl + d, dl);               // e^d - 1 = kl + d
@@ -176,14 +182,14 @@ __device__ __forceinline__ void merge_parts(float& m, float& rest, float m2, flo
 // the gradient costs one multiplication each; bf16 scores stay packed and are exponentiated a second time.
 constexpr int kMaxCluster = 8;
 template <typename T, int THREADS, int I, int MODE>
-__global__ void __launch_bounds__(THREADS == 32 ? 256 : THREADS, THREADS == 32 ? (I == 8 ? 3 : 4) : 1024 / THREADS)
+__global__ void __launch_bounds__(THREADS == 32 ? 256 : THREADS, THREADS == 32 ? 4 : (I == 8 ? 1024 : 1280) / THREADS)
 cand_cached_kernel(CandArgs a) {
     constexpr int V = Vec<T>::V;
     constexpr bool kWarp32 = THREADS == 32;
     constexpr bool kKeepExp = sizeof(T) == 4;
     constexpr int kWarps = THREADS / 32;
     __shared__ float2 parts[kWarp32 ? 1 : kWarps];
-    __shared__ float bcast;
+    __shared__ float bcast, sides[4];
     __shared__ double red[8];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int tid = kWarp32 ? lane : threadIdx.x;
@@ -203,9 +209,12 @@ cand_cached_kernel(CandArgs a) {
         const int cnt = cand_count(a, row);
         const int act = cand_action(a, row, cnt, tid == 0 && rank == 0);
         const float sa = act >= 0 ? cand_get(s + act) : 0.f;
+        float side = 0.f;                 // thread k < 4 requests operand k now: the finish of the row must not wait for memory
+        if (MODE == CM_POLICY && tid < 4) side = cand_side(a, row, tid);
         const int head = head_of(s, a.n), nv = (a.n - head) / V;
         const int share = (nv + static_cast<int>(csize) - 1) >> cshift;       // this CTA's vectors: [v0, v1)
         const int v0 = static_cast<int>(rank) * share, v1 = min(nv, v0 + share);
+        const int used = (v1 - v0 + THREADS - 1) / THREADS;      // registers of a thread that hold anything (the same for all)
         // the extra element of this thread, if any
         int xi = -1;
         if (rank == 0 && tid < 16) {
@@ -230,7 +239,7 @@ cand_cached_kernel(CandArgs a) {
         }
         float mw = xe;
 #pragma unroll
-        for (int i = 0; i < I; ++i) mw = fmaxf(mw, Vec<T>::max(r[i]));
+        for (int i = 0; i < I; ++i) if (i < used) mw = fmaxf(mw, Vec<T>::max(r[i]));
         mw = warp_max(mw);
         const float mz = finite_or_zero(mw);
         // the vector (register index) of this thread that holds the chosen candidate
@@ -247,6 +256,7 @@ cand_cached_kernel(CandArgs a) {
         }
 #pragma unroll
         for (int i = 0; i < I; ++i) {
+            if (i >= used) continue;
             float f[V];
             Vec<T>::open(r[i], f);
 #pragma unroll
@@ -268,10 +278,16 @@ cand_cached_kernel(CandArgs a) {
         }
         float m = mw, ga = 0.f;
         if (kWarp32) {
-            if (lane == 0) total += cand_finish<MODE>(a, row, act, sa, finite_or_zero(m), rest, true, &ga);
+            RowSide o = {};
+            if (MODE == CM_POLICY) {
+                o.w = __shfl_sync(kFull, side, 0); o.adv = __shfl_sync(kFull, side, 1);
+                o.old = __shfl_sync(kFull, side, 2); o.ref = __shfl_sync(kFull, side, 3);
+            }
+            if (lane == 0) total += cand_finish<MODE>(a, row, act, sa, finite_or_zero(m), rest, true, o, &ga);
             if (MODE != CM_LOGP) ga = __shfl_sync(kFull, ga, 0);
         } else {
             if (lane == 0) parts[warp] = make_float2(mw, rest);
+            if (MODE == CM_POLICY && tid < 4) sides[tid] = side;
             if (csize == 1) {
                 __syncthreads();
             } else {
@@ -297,10 +313,10 @@ cand_cached_kernel(CandArgs a) {
             m = warp_max(m);
             rest = warp_sum(rest * cand_ex2((mine - finite_or_zero(m)) * c));
             if (MODE == CM_LOGP) {
-                if (threadIdx.x == 0 && rank == 0) cand_finish<MODE>(a, row, act, sa, finite_or_zero(m), rest, true, &ga);
+                if (threadIdx.x == 0 && rank == 0) cand_finish<MODE>(a, row, act, sa, finite_or_zero(m), rest, true, RowSide{}, &ga);
             } else {
                 if (threadIdx.x == 0) {
-                    const double l = cand_finish<MODE>(a, row, act, sa, finite_or_zero(m), rest, rank == 0, &ga);
+                    const double l = cand_finish<MODE>(a, row, act, sa, finite_or_zero(m), rest, rank == 0, RowSide{sides[0], sides[1], sides[2], sides[3]}, &ga);
                     if (rank == 0) total += l;
                     bcast = ga;
                 }
@@ -452,7 +468,9 @@ __global__ void __launch_bounds__(256) cand_join_kernel(CandArgs a, const float2
             const int act = cand_action(a, row, cand_count(a, row), false);
             const float sa = act >= 0 ? cand_get(static_cast<const T*>(a.scores) + row * a.ld + act) : 0.f;
             float ga;
-            total += cand_finish<MODE>(a, row, act, sa, finite_or_zero(m), rest, true, &ga);
+            RowSide o = {};
+            if (MODE == CM_POLICY) o = RowSide{cand_side(a, row, 0), cand_side(a, row, 1), cand_side(a, row, 2), cand_side(a, row, 3)};
+            total += cand_finish<MODE>(a, row, act, sa, finite_or_zero(m), rest, true, o, &ga);
             if (MODE == CM_POLICY) { coef[3 * row] = finite_or_zero(m); coef[3 * row + 1] = rest; coef[3 * row + 2] = ga; }
         }
     }
@@ -595,7 +613,7 @@ template <typename T>
 static int cand_gradient(const CandArgs& a, const float* coef, bool aligned, cudaStream_t s) {
     const int per = 128 * (aligned ? Vec<T>::V : 1);
     const long long pieces = a.n > 0 ? (a.n + per - 1) / per : 1, want = (a.rows * pieces + 7) / 8;
-    const unsigned blocks = static_cast<unsigned>(want < 148 * 64 ? want : 148 * 64);
+    const unsigned blocks = static_cast<unsigned>(want < (1 << 30) ? want : (1 << 30));       // (short CTAs copy faster than a loop)
     if (aligned) cand_grad_kernel<T, true><<<blocks, 256, 0, s>>>(a, coef, pieces);
     else cand_grad_kernel<T, false><<<blocks, 256, 0, s>>>(a, coef, pieces);
     KGE_LAUNCH_CHECK("cand_grad_kernel");
@@ -632,10 +650,11 @@ static int cand_go(const CandArgs& a, void* ws, int* n_partial, cudaStream_t s) 
     if (nv <= 32) return cand_cached<T, 32, 1, MODE>(a, 1, n_partial, s);
     if (nv <= 64) return cand_cached<T, 32, 2, MODE>(a, 1, n_partial, s);
     if (nv <= 128) return cand_cached<T, 32, 4, MODE>(a, 1, n_partial, s);
-    if (nv <= 256) return cand_cached<T, 32, 8, MODE>(a, 1, n_partial, s);
     if (a.rows >= (1LL << 31)) return cand_passes<T, MODE>(a, ws, n_partial, s);      // (beyond a grid of one CTA a row)
-    if (nv <= 128 * 8) return cand_cached<T, 128, 8, MODE>(a, 1, n_partial, s);
-    if (nv <= 256 * 8) return cand_cached<T, 256, 8, MODE>(a, 1, n_partial, s);
+    if (nv <= 64 * 4) return cand_cached<T, 64, 4, MODE>(a, 1, n_partial, s);
+    if (nv <= 128 * 4) return cand_cached<T, 128, 4, MODE>(a, 1, n_partial, s);
+    if (nv <= 256 * 4) return cand_cached<T, 256, 4, MODE>(a, 1, n_partial, s);
+    if (nv <= 512 * 4) return cand_cached<T, 512, 4, MODE>(a, 1, n_partial, s);
     int cluster = 1;
     while (cluster <= kMaxCluster && nv > cluster * 512LL * 8) cluster *= 2;
     if (cluster > kMaxCluster || a.rows * cluster < 32 || a.rows >= (1LL << 31) / kMaxCluster) return cand_passes<T, MODE>(a, ws, n_partial, s);

@@ -83,20 +83,23 @@ template <> struct DropVec<__nv_bfloat16> {
     }
 };
 
+// Each CTA has 256 x kDropU adjacent vectors and ends: a plain copy in this form runs at 6.6 TB/s, at 5.7 TB/s as a loop of
+// eight resident CTAs per SM and at 6.4 TB/s with the vectors of a thread a grid apart.
+constexpr int kDropU = 2;
 template <typename T, bool PACKED>
 __global__ void __launch_bounds__(256) dropout_vec_kernel(DropoutArgs a, RoundKeys keys, long long vectors, int per_row) {
-    constexpr int V = DropVec<T>::V, U = 4;
+    constexpr int V = DropVec<T>::V, U = kDropU;
     const uint32_t step = 0x80000000u | (a.step_dev ? static_cast<uint32_t>(*a.step_dev) + a.step : a.step);
-    const long long stride = (long long)gridDim.x * 256;
     const uint4* x = static_cast<const uint4*>(a.x);
     const uint4* res = static_cast<const uint4*>(a.res);
     uint4* out = static_cast<uint4*>(a.out);
-    for (long long v0 = (long long)blockIdx.x * 256 + threadIdx.x; v0 < vectors; v0 += stride * U) {
+    {
+        const long long v0 = (long long)blockIdx.x * (256 * U) + threadIdx.x;
         uint4 r[U], q[U];
         long long ox[U], orr[U], oo[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const long long v = v0 + u * stride;
+            const long long v = v0 + u * 256;
             if (v >= vectors) break;
             if (PACKED) {
                 ox[u] = orr[u] = oo[u] = v;
@@ -111,7 +114,7 @@ __global__ void __launch_bounds__(256) dropout_vec_kernel(DropoutArgs a, RoundKe
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const long long v = v0 + u * stride;
+            const long long v = v0 + u * 256;
             if (v >= vectors) break;
             float f[V], g[V];
             DropVec<T>::open(r[u], f);
@@ -161,8 +164,9 @@ static int drop_go(const DropoutArgs& a, cudaStream_t s) {
     RoundKeys keys;
     uint32_t k0 = a.k0, k1 = a.k1;
     for (int i = 0; i < 10; ++i, k0 += 0x9E3779B9u, k1 += 0xBB67AE85u) { keys.a[i] = k0; keys.b[i] = k1; }
-    const long long vectors = a.rows * a.dim / DropVec<T>::V, want = (vectors + 255) / 256;
-    const unsigned blocks = static_cast<unsigned>(want < 148 * 64 ? want : 148 * 64);
+    const long long vectors = a.rows * a.dim / DropVec<T>::V, want = (vectors + 256 * kDropU - 1) / (256 * kDropU);
+    if (want >= (1LL << 31)) { set_error("kge_dropout: more than 2^40 vectors"); return KGE_E_RANGE; }
+    const unsigned blocks = static_cast<unsigned>(want);
     const int per_row = a.dim / DropVec<T>::V;
     if (packed) dropout_vec_kernel<T, true><<<blocks, 256, 0, s>>>(a, keys, vectors, per_row);
     else dropout_vec_kernel<T, false><<<blocks, 256, 0, s>>>(a, keys, vectors, per_row);
