@@ -8,7 +8,8 @@
 // The sum is kept as S = e_a + S', S' over the other candidates: 1 - p_a = S' / S and (where a is the maximum)
 // logp = -log1p(S') then keep their digits when the chosen candidate has nearly all the mass.
 // Row statistics are fp32, the loss is summed over rows in 64 bits.
-#include "common.cuh"
+#include <atomic>
+#include "umma.cuh"
 
 namespace kge {
 
@@ -176,84 +177,77 @@ __device__ __forceinline__ void merge_parts(float& m, float& rest, float m2, flo
 }
 
 // ---- rows kept in registers -------------------------------------------------------------------------------------------
-// A group of 32 lanes (one warp a row), or of THREADS x cluster size, reads its row once, as I vectors a thread, and keeps it
-// until the gradient is written: 8 bytes of traffic per fp32 score, 4 per bf16.  Each warp takes its own maximum and sum; the
-// (m, rest) pairs of a row's warps are merged after one barrier.  fp32 scores are replaced by their exponentials in place, so
-// the gradient costs one multiplication each; bf16 scores stay packed and are exponentiated a second time.
-constexpr int kMaxCluster = 8;
-template <typename T, int THREADS, int I, int MODE>
-__global__ void __launch_bounds__(THREADS == 32 ? 256 : THREADS, THREADS == 32 ? 4 : (I == 8 ? 1024 : 1280) / THREADS)
-cand_cached_kernel(CandArgs a) {
-    constexpr int V = Vec<T>::V;
-    constexpr bool kWarp32 = THREADS == 32;
-    constexpr bool kKeepExp = sizeof(T) == 4;
-    constexpr int kWarps = THREADS / 32;
-    __shared__ float2 parts[kWarp32 ? 1 : kWarps];
-    __shared__ float bcast, sides[4];
-    __shared__ double red[8];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int tid = kWarp32 ? lane : threadIdx.x;
-    uint32_t rank = 0, csize = 1;
-    if (!kWarp32) {
-        asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
-        asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(csize));
+// A warp, a CTA or a cluster of CTAs reads a row once, as I vectors a thread, and keeps it until the gradient is written:
+// 8 bytes of traffic per fp32 score, 4 per bf16.  Each warp takes its own maximum and sum; the (m, rest) pairs of a row's
+// warps are merged after one barrier.  fp32 scores are replaced by their exponentials in place, so the gradient costs one
+// multiplication each; bf16 scores stay packed and are exponentiated a second time.
+struct Slice {                    // a CTA's part of a row
+    int head, nv, v0, v1;         // elements before the first vector, vectors of the row, vectors [v0, v1) of this CTA
+};
+template <typename T>
+__device__ __forceinline__ Slice cand_slice(const T* s, int n, uint32_t rank, uint32_t csize) {
+    Slice q;
+    q.head = head_of(s, n);
+    q.nv = (n - q.head) / Vec<T>::V;
+    const int shift = 31 - __clz(static_cast<int>(csize));        // cluster sizes are powers of two
+    const int share = (q.nv + static_cast<int>(csize) - 1) >> shift;
+    q.v0 = min(q.nv, static_cast<int>(rank) * share);
+    q.v1 = min(q.nv, q.v0 + share);
+    return q;
+}
+// The head or tail element that thread tid < 16 of the row's first CTA takes, or -1.
+template <typename T>
+__device__ __forceinline__ int extra_index(const Slice& q, int n, int tid) {
+    if (tid < 8) return tid < q.head ? tid : -1;
+    const int j = q.head + q.nv * Vec<T>::V + tid - 8;
+    return tid < 16 && j < n ? j : -1;
+}
+
+// A thread's part of one row between the loads and the gradient: register i holds vector v0 + tid + i THREADS.
+template <typename T, int THREADS, int I>
+struct RowPart {
+    static constexpr int V = Vec<T>::V;
+    static constexpr bool kKeepExp = sizeof(T) == 4;
+    uint4 r[I];
+    float xe;                     // the extra element
+    int xi, own;                  // its index; the register that holds the chosen candidate, or -1
+    float mw, mz;                 // maximum of this warp's part, and with 0 in the place of -infinity
+
+    // first vector (in units of THREADS) past this thread's vectors that hold a candidate
+    __device__ __forceinline__ static int filled(const Slice& q, int cnt, int tid) {
+        const int nvc = cnt <= q.head ? 0 : (cnt - q.head + V - 1) / V;
+        return min(q.v1, nvc) - q.v0 - tid;
     }
-    const int cshift = 31 - __clz(static_cast<int>(csize));        // cluster sizes are powers of two
-    const long long groups = kWarp32 ? (long long)gridDim.x * 8 : 1;
-    const long long first_row = kWarp32 ? (long long)blockIdx.x * 8 + warp : blockIdx.x >> cshift;
-    const long long rows = kWarp32 ? a.rows : first_row + 1;        // a CTA or cluster has one row, a warp goes on
-    const float c = a.inv_temp * 1.4426950408889634f;
-    double total = 0.0;
-    for (long long row = first_row; row < rows; row += groups) {
-        const T* s = static_cast<const T*>(a.scores) + row * a.ld;
-        const int cnt = cand_count(a, row);
-        const int act = cand_action(a, row, cnt, tid == 0 && rank == 0);
-        const float sa = act >= 0 ? cand_get(s + act) : 0.f;
-        float side = 0.f;                 // thread k < 4 requests operand k now: the finish of the row must not wait for memory
-        if (MODE == CM_POLICY && tid < 4) side = cand_side(a, row, tid);
-        const int head = head_of(s, a.n), nv = (a.n - head) / V;
-        const int share = (nv + static_cast<int>(csize) - 1) >> cshift;       // this CTA's vectors: [v0, v1)
-        const int v0 = static_cast<int>(rank) * share, v1 = min(nv, v0 + share);
-        const int used = (v1 - v0 + THREADS - 1) / THREADS;      // registers of a thread that hold anything (the same for all)
-        // the extra element of this thread, if any
-        int xi = -1;
-        if (rank == 0 && tid < 16) {
-            if (tid < 8) { if (tid < head) xi = tid; }
-            else if (head + nv * V + tid - 8 < a.n) xi = head + nv * V + tid - 8;
-        }
-        const uint4* sv = reinterpret_cast<const uint4*>(s + head);
-        uint4 r[I];
+    __device__ __forceinline__ void load(const uint4* src, int left) {        // src: vector v0 + tid
 #pragma unroll
         for (int i = 0; i < I; ++i) {
-            const int v = v0 + tid + i * THREADS;
             r[i] = make_uint4(Vec<T>::kLow, Vec<T>::kLow, Vec<T>::kLow, Vec<T>::kLow);
-            if (v < v1 && head + v * V < cnt) r[i] = __ldcs(sv + v);
+            if (i * THREADS < left) r[i] = __ldcs(src + i * THREADS);
         }
-        float xe = xi >= 0 && xi < cnt ? cand_get(s + xi) : -INFINITY;
-        if (a.n_cand) {
+    }
+    __device__ __forceinline__ float stats(const Slice& q, int n, int cnt, int act, int tid, float c) {
+        const int used = (q.v1 - q.v0 + THREADS - 1) / THREADS;               // registers that hold anything, the same for all
+        if (cnt < n) {
 #pragma unroll
             for (int i = 0; i < I; ++i) {
-                const int at = head + (v0 + tid + i * THREADS) * V;
+                const int at = q.head + (q.v0 + tid + i * THREADS) * V;
                 if (at < cnt && at + V > cnt) r[i] = mask_past<T>(r[i], at, cnt);
             }
         }
-        float mw = xe;
+        mw = xe;
 #pragma unroll
         for (int i = 0; i < I; ++i) if (i < used) mw = fmaxf(mw, Vec<T>::max(r[i]));
         mw = warp_max(mw);
-        const float mz = finite_or_zero(mw);
-        // the vector (register index) of this thread that holds the chosen candidate
-        int own = -1;
-        if (act >= head && act < head + nv * V) {
-            const int v = (act - head) / V - v0;
-            if (v >= 0 && v % THREADS == tid && v0 + v < v1) own = v / THREADS;
+        mz = finite_or_zero(mw);
+        own = -1;
+        if (act >= q.head && act < q.head + q.nv * V) {
+            const int v = (act - q.head) / V - q.v0;
+            if (v >= 0 && v % THREADS == tid && q.v0 + v < q.v1) own = v / THREADS;
         }
         float rest = 0.f;
-        {
-            const float e = cand_ex2((xe - mz) * c);
-            if (xi != act) rest = e;
-            if (kKeepExp) xe = e;
-        }
+        const float e = cand_ex2((xe - mz) * c);
+        if (xi != act) rest = e;
+        if (kKeepExp) xe = e;
 #pragma unroll
         for (int i = 0; i < I; ++i) {
             if (i >= used) continue;
@@ -264,118 +258,238 @@ cand_cached_kernel(CandArgs a) {
             if (kKeepExp) r[i] = Vec<T>::close(f);
             if (i == own) {
 #pragma unroll
-                for (int k = 0; k < V; ++k) if ((act - head) % V == k) f[k] = 0.f;
+                for (int k = 0; k < V; ++k) if ((act - q.head) % V == k) f[k] = 0.f;
             }
             float t = 0.f;
 #pragma unroll
             for (int k = 0; k < V; k += 4) t += (f[k] + f[k + 1]) + (f[k + 2] + f[k + 3]);
             rest += t;
         }
-        rest = warp_sum(rest);
         if (!kKeepExp) {          // keep the packed words, not their unpacked values, in registers until the gradient
 #pragma unroll
             for (int i = 0; i < I; ++i) asm volatile("" : "+r"(r[i].x), "+r"(r[i].y), "+r"(r[i].z), "+r"(r[i].w));
         }
-        float m = mw, ga = 0.f;
-        if (kWarp32) {
-            RowSide o = {};
-            if (MODE == CM_POLICY) {
-                o.w = __shfl_sync(kFull, side, 0); o.adv = __shfl_sync(kFull, side, 1);
-                o.old = __shfl_sync(kFull, side, 2); o.ref = __shfl_sync(kFull, side, 3);
-            }
-            if (lane == 0) total += cand_finish<MODE>(a, row, act, sa, finite_or_zero(m), rest, true, o, &ga);
-            if (MODE != CM_LOGP) ga = __shfl_sync(kFull, ga, 0);
-        } else {
-            if (lane == 0) parts[warp] = make_float2(mw, rest);
-            if (MODE == CM_POLICY && tid < 4) sides[tid] = side;
-            if (csize == 1) {
-                __syncthreads();
-            } else {
-                asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-            }
-            // every warp merges all parts of the row, in the same order
-            m = -INFINITY; rest = 0.f;
-            if (csize == 1) {
-                if (lane < kWarps) { m = parts[lane].x; rest = parts[lane].y; }
-            } else {
-                for (int j = lane; j < kWarps * static_cast<int>(csize); j += 32) {
-                    float2 q;
-                    const uint32_t addr = static_cast<uint32_t>(__cvta_generic_to_shared(&parts[j % kWarps]));
-                    uint32_t remote;
-                    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(static_cast<uint32_t>(j / kWarps)));
-                    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(q.x), "=f"(q.y) : "r"(remote) : "memory");
-                    merge_parts(m, rest, q.x, q.y, c);
+        return warp_sum(rest);
+    }
+    __device__ __forceinline__ void write(T* d, const Slice& q, int n, int cnt, int act, int tid, float c, float m, float rest, float ga) const {
+        uint4* dv = reinterpret_cast<uint4*>(d + q.head) + q.v0 + tid;
+        const int left = q.v1 - q.v0 - tid;
+        const float mall = finite_or_zero(m);
+        // (a warp without a finite score has only zeros to scale: mz = 0 stands for nothing there)
+        const float f0 = ga == 0.f || (kKeepExp && mw == -INFINITY) ? 0.f : kKeepExp ? -ga * cand_ex2((mz - mall) * c) : -ga;
+        const float fa = ga == 0.f ? 0.f : ga * rest;
+        const bool plain = cnt == n && ga != 0.f;                 // no padding, and something to write
+#pragma unroll
+        for (int i = 0; i < I; ++i) {
+            if (i * THREADS < left) {
+                float f[V];
+                Vec<T>::open(r[i], f);
+#pragma unroll
+                for (int k = 0; k < V; ++k) f[k] = f0 * (kKeepExp ? f[k] : cand_ex2((f[k] - mall) * c));
+                if (!plain) {
+                    const int at = q.head + (q.v0 + tid + i * THREADS) * V;
+#pragma unroll
+                    for (int k = 0; k < V; ++k) if (ga == 0.f || at + k >= cnt) f[k] = 0.f;
                 }
-                // the parts have been read: no CTA of the cluster leaves before the others have got here
-                asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-            }
-            const float mine = m;
-            m = warp_max(m);
-            rest = warp_sum(rest * cand_ex2((mine - finite_or_zero(m)) * c));
-            if (MODE == CM_LOGP) {
-                if (threadIdx.x == 0 && rank == 0) cand_finish<MODE>(a, row, act, sa, finite_or_zero(m), rest, true, RowSide{}, &ga);
-            } else {
-                if (threadIdx.x == 0) {
-                    const double l = cand_finish<MODE>(a, row, act, sa, finite_or_zero(m), rest, rank == 0, RowSide{sides[0], sides[1], sides[2], sides[3]}, &ga);
-                    if (rank == 0) total += l;
-                    bcast = ga;
-                }
-                __syncthreads();
-                ga = bcast;
+                __stcs(dv + i * THREADS, Vec<T>::close(f));
             }
         }
-        if (MODE != CM_LOGP) {
-            T* d = static_cast<T*>(a.dscores) + row * a.ldd;
-            uint4* dv = reinterpret_cast<uint4*>(d + head);
-            const float mall = finite_or_zero(m);
-            // (a warp without a finite score has only zeros to scale: mz = 0 stands for nothing there)
-            const float f0 = ga == 0.f || (kKeepExp && mw == -INFINITY) ? 0.f : kKeepExp ? -ga * cand_ex2((mz - mall) * c) : -ga;
-            const float fa = ga == 0.f ? 0.f : ga * rest;
-#pragma unroll
-            for (int i = 0; i < I; ++i) {
-                const int v = v0 + tid + i * THREADS;
-                if (v < v1) {
-                    const int at = head + v * V;
-                    float f[V];
-                    if (at >= cnt || ga == 0.f) {
-#pragma unroll
-                        for (int k = 0; k < V; ++k) f[k] = 0.f;
-                    } else {
-                        Vec<T>::open(r[i], f);
-#pragma unroll
-                        for (int k = 0; k < V; ++k) f[k] = f0 * (kKeepExp ? f[k] : cand_ex2((f[k] - mall) * c));
-                        if (i == own) {
-#pragma unroll
-                            for (int k = 0; k < V; ++k) if (at + k == act) f[k] = fa;
-                        }
-                        if (at + V > cnt) {
-#pragma unroll
-                            for (int k = 0; k < V; ++k) if (at + k >= cnt) f[k] = 0.f;
-                        }
-                    }
-                    __stcs(dv + v, Vec<T>::close(f));
-                }
-            }
-            if (xi >= 0) {
-                float v = 0.f;
-                if (xi < cnt && ga != 0.f) v = xi == act ? fa : f0 * (kKeepExp ? xe : cand_ex2((xe - mall) * c));
-                cand_put(d + xi, v);
-            }
+        if (own >= 0) cand_put(d + act, fa);                      // over the vector just stored by this thread
+        if (xi >= 0) {
+            float v = 0.f;
+            if (xi < cnt && ga != 0.f) v = xi == act ? fa : f0 * (kKeepExp ? xe : cand_ex2((xe - mall) * c));
+            cand_put(d + xi, v);
         }
     }
-    if (!kWarp32 && csize > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+};
+
+// One warp per row: rows of up to 32 I vectors.
+template <typename T, int I, int MODE>
+__global__ void __launch_bounds__(256, 4) cand_warp_kernel(CandArgs a) {
+    __shared__ double red[8];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const float c = a.inv_temp * 1.4426950408889634f;
+    double total = 0.0;
+    for (long long row = (long long)blockIdx.x * 8 + warp; row < a.rows; row += (long long)gridDim.x * 8) {
+        const T* s = static_cast<const T*>(a.scores) + row * a.ld;
+        const int cnt = cand_count(a, row);
+        const int act = cand_action(a, row, cnt, lane == 0);
+        const float sa = act >= 0 ? cand_get(s + act) : 0.f;
+        float side = 0.f;                 // lane k < 4 requests operand k now: the finish of the row must not wait for memory
+        if (MODE == CM_POLICY && lane < 4) side = cand_side(a, row, lane);
+        const Slice q = cand_slice(s, a.n, 0, 1);
+        RowPart<T, 32, I> p;
+        p.load(reinterpret_cast<const uint4*>(s + q.head) + lane, RowPart<T, 32, I>::filled(q, cnt, lane));
+        p.xi = extra_index<T>(q, a.n, lane);
+        p.xe = p.xi >= 0 && p.xi < cnt ? cand_get(s + p.xi) : -INFINITY;
+        const float rest = p.stats(q, a.n, cnt, act, lane, c);
+        RowSide o = {};
+        if (MODE == CM_POLICY) {
+            o.w = __shfl_sync(kFull, side, 0); o.adv = __shfl_sync(kFull, side, 1);
+            o.old = __shfl_sync(kFull, side, 2); o.ref = __shfl_sync(kFull, side, 3);
+        }
+        float ga = 0.f;
+        if (lane == 0) total += cand_finish<MODE>(a, row, act, sa, p.mz, rest, true, o, &ga);
+        if (MODE == CM_POLICY) p.write(static_cast<T*>(a.dscores) + row * a.ldd, q, a.n, cnt, act, lane, c, p.mw, rest, __shfl_sync(kFull, ga, 0));
+    }
     if (MODE == CM_POLICY) {
-        if (kWarp32) {
-            if (lane == 0) red[warp] = total;
-            __syncthreads();
-            if (threadIdx.x == 0) {
-                for (int w = 1; w < 8; ++w) total += red[w];
-                a.partial[blockIdx.x] = total;
-            }
-        } else if (threadIdx.x == 0 && rank == 0) {
-            a.partial[blockIdx.x >> cshift] = total;
+        if (lane == 0) red[warp] = total;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            for (int w = 1; w < 8; ++w) total += red[w];
+            a.partial[blockIdx.x] = total;
         }
     }
+}
+
+// ---- rows kept in shared memory -----------------------------------------------------------------------------------------
+// A CTA, or a cluster, with one row each.  Its part of the row arrives by one bulk copy (in flight before anything else is
+// known about the row), is read twice from shared memory - online maximum and sum, then the gradient - and leaves by 16-byte
+// stores.  As many CTAs as shared memory holds (3 at 60 KB) share an SM, so that copies, arithmetic and stores of different
+// rows overlap.  Measured against rows in registers (4096 x 15000 fp32 / 1024 x 100000 bf16, us): see the launch code.
+constexpr int kMaxCluster = 8;
+constexpr int kRowSlot = 4608, kRowSmem = 216 * 1024;          // vectors of a row per CTA, at most (72 KB: three CTAs per SM)
+template <typename T, int THREADS, int CTAS, int MODE>
+__global__ void __launch_bounds__(THREADS, CTAS) cand_row_kernel(CandArgs a) {
+    constexpr int kWarps = THREADS / 32, V = Vec<T>::V;
+    extern __shared__ __align__(128) uint8_t row_smem[];
+    __shared__ __align__(8) uint64_t full;
+    __shared__ float2 parts[kWarps];
+    __shared__ float bcast, sides[4];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    uint32_t rank, csize;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(csize));
+    const long long row = blockIdx.x / csize;
+    const float c = a.inv_temp * 1.4426950408889634f;
+    const T* s = static_cast<const T*>(a.scores) + row * a.ld;
+    const int cnt = cand_count(a, row);
+    const Slice q = cand_slice(s, a.n, rank, csize);
+    const int nvc = cnt <= q.head ? 0 : (cnt - q.head + V - 1) / V;         // vectors of the row that hold a candidate
+    const int have = max(0, min(q.v1, nvc) - q.v0);                         // of this CTA
+    if (tid == 0) {
+        umma::mbar_init(&full, 1);
+        umma::fence_barrier_init();
+        if (have > 0) {
+            umma::mbar_expect_tx(&full, static_cast<uint32_t>(have) * 16u);
+            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                         ::"r"(umma::smem_u32(row_smem)), "l"(reinterpret_cast<const uint4*>(s + q.head) + q.v0),
+                           "r"(static_cast<uint32_t>(have) * 16u), "r"(umma::smem_u32(&full)) : "memory");
+        } else {
+            umma::mbar_arrive(&full);
+        }
+    }
+    const int act = cand_action(a, row, cnt, tid == 0 && rank == 0);
+    const float sa = act >= 0 && tid == 0 ? cand_get(s + act) : 0.f;
+    float side = 0.f;                     // thread k < 4 requests operand k now: the finish of the row must not wait for memory
+    if (MODE == CM_POLICY && tid < 4) side = cand_side(a, row, tid);
+    const int xi = rank == 0 ? extra_index<T>(q, a.n, tid) : -1;
+    const float xe = xi >= 0 && xi < cnt ? cand_get(s + xi) : -INFINITY;
+    // this CTA's vector that holds the chosen candidate, and its place in it
+    const int av = act >= q.head && act < q.head + q.nv * V ? (act - q.head) / V - q.v0 : -1, ak = (act - q.head) % V;
+    float m = xe, rest = 0.f, mz = finite_or_zero(m);
+    if (xi != act) rest = cand_ex2((xe - mz) * c);
+    __syncthreads();                      // the barrier exists
+    if (!umma::mbar_wait(&full, 0)) {     // (the row's outputs are invalid; its copy is waited for once more)
+        atomicOr(a.err, KGE_ERR_WAIT_TIMEOUT);
+        umma::mbar_wait(&full, 0);
+    }
+    const uint4* sv = reinterpret_cast<const uint4*>(row_smem);
+    const int whole = cnt >= a.n ? have : min(have, max(0, (cnt - q.head) / V - q.v0));      // vectors without padding in them
+#pragma unroll 2
+    for (int v = tid; v < have; v += THREADS) {
+        uint4 r = sv[v];
+        if (v >= whole) r = mask_past<T>(r, q.head + (q.v0 + v) * V, cnt);
+        const float vm = Vec<T>::max(r);
+        if (vm > m) {                     // a new maximum of this thread: rescale what it has (rare after the first vectors)
+            mz = finite_or_zero(vm);
+            rest *= cand_ex2((m - mz) * c);
+            m = vm;
+        }
+        float f[V];
+        Vec<T>::open(r, f);
+#pragma unroll
+        for (int k = 0; k < V; ++k) f[k] = cand_ex2((f[k] - mz) * c);
+        if (v == av) {
+#pragma unroll
+            for (int k = 0; k < V; ++k) if (k == ak) f[k] = 0.f;
+        }
+        float t = (f[0] + f[1]) + (f[2] + f[3]);
+        if (V == 8) t += (f[V - 4] + f[V - 3]) + (f[V - 2] + f[V - 1]);
+        rest += t;
+    }
+    {
+        const float mine = m;
+        m = warp_max(m);
+        rest = warp_sum(rest * cand_ex2((mine - finite_or_zero(m)) * c));
+    }
+    if (lane == 0) parts[warp] = make_float2(m, rest);
+    if (MODE == CM_POLICY && tid < 4) sides[tid] = side;
+    if (csize == 1) __syncthreads();
+    else asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    // every warp merges all parts of the row, in the same order
+    m = -INFINITY;
+    rest = 0.f;
+    if (csize == 1) {
+        if (lane < kWarps) { m = parts[lane].x; rest = parts[lane].y; }
+    } else {
+        for (int j = lane; j < kWarps * static_cast<int>(csize); j += 32) {
+            float2 o;
+            uint32_t remote;
+            asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(umma::smem_u32(&parts[j % kWarps])), "r"(static_cast<uint32_t>(j / kWarps)));
+            asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(o.x), "=f"(o.y) : "r"(remote) : "memory");
+            merge_parts(m, rest, o.x, o.y, c);
+        }
+        // the parts have been read: no CTA of the cluster leaves before the others have got here
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    }
+    {
+        const float mine = m;
+        m = warp_max(m);
+        mz = finite_or_zero(m);
+        rest = warp_sum(rest * cand_ex2((mine - mz) * c));
+    }
+    if (tid == 0) {
+        float ga = 0.f;
+        const RowSide o = {sides[0], sides[1], sides[2], sides[3]};
+        const double l = cand_finish<MODE>(a, row, act, sa, mz, rest, rank == 0, o, &ga);
+        bcast = ga;
+        if (MODE == CM_POLICY && rank == 0) a.partial[row] = l;
+    }
+    if (MODE == CM_POLICY) {
+        __syncthreads();
+        const float ga = bcast, fa = ga == 0.f ? 0.f : ga * rest;
+        T* d = static_cast<T*>(a.dscores) + row * a.ldd;
+        uint4* dv = reinterpret_cast<uint4*>(d + q.head) + q.v0;
+        const int mine = q.v1 - q.v0, full_to = ga == 0.f ? 0 : whole;
+#pragma unroll 2
+        for (int v = tid; v < full_to; v += THREADS) {
+            float f[V];
+            Vec<T>::open(sv[v], f);
+#pragma unroll
+            for (int k = 0; k < V; ++k) f[k] = -ga * cand_ex2((f[k] - mz) * c);
+            if (v == av) {
+#pragma unroll
+                for (int k = 0; k < V; ++k) if (k == ak) f[k] = fa;
+            }
+            __stcs(dv + v, Vec<T>::close(f));
+        }
+        for (int v = full_to + tid; v < mine; v += THREADS) {               // the vector that the count cuts, padding, dead rows
+            float f[V];
+#pragma unroll
+            for (int k = 0; k < V; ++k) f[k] = 0.f;
+            const int at = q.head + (q.v0 + v) * V;
+            if (ga != 0.f && at < cnt) {
+                float g[V];
+                Vec<T>::open(sv[v], g);
+#pragma unroll
+                for (int k = 0; k < V; ++k) if (at + k < cnt) f[k] = at + k == act ? fa : -ga * cand_ex2((g[k] - mz) * c);
+            }
+            __stcs(dv + v, Vec<T>::close(f));
+        }
+        if (xi >= 0) cand_put(d + xi, xi >= cnt || ga == 0.f ? 0.f : xi == act ? fa : -ga * cand_ex2((xe - mz) * c));
+    }
+    if (csize > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // ---- rows cut over several CTAs, in passes ----------------------------------------------------------------------------
@@ -570,7 +684,7 @@ int launch_sum_partials(const double* partial, int n, float* out, cudaStream_t s
     return 0;
 }
 
-constexpr int kCandMaxBlocks = 148 * 8;            // CTAs that leave a partial sum of the loss, where they take rows in turn
+constexpr int kCandMaxBlocks = 148 * 16;           // groups that take rows in turn; each leaves a partial sum of the loss
 
 // Workspace: partial sums of the loss, then per-chunk (m, rest) and per-row coefficients of the multi-pass form.
 struct CandLayout { int chunk, chunks; size_t off_parts, off_coef, total; };
@@ -589,23 +703,39 @@ static CandLayout cand_layout(long long rows, long long n) {
     return L;
 }
 
-template <typename T, int THREADS, int I, int MODE>
-static int cand_cached(const CandArgs& a, int cluster, int* n_partial, cudaStream_t s) {
-    // warps take rows in turn; a CTA or cluster has one row, so that its loads start while others write
-    const long long want = THREADS == 32 ? (a.rows + 7) / 8 : a.rows;
-    const long long groups = THREADS == 32 && want > kCandMaxBlocks ? kCandMaxBlocks : want;
+template <typename T, int I, int MODE>
+static int cand_warps(const CandArgs& a, int* n_partial, cudaStream_t s) {
+    const long long want = (a.rows + 7) / 8;
+    *n_partial = static_cast<int>(want < kCandMaxBlocks ? want : kCandMaxBlocks);
+    cand_warp_kernel<T, I, MODE><<<*n_partial, 256, 0, s>>>(a);
+    KGE_LAUNCH_CHECK("cand_warp_kernel");
+    return 0;
+}
+
+// slot: vectors of a row that one CTA holds
+template <typename T, int THREADS, int CTAS, int MODE>
+static int cand_rows(const CandArgs& a, int cluster, long long slot, int* n_partial, cudaStream_t s) {
+    static std::atomic<bool> attr_set[128];          // the shared-memory opt-in is per device and kernel
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return cuda_status(cudaGetLastError(), "cudaGetDevice");
+    if (dev < 0 || dev >= 128 || !attr_set[dev].load(std::memory_order_acquire)) {
+        cudaError_t e = cudaFuncSetAttribute(cand_row_kernel<T, THREADS, CTAS, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowSmem);
+        if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(cand_row_kernel)");
+        if (dev >= 0 && dev < 128) attr_set[dev].store(true, std::memory_order_release);
+    }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(groups * cluster));
-    cfg.blockDim = dim3(THREADS == 32 ? 256 : THREADS);
+    cfg.gridDim = dim3(static_cast<unsigned>(a.rows * cluster));
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = static_cast<size_t>(slot) * 16;
     cfg.stream = s;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = cluster; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
     cfg.attrs = at; cfg.numAttrs = cluster > 1 ? 1 : 0;
-    *n_partial = static_cast<int>(groups);
-    cudaError_t e = cudaLaunchKernelEx(&cfg, cand_cached_kernel<T, THREADS, I, MODE>, a);
-    if (e != cudaSuccess) return cuda_status(e, "cand_cached_kernel");
-    KGE_LAUNCH_CHECK("cand_cached_kernel");
+    *n_partial = static_cast<int>(a.rows);
+    cudaError_t e = cudaLaunchKernelEx(&cfg, cand_row_kernel<T, THREADS, CTAS, MODE>, a);
+    if (e != cudaSuccess) return cuda_status(e, "cand_row_kernel");
+    KGE_LAUNCH_CHECK("cand_row_kernel");
     return 0;
 }
 
@@ -643,22 +773,31 @@ static int cand_passes(const CandArgs& a, void* ws, int* n_partial, cudaStream_t
 
 // Which form: the smallest group that holds a row in registers; passes where the rows are too long for a cluster, where the
 // groups of all rows would leave most SMs idle, or where the gradient's alignment differs.
+#ifndef VAR
+#define VAR 0
+#endif
 template <typename T, int MODE>
 static int cand_go(const CandArgs& a, void* ws, int* n_partial, cudaStream_t s) {
     const long long nv = a.n / Vec<T>::V;              // vectors of a row, at most
     if (MODE == CM_POLICY && !same_phase<T>(a)) return cand_passes<T, MODE>(a, ws, n_partial, s);
-    if (nv <= 32) return cand_cached<T, 32, 1, MODE>(a, 1, n_partial, s);
-    if (nv <= 64) return cand_cached<T, 32, 2, MODE>(a, 1, n_partial, s);
-    if (nv <= 128) return cand_cached<T, 32, 4, MODE>(a, 1, n_partial, s);
-    if (a.rows >= (1LL << 31)) return cand_passes<T, MODE>(a, ws, n_partial, s);      // (beyond a grid of one CTA a row)
-    if (nv <= 64 * 4) return cand_cached<T, 64, 4, MODE>(a, 1, n_partial, s);
-    if (nv <= 128 * 4) return cand_cached<T, 128, 4, MODE>(a, 1, n_partial, s);
-    if (nv <= 256 * 4) return cand_cached<T, 256, 4, MODE>(a, 1, n_partial, s);
-    if (nv <= 512 * 4) return cand_cached<T, 512, 4, MODE>(a, 1, n_partial, s);
+    if (nv <= 32) return cand_warps<T, 1, MODE>(a, n_partial, s);
+    if (nv <= 64) return cand_warps<T, 2, MODE>(a, n_partial, s);
+    if (nv <= 128) return cand_warps<T, 4, MODE>(a, n_partial, s);
+    if (a.rows >= (1LL << 31) / kMaxCluster) return cand_passes<T, MODE>(a, ws, n_partial, s);      // (beyond a grid of one CTA a row)
+    if (nv <= 512) return cand_rows<T, 64, 16, MODE>(a, 1, nv, n_partial, s);
+    if (nv <= 1024) return cand_rows<T, 128, 10, MODE>(a, 1, nv, n_partial, s);
     int cluster = 1;
-    while (cluster <= kMaxCluster && nv > cluster * 512LL * 8) cluster *= 2;
-    if (cluster > kMaxCluster || a.rows * cluster < 32 || a.rows >= (1LL << 31) / kMaxCluster) return cand_passes<T, MODE>(a, ws, n_partial, s);
-    return cand_cached<T, 512, 8, MODE>(a, cluster, n_partial, s);
+    while (cluster <= kMaxCluster && nv > cluster * static_cast<long long>(kRowSlot)) cluster *= 2;
+    if (cluster > kMaxCluster || a.rows * cluster < 32) return cand_passes<T, MODE>(a, ws, n_partial, s);
+#if VAR == 0
+    return cand_rows<T, 256, 5, MODE>(a, cluster, (nv + cluster - 1) / cluster, n_partial, s);
+#elif VAR == 1
+    return cand_rows<T, 512, 3, MODE>(a, cluster, (nv + cluster - 1) / cluster, n_partial, s);
+#elif VAR == 2
+    return cand_rows<T, 512, 2, MODE>(a, cluster, (nv + cluster - 1) / cluster, n_partial, s);
+#else
+    return cand_rows<T, 1024, 1, MODE>(a, cluster, (nv + cluster - 1) / cluster, n_partial, s);
+#endif
 }
 
 }  // namespace kge

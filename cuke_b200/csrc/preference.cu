@@ -32,22 +32,20 @@ __device__ __forceinline__ float pref_rcp(float x) { float r; asm("rcp.approx.ft
 // interpolation of degree 4 on [0, 1/9], 4e-9 relative), so small terms keep their digits at the cost of one reciprocal and six
 // fused multiply-adds: the loss is bound by memory only if a pair stays below some 40 instructions.
 template <bool SQUARE>
-__device__ __forceinline__ void pref_pair(const PrefArgs& a, float z, float& l, float& d) {
+__device__ __forceinline__ void pref_pair(const PrefArgs& a, float keep, float z, float& l, float& d) {
     if (SQUARE) { l = z * z; d = 2.f * z; return; }
     const float t = pref_ex2(fabsf(z) * -1.4426950408889634f);
     const float inv = pref_rcp(1.f + t), w = t * pref_rcp(2.f + t), x = w * w;
     const float q = fmaf(fmaf(fmaf(fmaf(0.14078890f, x, 0.13982579f), x, 0.20012298f), x, 0.33333161f), x, 1.f);
-    const float small = t * inv, down = z >= 0.f ? small : inv;                      // sigmoid(-z)
-    const float keep = 1.f - a.smooth;
+    const float small = t * inv;                                 // sigmoid(-|z|); inv is sigmoid(|z|)
+    const bool up = z >= 0.f;
+    d = fmaf(up ? a.smooth : -keep, inv, (up ? -keep : a.smooth) * small);
     l = fmaf(w + w, q, keep * fmaxf(-z, 0.f));
-    d = -keep * down;
-    if (a.smooth > 0.f) {                                                            // (0 x inf without the test)
-        l = fmaf(a.smooth, fmaxf(z, 0.f), l);
-        d = fmaf(a.smooth, z >= 0.f ? inv : small, d);
-    }
+    if (a.smooth > 0.f) l = fmaf(a.smooth, fmaxf(z, 0.f), l);    // (0 x inf without the test)
 }
 
-__device__ __forceinline__ int nonzero_bytes(uint32_t w) { return __popc(__vcmpne4(w, 0u)) >> 3; }
+// bytes of w that are not zero: the low seven bits carry into the eighth, or it is set already
+__device__ __forceinline__ int nonzero_bytes(uint32_t w) { return __popc((((w & 0x7F7F7F7Fu) + 0x7F7F7F7Fu) | w) & 0x80808080u); }
 
 template <int G>
 __device__ __forceinline__ float pref_group_sum(float v) {
@@ -67,7 +65,7 @@ __device__ __forceinline__ int pref_group_sum(int v) {
 // a row are counted first - the mask is a thirteenth of the traffic and comes from L1 the second time - so that the main pass
 // writes final gradients; it requests U accesses of each array before it uses the first.  Without VEC a thread has the same four
 // negatives, read one by one: the order of the additions, and so every bit of the result, does not depend on alignment.
-template <int G, bool VEC, bool SQUARE>
+template <int G, bool VEC, bool SQUARE, bool MASK>
 __global__ void __launch_bounds__(G > 256 ? G : 256) pref_kernel(PrefArgs a) {
     constexpr int BLOCK = G > 256 ? G : 256;
     constexpr int W = 4;                           // consecutive negatives of a thread
@@ -88,10 +86,10 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) pref_kernel(PrefArgs a) {
         const int n = live ? a.n : 0;
         const float* neg = a.neg + rr * a.ldn;
         const float* rneg = a.rneg ? a.rneg + rr * a.ldr : nullptr;
-        const unsigned char* mask = a.mask ? a.mask + rr * a.ldm : nullptr;
+        const unsigned char* mask = MASK ? a.mask + rr * a.ldm : nullptr;
         float* dneg = a.dneg + rr * a.ldd;
         int cnt = n;
-        if (mask) {
+        if (MASK) {
             cnt = 0;
             for (int j = gl * W; j < n; j += G * W) {
                 if (VEC) {
@@ -112,7 +110,8 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) pref_kernel(PrefArgs a) {
         const float base = a.pos[rr] - (a.rpos ? a.rpos[rr] : 0.f);
         const float weight = a.weight ? a.weight[rr] : 1.f;
         const float cw = cnt > 0 ? a.scale * weight / static_cast<float>(cnt) : 0.f;
-        const float dscale = -cw * a.beta;
+        const float dscale = -cw * a.beta, keep = 1.f - a.smooth;
+        const bool off = cw == 0.f;                    // nothing valid, or weight 0: zeros, whatever the scores hold
         float ls = 0.f, ds = 0.f;
         for (int j0 = gl * W; j0 < n; j0 += G * W * U) {
             float x[U][W], y[U][W];
@@ -126,7 +125,7 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) pref_kernel(PrefArgs a) {
                         const float4 f = __ldcs(reinterpret_cast<const float4*>(neg + j));
                         float4 g = make_float4(0.f, 0.f, 0.f, 0.f);
                         if (rneg) g = __ldcs(reinterpret_cast<const float4*>(rneg + j));
-                        m[u] = mask ? __vcmpne4(*reinterpret_cast<const uint32_t*>(mask + j), 0u) : 0xFFFFFFFFu;
+                        if (MASK) m[u] = *reinterpret_cast<const uint32_t*>(mask + j);
                         x[u][0] = f.x; x[u][1] = f.y; x[u][2] = f.z; x[u][3] = f.w;
                         y[u][0] = g.x; y[u][1] = g.y; y[u][2] = g.z; y[u][3] = g.w;
                     } else {
@@ -136,7 +135,7 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) pref_kernel(PrefArgs a) {
                             if (j + k < n) {
                                 x[u][k] = neg[j + k];
                                 if (rneg) y[u][k] = rneg[j + k];
-                                if (!mask || mask[j + k]) m[u] |= 0xFFu << (8 * k);
+                                if (!MASK || mask[j + k]) m[u] |= 0xFFu << (8 * k);
                             }
                         }
                     }
@@ -150,12 +149,13 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) pref_kernel(PrefArgs a) {
 #pragma unroll
                     for (int k = 0; k < W; ++k) {
                         float l, d;
-                        pref_pair<SQUARE>(a, fmaf(a.beta, base - (x[u][k] - y[u][k]), -a.margin), l, d);
-                        const bool on = (m[u] >> (8 * k)) & 1u;
-                        ls += on ? l : 0.f;
-                        ds += on ? d : 0.f;
-                        o[k] = on && cw != 0.f ? dscale * d : 0.f;
+                        pref_pair<SQUARE>(a, keep, fmaf(a.beta, base - (x[u][k] - y[u][k]), -a.margin), l, d);
+                        if ((MASK || !VEC) && !(m[u] & (0xFFu << (8 * k)))) { l = 0.f; d = 0.f; }
+                        ls += l;
+                        ds += d;
+                        o[k] = dscale * d;
                     }
+                    if (off) o[0] = o[1] = o[2] = o[3] = 0.f;
                     if (VEC) {
                         __stcs(reinterpret_cast<float4*>(dneg + j), make_float4(o[0], o[1], o[2], o[3]));
                     } else {
@@ -200,13 +200,17 @@ static long long pref_blocks(long long rows, int per) {
     return want < kPrefMaxBlocks ? want : kPrefMaxBlocks;
 }
 
-template <int G, bool VEC, bool SQUARE>
-static int pref_go(const PrefArgs& a, float* loss, cudaStream_t s) {
+template <int G, bool VEC, bool SQUARE, bool MASK>
+static int pref_go2(const PrefArgs& a, float* loss, cudaStream_t s) {
     constexpr int per = G > 256 ? 1 : 256 / G;
     const unsigned blocks = static_cast<unsigned>(pref_blocks(a.rows, per));
-    pref_kernel<G, VEC, SQUARE><<<blocks, G > 256 ? G : 256, 0, s>>>(a);
+    pref_kernel<G, VEC, SQUARE, MASK><<<blocks, G > 256 ? G : 256, 0, s>>>(a);
     KGE_LAUNCH_CHECK("pref_kernel");
     return launch_sum_partials(a.partial, static_cast<int>(blocks), loss, s);
+}
+template <int G, bool VEC, bool SQUARE>
+static int pref_go(const PrefArgs& a, float* loss, cudaStream_t s) {
+    return a.mask ? pref_go2<G, VEC, SQUARE, true>(a, loss, s) : pref_go2<G, VEC, SQUARE, false>(a, loss, s);
 }
 template <bool VEC, bool SQUARE>
 static int pref_pick(const PrefArgs& a, float* loss, cudaStream_t s) {
