@@ -154,6 +154,32 @@ __device__ __forceinline__ float warp_max(float v) {
     for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kFull, v, o));
     return v;
 }
+// exp((f - m) / T) of V scores, two at a time (packed fp32 pairs: half the instructions of the subtraction and the product)
+template <int V>
+__device__ __forceinline__ void cand_exps(float (&f)[V], float m, float c) {
+    const float2 nm = make_float2(-m, -m), c2 = make_float2(c, c);
+#pragma unroll
+    for (int k = 0; k < V; k += 2) {
+        const float2 p = __fmul2_rn(__fadd2_rn(make_float2(f[k], f[k + 1]), nm), c2);
+        f[k] = cand_ex2(p.x); f[k + 1] = cand_ex2(p.y);
+    }
+}
+template <int V>
+__device__ __forceinline__ void cand_scale(float (&f)[V], float by) {
+    const float2 b2 = make_float2(by, by);
+#pragma unroll
+    for (int k = 0; k < V; k += 2) {
+        const float2 p = __fmul2_rn(make_float2(f[k], f[k + 1]), b2);
+        f[k] = p.x; f[k + 1] = p.y;
+    }
+}
+// even and odd elements summed side by side
+template <int V>
+__device__ __forceinline__ void cand_add(float2& sum, const float (&f)[V]) {
+    float2 t = __fadd2_rn(make_float2(f[0], f[1]), make_float2(f[2], f[3]));
+    if (V == 8) t = __fadd2_rn(t, __fadd2_rn(make_float2(f[V - 4], f[V - 3]), make_float2(f[V - 2], f[V - 1])));
+    sum = __fadd2_rn(sum, t);
+}
 __device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY ? 0.f : m; }
 template <typename T>
 __device__ __forceinline__ int head_of(const T* p, int n) {
@@ -244,32 +270,27 @@ struct RowPart {
             const int v = (act - q.head) / V - q.v0;
             if (v >= 0 && v % THREADS == tid && q.v0 + v < q.v1) own = v / THREADS;
         }
-        float rest = 0.f;
         const float e = cand_ex2((xe - mz) * c);
-        if (xi != act) rest = e;
+        float2 sum = make_float2(xi != act ? e : 0.f, 0.f);
         if (kKeepExp) xe = e;
 #pragma unroll
         for (int i = 0; i < I; ++i) {
             if (i >= used) continue;
             float f[V];
             Vec<T>::open(r[i], f);
-#pragma unroll
-            for (int k = 0; k < V; ++k) f[k] = cand_ex2((f[k] - mz) * c);
+            cand_exps<V>(f, mz, c);
             if (kKeepExp) r[i] = Vec<T>::close(f);
             if (i == own) {
 #pragma unroll
                 for (int k = 0; k < V; ++k) if ((act - q.head) % V == k) f[k] = 0.f;
             }
-            float t = 0.f;
-#pragma unroll
-            for (int k = 0; k < V; k += 4) t += (f[k] + f[k + 1]) + (f[k + 2] + f[k + 3]);
-            rest += t;
+            cand_add<V>(sum, f);
         }
         if (!kKeepExp) {          // keep the packed words, not their unpacked values, in registers until the gradient
 #pragma unroll
             for (int i = 0; i < I; ++i) asm volatile("" : "+r"(r[i].x), "+r"(r[i].y), "+r"(r[i].z), "+r"(r[i].w));
         }
-        return warp_sum(rest);
+        return warp_sum(sum.x + sum.y);
     }
     __device__ __forceinline__ void write(T* d, const Slice& q, int n, int cnt, int act, int tid, float c, float m, float rest, float ga) const {
         uint4* dv = reinterpret_cast<uint4*>(d + q.head) + q.v0 + tid;
@@ -284,8 +305,8 @@ struct RowPart {
             if (i * THREADS < left) {
                 float f[V];
                 Vec<T>::open(r[i], f);
-#pragma unroll
-                for (int k = 0; k < V; ++k) f[k] = f0 * (kKeepExp ? f[k] : cand_ex2((f[k] - mall) * c));
+                if (!kKeepExp) cand_exps<V>(f, mall, c);
+                cand_scale<V>(f, f0);
                 if (!plain) {
                     const int at = q.head + (q.v0 + tid + i * THREADS) * V;
 #pragma unroll
@@ -388,7 +409,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) cand_row_kernel(CandArgs a) {
     // this CTA's vector that holds the chosen candidate, and its place in it
     const int av = act >= q.head && act < q.head + q.nv * V ? (act - q.head) / V - q.v0 : -1, ak = (act - q.head) % V;
     float m = xe, rest = 0.f, mz = finite_or_zero(m);
-    if (xi != act) rest = cand_ex2((xe - mz) * c);
+    float2 sum = make_float2(xi != act ? cand_ex2((xe - mz) * c) : 0.f, 0.f);
     __syncthreads();                      // the barrier exists
     if (!umma::mbar_wait(&full, 0)) {     // (the row's outputs are invalid; its copy is waited for once more)
         atomicOr(a.err, KGE_ERR_WAIT_TIMEOUT);
@@ -403,21 +424,20 @@ __global__ void __launch_bounds__(THREADS, CTAS) cand_row_kernel(CandArgs a) {
         const float vm = Vec<T>::max(r);
         if (vm > m) {                     // a new maximum of this thread: rescale what it has (rare after the first vectors)
             mz = finite_or_zero(vm);
-            rest *= cand_ex2((m - mz) * c);
+            const float by = cand_ex2((m - mz) * c);
+            sum = __fmul2_rn(sum, make_float2(by, by));
             m = vm;
         }
         float f[V];
         Vec<T>::open(r, f);
-#pragma unroll
-        for (int k = 0; k < V; ++k) f[k] = cand_ex2((f[k] - mz) * c);
+        cand_exps<V>(f, mz, c);
         if (v == av) {
 #pragma unroll
             for (int k = 0; k < V; ++k) if (k == ak) f[k] = 0.f;
         }
-        float t = (f[0] + f[1]) + (f[2] + f[3]);
-        if (V == 8) t += (f[V - 4] + f[V - 3]) + (f[V - 2] + f[V - 1]);
-        rest += t;
+        cand_add<V>(sum, f);
     }
+    rest = sum.x + sum.y;
     {
         const float mine = m;
         m = warp_max(m);
@@ -440,8 +460,8 @@ __global__ void __launch_bounds__(THREADS, CTAS) cand_row_kernel(CandArgs a) {
             asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(o.x), "=f"(o.y) : "r"(remote) : "memory");
             merge_parts(m, rest, o.x, o.y, c);
         }
-        // the parts have been read: no CTA of the cluster leaves before the others have got here
-        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        // the parts have been read: no CTA of the cluster leaves before the others have got here (nothing is handed over)
+        asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     }
     {
         const float mine = m;
@@ -466,8 +486,8 @@ __global__ void __launch_bounds__(THREADS, CTAS) cand_row_kernel(CandArgs a) {
         for (int v = tid; v < full_to; v += THREADS) {
             float f[V];
             Vec<T>::open(sv[v], f);
-#pragma unroll
-            for (int k = 0; k < V; ++k) f[k] = -ga * cand_ex2((f[k] - mz) * c);
+            cand_exps<V>(f, mz, c);
+            cand_scale<V>(f, -ga);
             if (v == av) {
 #pragma unroll
                 for (int k = 0; k < V; ++k) if (k == ak) f[k] = fa;
@@ -519,6 +539,7 @@ __global__ void __launch_bounds__(256) cand_stats_kernel(CandArgs a, float2* par
                 }
             }
             const int av = la >= head && la < head + nv * V ? (la - head) / V : -1;
+            float2 sum = make_float2(rest, 0.f);
             for (int base = tid; base < nv; base += 4 * 256) {
                 uint4 r[4];
 #pragma unroll
@@ -528,23 +549,24 @@ __global__ void __launch_bounds__(256) cand_stats_kernel(CandArgs a, float2* par
                 }
                 const float bm = fmaxf(fmaxf(Vec<T>::max(r[0]), Vec<T>::max(r[1])), fmaxf(Vec<T>::max(r[2]), Vec<T>::max(r[3])));
                 const float top = fmaxf(m, bm), mz = finite_or_zero(top);
-                if (bm > m) { rest *= cand_ex2((m - mz) * c); m = top; }
+                if (bm > m) {
+                    const float by = cand_ex2((m - mz) * c);
+                    sum = __fmul2_rn(sum, make_float2(by, by));
+                    m = top;
+                }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     float f[V];
                     Vec<T>::open(r[i], f);
-#pragma unroll
-                    for (int q = 0; q < V; ++q) f[q] = cand_ex2((f[q] - mz) * c);
+                    cand_exps<V>(f, mz, c);
                     if (base + i * 256 == av) {
 #pragma unroll
                         for (int q = 0; q < V; ++q) if ((la - head) % V == q) f[q] = 0.f;
                     }
-                    float t = 0.f;
-#pragma unroll
-                    for (int q = 0; q < V; q += 4) t += (f[q] + f[q + 1]) + (f[q + 2] + f[q + 3]);
-                    rest += t;
+                    cand_add<V>(sum, f);
                 }
             }
+            rest = sum.x + sum.y;
         }
 #pragma unroll
         for (int o = 16; o; o >>= 1) {
@@ -641,8 +663,8 @@ __global__ void __launch_bounds__(256) cand_grad_kernel(CandArgs a, const float*
 #pragma unroll
                         for (int k = 0; k < V; ++k) f[k] = one(at + k, f[k]);
                     } else {
-#pragma unroll
-                        for (int k = 0; k < V; ++k) f[k] = -ga * cand_ex2((f[k] - m) * c);
+                        cand_exps<V>(f, m, c);
+                        cand_scale<V>(f, -ga);
                     }
                 }
                 __stcs(dv + v, Vec<T>::close(f));
@@ -773,9 +795,6 @@ static int cand_passes(const CandArgs& a, void* ws, int* n_partial, cudaStream_t
 
 // Which form: the smallest group that holds a row in registers; passes where the rows are too long for a cluster, where the
 // groups of all rows would leave most SMs idle, or where the gradient's alignment differs.
-#ifndef VAR
-#define VAR 0
-#endif
 template <typename T, int MODE>
 static int cand_go(const CandArgs& a, void* ws, int* n_partial, cudaStream_t s) {
     const long long nv = a.n / Vec<T>::V;              // vectors of a row, at most
@@ -789,15 +808,7 @@ static int cand_go(const CandArgs& a, void* ws, int* n_partial, cudaStream_t s) 
     int cluster = 1;
     while (cluster <= kMaxCluster && nv > cluster * static_cast<long long>(kRowSlot)) cluster *= 2;
     if (cluster > kMaxCluster || a.rows * cluster < 32) return cand_passes<T, MODE>(a, ws, n_partial, s);
-#if VAR == 0
     return cand_rows<T, 256, 5, MODE>(a, cluster, (nv + cluster - 1) / cluster, n_partial, s);
-#elif VAR == 1
-    return cand_rows<T, 512, 3, MODE>(a, cluster, (nv + cluster - 1) / cluster, n_partial, s);
-#elif VAR == 2
-    return cand_rows<T, 512, 2, MODE>(a, cluster, (nv + cluster - 1) / cluster, n_partial, s);
-#else
-    return cand_rows<T, 1024, 1, MODE>(a, cluster, (nv + cluster - 1) / cluster, n_partial, s);
-#endif
 }
 
 }  // namespace kge

@@ -31,17 +31,26 @@ __device__ __forceinline__ float pref_rcp(float x) { float r; asm("rcp.approx.ft
 // softplus(-|z|) = log1p(t) = 2 atanh(w), w = t / (2 + t) in [0, 1/3]: atanh(w) / w as a polynomial in w^2 (Chebyshev
 // interpolation of degree 4 on [0, 1/9], 4e-9 relative), so small terms keep their digits at the cost of one reciprocal and six
 // fused multiply-adds: the loss is bound by memory only if a pair stays below some 40 instructions.
+// Two pairs at a time: additions, products and the polynomial run on packed fp32 pairs.
+__device__ __forceinline__ float2 f2(float v) { return make_float2(v, v); }
 template <bool SQUARE>
-__device__ __forceinline__ void pref_pair(const PrefArgs& a, float keep, float z, float& l, float& d) {
-    if (SQUARE) { l = z * z; d = 2.f * z; return; }
-    const float t = pref_ex2(fabsf(z) * -1.4426950408889634f);
-    const float inv = pref_rcp(1.f + t), w = t * pref_rcp(2.f + t), x = w * w;
-    const float q = fmaf(fmaf(fmaf(fmaf(0.14078890f, x, 0.13982579f), x, 0.20012298f), x, 0.33333161f), x, 1.f);
-    const float small = t * inv;                                 // sigmoid(-|z|); inv is sigmoid(|z|)
-    const bool up = z >= 0.f;
-    d = fmaf(up ? a.smooth : -keep, inv, (up ? -keep : a.smooth) * small);
-    l = fmaf(w + w, q, keep * fmaxf(-z, 0.f));
-    if (a.smooth > 0.f) l = fmaf(a.smooth, fmaxf(z, 0.f), l);    // (0 x inf without the test)
+__device__ __forceinline__ void pref_pairs(const PrefArgs& a, float keep, float2 z, float2& l, float2& d) {
+    if (SQUARE) { l = __fmul2_rn(z, z); d = __fadd2_rn(z, z); return; }
+    const float2 t = make_float2(pref_ex2(fabsf(z.x) * -1.4426950408889634f), pref_ex2(fabsf(z.y) * -1.4426950408889634f));
+    const float2 t1 = __fadd2_rn(t, f2(1.f)), t2 = __fadd2_rn(t, f2(2.f));
+    const float2 inv = make_float2(pref_rcp(t1.x), pref_rcp(t1.y));                        // sigmoid(|z|)
+    const float2 w = __fmul2_rn(t, make_float2(pref_rcp(t2.x), pref_rcp(t2.y))), x = __fmul2_rn(w, w);
+    float2 q = __ffma2_rn(f2(2.f * 0.14078890f), x, f2(2.f * 0.13982579f));
+    q = __ffma2_rn(q, x, f2(2.f * 0.20012298f));
+    q = __ffma2_rn(q, x, f2(2.f * 0.33333161f));
+    q = __ffma2_rn(q, x, f2(2.f));
+    const float2 small = __fmul2_rn(t, inv);                                               // sigmoid(-|z|)
+    const bool ux = z.x >= 0.f, uy = z.y >= 0.f;
+    const float2 hi = make_float2(ux ? a.smooth : -keep, uy ? a.smooth : -keep), lo = make_float2(ux ? -keep : a.smooth, uy ? -keep : a.smooth);
+    d = __ffma2_rn(hi, inv, __fmul2_rn(lo, small));
+    l = __ffma2_rn(f2(keep), make_float2(fmaxf(-z.x, 0.f), fmaxf(-z.y, 0.f)), __fmul2_rn(w, q));
+    if (a.smooth > 0.f)                                                                    // (0 x inf without the test)
+        l = __ffma2_rn(f2(a.smooth), make_float2(fmaxf(z.x, 0.f), fmaxf(z.y, 0.f)), l);
 }
 
 // bytes of w that are not zero: the low seven bits carry into the eighth, or it is set already
@@ -112,7 +121,7 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) pref_kernel(PrefArgs a) {
         const float cw = cnt > 0 ? a.scale * weight / static_cast<float>(cnt) : 0.f;
         const float dscale = -cw * a.beta, keep = 1.f - a.smooth;
         const bool off = cw == 0.f;                    // nothing valid, or weight 0: zeros, whatever the scores hold
-        float ls = 0.f, ds = 0.f;
+        float2 ls = f2(0.f), ds = f2(0.f);
         for (int j0 = gl * W; j0 < n; j0 += G * W * U) {
             float x[U][W], y[U][W];
             uint32_t m[U];
@@ -147,13 +156,18 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) pref_kernel(PrefArgs a) {
                 if (j < n) {
                     float o[W];
 #pragma unroll
-                    for (int k = 0; k < W; ++k) {
-                        float l, d;
-                        pref_pair<SQUARE>(a, keep, fmaf(a.beta, base - (x[u][k] - y[u][k]), -a.margin), l, d);
-                        if ((MASK || !VEC) && !(m[u] & (0xFFu << (8 * k)))) { l = 0.f; d = 0.f; }
-                        ls += l;
-                        ds += d;
-                        o[k] = dscale * d;
+                    for (int k = 0; k < W; k += 2) {
+                        float2 l, d;
+                        const float2 gap = __ffma2_rn(make_float2(x[u][k], x[u][k + 1]), f2(-1.f), make_float2(y[u][k], y[u][k + 1]));
+                        pref_pairs<SQUARE>(a, keep, __ffma2_rn(f2(a.beta), __fadd2_rn(f2(base), gap), f2(-a.margin)), l, d);
+                        if (MASK || !VEC) {
+                            if (!(m[u] & (0xFFu << (8 * k)))) { l.x = 0.f; d.x = 0.f; }
+                            if (!(m[u] & (0xFFu << (8 * k + 8)))) { l.y = 0.f; d.y = 0.f; }
+                        }
+                        ls = __fadd2_rn(ls, l);
+                        ds = __fadd2_rn(ds, d);
+                        const float2 g = __fmul2_rn(f2(dscale), d);
+                        o[k] = g.x; o[k + 1] = g.y;
                     }
                     if (off) o[0] = o[1] = o[2] = o[3] = 0.f;
                     if (VEC) {
@@ -165,16 +179,16 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) pref_kernel(PrefArgs a) {
                 }
             }
         }
-        ls = pref_group_sum<G>(ls); ds = pref_group_sum<G>(ds);
+        float lsum = pref_group_sum<G>(ls.x + ls.y), dsum = pref_group_sum<G>(ds.x + ds.y);
         if (G > 32) {
-            if (lane == 0) { rl[warp] = ls; rd[warp] = ds; }
+            if (lane == 0) { rl[warp] = lsum; rd[warp] = dsum; }
             __syncthreads();
             if (threadIdx.x == 0)
-                for (int w = 1; w < G / 32; ++w) { ls += rl[w]; ds += rd[w]; }
+                for (int w = 1; w < G / 32; ++w) { lsum += rl[w]; dsum += rd[w]; }
         }
         if (gl == 0 && live) {
-            a.dpos[row] = cw != 0.f ? -dscale * ds : 0.f;
-            if (cw != 0.f) total += static_cast<double>(cw) * ls;
+            a.dpos[row] = cw != 0.f ? -dscale * dsum : 0.f;
+            if (cw != 0.f) total += static_cast<double>(cw) * lsum;
         }
         if (G > 32) __syncthreads();               // rc, rl, rd are free for the next row
     }
