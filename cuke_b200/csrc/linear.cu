@@ -33,7 +33,7 @@ struct LinEpilogue {
     __half* slope;                                // (M, N) packed, or NULL
     float* part;                                  // LE_PARTIAL: (splits, M, N)
     int act;
-    int wide, wide_slope;                         // rows of out / slope start on 32-byte boundaries
+    int wide, wide_slope, wide_res;               // rows of out / slope / res start on 32-byte boundaries
 };
 struct LinGemm {
     int m, n;                                     // output rows and columns
@@ -46,25 +46,45 @@ struct LinGemm {
 // ---- elementwise pieces -------------------------------------------------------------------------------------------
 __device__ __forceinline__ float lin_ex2(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
 __device__ __forceinline__ float lin_rcp(float x) { float r; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
-// 1 / (1 + exp(-x)): exp overflows to +inf for very negative x and the reciprocal is then 0
-__device__ __forceinline__ float lin_sigmoid(float x) { return lin_rcp(1.f + lin_ex2(-1.4426950408889634f * x)); }
+__device__ __forceinline__ float lin_max(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ float lin_min(float a, float b) { float r; asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ float2 f2(float v) { return make_float2(v, v); }
+// 1 / (1 + 2^x): 2^x overflows to +inf for large x and the reciprocal is then 0
+__device__ __forceinline__ float2 lin_sigmoid2(float2 x) {
+    const float2 d = __fadd2_rn(make_float2(lin_ex2(x.x), lin_ex2(x.y)), f2(1.f));
+    return make_float2(lin_rcp(d.x), lin_rcp(d.y));
+}
 
-// (act(z), act'(z)); gelu is the tanh form, 0.5 z (1 + tanh u) = z sigmoid(2 u), u = sqrt(2 / pi) (z + 0.044715 z^3)
-template <int ACT>
-__device__ __forceinline__ float2 lin_act(float z) {
-    if (ACT == ACT_NONE) return make_float2(z, 1.f);
-    if (ACT == ACT_RELU) return make_float2(z > 0.f ? z : (z != z ? z : 0.f), z > 0.f ? 1.f : 0.f);
-    // s rounds to 0 or 1 far from the origin: z s and s (1 - s) are then taken as the limits they have, so that neither an
-    // infinite z nor the polynomial's overflow turns into NaN (a NaN z stays one)
-    if (ACT == ACT_SILU) {
-        const float s = lin_sigmoid(z), y = s == 0.f ? 0.f : z * s, om = 1.f - s;
-        return make_float2(y, om > 0.f ? fmaf(y, om, s) : s);
+// act(z) and, with SLOPE, act'(z) of two values: the epilogue has 13 instructions a value for the tensor core not to wait for it
+// (K = 1024), so additions and products are packed fp32 pairs.  gelu is the tanh form, 0.5 z (1 + tanh u) = z s(2 u),
+// u = sqrt(2 / pi) (z + 0.044715 z^3).  Far from the origin s rounds to 0 or 1; clamping z there (below at -3e4 for all, above at
+// 3e4 for the slope alone) keeps 0 x infinity out of the products and leaves every result as it is; NaN goes through.
+template <int ACT, bool SLOPE>
+__device__ __forceinline__ float2 lin_act(float2 z, float2& slope) {
+    if (ACT == ACT_NONE) { if (SLOPE) slope = f2(1.f); return z; }
+    if (ACT == ACT_RELU) {
+        if (SLOPE) slope = make_float2(z.x > 0.f ? 1.f : 0.f, z.y > 0.f ? 1.f : 0.f);
+        return make_float2(lin_max(z.x, 0.f), lin_max(z.y, 0.f));
     }
-    const float c = 1.5957691216057308f;          // 2 sqrt(2 / pi)
-    const float z2 = z * z;
-    const float s = lin_sigmoid(c * z * fmaf(0.044715f, z2, 1.f));
-    const float y = s == 0.f ? 0.f : z * s, om = 1.f - s;
-    return make_float2(y, om > 0.f && s != 0.f ? fmaf(y * om, c * fmaf(3.f * 0.044715f, z2, 1.f), s) : s);
+    const float lim = 3e4f;
+    z = make_float2(lin_max(z.x, -lim), lin_max(z.y, -lim));
+    if (ACT == ACT_SILU) {
+        const float2 s = lin_sigmoid2(__fmul2_rn(z, f2(-1.4426950408889634f)));
+        if (SLOPE) {
+            const float2 zc = make_float2(lin_min(z.x, lim), lin_min(z.y, lim));
+            slope = __ffma2_rn(__fmul2_rn(zc, s), __ffma2_rn(s, f2(-1.f), f2(1.f)), s);
+        }
+        return __fmul2_rn(z, s);
+    }
+    const float c = 1.5957691216057308f, l = -1.4426950408889634f * c;          // 2 sqrt(2 / pi), and times -log2 e
+    const float2 zc = make_float2(lin_min(z.x, lim), lin_min(z.y, lim));
+    const float2 z2 = __fmul2_rn(zc, zc);
+    const float2 s = lin_sigmoid2(__fmul2_rn(zc, __ffma2_rn(z2, f2(0.044715f * l), f2(l))));
+    if (SLOPE) {
+        const float2 t = __fmul2_rn(__fmul2_rn(zc, s), __ffma2_rn(s, f2(-1.f), f2(1.f)));
+        slope = __ffma2_rn(t, __ffma2_rn(z2, f2(3.f * 0.044715f * c), f2(c)), s);
+    }
+    return __fmul2_rn(z, s);
 }
 __device__ __forceinline__ uint32_t lin_bf2(float a, float b) {
     __nv_bfloat162 p = __floats2bfloat162_rn(a, b);
@@ -90,43 +110,55 @@ __device__ __forceinline__ void lin_store16(void* p, const uint32_t (&w)[16], in
         if (8 * i < lim) q[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
 }
 
-template <int ACT>
-__device__ __forceinline__ void lin_apply(float (&v)[32], const uint32_t (&bias)[16], const uint32_t (&res)[16], uint32_t (&slope)[16]) {
+// 32 bytes, 32-byte aligned
+__device__ __forceinline__ void lin_ld8(uint32_t* w, const void* p) {
+    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7]) : "l"(p) : "memory");
+}
+
+template <int ACT, bool SLOPE>
+__device__ __forceinline__ void lin_apply(float (&v)[32], const uint32_t (&bias)[16], const uint32_t (&res)[16], uint32_t (&out)[16], uint32_t (&slope)[16]) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-        const float2 a = lin_act<ACT>(v[2 * i] + lin_lo(bias[i])), b = lin_act<ACT>(v[2 * i + 1] + lin_hi(bias[i]));
-        v[2 * i] = a.x + lin_lo(res[i]);
-        v[2 * i + 1] = b.x + lin_hi(res[i]);
-        slope[i] = lin_h2(a.y, b.y);
+        float2 g;
+        const float2 z = __fadd2_rn(make_float2(v[2 * i], v[2 * i + 1]), make_float2(lin_lo(bias[i]), lin_hi(bias[i])));
+        const float2 y = __fadd2_rn(lin_act<ACT, SLOPE>(z, g), make_float2(lin_lo(res[i]), lin_hi(res[i])));
+        out[i] = lin_bf2(y.x, y.y);
+        if (SLOPE) slope[i] = lin_h2(g.x, g.y);
+    }
+}
+template <bool SLOPE>
+__device__ __forceinline__ void lin_apply(int act, float (&v)[32], const uint32_t (&bias)[16], const uint32_t (&res)[16], uint32_t (&out)[16],
+                                          uint32_t (&slope)[16]) {
+    switch (act) {
+        case ACT_NONE: lin_apply<ACT_NONE, SLOPE>(v, bias, res, out, slope); break;
+        case ACT_RELU: lin_apply<ACT_RELU, SLOPE>(v, bias, res, out, slope); break;
+        case ACT_SILU: lin_apply<ACT_SILU, SLOPE>(v, bias, res, out, slope); break;
+        default: lin_apply<ACT_GELU, SLOPE>(v, bias, res, out, slope); break;
     }
 }
 
 // 32 consecutive columns of one output row: fp32 sums in v -> bias, activation, residual -> bf16 row and fp16 slope
 __device__ __forceinline__ void lin_finish(const LinEpilogue& e, float (&v)[32], const uint32_t (&res)[16], long long row, int col, int lim, int n) {
-    uint32_t bias[16], slope[16];
+    uint32_t bias[16], w[16], slope[16];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         uint4 b = make_uint4(0u, 0u, 0u, 0u);
         if (e.bias && 8 * i < lim) b = __ldg(reinterpret_cast<const uint4*>(e.bias + col) + i);
         bias[4 * i] = b.x; bias[4 * i + 1] = b.y; bias[4 * i + 2] = b.z; bias[4 * i + 3] = b.w;
     }
-    switch (e.act) {
-        case ACT_NONE: lin_apply<ACT_NONE>(v, bias, res, slope); break;
-        case ACT_RELU: lin_apply<ACT_RELU>(v, bias, res, slope); break;
-        case ACT_SILU: lin_apply<ACT_SILU>(v, bias, res, slope); break;
-        default: lin_apply<ACT_GELU>(v, bias, res, slope); break;
-    }
-    uint32_t w[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) w[i] = lin_bf2(v[2 * i], v[2 * i + 1]);
+    if (e.slope) lin_apply<true>(e.act, v, bias, res, w, slope);
+    else lin_apply<false>(e.act, v, bias, res, w, slope);
     lin_store16(e.out + row * e.ldo + col, w, lim, e.wide);
     if (e.slope) lin_store16(e.slope + row * n + col, slope, lim, e.wide_slope);
 }
 __device__ __forceinline__ void lin_residual(const LinEpilogue& e, uint32_t (&res)[16], long long row, int col, int lim) {
+    const __nv_bfloat16* p = e.res + row * e.ldr + col;
+    if (e.res && e.wide_res && lim == 32) { lin_ld8(res, p); lin_ld8(res + 8, p + 16); return; }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         uint4 r = make_uint4(0u, 0u, 0u, 0u);
-        if (e.res && 8 * i < lim) r = *(reinterpret_cast<const uint4*>(e.res + row * e.ldr + col) + i);
+        if (e.res && 8 * i < lim) r = *(reinterpret_cast<const uint4*>(p) + i);
         res[4 * i] = r.x; res[4 * i + 1] = r.y; res[4 * i + 2] = r.z; res[4 * i + 3] = r.w;
     }
 }
@@ -323,16 +355,16 @@ __global__ void __launch_bounds__(256) linear_join_kernel(LinEpilogue e, long lo
             uint32_t sl[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                float2 lo, hi;
-                const float z0 = v[2 * k] + lin_lo(bw[k]), z1 = v[2 * k + 1] + lin_hi(bw[k]);
+                float2 g, y;
+                const float2 z = make_float2(v[2 * k] + lin_lo(bw[k]), v[2 * k + 1] + lin_hi(bw[k]));
                 switch (e.act) {
-                    case ACT_NONE: lo = lin_act<ACT_NONE>(z0); hi = lin_act<ACT_NONE>(z1); break;
-                    case ACT_RELU: lo = lin_act<ACT_RELU>(z0); hi = lin_act<ACT_RELU>(z1); break;
-                    case ACT_SILU: lo = lin_act<ACT_SILU>(z0); hi = lin_act<ACT_SILU>(z1); break;
-                    default: lo = lin_act<ACT_GELU>(z0); hi = lin_act<ACT_GELU>(z1); break;
+                    case ACT_NONE: y = lin_act<ACT_NONE, true>(z, g); break;
+                    case ACT_RELU: y = lin_act<ACT_RELU, true>(z, g); break;
+                    case ACT_SILU: y = lin_act<ACT_SILU, true>(z, g); break;
+                    default: y = lin_act<ACT_GELU, true>(z, g); break;
                 }
-                v[2 * k] = lo.x + lin_lo(rw[k]); v[2 * k + 1] = hi.x + lin_hi(rw[k]);
-                sl[k] = lin_h2(lo.y, hi.y);
+                v[2 * k] = y.x + lin_lo(rw[k]); v[2 * k + 1] = y.y + lin_hi(rw[k]);
+                sl[k] = lin_h2(g.x, g.y);
             }
             if (e.slope) *reinterpret_cast<uint4*>(e.slope + row * n + col) = make_uint4(sl[0], sl[1], sl[2], sl[3]);
         }
@@ -459,6 +491,7 @@ static int lin_gemm(const void* a, long long lda, int a_mn, const void* b, long 
     if (p.splits > 1 && (!part || part_bytes < sizeof(float) * static_cast<size_t>(p.splits) * m * n)) p.splits = 1;
     e.wide = (e.ldo & 15) == 0 && (reinterpret_cast<uintptr_t>(e.out) & 31) == 0;
     e.wide_slope = (n & 15) == 0 && (reinterpret_cast<uintptr_t>(e.slope) & 31) == 0;
+    e.wide_res = (e.ldr & 15) == 0 && (reinterpret_cast<uintptr_t>(e.res) & 31) == 0;
     e.part = part;
     p.e = e;
     p.err = device_error_word();
