@@ -22,8 +22,11 @@ constexpr int LG_BM = 128;                        // rows of a tile per CTA (a p
 constexpr int LG_BK = 64;                         // contraction per stage: one 128-byte swizzle row of bf16
 constexpr int LG_A_BYTES = LG_BM * LG_BK * 2;
 constexpr int LG_SLAB = LG_BK * 128;              // MN-major slab: 64 k-rows x 128 bytes
-constexpr int LG_THREADS = 320;                   // warp 0: TMA, warp 1: MMA and tensor memory, warps 2..9: epilogue
-constexpr int LG_EPI_WARPS = 8;
+// warp 0: TMA, warp 1: MMA and tensor memory, warps 2..17: epilogue.  An epilogue is a chain of latencies (residual, tensor
+// memory, bias, two special functions a value, stores): with eight warps on 32-column chunks it took 12.7 us a tile against 6 us
+// of products (65536 x 1024 x 1024 with gelu, residual and slope).  Sixteen warps on 16-column chunks fit the registers.
+constexpr int LG_EPI_WARPS = 16;
+constexpr int LG_THREADS = 64 + 32 * LG_EPI_WARPS;
 constexpr int LG_MAX_SMEM = 227 * 1024;
 constexpr int LG_ACC_COLS = 256;
 
@@ -101,13 +104,12 @@ __device__ __forceinline__ void lin_st8(void* p, const uint32_t* w) {      // 32
     asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
                  :: "l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
 }
-// 16 packed words (32 16-bit elements) of one row, `lim` of them valid (a multiple of 8 elements)
-__device__ __forceinline__ void lin_store16(void* p, const uint32_t (&w)[16], int lim, bool wide) {
+// 8 packed words (16 16-bit elements) of one row, `lim` of them valid (8 or 16 elements)
+__device__ __forceinline__ void lin_store(void* p, const uint32_t (&w)[8], int lim, bool wide) {
     uint4* q = static_cast<uint4*>(p);
-    if (wide && lim == 32) { lin_st8(p, w); lin_st8(q + 2, w + 8); return; }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (8 * i < lim) q[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+    if (wide && lim == 16) { lin_st8(p, w); return; }
+    q[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    if (lim > 8) q[1] = make_uint4(w[4], w[5], w[6], w[7]);
 }
 
 // 32 bytes, 32-byte aligned
@@ -117,9 +119,9 @@ __device__ __forceinline__ void lin_ld8(uint32_t* w, const void* p) {
 }
 
 template <int ACT, bool SLOPE>
-__device__ __forceinline__ void lin_apply(float (&v)[32], const uint32_t (&bias)[16], const uint32_t (&res)[16], uint32_t (&out)[16], uint32_t (&slope)[16]) {
+__device__ __forceinline__ void lin_apply(const float (&v)[16], const uint32_t (&bias)[8], const uint32_t (&res)[8], uint32_t (&out)[8], uint32_t (&slope)[8]) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < 8; ++i) {
         float2 g;
         const float2 z = __fadd2_rn(make_float2(v[2 * i], v[2 * i + 1]), make_float2(lin_lo(bias[i]), lin_hi(bias[i])));
         const float2 y = __fadd2_rn(lin_act<ACT, SLOPE>(z, g), make_float2(lin_lo(res[i]), lin_hi(res[i])));
@@ -128,8 +130,8 @@ __device__ __forceinline__ void lin_apply(float (&v)[32], const uint32_t (&bias)
     }
 }
 template <bool SLOPE>
-__device__ __forceinline__ void lin_apply(int act, float (&v)[32], const uint32_t (&bias)[16], const uint32_t (&res)[16], uint32_t (&out)[16],
-                                          uint32_t (&slope)[16]) {
+__device__ __forceinline__ void lin_apply(int act, const float (&v)[16], const uint32_t (&bias)[8], const uint32_t (&res)[8], uint32_t (&out)[8],
+                                          uint32_t (&slope)[8]) {
     switch (act) {
         case ACT_NONE: lin_apply<ACT_NONE, SLOPE>(v, bias, res, out, slope); break;
         case ACT_RELU: lin_apply<ACT_RELU, SLOPE>(v, bias, res, out, slope); break;
@@ -137,30 +139,45 @@ __device__ __forceinline__ void lin_apply(int act, float (&v)[32], const uint32_
         default: lin_apply<ACT_GELU, SLOPE>(v, bias, res, out, slope); break;
     }
 }
-
-// 32 consecutive columns of one output row: fp32 sums in v -> bias, activation, residual -> bf16 row and fp16 slope
-__device__ __forceinline__ void lin_finish(const LinEpilogue& e, float (&v)[32], const uint32_t (&res)[16], long long row, int col, int lim, int n) {
-    uint32_t bias[16], w[16], slope[16];
+// 16 consecutive bf16 values, `lim` of them (8, 16; or none) existing
+__device__ __forceinline__ void lin_load(uint32_t (&w)[8], const __nv_bfloat16* p, int lim, bool wide) {
+    if (wide && lim == 16) { lin_ld8(w, p); return; }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 2; ++i) {
+        uint4 r = make_uint4(0u, 0u, 0u, 0u);
+        if (8 * i < lim) r = *(reinterpret_cast<const uint4*>(p) + i);
+        w[4 * i] = r.x; w[4 * i + 1] = r.y; w[4 * i + 2] = r.z; w[4 * i + 3] = r.w;
+    }
+}
+// 16 consecutive columns of one output row: fp32 sums in v -> bias, activation, residual -> bf16 row and fp16 slope
+__device__ __forceinline__ void lin_finish(const LinEpilogue& e, const float (&v)[16], const uint32_t (&res)[8], long long row, int col, int lim, int n) {
+    uint32_t bias[8], w[8], slope[8];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
         uint4 b = make_uint4(0u, 0u, 0u, 0u);
         if (e.bias && 8 * i < lim) b = __ldg(reinterpret_cast<const uint4*>(e.bias + col) + i);
         bias[4 * i] = b.x; bias[4 * i + 1] = b.y; bias[4 * i + 2] = b.z; bias[4 * i + 3] = b.w;
     }
-    if (e.slope) lin_apply<true>(e.act, v, bias, res, w, slope);
-    else lin_apply<false>(e.act, v, bias, res, w, slope);
-    lin_store16(e.out + row * e.ldo + col, w, lim, e.wide);
-    if (e.slope) lin_store16(e.slope + row * n + col, slope, lim, e.wide_slope);
-}
-__device__ __forceinline__ void lin_residual(const LinEpilogue& e, uint32_t (&res)[16], long long row, int col, int lim) {
-    const __nv_bfloat16* p = e.res + row * e.ldr + col;
-    if (e.res && e.wide_res && lim == 32) { lin_ld8(res, p); lin_ld8(res + 8, p + 16); return; }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        uint4 r = make_uint4(0u, 0u, 0u, 0u);
-        if (e.res && 8 * i < lim) r = *(reinterpret_cast<const uint4*>(p) + i);
-        res[4 * i] = r.x; res[4 * i + 1] = r.y; res[4 * i + 2] = r.z; res[4 * i + 3] = r.w;
+    if (e.slope) {
+        lin_apply<true>(e.act, v, bias, res, w, slope);
+        lin_store(e.slope + row * n + col, slope, lim, e.wide_slope);
+    } else {
+        lin_apply<false>(e.act, v, bias, res, w, slope);
     }
+    lin_store(e.out + row * e.ldo + col, w, lim, e.wide);
+}
+// 32 lanes x 16 consecutive fp32 columns of tensor memory, complete on return
+__device__ __forceinline__ void lin_tmem16(uint32_t taddr, float (&v)[16]) {
+    uint32_t r[16];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr) : "memory");
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 
 // ---- the product ----------------------------------------------------------------------------------------------------
@@ -272,9 +289,9 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
             }
         }
     } else {
-        // thread = row of the tile; the two warps of a lane quarter take alternate 32-column chunks
-        const int q = warp & 3, half = (warp - 2) >> 2;
-        const int chunks = (p.bn + 31) / 32;
+        // thread = row of the tile; the four warps of a lane quarter take 16-column chunks in turn
+        const int q = warp & 3, part = (warp - 2) >> 2;
+        const int chunks = (p.bn + 15) / 16;
         int lt = 0;
         for (int item = pair; item < items; item += n_pairs, ++lt) {
             const int split = item / tiles, tile = item - split * tiles;
@@ -287,39 +304,46 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
             bool ready = false;
             // one vote per wait: the whole warp goes on, or the whole warp gives up
             auto wait_full = [&]() { return __all_sync(kFull, umma::mbar_wait(&acc_full[buf], static_cast<uint32_t>(lt >> 1) & 1)) != 0; };
+            // the residual of the next chunk is requested before this one is worked on
+            auto columns = [&](int c) { return c < chunks && row_ok ? min(16, p.n - (n0 + c * 16)) : 0; };
+            uint32_t next[8];
+            const bool has_res = EPI == LE_FORWARD && p.e.res != nullptr;
+            if (EPI == LE_FORWARD) lin_load(next, p.e.res + row * p.e.ldr + n0 + part * 16, has_res ? columns(part) : 0, p.e.wide_res);
 #pragma unroll 1
-            for (int c = half; c < chunks; c += 2) {
-                const int col = n0 + c * 32;
-                const int lim = min(32, min(p.bn - c * 32, p.n - col));
-                const bool live = row_ok && lim > 0;
-                uint32_t res[16];
-                if (EPI == LE_FORWARD) lin_residual(p.e, res, row, col, live ? lim : 0);
+            for (int c = part; c < chunks; c += 4) {
+                const int col = n0 + c * 16;
+                const int lim = columns(c);
+                uint32_t res[8];
+                if (EPI == LE_FORWARD) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) res[i] = next[i];
+                    lin_load(next, p.e.res + row * p.e.ldr + col + 64, has_res ? columns(c + 4) : 0, p.e.wide_res);
+                }
                 if (!ready) {
                     ready = wait_full();
                     if (!ready) break;
                     umma::tc_fence_after();
                 }
-                float v[32];
+                float v[16];
                 __syncwarp();                     // tensor-memory reads are warp-collective
-                umma::tmem_ld32(taddr + c * 32, v);
-                if (live) {
+                lin_tmem16(taddr + c * 16, v);
+                if (lim > 0) {
                     if (EPI == LE_FORWARD) {
                         lin_finish(p.e, v, res, row, col, lim, p.n);
                     } else if (EPI == LE_STORE) {
-                        uint32_t w[16];
+                        uint32_t w[8];
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) w[i] = lin_bf2(v[2 * i], v[2 * i + 1]);
-                        lin_store16(p.e.out + row * p.e.ldo + col, w, lim, p.e.wide);
+                        for (int i = 0; i < 8; ++i) w[i] = lin_bf2(v[2 * i], v[2 * i + 1]);
+                        lin_store(p.e.out + row * p.e.ldo + col, w, lim, p.e.wide);
                     } else {
                         float* d = p.e.part + (static_cast<long long>(split) * p.m + row) * p.n + col;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (8 * i < lim) lin_st8(d + 8 * i, reinterpret_cast<const uint32_t*>(v) + 8 * i);
+                        lin_st8(d, reinterpret_cast<const uint32_t*>(v));
+                        if (lim > 8) lin_st8(d + 8, reinterpret_cast<const uint32_t*>(v) + 8);
                     }
                 }
                 __syncwarp();
             }
-            if (!ready && (half < chunks || !wait_full())) {      // (a warp without a chunk only keeps step)
+            if (!ready && (part < chunks || !wait_full())) {      // (a warp without a chunk only keeps step)
                 if (lane == 0) atomicOr(p.err, KGE_ERR_WAIT_TIMEOUT);
                 break;
             }
@@ -375,13 +399,15 @@ __global__ void __launch_bounds__(256) linear_join_kernel(LinEpilogue e, long lo
 
 // dz = dout * slope (skipped when slope is NULL: dz is dout itself) and the column sums of dz per block of LZ_ROWS rows.
 // A warp covers 256 columns of a row (8 per lane), the 8 warps of a CTA take rows in turn.
-constexpr int LZ_ROWS = 256;
+constexpr int LZ_ROWS = 64;
 __global__ void __launch_bounds__(256) linear_dz_kernel(const __nv_bfloat16* __restrict__ dout, long long ldd, const __half* __restrict__ slope,
-                                                        __nv_bfloat16* __restrict__ dz, float* __restrict__ colpart, long long m, int n) {
+                                                        __nv_bfloat16* __restrict__ dz, float* __restrict__ colpart, long long m, int n,
+                                                        unsigned strips) {
     __shared__ float red[8][256];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int col = blockIdx.y * 256 + lane * 8;
-    const long long r0 = static_cast<long long>(blockIdx.x) * LZ_ROWS, r1 = min(m, r0 + LZ_ROWS);
+    const long long block = blockIdx.x / strips;                  // strips of 256 columns of the same rows follow one another
+    const int c0 = static_cast<int>(blockIdx.x - block * strips) * 256, col = c0 + lane * 8;
+    const long long r0 = block * LZ_ROWS, r1 = min(m, r0 + LZ_ROWS);
     float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (col < n) {
 #pragma unroll 4
@@ -410,25 +436,27 @@ __global__ void __launch_bounds__(256) linear_dz_kernel(const __nv_bfloat16* __r
 #pragma unroll
     for (int k = 0; k < 8; ++k) red[warp][lane * 8 + k] = sum[k];
     __syncthreads();
-    const int c = blockIdx.y * 256 + threadIdx.x;
+    const int c = c0 + threadIdx.x;
     if (c < n) {
         float t = 0.f;
         for (int w = 0; w < 8; ++w) t += red[w][threadIdx.x];
-        colpart[static_cast<long long>(blockIdx.x) * n + c] = t;
+        colpart[block * n + c] = t;
     }
 }
-// db[c] = sum over row blocks, in fp32 and in a fixed order (8 interleaved partial sums per column)
-__global__ void __launch_bounds__(256) linear_db_kernel(const float* colpart, long long blocks, int n, __nv_bfloat16* db) {
-    __shared__ float red[8][33];
+// db[c] = sum over row blocks, in fp32 and in a fixed order (32 interleaved partial sums per column)
+__global__ void __launch_bounds__(1024) linear_db_kernel(const float* colpart, long long blocks, int n, __nv_bfloat16* db) {
+    __shared__ float red[32][33];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int c = blockIdx.x * 32 + lane;
     float t = 0.f;
-    if (c < n)
-        for (long long b = warp; b < blocks; b += 8) t += colpart[b * n + c];
+    if (c < n) {
+#pragma unroll 8
+        for (long long b = warp; b < blocks; b += 32) t += colpart[b * n + c];
+    }
     red[warp][lane] = t;
     __syncthreads();
     if (warp == 0 && c < n) {
-        for (int w = 1; w < 8; ++w) t += red[w][lane];
+        for (int w = 1; w < 32; ++w) t += red[w][lane];
         db[c] = __float2bfloat16_rn(t);
     }
 }
@@ -620,13 +648,15 @@ int kge_linear_backward(const void* dout, int64_t ldd, const void* x, int64_t ld
     const size_t part_bytes = workspace_bytes - static_cast<size_t>(ws - static_cast<char*>(workspace));
     ldd = pitch_of(ldd, m, n);
     if (dz || dbias) {
-        linear_dz_kernel<<<dim3(static_cast<unsigned>(blocks), static_cast<unsigned>((n + 255) / 256)), 256, 0, s>>>(
+        const long long strips = (n + 255) / 256;
+        if (blocks * strips >= (1LL << 31)) { set_error("%s: m x n too large", fn); return KGE_E_RANGE; }
+        linear_dz_kernel<<<static_cast<unsigned>(blocks * strips), 256, 0, s>>>(
             static_cast<const __nv_bfloat16*>(dout), ldd, dz ? static_cast<const __half*>(slope) : nullptr, dz, dbias ? colpart : nullptr, m,
-            static_cast<int>(n));
+            static_cast<int>(n), static_cast<unsigned>(strips));
         KGE_LAUNCH_CHECK("linear_dz_kernel");
     }
     if (dbias) {
-        linear_db_kernel<<<static_cast<unsigned>((n + 31) / 32), 256, 0, s>>>(colpart, blocks, static_cast<int>(n), static_cast<__nv_bfloat16*>(dbias));
+        linear_db_kernel<<<static_cast<unsigned>((n + 31) / 32), 1024, 0, s>>>(colpart, blocks, static_cast<int>(n), static_cast<__nv_bfloat16*>(dbias));
         KGE_LAUNCH_CHECK("linear_db_kernel");
     }
     const void* g = dz ? static_cast<const void*>(dz) : dout;
