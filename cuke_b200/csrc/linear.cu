@@ -29,6 +29,13 @@ constexpr int LG_EPI_WARPS = 16;
 constexpr int LG_THREADS = 64 + 32 * LG_EPI_WARPS;
 constexpr int LG_MAX_SMEM = 227 * 1024;
 constexpr int LG_ACC_COLS = 256;
+// An epilogue warp works on blocks of 32 rows x 32 columns, staged in shared memory as 64-byte rows: a residual block arrives by
+// a tiled load, the finished block and its slope leave by tiled stores.  (Thread-per-row accesses to global memory touch 32 cache
+// lines an instruction: with them residual and slope cost 50 us of 172.)  Two residual / output blocks and one slope block a warp.
+constexpr int LG_BLOCK = 32 * 64;
+constexpr int LG_WARP_STAGE = 3 * LG_BLOCK;
+constexpr int LG_STAGING = LG_EPI_WARPS * LG_WARP_STAGE;
+constexpr int LG_TAIL = 512;                      // barriers and the tensor-memory slot
 
 struct LinEpilogue {
     const __nv_bfloat16* bias; const __nv_bfloat16* res; long long ldr;
@@ -36,7 +43,6 @@ struct LinEpilogue {
     __half* slope;                                // (M, N) packed, or NULL
     float* part;                                  // LE_PARTIAL: (splits, M, N)
     int act;
-    int wide, wide_slope, wide_res;               // rows of out / slope / res start on 32-byte boundaries
 };
 struct LinGemm {
     int m, n;                                     // output rows and columns
@@ -104,20 +110,6 @@ __device__ __forceinline__ void lin_st8(void* p, const uint32_t* w) {      // 32
     asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
                  :: "l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
 }
-// 8 packed words (16 16-bit elements) of one row, `lim` of them valid (8 or 16 elements)
-__device__ __forceinline__ void lin_store(void* p, const uint32_t (&w)[8], int lim, bool wide) {
-    uint4* q = static_cast<uint4*>(p);
-    if (wide && lim == 16) { lin_st8(p, w); return; }
-    q[0] = make_uint4(w[0], w[1], w[2], w[3]);
-    if (lim > 8) q[1] = make_uint4(w[4], w[5], w[6], w[7]);
-}
-
-// 32 bytes, 32-byte aligned
-__device__ __forceinline__ void lin_ld8(uint32_t* w, const void* p) {
-    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7]) : "l"(p) : "memory");
-}
-
 template <int ACT, bool SLOPE>
 __device__ __forceinline__ void lin_apply(const float (&v)[16], const uint32_t (&bias)[8], const uint32_t (&res)[8], uint32_t (&out)[8], uint32_t (&slope)[8]) {
 #pragma unroll
@@ -139,33 +131,28 @@ __device__ __forceinline__ void lin_apply(int act, const float (&v)[16], const u
         default: lin_apply<ACT_GELU, SLOPE>(v, bias, res, out, slope); break;
     }
 }
-// 16 consecutive bf16 values, `lim` of them (8, 16; or none) existing
-__device__ __forceinline__ void lin_load(uint32_t (&w)[8], const __nv_bfloat16* p, int lim, bool wide) {
-    if (wide && lim == 16) { lin_ld8(w, p); return; }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        uint4 r = make_uint4(0u, 0u, 0u, 0u);
-        if (8 * i < lim) r = *(reinterpret_cast<const uint4*>(p) + i);
-        w[4 * i] = r.x; w[4 * i + 1] = r.y; w[4 * i + 2] = r.z; w[4 * i + 3] = r.w;
-    }
-}
 // 16 consecutive columns of one output row: fp32 sums in v -> bias, activation, residual -> bf16 row and fp16 slope
-__device__ __forceinline__ void lin_finish(const LinEpilogue& e, const float (&v)[16], const uint32_t (&res)[8], long long row, int col, int lim, int n) {
-    uint32_t bias[8], w[8], slope[8];
+__device__ __forceinline__ void lin_finish(const LinEpilogue& e, const float (&v)[16], const uint32_t (&res)[8], int col, int n, uint32_t (&w)[8],
+                                           uint32_t (&slope)[8]) {
+    uint32_t bias[8];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         uint4 b = make_uint4(0u, 0u, 0u, 0u);
-        if (e.bias && 8 * i < lim) b = __ldg(reinterpret_cast<const uint4*>(e.bias + col) + i);
+        if (e.bias && col + 8 * i < n) b = __ldg(reinterpret_cast<const uint4*>(e.bias + col) + i);
         bias[4 * i] = b.x; bias[4 * i + 1] = b.y; bias[4 * i + 2] = b.z; bias[4 * i + 3] = b.w;
     }
-    if (e.slope) {
-        lin_apply<true>(e.act, v, bias, res, w, slope);
-        lin_store(e.slope + row * n + col, slope, lim, e.wide_slope);
-    } else {
-        lin_apply<false>(e.act, v, bias, res, w, slope);
-    }
-    lin_store(e.out + row * e.ldo + col, w, lim, e.wide);
+    if (e.slope) lin_apply<true>(e.act, v, bias, res, w, slope);
+    else lin_apply<false>(e.act, v, bias, res, w, slope);
 }
+// tiled store of a staged block, and its bookkeeping (one thread of a warp issues and waits)
+__device__ __forceinline__ void lin_store_block(const CUtensorMap* map, const void* src, int x, int y) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];"
+                 ::"l"(map), "r"(x), "r"(y), "r"(umma::smem_u32(src)) : "memory");
+}
+__device__ __forceinline__ void lin_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void lin_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }     // the staged bytes have been read
+__device__ __forceinline__ void lin_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
 // 32 lanes x 16 consecutive fp32 columns of tensor memory, complete on return
 __device__ __forceinline__ void lin_tmem16(uint32_t taddr, float (&v)[16]) {
     uint32_t r[16];
@@ -180,12 +167,15 @@ __device__ __forceinline__ void lin_tmem16(uint32_t taddr, float (&v)[16]) {
     for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 
+__device__ __forceinline__ int split_of(int item, int tiles) { return item / tiles; }
+
 // ---- the product ----------------------------------------------------------------------------------------------------
 // Work item = (output tile, share of the contraction); items of the same share run over the column tiles first, so the
 // pairs working at one time read the same rows of A.  Pair p takes items p, p + pairs, ...
 template <int EPI>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LG_THREADS, 1)
-linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, LinGemm p) {
+linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_out,
+                   const __grid_constant__ CUtensorMap map_slope, const __grid_constant__ CUtensorMap map_res, LinGemm p) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     const int half_n = p.bn / 2;                                   // B columns staged by each CTA
@@ -193,11 +183,13 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
     const int b_bytes = p.b_mn ? b_slabs * LG_SLAB : half_n * 128;
     const int b_room = (b_bytes + 1023) & ~1023;                   // swizzle atoms start on 1024-byte boundaries
     const int stage_bytes = LG_A_BYTES + b_room;
-    uint64_t* full = reinterpret_cast<uint64_t*>(smem + p.stages * stage_bytes);
+    uint8_t* staging = smem + p.stages * stage_bytes;
+    uint64_t* full = reinterpret_cast<uint64_t*>(staging + (EPI == LE_PARTIAL ? 0 : LG_STAGING));
     uint64_t* empty = full + p.stages;
     uint64_t* acc_full = empty + p.stages;
     uint64_t* acc_empty = acc_full + 2;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+    uint64_t* res_full = acc_empty + 2;                            // two per epilogue warp: its residual blocks
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(res_full + 2 * LG_EPI_WARPS);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = umma::cluster_ctarank();
@@ -207,6 +199,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
     if (threadIdx.x == 0) {
         for (int s = 0; s < p.stages; ++s) { umma::mbar_init(&full[s], 1); umma::mbar_init(&empty[s], 1); }
         for (int s = 0; s < 2; ++s) { umma::mbar_init(&acc_full[s], 1); umma::mbar_init(&acc_empty[s], 2 * LG_EPI_WARPS); }
+        for (int s = 0; s < 2 * LG_EPI_WARPS; ++s) umma::mbar_init(&res_full[s], 1);
         umma::fence_barrier_init();
     }
     if (warp == 1) { umma::tmem_alloc_pair(tmem_slot, 2 * LG_ACC_COLS); umma::tmem_relinquish_pair(); }
@@ -289,68 +282,124 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
             }
         }
     } else {
-        // thread = row of the tile; the four warps of a lane quarter take 16-column chunks in turn
+        // thread = row of a block; the four warps of a lane quarter take the 32-column blocks of their rows in turn
         const int q = warp & 3, part = (warp - 2) >> 2;
-        const int chunks = (p.bn + 15) / 16;
-        int lt = 0;
+        const int blocks = (p.bn + 31) / 32;
+        uint8_t* mine = staging + (warp - 2) * LG_WARP_STAGE;
+        uint64_t* res_bar = res_full + 2 * (warp - 2);
+        const bool has_res = EPI == LE_FORWARD && p.e.res != nullptr;
+        const uint32_t swz = static_cast<uint32_t>(lane >> 1) & 3u;               // 64-byte swizzle: 16-byte piece c of row `lane` lies at c ^ swz
+        // first row and column of a block; false where nothing of it exists
+        auto place = [&](int item, int blk, int& row, int& col) {
+            const int split = item / tiles, tile = item - split * tiles, tm = tile / p.tiles_n;
+            row = tm * 2 * LG_BM + static_cast<int>(rank) * LG_BM + q * 32;
+            col = (tile - tm * p.tiles_n) * p.bn + blk * 32;
+            return item < items && blk < blocks && row < p.m && col < p.n;
+        };
+        int lt = 0, b = 0;
+        uint32_t res_phase = 0, pending = 0;                                      // bit b: parity of buffer b's next load; a load is under way
+        auto fetch = [&](int item, int blk, int b) {                              // residual block -> buffer b (whole warp calls)
+            int row, col;
+            if (!has_res || !place(item, blk, row, col)) return;
+            pending |= 1u << b;
+            if (lane == 0) {
+                umma::mbar_expect_tx(&res_bar[b], LG_BLOCK);
+                umma::tma_load_2d(mine + b * LG_BLOCK, &map_res, col, row, &res_bar[b]);
+            }
+        };
+        fetch(pair, part, 0);
         for (int item = pair; item < items; item += n_pairs, ++lt) {
-            const int split = item / tiles, tile = item - split * tiles;
-            const int tm = tile / p.tiles_n;
-            const int row = tm * 2 * LG_BM + static_cast<int>(rank) * LG_BM + q * 32 + lane;
-            const int n0 = (tile - tm * p.tiles_n) * p.bn;
             const int buf = lt & 1;
-            const bool row_ok = row < p.m;
             const uint32_t taddr = tmem_base + buf * LG_ACC_COLS + (static_cast<uint32_t>(q * 32) << 16);
             bool ready = false;
             // one vote per wait: the whole warp goes on, or the whole warp gives up
             auto wait_full = [&]() { return __all_sync(kFull, umma::mbar_wait(&acc_full[buf], static_cast<uint32_t>(lt >> 1) & 1)) != 0; };
-            // the residual of the next chunk is requested before this one is worked on
-            auto columns = [&](int c) { return c < chunks && row_ok ? min(16, p.n - (n0 + c * 16)) : 0; };
-            uint32_t next[8];
-            const bool has_res = EPI == LE_FORWARD && p.e.res != nullptr;
-            if (EPI == LE_FORWARD) lin_load(next, p.e.res + row * p.e.ldr + n0 + part * 16, has_res ? columns(part) : 0, p.e.wide_res);
+            auto drained = [&]() {                                                // this warp is done with the accumulator
+                umma::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) umma::mbar_arrive_cluster(umma::map_to_cta(umma::smem_u32(&acc_empty[buf]), 0));
+            };
+            bool ok = true;
 #pragma unroll 1
-            for (int c = part; c < chunks; c += 4) {
-                const int col = n0 + c * 16;
-                const int lim = columns(c);
-                uint32_t res[8];
-                if (EPI == LE_FORWARD) {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) res[i] = next[i];
-                    lin_load(next, p.e.res + row * p.e.ldr + col + 64, has_res ? columns(c + 4) : 0, p.e.wide_res);
+            for (int blk = part; blk < blocks; blk += 4, b ^= 1) {
+                int row, col;
+                const bool live = place(item, blk, row, col);
+                const bool last = blk + 4 >= blocks;
+                if (EPI != LE_PARTIAL) {
+                    if (lane == 0) lin_wait_read();                               // the other buffer and the slope block are free again
+                    __syncwarp();
+                    fetch(last ? item + n_pairs : item, last ? part : blk + 4, b ^ 1);
+                    if (has_res && live) {
+                        ok = __all_sync(kFull, umma::mbar_wait(&res_bar[b], (res_phase >> b) & 1u)) != 0;
+                        if (!ok) break;
+                        res_phase ^= 1u << b;
+                        pending &= ~(1u << b);
+                    }
                 }
                 if (!ready) {
-                    ready = wait_full();
+                    ready = ok = wait_full();
                     if (!ready) break;
                     umma::tc_fence_after();
                 }
-                float v[16];
-                __syncwarp();                     // tensor-memory reads are warp-collective
-                lin_tmem16(taddr + c * 16, v);
-                if (lim > 0) {
+                uint8_t* rows = mine + b * LG_BLOCK + lane * 64;
+                uint8_t* srow = mine + 2 * LG_BLOCK + lane * 64;
+#pragma unroll 1
+                for (int h = 0; h < 2; ++h) {
+                    float v[16];
+                    __syncwarp();                 // tensor-memory reads are warp-collective
+                    lin_tmem16(taddr + blk * 32 + h * 16, v);
+                    if (last && h == 1) drained();
+                    if (EPI == LE_PARTIAL) {
+                        const int lim = live && row + lane < p.m && blk * 32 + h * 16 < p.bn ? p.n - (col + h * 16) : 0;
+                        float* d = p.e.part + (static_cast<long long>(split_of(item, tiles)) * p.m + row + lane) * p.n + col + h * 16;
+                        if (lim > 0) lin_st8(d, reinterpret_cast<const uint32_t*>(v));
+                        if (lim > 8) lin_st8(d + 8, reinterpret_cast<const uint32_t*>(v) + 8);
+                        continue;
+                    }
+                    uint4* p0 = reinterpret_cast<uint4*>(rows + (((2 * h) ^ swz) << 4));
+                    uint4* p1 = reinterpret_cast<uint4*>(rows + (((2 * h + 1) ^ swz) << 4));
+                    uint32_t w[8];
                     if (EPI == LE_FORWARD) {
-                        lin_finish(p.e, v, res, row, col, lim, p.n);
-                    } else if (EPI == LE_STORE) {
-                        uint32_t w[8];
+                        uint32_t res[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u}, sl[8];
+                        if (has_res && live) {
+                            const uint4 r0 = *p0, r1 = *p1;
+                            res[0] = r0.x; res[1] = r0.y; res[2] = r0.z; res[3] = r0.w; res[4] = r1.x; res[5] = r1.y; res[6] = r1.z; res[7] = r1.w;
+                        }
+                        lin_finish(p.e, v, res, col + h * 16, p.n, w, sl);
+                        if (p.e.slope) {
+                            *reinterpret_cast<uint4*>(srow + (((2 * h) ^ swz) << 4)) = make_uint4(sl[0], sl[1], sl[2], sl[3]);
+                            *reinterpret_cast<uint4*>(srow + (((2 * h + 1) ^ swz) << 4)) = make_uint4(sl[4], sl[5], sl[6], sl[7]);
+                        }
+                    } else {
 #pragma unroll
                         for (int i = 0; i < 8; ++i) w[i] = lin_bf2(v[2 * i], v[2 * i + 1]);
-                        lin_store(p.e.out + row * p.e.ldo + col, w, lim, p.e.wide);
-                    } else {
-                        float* d = p.e.part + (static_cast<long long>(split) * p.m + row) * p.n + col;
-                        lin_st8(d, reinterpret_cast<const uint32_t*>(v));
-                        if (lim > 8) lin_st8(d + 8, reinterpret_cast<const uint32_t*>(v) + 8);
+                    }
+                    *p0 = make_uint4(w[0], w[1], w[2], w[3]);
+                    *p1 = make_uint4(w[4], w[5], w[6], w[7]);
+                }
+                if (EPI != LE_PARTIAL) {
+                    umma::fence_proxy_async();                                    // the staged block is visible to the copy engine
+                    __syncwarp();
+                    if (lane == 0 && live) {                                      // (rows and columns past the end are not written)
+                        lin_store_block(&map_out, mine + b * LG_BLOCK, col, row);
+                        if (EPI == LE_FORWARD && p.e.slope) lin_store_block(&map_slope, mine + 2 * LG_BLOCK, col, row);
+                        lin_commit();
                     }
                 }
                 __syncwarp();
             }
-            if (!ready && (part < chunks || !wait_full())) {      // (a warp without a chunk only keeps step)
+            if (part >= blocks) {                                                 // a warp without a block only keeps step
+                ok = wait_full();
+                drained();
+            }
+            if (!ok) {
                 if (lane == 0) atomicOr(p.err, KGE_ERR_WAIT_TIMEOUT);
                 break;
             }
-            umma::tc_fence_before();
-            __syncwarp();
-            if (lane == 0) umma::mbar_arrive_cluster(umma::map_to_cta(umma::smem_u32(&acc_empty[buf]), 0));
         }
+        for (int i = 0; i < 2; ++i)                                               // only after a wait ran out: copies still under way
+            if ((pending >> i) & 1u) umma::mbar_wait(&res_bar[i], (res_phase >> i) & 1u);
+        if (EPI != LE_PARTIAL && lane == 0) lin_wait_all();
     }
     umma::tc_fence_before();
     __syncthreads();
@@ -470,9 +519,9 @@ static int lin_sms() {
     }
     return sms;
 }
-static int lin_bn(long long n) {          // equal tiles of at most 256 columns, multiples of 16
-    const long long tiles = (n + 255) / 256;
-    return static_cast<int>(((n + tiles - 1) / tiles + 15) / 16 * 16);
+static int lin_bn(long long n) {          // equal tiles of at most 256 columns: whole 32-column blocks, or one tile in units of 16
+    const long long tiles = (n + 255) / 256, unit = tiles > 1 ? 32 : 16;
+    return static_cast<int>(((n + tiles - 1) / tiles + unit - 1) / unit * unit);
 }
 // Shares of the contraction: the count with the least (rounds of work items x stages per item + cost of the join).
 static int lin_splits(long long m, long long n, long long k, int sms) {
@@ -491,7 +540,7 @@ static int lin_splits(long long m, long long n, long long k, int sms) {
 }
 
 template <int EPI>
-static int lin_launch(const CUtensorMap& a, const CUtensorMap& b, const LinGemm& p, unsigned ctas, size_t smem, cudaStream_t s) {
+static int lin_launch(const CUtensorMap (&maps)[5], const LinGemm& p, unsigned ctas, size_t smem, cudaStream_t s) {
     static std::atomic<bool> attr_set[128];          // the shared-memory opt-in is per device and kernel
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return cuda_status(cudaGetLastError(), "cudaGetDevice");
@@ -500,7 +549,7 @@ static int lin_launch(const CUtensorMap& a, const CUtensorMap& b, const LinGemm&
         if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(linear_pair_kernel)");
         if (dev >= 0 && dev < 128) attr_set[dev].store(true, std::memory_order_release);
     }
-    linear_pair_kernel<EPI><<<ctas, LG_THREADS, smem, s>>>(a, b, p);
+    linear_pair_kernel<EPI><<<ctas, LG_THREADS, smem, s>>>(maps[0], maps[1], maps[2], maps[3], maps[4], p);
     KGE_LAUNCH_CHECK("linear_pair_kernel");
     return 0;
 }
@@ -517,15 +566,17 @@ static int lin_gemm(const void* a, long long lda, int a_mn, const void* b, long 
     p.tiles_n = static_cast<int>((n + p.bn - 1) / p.bn);
     p.splits = lin_splits(m, n, k, sms);
     if (p.splits > 1 && (!part || part_bytes < sizeof(float) * static_cast<size_t>(p.splits) * m * n)) p.splits = 1;
-    e.wide = (e.ldo & 15) == 0 && (reinterpret_cast<uintptr_t>(e.out) & 31) == 0;
-    e.wide_slope = (n & 15) == 0 && (reinterpret_cast<uintptr_t>(e.slope) & 31) == 0;
-    e.wide_res = (e.ldr & 15) == 0 && (reinterpret_cast<uintptr_t>(e.res) & 31) == 0;
     e.part = part;
     p.e = e;
     p.err = device_error_word();
     if (!p.err) { set_error("linear: no usable device"); return KGE_E_DEVICE; }
-    CUtensorMap ma, mb;
+    CUtensorMap maps[5];                        // A, B, out, slope, residual (the last three: one that exists stands in for one that does not)
+    CUtensorMap &ma = maps[0], &mb = maps[1];
     int rc;
+    if ((rc = make_tensor_map_64b(&maps[2], e.out, m, n, static_cast<uint64_t>(e.ldo) * 2, 32))) return rc;
+    maps[3] = maps[4] = maps[2];
+    if (e.slope && (rc = make_tensor_map_64b(&maps[3], e.slope, m, n, static_cast<uint64_t>(n) * 2, 32))) return rc;
+    if (e.res && (rc = make_tensor_map_64b(&maps[4], e.res, m, n, static_cast<uint64_t>(e.ldr) * 2, 32))) return rc;
     if (a_mn) rc = make_tensor_map_2d(&ma, a, 2, k, m, lda * 2, LG_BK, 64);
     else rc = make_tensor_map_2d(&ma, a, 2, m, k, lda * 2, LG_BM, LG_BK);
     if (rc) return rc;
@@ -535,14 +586,15 @@ static int lin_gemm(const void* a, long long lda, int a_mn, const void* b, long 
     const int half_n = p.bn / 2;
     const int b_room = ((b_mn ? (half_n + 63) / 64 * LG_SLAB : half_n * 128) + 1023) & ~1023;
     const int stage = LG_A_BYTES + b_room;
-    p.stages = (LG_MAX_SMEM - 1024 - 256) / stage;
+    const int staging = p.splits > 1 ? 0 : LG_STAGING;
+    p.stages = (LG_MAX_SMEM - 1024 - LG_TAIL - staging) / stage;          // 4 at 256 columns; 3 cost 6 %, 5 to 7 gain nothing
     if (p.stages > 8) p.stages = 8;
-    const size_t smem = static_cast<size_t>(p.stages) * stage + 1024 + 256;
+    const size_t smem = static_cast<size_t>(p.stages) * stage + staging + 1024 + LG_TAIL;
     const long long items = static_cast<long long>(p.tiles_m) * p.tiles_n * p.splits;
     if (items >= (1LL << 30)) { set_error("linear: %lld tiles exceed the tile index", items); return KGE_E_RANGE; }
     const unsigned ctas = 2u * static_cast<unsigned>(items < sms / 2 ? items : sms / 2);
-    if (p.splits == 1) return forward ? lin_launch<LE_FORWARD>(ma, mb, p, ctas, smem, s) : lin_launch<LE_STORE>(ma, mb, p, ctas, smem, s);
-    if ((rc = lin_launch<LE_PARTIAL>(ma, mb, p, ctas, smem, s))) return rc;
+    if (p.splits == 1) return forward ? lin_launch<LE_FORWARD>(maps, p, ctas, smem, s) : lin_launch<LE_STORE>(maps, p, ctas, smem, s);
+    if ((rc = lin_launch<LE_PARTIAL>(maps, p, ctas, smem, s))) return rc;
     const long long groups = (m * (n / 8) + 255) / 256;
     const unsigned blocks = static_cast<unsigned>(groups < 148 * 8 ? groups : 148 * 8);
     if (forward) linear_join_kernel<LE_FORWARD><<<blocks, 256, 0, s>>>(e, m, p.n, p.splits);

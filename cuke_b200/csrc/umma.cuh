@@ -236,4 +236,8 @@ int make_tensor_map_3d(CUtensorMap* out, const void* base, int elem_bytes, uint6
 int make_tensor_map_slabs(CUtensorMap* out, const void* base, int elem_bytes, uint64_t batch, uint64_t krows, uint64_t cols_padded,
                           uint64_t row_stride_bytes, uint64_t batch_stride_bytes, uint32_t box_krows, uint32_t box_slabs);
 
+// 2-D map of 16-bit elements with a box of box_rows x 32 columns (64-byte rows, 64-byte swizzle): epilogue blocks that are
+// staged in shared memory and travel by tiled loads and stores; what lies outside reads as zero and is not written.
+int make_tensor_map_64b(CUtensorMap* out, const void* base, uint64_t rows, uint64_t cols, uint64_t row_stride_bytes, uint32_t box_rows);
+
 }  // namespace kge
