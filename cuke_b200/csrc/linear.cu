@@ -167,6 +167,42 @@ __device__ __forceinline__ void lin_tmem16(uint32_t taddr, float (&v)[16]) {
     for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 
+// Arrives on the barrier at `bar` (same offset) of both CTAs of the pair once all MMAs issued so far have completed.
+__device__ __forceinline__ void lin_commit_both(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                 ::"r"(bar), "h"(static_cast<uint16_t>(3)) : "memory");
+}
+// One lane of the (converged) warp.
+__device__ __forceinline__ bool lin_elect() {
+    uint32_t is;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(is));
+    return is != 0;
+}
+// Bounded wait by a whole warp on the barrier at a shared address; false = gave up.
+__device__ __forceinline__ bool lin_wait(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .u32 n;\n\t"
+        "mov.u32 n, %3;\n"
+        "WAIT:\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "@p bra DONE;\n\t"
+        "sub.u32 n, n, 1;\n\t"
+        "setp.eq.u32 p, n, 0;\n\t"
+        "@!p bra WAIT;\n\t"
+        "setp.ne.u32 p, n, n;\n"
+        "DONE:\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok) : "r"(bar), "r"(parity), "n"(1 << 22) : "memory");
+    return __all_sync(kFull, ok != 0) != 0;
+}
+__device__ __forceinline__ void lin_expect_tx(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void lin_tma_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t leader_bar) {
+    asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(0), "r"(leader_bar) : "memory");
+}
 __device__ __forceinline__ int split_of(int item, int tiles) { return item / tiles; }
 
 // ---- the product ----------------------------------------------------------------------------------------------------
@@ -191,7 +227,8 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
     uint64_t* res_full = acc_empty + 2;                            // two per epilogue warp: its residual blocks
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(res_full + 2 * LG_EPI_WARPS);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // (a shuffle makes the warp number uniform for the compiler too: see the producer)
+    const int warp = __shfl_sync(kFull, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const uint32_t rank = umma::cluster_ctarank();
     const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
     const int tiles = p.tiles_m * p.tiles_n, items = tiles * p.splits;
@@ -209,47 +246,57 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
     umma::tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
 
+    const uint32_t smem0 = umma::smem_u32(smem), full0 = umma::smem_u32(full), empty0 = umma::smem_u32(empty);
+    const uint32_t acc_full0 = umma::smem_u32(acc_full), acc_empty0 = umma::smem_u32(acc_empty);
     if (warp == 0) {
-        if (lane == 0) {
-            umma::prefetch_tensormap(&map_a); umma::prefetch_tensormap(&map_b);
-            int s = 0; uint32_t ph = 0;
-            bool ok = true;
-            const uint32_t tx_pair = 2u * (LG_A_BYTES + b_bytes);
-            for (int item = pair; item < items && ok; item += n_pairs) {
-                const int split = item / tiles, tile = item - split * tiles;
-                const int tm = tile / p.tiles_n;
-                const int m0 = tm * 2 * LG_BM + static_cast<int>(rank) * LG_BM;
-                const int nb0 = (tile - tm * p.tiles_n) * p.bn + static_cast<int>(rank) * half_n;
-                const int kb0 = static_cast<int>(static_cast<long long>(p.kb) * split / p.splits);
-                const int kb1 = static_cast<int>(static_cast<long long>(p.kb) * (split + 1) / p.splits);
-                for (int kb = kb0; kb < kb1; ++kb) {
-                    if (!umma::mbar_wait(&empty[s], ph ^ 1)) { atomicOr(p.err, KGE_ERR_WAIT_TIMEOUT); ok = false; break; }
-                    uint8_t* a = smem + s * stage_bytes;
-                    uint8_t* b = a + LG_A_BYTES;
-                    const uint32_t lead = umma::map_to_cta(umma::smem_u32(&full[s]), 0);
-                    if (rank == 0) umma::mbar_expect_tx(&full[s], tx_pair);
+        // TMA producer.  The whole warp runs the loop and one elected lane issues: inside a branch on the lane the compiler has no
+        // uniform registers, every copy and MMA gets its operands through moves, and a stage took its threads 650 cycles where
+        // the MMAs take 512.
+        const bool elected = lin_elect();
+        if (elected) { umma::prefetch_tensormap(&map_a); umma::prefetch_tensormap(&map_b); }
+        const uint32_t lead0 = umma::map_to_cta(full0, 0);          // the leader's `full` barriers count the bytes of both CTAs
+        const uint32_t tx_pair = 2u * (LG_A_BYTES + b_bytes);
+        int s = 0; uint32_t ph = 0;
+        bool ok = true;
+        for (int item = pair; item < items && ok; item += n_pairs) {
+            const int split = item / tiles, tile = item - split * tiles;
+            const int tm = tile / p.tiles_n;
+            const int m0 = tm * 2 * LG_BM + static_cast<int>(rank) * LG_BM;
+            const int nb0 = (tile - tm * p.tiles_n) * p.bn + static_cast<int>(rank) * half_n;
+            const int kb0 = static_cast<int>(static_cast<long long>(p.kb) * split / p.splits);
+            const int kb1 = static_cast<int>(static_cast<long long>(p.kb) * (split + 1) / p.splits);
+            for (int kb = kb0; kb < kb1; ++kb) {
+                ok = lin_wait(empty0 + 8 * s, ph ^ 1);
+                if (!ok) break;
+                if (elected) {
+                    const uint32_t a = smem0 + s * stage_bytes, b = a + LG_A_BYTES, lead = lead0 + 8 * s;
+                    if (rank == 0) lin_expect_tx(full0 + 8 * s, tx_pair);
                     const int k0 = kb * LG_BK;
                     if (!p.a_mn) {
-                        umma::tma_load_3d_pair(a, &map_a, k0, m0, 0, lead);
+                        lin_tma_pair(a, &map_a, k0, m0, lead);
                     } else {
-                        umma::tma_load_3d_pair(a, &map_a, m0, k0, 0, lead);
-                        umma::tma_load_3d_pair(a + LG_SLAB, &map_a, m0 + 64, k0, 0, lead);
+                        lin_tma_pair(a, &map_a, m0, k0, lead);
+                        lin_tma_pair(a + LG_SLAB, &map_a, m0 + 64, k0, lead);
                     }
                     if (!p.b_mn) {
-                        umma::tma_load_3d_pair(b, &map_b, k0, nb0, 0, lead);
+                        lin_tma_pair(b, &map_b, k0, nb0, lead);
                     } else {
-                        for (int sl = 0; sl < b_slabs; ++sl) umma::tma_load_3d_pair(b + sl * LG_SLAB, &map_b, nb0 + 64 * sl, k0, 0, lead);
+                        lin_tma_pair(b, &map_b, nb0, k0, lead);
+                        if (b_slabs > 1) lin_tma_pair(b + LG_SLAB, &map_b, nb0 + 64, k0, lead);
                     }
-                    if (++s == p.stages) { s = 0; ph ^= 1; }
                 }
-            }
-            for (int i = 0; i < p.stages && ok; ++i) {         // every commit aimed at this CTA has landed before it may exit
-                if (!umma::mbar_wait(&empty[s], ph ^ 1)) { atomicOr(p.err, KGE_ERR_WAIT_TIMEOUT); ok = false; }
+                __syncwarp();
                 if (++s == p.stages) { s = 0; ph ^= 1; }
             }
         }
+        for (int i = 0; i < p.stages && ok; ++i) {                  // every commit aimed at this CTA has landed before it may exit
+            ok = lin_wait(empty0 + 8 * s, ph ^ 1);
+            if (++s == p.stages) { s = 0; ph ^= 1; }
+        }
+        if (!ok && lane == 0) atomicOr(p.err, KGE_ERR_WAIT_TIMEOUT);
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
+        if (rank == 0) {
+            const bool elected = lin_elect();
             const uint64_t a_tmpl = p.a_mn ? umma::smem_desc_mn(0, LG_SLAB, 1024u, 2u) : umma::smem_desc_k_sw128(0);
             const uint64_t b_tmpl = p.b_mn ? umma::smem_desc_mn(0, LG_SLAB, 1024u, 2u) : umma::smem_desc_k_sw128(0);
             const uint32_t a_step = (p.a_mn ? 2048u : 32u) >> 4, b_step = (p.b_mn ? 2048u : 32u) >> 4;
@@ -261,25 +308,29 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
                 const int nkb = static_cast<int>(static_cast<long long>(p.kb) * (split + 1) / p.splits) -
                                 static_cast<int>(static_cast<long long>(p.kb) * split / p.splits);
                 const int buf = lt & 1;
-                if (!umma::mbar_wait(&acc_empty[buf], (static_cast<uint32_t>(lt >> 1) & 1) ^ 1)) { atomicOr(p.err, KGE_ERR_WAIT_TIMEOUT); ok = false; break; }
+                ok = lin_wait(acc_empty0 + 8 * buf, (static_cast<uint32_t>(lt >> 1) & 1) ^ 1);
+                if (!ok) break;
                 umma::tc_fence_after();
                 const uint32_t tmem_d = tmem_base + buf * LG_ACC_COLS;
                 for (int kb = 0; kb < nkb; ++kb) {
-                    if (!umma::mbar_wait(&full[s], ph)) { atomicOr(p.err, KGE_ERR_WAIT_TIMEOUT); ok = false; break; }
-                    umma::tc_fence_after();
-                    const uint32_t st = (umma::smem_u32(smem + s * stage_bytes) & 0x3FFFFu) >> 4;
-                    uint64_t da = a_tmpl | st, db = b_tmpl | (st + (LG_A_BYTES >> 4));
-#pragma unroll
-                    for (int k = 0; k < 4; ++k, da += a_step, db += b_step) umma::mma_f16_pair(tmem_d, da, db, idesc, (kb > 0 || k > 0) ? 1u : 0u);
-                    const uint32_t e0 = umma::smem_u32(&empty[s]);
-                    umma::mma_commit_pair(e0);
-                    umma::mma_commit_pair(umma::map_to_cta(e0, 1));
+                    ok = lin_wait(full0 + 8 * s, ph);
+                    if (!ok) break;
+                    const uint32_t st = ((smem0 + s * stage_bytes) & 0x3FFFFu) >> 4;
+                    const uint64_t da = a_tmpl | st, db = b_tmpl | (st + (LG_A_BYTES >> 4));
+                    if (elected) {
+                        umma::mma_f16_pair(tmem_d, da, db, idesc, kb > 0 ? 1u : 0u);
+                        umma::mma_f16_pair(tmem_d, da + a_step, db + b_step, idesc, 1u);
+                        umma::mma_f16_pair(tmem_d, da + 2 * a_step, db + 2 * b_step, idesc, 1u);
+                        umma::mma_f16_pair(tmem_d, da + 3 * a_step, db + 3 * b_step, idesc, 1u);
+                        lin_commit_both(empty0 + 8 * s);
+                    }
+                    __syncwarp();
                     if (++s == p.stages) { s = 0; ph ^= 1; }
                 }
-                const uint32_t f0 = umma::smem_u32(&acc_full[buf]);
-                umma::mma_commit_pair(f0);
-                umma::mma_commit_pair(umma::map_to_cta(f0, 1));
+                if (elected) lin_commit_both(acc_full0 + 8 * buf);
+                __syncwarp();
             }
+            if (!ok && lane == 0) atomicOr(p.err, KGE_ERR_WAIT_TIMEOUT);
         }
     } else {
         // thread = row of a block; the four warps of a lane quarter take the 32-column blocks of their rows in turn
