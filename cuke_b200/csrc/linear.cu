@@ -498,48 +498,55 @@ __global__ void __launch_bounds__(256) linear_join_kernel(LinEpilogue e, long lo
 }
 
 // dz = dout * slope (skipped when slope is NULL: dz is dout itself) and the column sums of dz per block of LZ_ROWS rows.
-// A warp covers 256 columns of a row (8 per lane), the 8 warps of a CTA take rows in turn.
+// A warp has 4 rows of a strip of 256 columns (8 per lane), all requested before the first is used; strips of the same rows
+// follow one another, so whole rows leave and arrive together.
 constexpr int LZ_ROWS = 64;
-__global__ void __launch_bounds__(256) linear_dz_kernel(const __nv_bfloat16* __restrict__ dout, long long ldd, const __half* __restrict__ slope,
+__global__ void __launch_bounds__(512) linear_dz_kernel(const __nv_bfloat16* __restrict__ dout, long long ldd, const __half* __restrict__ slope,
                                                         __nv_bfloat16* __restrict__ dz, float* __restrict__ colpart, long long m, int n,
                                                         unsigned strips) {
-    __shared__ float red[8][256];
+    constexpr int W = 16, R = LZ_ROWS / W;
+    __shared__ __align__(16) float red[W][256];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const long long block = blockIdx.x / strips;                  // strips of 256 columns of the same rows follow one another
+    const long long block = blockIdx.x / strips;
     const int c0 = static_cast<int>(blockIdx.x - block * strips) * 256, col = c0 + lane * 8;
-    const long long r0 = block * LZ_ROWS, r1 = min(m, r0 + LZ_ROWS);
-    float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    const long long r0 = block * LZ_ROWS + warp;
+    float2 sum[4] = {f2(0.f), f2(0.f), f2(0.f), f2(0.f)};
     if (col < n) {
-#pragma unroll 4
-        for (long long r = r0 + warp; r < r1; r += 8) {
-            const uint4 d = __ldcs(reinterpret_cast<const uint4*>(dout + r * ldd + col));
-            const uint32_t dw[4] = {d.x, d.y, d.z, d.w};
-            float v[8];
+        uint4 d[R], g[R];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) { v[2 * k] = lin_lo(dw[k]); v[2 * k + 1] = lin_hi(dw[k]); }
-            if (slope) {
-                const uint4 s = __ldcs(reinterpret_cast<const uint4*>(slope + r * n + col));
-                const uint32_t sw[4] = {s.x, s.y, s.z, s.w};
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&sw[k]));
-                    v[2 * k] *= f.x; v[2 * k + 1] *= f.y;
-                }
-                *reinterpret_cast<uint4*>(dz + r * n + col) =
-                    make_uint4(lin_bf2(v[0], v[1]), lin_bf2(v[2], v[3]), lin_bf2(v[4], v[5]), lin_bf2(v[6], v[7]));
+        for (int i = 0; i < R; ++i) {
+            const long long r = r0 + i * W;
+            d[i] = g[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (r < m) {
+                d[i] = __ldcs(reinterpret_cast<const uint4*>(dout + r * ldd + col));
+                if (slope) g[i] = __ldcs(reinterpret_cast<const uint4*>(slope + r * n + col));
             }
+        }
 #pragma unroll
-            for (int k = 0; k < 8; ++k) sum[k] += v[k];
+        for (int i = 0; i < R; ++i) {
+            const long long r = r0 + i * W;
+            const uint32_t dw[4] = {d[i].x, d[i].y, d[i].z, d[i].w}, gw[4] = {g[i].x, g[i].y, g[i].z, g[i].w};
+            uint32_t o[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                float2 v = make_float2(lin_lo(dw[k]), lin_hi(dw[k]));
+                if (slope) v = __fmul2_rn(v, __half22float2(*reinterpret_cast<const __half2*>(&gw[k])));
+                o[k] = lin_bf2(v.x, v.y);
+                sum[k] = __fadd2_rn(sum[k], v);
+            }
+            if (slope && r < m) *reinterpret_cast<uint4*>(dz + r * n + col) = make_uint4(o[0], o[1], o[2], o[3]);
         }
     }
     if (!colpart) return;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) red[warp][lane * 8 + k] = sum[k];
+    float4* mine = reinterpret_cast<float4*>(&red[warp][lane * 8]);
+    mine[0] = make_float4(sum[0].x, sum[0].y, sum[1].x, sum[1].y);
+    mine[1] = make_float4(sum[2].x, sum[2].y, sum[3].x, sum[3].y);
     __syncthreads();
     const int c = c0 + threadIdx.x;
-    if (c < n) {
+    if (threadIdx.x < 256 && c < n) {
         float t = 0.f;
-        for (int w = 0; w < 8; ++w) t += red[w][threadIdx.x];
+#pragma unroll
+        for (int w = 0; w < W; ++w) t += red[w][threadIdx.x];
         colpart[block * n + c] = t;
     }
 }
@@ -753,7 +760,7 @@ int kge_linear_backward(const void* dout, int64_t ldd, const void* x, int64_t ld
     if (dz || dbias) {
         const long long strips = (n + 255) / 256;
         if (blocks * strips >= (1LL << 31)) { set_error("%s: m x n too large", fn); return KGE_E_RANGE; }
-        linear_dz_kernel<<<static_cast<unsigned>(blocks * strips), 256, 0, s>>>(
+        linear_dz_kernel<<<static_cast<unsigned>(blocks * strips), 512, 0, s>>>(
             static_cast<const __nv_bfloat16*>(dout), ldd, dz ? static_cast<const __half*>(slope) : nullptr, dz, dbias ? colpart : nullptr, m,
             static_cast<int>(n), static_cast<unsigned>(strips));
         KGE_LAUNCH_CHECK("linear_dz_kernel");
