@@ -34,7 +34,8 @@ constexpr int LG_ACC_COLS = 256;
 // lines an instruction: with them residual and slope cost 50 us of 172.)  Two residual / output blocks and one slope block a warp.
 constexpr int LG_BLOCK = 32 * 64;
 constexpr int LG_WARP_STAGE = 3 * LG_BLOCK;
-constexpr int LG_STAGING = LG_EPI_WARPS * LG_WARP_STAGE;
+constexpr int LG_STRIP = 32 * 4;                  // a block's bias in fp32, read by broadcast
+constexpr int LG_STAGING = LG_EPI_WARPS * (LG_WARP_STAGE + LG_STRIP);
 constexpr int LG_TAIL = 512;                      // barriers and the tensor-memory slot
 
 struct LinEpilogue {
@@ -110,44 +111,26 @@ __device__ __forceinline__ void lin_st8(void* p, const uint32_t* w) {      // 32
     asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
                  :: "l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
 }
-template <int ACT, bool SLOPE>
-__device__ __forceinline__ void lin_apply(const float (&v)[16], const uint32_t (&bias)[8], const uint32_t (&res)[8], uint32_t (&out)[8], uint32_t (&slope)[8]) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        float2 g;
-        const float2 z = __fadd2_rn(make_float2(v[2 * i], v[2 * i + 1]), make_float2(lin_lo(bias[i]), lin_hi(bias[i])));
-        const float2 y = __fadd2_rn(lin_act<ACT, SLOPE>(z, g), make_float2(lin_lo(res[i]), lin_hi(res[i])));
-        out[i] = lin_bf2(y.x, y.y);
-        if (SLOPE) slope[i] = lin_h2(g.x, g.y);
-    }
-}
-template <bool SLOPE>
-__device__ __forceinline__ void lin_apply(int act, const float (&v)[16], const uint32_t (&bias)[8], const uint32_t (&res)[8], uint32_t (&out)[8],
-                                          uint32_t (&slope)[8]) {
-    switch (act) {
-        case ACT_NONE: lin_apply<ACT_NONE, SLOPE>(v, bias, res, out, slope); break;
-        case ACT_RELU: lin_apply<ACT_RELU, SLOPE>(v, bias, res, out, slope); break;
-        case ACT_SILU: lin_apply<ACT_SILU, SLOPE>(v, bias, res, out, slope); break;
-        default: lin_apply<ACT_GELU, SLOPE>(v, bias, res, out, slope); break;
-    }
-}
 // 16 consecutive columns of one output row: fp32 sums in v -> bias, activation, residual -> bf16 row and fp16 slope
-__device__ __forceinline__ void lin_finish(const LinEpilogue& e, const float (&v)[16], const uint32_t (&res)[8], int col, int n, uint32_t (&w)[8],
-                                           uint32_t (&slope)[8]) {
-    uint32_t bias[8];
+template <int ACT, bool SLOPE>
+__device__ __forceinline__ void lin_apply(const float (&v)[16], const float4* bias, const uint32_t (&res)[8], uint32_t (&out)[8], uint32_t (&slope)[8]) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        uint4 b = make_uint4(0u, 0u, 0u, 0u);
-        if (e.bias && col + 8 * i < n) b = __ldg(reinterpret_cast<const uint4*>(e.bias + col) + i);
-        bias[4 * i] = b.x; bias[4 * i + 1] = b.y; bias[4 * i + 2] = b.z; bias[4 * i + 3] = b.w;
+    for (int i = 0; i < 8; i += 2) {
+        const float4 b = bias[i / 2];
+        float2 g0, g1;
+        float2 y0 = lin_act<ACT, SLOPE>(__fadd2_rn(make_float2(v[2 * i], v[2 * i + 1]), make_float2(b.x, b.y)), g0);
+        float2 y1 = lin_act<ACT, SLOPE>(__fadd2_rn(make_float2(v[2 * i + 2], v[2 * i + 3]), make_float2(b.z, b.w)), g1);
+        y0 = __fadd2_rn(y0, make_float2(lin_lo(res[i]), lin_hi(res[i])));
+        y1 = __fadd2_rn(y1, make_float2(lin_lo(res[i + 1]), lin_hi(res[i + 1])));
+        out[i] = lin_bf2(y0.x, y0.y);
+        out[i + 1] = lin_bf2(y1.x, y1.y);
+        if (SLOPE) { slope[i] = lin_h2(g0.x, g0.y); slope[i + 1] = lin_h2(g1.x, g1.y); }
     }
-    if (e.slope) lin_apply<true>(e.act, v, bias, res, w, slope);
-    else lin_apply<false>(e.act, v, bias, res, w, slope);
 }
 // tiled store of a staged block, and its bookkeeping (one thread of a warp issues and waits)
-__device__ __forceinline__ void lin_store_block(const CUtensorMap* map, const void* src, int x, int y) {
+__device__ __forceinline__ void lin_store_block(const CUtensorMap* map, uint32_t src, int x, int y) {
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];"
-                 ::"l"(map), "r"(x), "r"(y), "r"(umma::smem_u32(src)) : "memory");
+                 ::"l"(map), "r"(x), "r"(y), "r"(src) : "memory");
 }
 __device__ __forceinline__ void lin_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 __device__ __forceinline__ void lin_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }     // the staged bytes have been read
@@ -196,6 +179,11 @@ __device__ __forceinline__ bool lin_wait(uint32_t bar, uint32_t parity) {
         : "=r"(ok) : "r"(bar), "r"(parity), "n"(1 << 22) : "memory");
     return __all_sync(kFull, ok != 0) != 0;
 }
+// Arrival that hands nothing over but tensor memory, whose reads have completed (wait::ld) and are fenced by the caller: the
+// releasing form waits for the warp's stores and copies too, 2500 cycles in the middle of a tile's epilogue.
+__device__ __forceinline__ void lin_arrive_relaxed(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
 __device__ __forceinline__ void lin_expect_tx(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
@@ -203,17 +191,18 @@ __device__ __forceinline__ void lin_tma_pair(uint32_t dst, const CUtensorMap* ma
     asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
                  ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(0), "r"(leader_bar) : "memory");
 }
-__device__ __forceinline__ int split_of(int item, int tiles) { return item / tiles; }
-
 // ---- the product ----------------------------------------------------------------------------------------------------
 // Work item = (output tile, share of the contraction); items of the same share run over the column tiles first, so the
 // pairs working at one time read the same rows of A.  Pair p takes items p, p + pairs, ...
-template <int EPI>
+template <int EPI, int ACT, bool SLOPE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LG_THREADS, 1)
 linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_out,
                    const __grid_constant__ CUtensorMap map_slope, const __grid_constant__ CUtensorMap map_res, LinGemm p) {
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    extern __shared__ __align__(1024) uint8_t smem[];              // swizzle atoms start on 1024-byte boundaries; no room to round up
+    if ((umma::smem_u32(smem) & 1023u) != 0) {                     // (every thread of both CTAs leaves: the launch reports itself)
+        if (threadIdx.x == 0) atomicOr(p.err, KGE_ERR_WAIT_TIMEOUT);
+        return;
+    }
     const int half_n = p.bn / 2;                                   // B columns staged by each CTA
     const int b_slabs = (half_n + 63) / 64;
     const int b_bytes = p.b_mn ? b_slabs * LG_SLAB : half_n * 128;
@@ -340,48 +329,52 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
         uint64_t* res_bar = res_full + 2 * (warp - 2);
         const bool has_res = EPI == LE_FORWARD && p.e.res != nullptr;
         const uint32_t swz = static_cast<uint32_t>(lane >> 1) & 3u;               // 64-byte swizzle: 16-byte piece c of row `lane` lies at c ^ swz
-        // first row and column of a block; false where nothing of it exists
-        auto place = [&](int item, int blk, int& row, int& col) {
-            const int split = item / tiles, tile = item - split * tiles, tm = tile / p.tiles_n;
-            row = tm * 2 * LG_BM + static_cast<int>(rank) * LG_BM + q * 32;
-            col = (tile - tm * p.tiles_n) * p.bn + blk * 32;
-            return item < items && blk < blocks && row < p.m && col < p.n;
-        };
+        float* strip = reinterpret_cast<float*>(staging + LG_EPI_WARPS * LG_WARP_STAGE) + 32 * (warp - 2);
+        const uint32_t out_addr = umma::smem_u32(mine);
+        // tile coordinates of this item and the next, kept by addition (items of a split product: the tile within its share)
+        const int step_m = n_pairs / p.tiles_n, step_n = n_pairs - step_m * p.tiles_n;
+        int tm = pair / p.tiles_n, tn = pair - tm * p.tiles_n;                    // (in units of tiles over all shares)
+        const int row_in = static_cast<int>(rank) * LG_BM + q * 32;
         int lt = 0, b = 0;
         uint32_t res_phase = 0, pending = 0;                                      // bit b: parity of buffer b's next load; a load is under way
-        auto fetch = [&](int item, int blk, int b) {                              // residual block -> buffer b (whole warp calls)
-            int row, col;
-            if (!has_res || !place(item, blk, row, col)) return;
+        float bias_next = 0.f;
+        // what the block at (row, col) needs from memory: its residual into buffer b, its bias into a register (whole warp calls)
+        auto fetch = [&](bool exists, int row, int col, int b) {
+            if (EPI != LE_FORWARD) return;
+            bias_next = exists && p.e.bias != nullptr && col + lane < p.n ? __bfloat162float(p.e.bias[col + lane]) : 0.f;
+            if (!has_res || !exists || row >= p.m || col >= p.n) return;
             pending |= 1u << b;
             if (lane == 0) {
                 umma::mbar_expect_tx(&res_bar[b], LG_BLOCK);
                 umma::tma_load_2d(mine + b * LG_BLOCK, &map_res, col, row, &res_bar[b]);
             }
+            __syncwarp();
         };
-        fetch(pair, part, 0);
+        fetch(pair < items && part < blocks, tm * 2 * LG_BM + row_in, tn * p.bn + part * 32, 0);
         for (int item = pair; item < items; item += n_pairs, ++lt) {
+            int tm_next = tm + step_m, tn_next = tn + step_n;
+            if (tn_next >= p.tiles_n) { tn_next -= p.tiles_n; ++tm_next; }
+            const int split = EPI == LE_PARTIAL ? item / tiles : 0;
+            const int row = (tm - split * p.tiles_m) * 2 * LG_BM + row_in;
             const int buf = lt & 1;
             const uint32_t taddr = tmem_base + buf * LG_ACC_COLS + (static_cast<uint32_t>(q * 32) << 16);
             bool ready = false;
-            // one vote per wait: the whole warp goes on, or the whole warp gives up
-            auto wait_full = [&]() { return __all_sync(kFull, umma::mbar_wait(&acc_full[buf], static_cast<uint32_t>(lt >> 1) & 1)) != 0; };
+            auto wait_full = [&]() { return lin_wait(acc_full0 + 8 * buf, static_cast<uint32_t>(lt >> 1) & 1); };
             auto drained = [&]() {                                                // this warp is done with the accumulator
                 umma::tc_fence_before();
                 __syncwarp();
-                if (lane == 0) umma::mbar_arrive_cluster(umma::map_to_cta(umma::smem_u32(&acc_empty[buf]), 0));
+                if (lane == 0) lin_arrive_relaxed(umma::map_to_cta(acc_empty0 + 8 * buf, 0));
             };
             bool ok = true;
 #pragma unroll 1
             for (int blk = part; blk < blocks; blk += 4, b ^= 1) {
-                int row, col;
-                const bool live = place(item, blk, row, col);
+                const int col = tn * p.bn + blk * 32;
+                const bool live = row < p.m && col < p.n;                         // something of the block exists
                 const bool last = blk + 4 >= blocks;
-                if (EPI != LE_PARTIAL) {
-                    if (lane == 0) lin_wait_read();                               // the other buffer and the slope block are free again
-                    __syncwarp();
-                    fetch(last ? item + n_pairs : item, last ? part : blk + 4, b ^ 1);
+                if (EPI == LE_FORWARD) {
+                    strip[lane] = bias_next;
                     if (has_res && live) {
-                        ok = __all_sync(kFull, umma::mbar_wait(&res_bar[b], (res_phase >> b) & 1u)) != 0;
+                        ok = lin_wait(umma::smem_u32(&res_bar[b]), (res_phase >> b) & 1u);
                         if (!ok) break;
                         res_phase ^= 1u << b;
                         pending &= ~(1u << b);
@@ -392,19 +385,20 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
                     if (!ready) break;
                     umma::tc_fence_after();
                 }
+                __syncwarp();                     // the strip is written; tensor-memory reads are warp-collective
                 uint8_t* rows = mine + b * LG_BLOCK + lane * 64;
                 uint8_t* srow = mine + 2 * LG_BLOCK + lane * 64;
-#pragma unroll 1
+#pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     float v[16];
-                    __syncwarp();                 // tensor-memory reads are warp-collective
                     lin_tmem16(taddr + blk * 32 + h * 16, v);
                     if (last && h == 1) drained();
                     if (EPI == LE_PARTIAL) {
                         const int lim = live && row + lane < p.m && blk * 32 + h * 16 < p.bn ? p.n - (col + h * 16) : 0;
-                        float* d = p.e.part + (static_cast<long long>(split_of(item, tiles)) * p.m + row + lane) * p.n + col + h * 16;
+                        float* d = p.e.part + (static_cast<long long>(split) * p.m + row + lane) * p.n + col + h * 16;
                         if (lim > 0) lin_st8(d, reinterpret_cast<const uint32_t*>(v));
                         if (lim > 8) lin_st8(d + 8, reinterpret_cast<const uint32_t*>(v) + 8);
+                        __syncwarp();
                         continue;
                     }
                     uint4* p0 = reinterpret_cast<uint4*>(rows + (((2 * h) ^ swz) << 4));
@@ -412,18 +406,28 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
                     uint32_t w[8];
                     if (EPI == LE_FORWARD) {
                         uint32_t res[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u}, sl[8];
-                        if (has_res && live) {
+                        if (has_res) {            // (a block that does not exist reads what lies there and is not stored)
                             const uint4 r0 = *p0, r1 = *p1;
                             res[0] = r0.x; res[1] = r0.y; res[2] = r0.z; res[3] = r0.w; res[4] = r1.x; res[5] = r1.y; res[6] = r1.z; res[7] = r1.w;
                         }
-                        lin_finish(p.e, v, res, col + h * 16, p.n, w, sl);
-                        if (p.e.slope) {
+                        lin_apply<ACT, SLOPE>(v, reinterpret_cast<const float4*>(strip) + 4 * h, res, w, sl);
+                        if (h == 0) {             // the last block's copies have been read by now: its buffers take the next block
+                            if (lane == 0) lin_wait_read();
+                            __syncwarp();
+                            if (last) fetch(item + n_pairs < items, tm_next * 2 * LG_BM + row_in, tn_next * p.bn + part * 32, b ^ 1);
+                            else fetch(true, row, col + 128, b ^ 1);
+                        }
+                        if (SLOPE) {
                             *reinterpret_cast<uint4*>(srow + (((2 * h) ^ swz) << 4)) = make_uint4(sl[0], sl[1], sl[2], sl[3]);
                             *reinterpret_cast<uint4*>(srow + (((2 * h + 1) ^ swz) << 4)) = make_uint4(sl[4], sl[5], sl[6], sl[7]);
                         }
                     } else {
 #pragma unroll
                         for (int i = 0; i < 8; ++i) w[i] = lin_bf2(v[2 * i], v[2 * i + 1]);
+                        if (h == 0) {
+                            if (lane == 0) lin_wait_read();
+                            __syncwarp();
+                        }
                     }
                     *p0 = make_uint4(w[0], w[1], w[2], w[3]);
                     *p1 = make_uint4(w[4], w[5], w[6], w[7]);
@@ -432,8 +436,8 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
                     umma::fence_proxy_async();                                    // the staged block is visible to the copy engine
                     __syncwarp();
                     if (lane == 0 && live) {                                      // (rows and columns past the end are not written)
-                        lin_store_block(&map_out, mine + b * LG_BLOCK, col, row);
-                        if (EPI == LE_FORWARD && p.e.slope) lin_store_block(&map_slope, mine + 2 * LG_BLOCK, col, row);
+                        lin_store_block(&map_out, out_addr + b * LG_BLOCK, col, row);
+                        if (SLOPE) lin_store_block(&map_slope, out_addr + 2 * LG_BLOCK, col, row);
                         lin_commit();
                     }
                 }
@@ -447,6 +451,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
                 if (lane == 0) atomicOr(p.err, KGE_ERR_WAIT_TIMEOUT);
                 break;
             }
+            tm = tm_next; tn = tn_next;
         }
         for (int i = 0; i < 2; ++i)                                               // only after a wait ran out: copies still under way
             if ((pending >> i) & 1u) umma::mbar_wait(&res_bar[i], (res_phase >> i) & 1u);
@@ -597,19 +602,24 @@ static int lin_splits(long long m, long long n, long long k, int sms) {
     return pick;
 }
 
-template <int EPI>
+template <int EPI, int ACT, bool SLOPE>
 static int lin_launch(const CUtensorMap (&maps)[5], const LinGemm& p, unsigned ctas, size_t smem, cudaStream_t s) {
     static std::atomic<bool> attr_set[128];          // the shared-memory opt-in is per device and kernel
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return cuda_status(cudaGetLastError(), "cudaGetDevice");
     if (dev < 0 || dev >= 128 || !attr_set[dev].load(std::memory_order_acquire)) {
-        cudaError_t e = cudaFuncSetAttribute(linear_pair_kernel<EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, LG_MAX_SMEM);
+        cudaError_t e = cudaFuncSetAttribute(linear_pair_kernel<EPI, ACT, SLOPE>, cudaFuncAttributeMaxDynamicSharedMemorySize, LG_MAX_SMEM);
         if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(linear_pair_kernel)");
         if (dev >= 0 && dev < 128) attr_set[dev].store(true, std::memory_order_release);
     }
-    linear_pair_kernel<EPI><<<ctas, LG_THREADS, smem, s>>>(maps[0], maps[1], maps[2], maps[3], maps[4], p);
+    linear_pair_kernel<EPI, ACT, SLOPE><<<ctas, LG_THREADS, smem, s>>>(maps[0], maps[1], maps[2], maps[3], maps[4], p);
     KGE_LAUNCH_CHECK("linear_pair_kernel");
     return 0;
+}
+
+template <int ACT>
+static int lin_launch_forward(const CUtensorMap (&maps)[5], const LinGemm& p, unsigned ctas, size_t smem, cudaStream_t s) {
+    return p.e.slope ? lin_launch<LE_FORWARD, ACT, true>(maps, p, ctas, smem, s) : lin_launch<LE_FORWARD, ACT, false>(maps, p, ctas, smem, s);
 }
 
 // out[m][n] (+ epilogue) = sum_k A[m][k] B[n][k].  a_mn / b_mn: the operand lies as (k rows, m or n columns).
@@ -645,14 +655,22 @@ static int lin_gemm(const void* a, long long lda, int a_mn, const void* b, long 
     const int b_room = ((b_mn ? (half_n + 63) / 64 * LG_SLAB : half_n * 128) + 1023) & ~1023;
     const int stage = LG_A_BYTES + b_room;
     const int staging = p.splits > 1 ? 0 : LG_STAGING;
-    p.stages = (LG_MAX_SMEM - 1024 - LG_TAIL - staging) / stage;          // 4 at 256 columns; 3 cost 6 %, 5 to 7 gain nothing
+    p.stages = (LG_MAX_SMEM - LG_TAIL - staging) / stage;          // 4 at 256 columns; 3 cost 6 %, 5 to 7 gain nothing
     if (p.stages > 8) p.stages = 8;
-    const size_t smem = static_cast<size_t>(p.stages) * stage + staging + 1024 + LG_TAIL;
+    const size_t smem = static_cast<size_t>(p.stages) * stage + staging + LG_TAIL;
     const long long items = static_cast<long long>(p.tiles_m) * p.tiles_n * p.splits;
     if (items >= (1LL << 30)) { set_error("linear: %lld tiles exceed the tile index", items); return KGE_E_RANGE; }
     const unsigned ctas = 2u * static_cast<unsigned>(items < sms / 2 ? items : sms / 2);
-    if (p.splits == 1) return forward ? lin_launch<LE_FORWARD>(maps, p, ctas, smem, s) : lin_launch<LE_STORE>(maps, p, ctas, smem, s);
-    if ((rc = lin_launch<LE_PARTIAL>(maps, p, ctas, smem, s))) return rc;
+    if (p.splits == 1) {
+        if (!forward) return lin_launch<LE_STORE, ACT_NONE, false>(maps, p, ctas, smem, s);
+        switch (e.act) {
+            case ACT_NONE: return lin_launch<LE_FORWARD, ACT_NONE, false>(maps, p, ctas, smem, s);
+            case ACT_RELU: return lin_launch_forward<ACT_RELU>(maps, p, ctas, smem, s);
+            case ACT_SILU: return lin_launch_forward<ACT_SILU>(maps, p, ctas, smem, s);
+            default: return lin_launch_forward<ACT_GELU>(maps, p, ctas, smem, s);
+        }
+    }
+    if ((rc = lin_launch<LE_PARTIAL, ACT_NONE, false>(maps, p, ctas, smem, s))) return rc;
     const long long groups = (m * (n / 8) + 255) / 256;
     const unsigned blocks = static_cast<unsigned>(groups < 148 * 8 ? groups : 148 * 8);
     if (forward) linear_join_kernel<LE_FORWARD><<<blocks, 256, 0, s>>>(e, m, p.n, p.splits);
