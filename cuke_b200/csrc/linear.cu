@@ -33,9 +33,11 @@ constexpr int LG_ACC_COLS = 256;
 // a tiled load, the finished block and its slope leave by tiled stores.  (Thread-per-row accesses to global memory touch 32 cache
 // lines an instruction: with them residual and slope cost 50 us of 172.)  Two residual / output blocks and one slope block a warp.
 constexpr int LG_BLOCK = 32 * 64;
-constexpr int LG_WARP_STAGE = 3 * LG_BLOCK;
 constexpr int LG_STRIP = 32 * 4;                  // a block's bias in fp32, read by broadcast
-constexpr int LG_STAGING = LG_EPI_WARPS * (LG_WARP_STAGE + LG_STRIP);
+__host__ __device__ constexpr int lin_warp_stage(bool slope) { return (slope ? 3 : 2) * LG_BLOCK; }
+__host__ __device__ constexpr int lin_staging(int epi, bool slope) {
+    return epi == LE_PARTIAL ? 0 : LG_EPI_WARPS * (lin_warp_stage(slope) + (epi == LE_FORWARD ? LG_STRIP : 0));
+}
 constexpr int LG_TAIL = 512;                      // barriers and the tensor-memory slot
 
 struct LinEpilogue {
@@ -209,7 +211,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
     const int b_room = (b_bytes + 1023) & ~1023;                   // swizzle atoms start on 1024-byte boundaries
     const int stage_bytes = LG_A_BYTES + b_room;
     uint8_t* staging = smem + p.stages * stage_bytes;
-    uint64_t* full = reinterpret_cast<uint64_t*>(staging + (EPI == LE_PARTIAL ? 0 : LG_STAGING));
+    uint64_t* full = reinterpret_cast<uint64_t*>(staging + lin_staging(EPI, SLOPE));
     uint64_t* empty = full + p.stages;
     uint64_t* acc_full = empty + p.stages;
     uint64_t* acc_empty = acc_full + 2;
@@ -325,11 +327,11 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
         // thread = row of a block; the four warps of a lane quarter take the 32-column blocks of their rows in turn
         const int q = warp & 3, part = (warp - 2) >> 2;
         const int blocks = (p.bn + 31) / 32;
-        uint8_t* mine = staging + (warp - 2) * LG_WARP_STAGE;
+        uint8_t* mine = staging + (warp - 2) * lin_warp_stage(SLOPE);
         uint64_t* res_bar = res_full + 2 * (warp - 2);
         const bool has_res = EPI == LE_FORWARD && p.e.res != nullptr;
         const uint32_t swz = static_cast<uint32_t>(lane >> 1) & 3u;               // 64-byte swizzle: 16-byte piece c of row `lane` lies at c ^ swz
-        float* strip = reinterpret_cast<float*>(staging + LG_EPI_WARPS * LG_WARP_STAGE) + 32 * (warp - 2);
+        float* strip = reinterpret_cast<float*>(staging + LG_EPI_WARPS * lin_warp_stage(SLOPE)) + 32 * (warp - 2);
         const uint32_t out_addr = umma::smem_u32(mine);
         // tile coordinates of this item and the next, kept by addition (items of a split product: the tile within its share)
         const int step_m = n_pairs / p.tiles_n, step_n = n_pairs - step_m * p.tiles_n;
@@ -654,8 +656,8 @@ static int lin_gemm(const void* a, long long lda, int a_mn, const void* b, long 
     const int half_n = p.bn / 2;
     const int b_room = ((b_mn ? (half_n + 63) / 64 * LG_SLAB : half_n * 128) + 1023) & ~1023;
     const int stage = LG_A_BYTES + b_room;
-    const int staging = p.splits > 1 ? 0 : LG_STAGING;
-    p.stages = (LG_MAX_SMEM - LG_TAIL - staging) / stage;          // 4 at 256 columns; 3 cost 6 %, 5 to 7 gain nothing
+    const int staging = lin_staging(p.splits > 1 ? LE_PARTIAL : forward ? LE_FORWARD : LE_STORE, forward && e.slope != nullptr);
+    p.stages = (LG_MAX_SMEM - LG_TAIL - staging) / stage;          // 4 or 5 at 256 columns; 3 cost 6 %
     if (p.stages > 8) p.stages = 8;
     const size_t smem = static_cast<size_t>(p.stages) * stage + staging + LG_TAIL;
     const long long items = static_cast<long long>(p.tiles_m) * p.tiles_n * p.splits;
