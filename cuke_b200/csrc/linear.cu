@@ -504,6 +504,115 @@ __global__ void __launch_bounds__(256) linear_join_kernel(LinEpilogue e, long lo
     }
 }
 
+// ---- few rows ------------------------------------------------------------------------------------------------------------
+// Up to 8 rows (one entity while serving): bound by reading w once, so w streams past fp32 registers instead of filling a
+// 128-row tensor tile.  A CTA has 32 columns (4 lanes of 8 columns, 64-byte pieces of a w row) and a share of K: 8 warps x 8 rows
+// of w at a time.  A cluster's CTAs share the columns and sum up over distributed shared memory in rank order.
+// One row, K = 1024, N = 512: 4.2 us, against 10.3 us for the split tensor product and its join.
+constexpr int LF_ROWS = 8;                        // rows of x, at most
+constexpr int LF_KC = 512;                        // k-values of x staged at a time
+template <int M>
+__global__ void __launch_bounds__(256) linear_few_kernel(const __nv_bfloat16* __restrict__ x, long long ldx, const __nv_bfloat16* __restrict__ w,
+                                                         long long ldw, int m, int k, int n, LinEpilogue e) {
+    __shared__ float xs[M][LF_KC];
+    __shared__ float part[8][M][32];
+    __shared__ float sum[M][32];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    uint32_t rank, csize;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(csize));
+    const int n0 = static_cast<int>(blockIdx.x / csize) * 32, col = n0 + (lane & 3) * 8;
+    const int k_lo = static_cast<int>(static_cast<long long>(k) * rank / csize), k_hi = static_cast<int>(static_cast<long long>(k) * (rank + 1) / csize);
+    float2 acc[M][4];
+#pragma unroll
+    for (int i = 0; i < M; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = f2(0.f);
+    for (int kc = k_lo; kc < k_hi; kc += LF_KC) {
+        const int len = min(LF_KC, k_hi - kc);
+        for (int i = tid; i < M * LF_KC; i += 256) {
+            const int r = i / LF_KC, c = i % LF_KC;
+            if (c < len) xs[r][c] = r < m ? __bfloat162float(x[r * ldx + kc + c]) : 0.f;
+        }
+        __syncthreads();
+        if (col < n) {
+            const int first = warp * 8 + (lane >> 2);
+            for (int c0 = first; c0 < len; c0 += 256) {
+                uint4 v[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    v[u] = make_uint4(0u, 0u, 0u, 0u);
+                    if (c0 + 64 * u < len) v[u] = __ldg(reinterpret_cast<const uint4*>(w + (kc + c0 + 64 * u) * ldw + col));
+                }
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    if (c0 + 64 * u >= len) continue;
+                    const uint32_t ww[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+#pragma unroll
+                    for (int i = 0; i < M; ++i) {
+                        const float2 xi = f2(xs[i][c0 + 64 * u]);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) acc[i][j] = __ffma2_rn(xi, make_float2(lin_lo(ww[j]), lin_hi(ww[j])), acc[i][j]);
+                    }
+                }
+            }
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < M; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) {
+                acc[i][j].x += __shfl_xor_sync(kFull, acc[i][j].x, o);
+                acc[i][j].y += __shfl_xor_sync(kFull, acc[i][j].y, o);
+            }
+            if (lane < 4) {
+                part[warp][i][lane * 8 + 2 * j] = acc[i][j].x;
+                part[warp][i][lane * 8 + 2 * j + 1] = acc[i][j].y;
+            }
+        }
+    __syncthreads();
+    for (int i = tid; i < M * 32; i += 256) {
+        float t = 0.f;
+#pragma unroll
+        for (int v = 0; v < 8; ++v) t += part[v][i / 32][i % 32];
+        sum[i / 32][i % 32] = t;
+    }
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    // pairs of columns, dealt out over the CTAs of the cluster
+    for (int i = static_cast<int>(rank) * 256 + tid; i < M * 16; i += static_cast<int>(csize) * 256) {
+        const int r = i / 16, c = (i % 16) * 2;
+        if (r >= m || n0 + c >= n) continue;
+        float2 z = f2(0.f), g, y;
+        const uint32_t addr = umma::smem_u32(&sum[r][c]);
+        for (uint32_t q = 0; q < csize; ++q) {
+            float2 o;
+            asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(o.x), "=f"(o.y) : "r"(umma::map_to_cta(addr, q)) : "memory");
+            z.x += o.x; z.y += o.y;
+        }
+        if (e.bias) {
+            const uint32_t b = *reinterpret_cast<const uint32_t*>(e.bias + n0 + c);
+            z.x += lin_lo(b); z.y += lin_hi(b);
+        }
+        switch (e.act) {
+            case ACT_NONE: y = lin_act<ACT_NONE, true>(z, g); break;
+            case ACT_RELU: y = lin_act<ACT_RELU, true>(z, g); break;
+            case ACT_SILU: y = lin_act<ACT_SILU, true>(z, g); break;
+            default: y = lin_act<ACT_GELU, true>(z, g); break;
+        }
+        if (e.res) {
+            const uint32_t v = *reinterpret_cast<const uint32_t*>(e.res + r * e.ldr + n0 + c);
+            y.x += lin_lo(v); y.y += lin_hi(v);
+        }
+        *reinterpret_cast<uint32_t*>(e.out + r * e.ldo + n0 + c) = lin_bf2(y.x, y.y);
+        if (e.slope) *reinterpret_cast<uint32_t*>(e.slope + static_cast<long long>(r) * n + n0 + c) = lin_h2(g.x, g.y);
+    }
+    // no CTA leaves while another may still read its sums
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 // dz = dout * slope (skipped when slope is NULL: dz is dout itself) and the column sums of dz per block of LZ_ROWS rows.
 // A warp has 4 rows of a strip of 256 columns (8 per lane), all requested before the first is used; strips of the same rows
 // follow one another, so whole rows leave and arrive together.
@@ -681,6 +790,25 @@ static int lin_gemm(const void* a, long long lda, int a_mn, const void* b, long 
     return 0;
 }
 
+template <int M>
+static int lin_few(const void* x, long long ldx, const void* w, long long ldw, long long m, long long k, long long n, const LinEpilogue& e, cudaStream_t s) {
+    int cluster = 8;
+    while (cluster > 1 && k < cluster * 64) cluster /= 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>((n + 31) / 32 * cluster));
+    cfg.blockDim = dim3(256);
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = cluster; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+    cfg.attrs = at; cfg.numAttrs = 1;
+    cudaError_t err = cudaLaunchKernelEx(&cfg, linear_few_kernel<M>, static_cast<const __nv_bfloat16*>(x), ldx, static_cast<const __nv_bfloat16*>(w), ldw,
+                                         static_cast<int>(m), static_cast<int>(k), static_cast<int>(n), e);
+    if (err != cudaSuccess) return cuda_status(err, "linear_few_kernel");
+    KGE_LAUNCH_CHECK("linear_few_kernel");
+    return 0;
+}
+
 static size_t lin_up(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
 static size_t lin_part_bytes(long long m, long long n, long long k, int sms) {
     const int s = lin_splits(m, n, k, sms);
@@ -722,7 +850,7 @@ extern "C" {
 size_t kge_linear_workspace_bytes(int64_t m, int64_t k, int64_t n, int32_t act, int32_t backward) {
     if (m <= 0 || k <= 0 || n <= 0 || check_linear("kge_linear_workspace_bytes", m, k, n, act)) return 0;
     const int sms = lin_sms();
-    if (!backward) return lin_part_bytes(m, n, k, sms);
+    if (!backward) return m <= LF_ROWS ? 0 : lin_part_bytes(m, n, k, sms);
     const size_t dx = lin_part_bytes(m, k, n, sms), dw = lin_part_bytes(k, n, m, sms);
     return (act != ACT_NONE ? lin_up(2 * static_cast<size_t>(m) * n) : 0) + lin_up(sizeof(float) * ((m + LZ_ROWS - 1) / LZ_ROWS) * n) + (dx > dw ? dx : dw);
 }
@@ -746,6 +874,14 @@ int kge_linear_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, c
     e.out = static_cast<__nv_bfloat16*>(out); e.ldo = pitch_of(ldo, m, n);
     e.slope = act == ACT_NONE ? nullptr : static_cast<__half*>(slope);
     e.act = act;
+    if (m <= LF_ROWS) {
+        cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+        ldx = pitch_of(ldx, m, k); ldw = pitch_of(ldw, k, n);
+        if (m == 1) return lin_few<1>(x, ldx, w, ldw, m, k, n, e, s);
+        if (m == 2) return lin_few<2>(x, ldx, w, ldw, m, k, n, e, s);
+        if (m <= 4) return lin_few<4>(x, ldx, w, ldw, m, k, n, e, s);
+        return lin_few<8>(x, ldx, w, ldw, m, k, n, e, s);
+    }
     return lin_gemm(x, pitch_of(ldx, m, k), 0, w, pitch_of(ldw, k, n), 1, m, n, k, e, true, static_cast<float*>(workspace), workspace_bytes,
                     reinterpret_cast<cudaStream_t>(stream));
 }
