@@ -12,30 +12,40 @@ import torch
 
 from . import _lib
 from ._lib import ACTIVATIONS, DTYPES, check
-from .scoring import _dtype_of, _ptr, _stream
+from .scoring import _ptr, _stream
+
+
+_CODES = {torch.float32: DTYPES["f32"], torch.bfloat16: DTYPES["bf16"]}
 
 
 def need_here(*ts) -> None:
     """The tensors are on the current CUDA device (the library launches on its current stream)."""
+    here = torch.cuda.current_device() if torch.cuda.is_available() else -2
     for t in ts:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise ValueError("expected CUDA tensors")
-        if t.device.index != torch.cuda.current_device():
-            raise ValueError(f"a tensor is on {t.device}, the current device is cuda:{torch.cuda.current_device()}; "
-                             "use torch.cuda.device(...)")
+        if t is not None and t.get_device() != here:
+            if not t.is_cuda:
+                raise ValueError("expected CUDA tensors")
+            raise ValueError(f"a tensor is on {t.device}, the current device is cuda:{here}; use torch.cuda.device(...)")
+
+
+def dtype_code(t: torch.Tensor) -> int:
+    code = _CODES.get(t.dtype)
+    if code is None:
+        raise TypeError(f"expected float32 or bfloat16, got {t.dtype}")
+    return code
 
 
 def pitch(t: torch.Tensor, name: str) -> int:
     """Row pitch in elements of a 2-D tensor whose columns are adjacent."""
-    if t.shape[1] > 1 and t.stride(1) != 1:
+    rows, cols = t.shape
+    by_row, by_col = t.stride()
+    if cols > 1 and by_col != 1:
         raise ValueError(f"{name}: the last dimension must be contiguous")
-    if t.shape[0] <= 1:
-        return max(t.shape[1], 1)
-    if t.stride(0) < t.shape[1]:
-        raise ValueError(f"{name}: rows overlap (stride {t.stride(0)} for {t.shape[1]} columns)")
-    return t.stride(0)
+    if rows <= 1:
+        return cols or 1
+    if by_row < cols:
+        raise ValueError(f"{name}: rows overlap (stride {by_row} for {cols} columns)")
+    return by_row
 
 
 def dropout(x: torch.Tensor, p: float, seed: int, stream_id: int = 0, step: Union[int, torch.Tensor] = 0,
@@ -48,34 +58,38 @@ def dropout(x: torch.Tensor, p: float, seed: int, stream_id: int = 0, step: Unio
     CUDA tensor: it is read when the kernel runs, so a captured graph draws a new mask whenever that tensor is advanced
     between replays.  out may be x or residual itself."""
     need_here(x, residual, out)
-    dt = DTYPES[_dtype_of(x)]
+    dt = dtype_code(x)
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
         raise ValueError("residual must have the shape and dtype of x")
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
     elif out.shape != x.shape or out.dtype != x.dtype:
         raise ValueError("out must have the shape and dtype of x")
     step_dev = None
     if isinstance(step, torch.Tensor):
-        if step.dtype != torch.int64 or step.numel() != 1 or not step.is_cuda:
+        if step.dtype != torch.int64 or step.numel() != 1:
             raise ValueError("step must be an int or a one-element int64 CUDA tensor")
         need_here(step)
-        step_dev, step = step, 0
-    if x.dim() == 2 and x.shape[1] > 0:
+        step_dev, step = step.data_ptr(), 0
+    ldr = 0
+    if x.is_contiguous() and out.is_contiguous() and (residual is None or residual.is_contiguous()):
+        n = x.numel()                                     # one run of elements, whatever the shape
+        rows, dim = (1, n) if n < 1 << 31 else (n, 1)
+        ldx = ldo = dim
+        if residual is not None:
+            ldr = dim
+    else:
+        if x.dim() != 2:
+            raise ValueError("tensors that are not 2-D must be contiguous")
         rows, dim = x.shape
         ldx, ldo = pitch(x, "x"), pitch(out, "out")
-        ldr = 0 if residual is None else pitch(residual, "residual")
-    else:
-        if not (x.is_contiguous() and out.is_contiguous() and (residual is None or residual.is_contiguous())):
-            raise ValueError("tensors that are not 2-D must be contiguous")
-        rows, dim = x.numel(), 1
-        ldx = ldo = 1
-        ldr = 0 if residual is None else 1
-    for other, ld in ((x, ldx), (residual, ldr)):
-        if other is not None and other.data_ptr() == out.data_ptr() and rows > 1 and ld != ldo:
-            raise ValueError("out may be x or residual only with the same row pitch")
-    check(_lib.lib().kge_dropout(_ptr(x), dt, rows, dim, ldx, _ptr(residual), ldr, _ptr(out), ldo, float(p),
-                                 int(seed) & 0xFFFFFFFFFFFFFFFF, int(stream_id) & 0xFFFFFFFF, int(step) & 0x7FFFFFFF, _ptr(step_dev), _stream()))
+        if residual is not None:
+            ldr = pitch(residual, "residual")
+        for other, ld in ((x, ldx), (residual, ldr)):
+            if other is not None and other.data_ptr() == out.data_ptr() and rows > 1 and ld != ldo:
+                raise ValueError("out may be x or residual only with the same row pitch")
+    check(_lib.lib().kge_dropout(x.data_ptr(), dt, rows, dim, ldx, _ptr(residual), ldr, out.data_ptr(), ldo, p, int(seed) & 0xFFFFFFFFFFFFFFFF,
+                                 int(stream_id) & 0xFFFFFFFF, int(step) & 0x7FFFFFFF, step_dev, _stream()))
     return out
 
 
@@ -112,14 +126,15 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None
     if bias is not None and (bias.dtype != torch.bfloat16 or bias.shape != (n,) or not bias.is_contiguous()):
         raise ValueError(f"bias must be a contiguous bfloat16 vector of {n}")
     if out is None:
-        out = torch.empty((m, n), dtype=torch.bfloat16, device=x.device)
-    ldo = _matrix(out, "out", m, n)
+        out, ldo = x.new_empty((m, n)), n
+    else:
+        ldo = _matrix(out, "out", m, n)
     if residual is not None and residual.data_ptr() == out.data_ptr() and ldr != ldo:
         raise ValueError("out may be residual only with the same row pitch")
-    preact = torch.empty((m, n), dtype=torch.float16, device=x.device) if save_preact and code else None
+    preact = x.new_empty((m, n), dtype=torch.float16) if save_preact and code else None
     L = _lib.lib()
     need = L.kge_linear_workspace_bytes(m, k, n, code, 0)
-    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    ws = x.new_empty(need, dtype=torch.uint8) if need else None
     check(L.kge_linear_forward(_ptr(x), ldx, _ptr(w), ldw, _ptr(bias), _ptr(residual), ldr, m, k, n, code, _ptr(out), ldo, _ptr(preact),
                                _ptr(ws), need, _stream()))
     return (out, preact) if save_preact else out
@@ -138,13 +153,12 @@ def linear_backward(dout: torch.Tensor, x: torch.Tensor, w: torch.Tensor, preact
     ldd, ldx, ldw = _matrix(dout, "dout", m, n), _matrix(x, "x", m, k), _matrix(w, "w", k, n)
     if code and (preact is None or preact.dtype != torch.float16 or preact.shape != (m, n) or not preact.is_contiguous()):
         raise ValueError("preact must be what linear(..., save_preact=True) returned")
-    dev = x.device
-    dx = torch.empty((m, k), dtype=torch.bfloat16, device=dev) if need_dx else None
-    dw = torch.empty((k, n), dtype=torch.bfloat16, device=dev) if need_dw else None
-    db = torch.empty(n, dtype=torch.bfloat16, device=dev) if need_dbias else None
+    dx = x.new_empty((m, k)) if need_dx else None
+    dw = x.new_empty((k, n)) if need_dw else None
+    db = x.new_empty(n) if need_dbias else None
     L = _lib.lib()
     need = L.kge_linear_workspace_bytes(m, k, n, code, 1)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    ws = x.new_empty(need, dtype=torch.uint8) if need else None
     check(L.kge_linear_backward(_ptr(dout), ldd, _ptr(x), ldx, _ptr(w), ldw, _ptr(preact) if code else None, m, k, n, code, _ptr(dx), k, _ptr(dw),
                                 _ptr(db), _ptr(ws), need, _stream()))
     return dx, dw, db

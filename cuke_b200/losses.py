@@ -12,9 +12,9 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from ._lib import DTYPES, PREFERENCE_KINDS, check
-from .features import need_here, pitch
-from .scoring import _dtype_of, _id_bits, _ptr, _stream
+from ._lib import PREFERENCE_KINDS, check
+from .features import dtype_code, need_here, pitch
+from .scoring import _id_bits, _ptr, _stream
 
 
 def _floats(t: Optional[torch.Tensor], rows: int, name: str) -> Optional[torch.Tensor]:
@@ -65,11 +65,11 @@ def preference_loss(pos: torch.Tensor, neg: torch.Tensor, ref_pos: Optional[torc
     ref_neg, ldr = flat(ref_neg, "ref_neg", torch.float32)
     mask, ldm = flat(mask, "mask", torch.bool)
     _floats(pos, rows, "pos"), _floats(ref_pos, rows, "ref_pos"), _floats(weight, rows, "weight")
-    loss = torch.empty(1, dtype=torch.float32, device=pos.device)
-    dpos, dneg = torch.empty(pos.shape, dtype=torch.float32, device=pos.device), torch.empty(neg.shape, dtype=torch.float32, device=pos.device)
+    loss = pos.new_empty(1)
+    dpos, dneg = torch.empty_like(pos), torch.empty_like(neg, memory_format=torch.contiguous_format)
     L = _lib.lib()
     need = L.kge_preference_workspace_bytes(rows, n)
-    ws = torch.empty(need, dtype=torch.uint8, device=pos.device)
+    ws = pos.new_empty(need, dtype=torch.uint8)
     check(L.kge_preference_loss(_ptr(pos), _ptr(ref_pos), _ptr(neg), ldn, _ptr(ref_neg), ldr, _ptr(mask), ldm, _ptr(weight), rows, n,
                                 PREFERENCE_KINDS[kind], float(beta), float(margin), float(smoothing), _scale(reduction, rows),
                                 _ptr(loss), _ptr(dpos), _ptr(dneg), max(n, 1), _ptr(ws), need, _stream()))
@@ -85,7 +85,7 @@ def _candidates(scores, action, n_cand):
         raise ValueError("action must hold one id per row of scores")
     if n_cand is not None and (n_cand.dtype != torch.int32 or n_cand.numel() != rows or not n_cand.is_contiguous()):
         raise ValueError("n_cand must be a contiguous int32 tensor with one count per row of scores")
-    return _ptr(scores), DTYPES[_dtype_of(scores)], pitch(scores, "scores"), rows, scores.shape[1], _ptr(n_cand), _ptr(action), _id_bits(action)
+    return _ptr(scores), dtype_code(scores), pitch(scores, "scores"), rows, scores.shape[1], _ptr(n_cand), _ptr(action), _id_bits(action)
 
 
 def log_prob(scores: torch.Tensor, action: torch.Tensor, n_cand: Optional[torch.Tensor] = None,
@@ -96,11 +96,11 @@ def log_prob(scores: torch.Tensor, action: torch.Tensor, n_cand: Optional[torch.
     int32 / int64, -1 where nothing was chosen (logp 0, zero gradient).  stats is what log_prob_backward needs."""
     how = _candidates(scores, action, n_cand)
     rows, n = how[3], how[4]
-    logp = torch.empty(rows, dtype=torch.float32, device=scores.device)
-    stats = torch.empty((rows, 3), dtype=torch.float32, device=scores.device)
+    logp = scores.new_empty(rows, dtype=torch.float32)
+    stats = scores.new_empty((rows, 3), dtype=torch.float32)
     L = _lib.lib()
     need = L.kge_candidates_workspace_bytes(rows, n)
-    ws = torch.empty(need, dtype=torch.uint8, device=scores.device)
+    ws = scores.new_empty(need, dtype=torch.uint8)
     check(L.kge_log_prob(*how, float(temperature), _ptr(logp), _ptr(stats), _ptr(ws), need, _stream()))
     return logp, stats
 
@@ -111,7 +111,7 @@ def log_prob_backward(scores: torch.Tensor, action: torch.Tensor, stats: torch.T
     how = _candidates(scores, action, n_cand)
     need_here(stats, dlogp)
     _floats(stats, 3 * how[3], "stats"), _floats(dlogp, how[3], "dlogp")
-    dscores = torch.empty(scores.shape, dtype=scores.dtype, device=scores.device)
+    dscores = torch.empty_like(scores, memory_format=torch.contiguous_format)
     check(_lib.lib().kge_log_prob_backward(*how, float(temperature), _ptr(stats), _ptr(dlogp), _ptr(dscores), max(how[4], 1), _stream()))
     return dscores
 
@@ -133,13 +133,12 @@ def policy_loss(scores: torch.Tensor, action: torch.Tensor, old_logp: torch.Tens
     _floats(ref_logp, rows, "ref_logp"), _floats(weight, rows, "weight")
     if kl_coef and ref_logp is None:
         raise ValueError("kl_coef needs ref_logp")
-    dev = scores.device
-    loss = torch.empty(1, dtype=torch.float32, device=dev)
-    logp, kl = torch.empty(rows, dtype=torch.float32, device=dev), torch.empty(rows, dtype=torch.float32, device=dev)
-    dscores = torch.empty(scores.shape, dtype=scores.dtype, device=dev)
+    loss = old_logp.new_empty(1)
+    logp, kl = old_logp.new_empty(rows), old_logp.new_empty(rows)
+    dscores = torch.empty_like(scores, memory_format=torch.contiguous_format)
     L = _lib.lib()
     need = L.kge_candidates_workspace_bytes(rows, n)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    ws = old_logp.new_empty(need, dtype=torch.uint8)
     check(L.kge_policy_loss(*how, float(temperature), _ptr(old_logp), _ptr(ref_logp), _ptr(advantage), _ptr(weight), float(clip_low),
                             float(clip_high), float(kl_coef), _scale(reduction, rows), _ptr(loss), _ptr(logp), _ptr(kl), _ptr(dscores),
                             max(n, 1), _ptr(ws), need, _stream()))
