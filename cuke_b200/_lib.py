@@ -101,9 +101,9 @@ SIGNATURES = {
     "kge_preference_loss": (C.c_int, [_vp, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i32, _f32, _f32, _f32, _f32, _vp, _vp,
                                       _vp, _i64, _vp, _sz, _vp]),
     "kge_candidates_workspace_bytes": (_sz, [_i64, _i64]),
-    "kge_log_prob": (C.c_int, [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _i32, _f32, _vp, _vp, _vp, _sz, _vp]),
-    "kge_log_prob_backward": (C.c_int, [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _i32, _f32, _vp, _vp, _vp, _i64, _vp]),
-    "kge_policy_loss": (C.c_int, [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _i32, _f32, _vp, _vp, _vp, _vp, _f32, _f32, _f32, _f32, _vp, _vp,
+    "kge_log_prob": (C.c_int, [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _i32, C.c_double, _vp, _vp, _vp, _sz, _vp]),
+    "kge_log_prob_backward": (C.c_int, [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _i32, C.c_double, _vp, _vp, _vp, _i64, _vp]),
+    "kge_policy_loss": (C.c_int, [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _i32, C.c_double, _vp, _vp, _vp, _vp, _f32, _f32, _f32, _f32, _vp, _vp,
                                   _vp, _vp, _i64, _vp, _sz, _vp]),
     "kge_linear_workspace_bytes": (_sz, [_i64, _i64, _i64, _i32, _i32]),
     "kge_linear_forward": (C.c_int, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _i32, _vp, _i64, _vp, _vp, _sz, _vp]),

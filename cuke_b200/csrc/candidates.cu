@@ -8,6 +8,7 @@
 // The sum is kept as S = e_a + S', S' over the other candidates: 1 - p_a = S' / S and (where a is the maximum)
 // logp = -log1p(S') then keep their digits when the chosen candidate has nearly all the mass.
 // Row statistics are fp32, the loss is summed over rows in 64 bits.
+#include <math.h>
 #include <atomic>
 #include "umma.cuh"
 
@@ -19,7 +20,8 @@ struct CandArgs {
     int n, id64;
     const int* n_cand;               // optional (rows)
     const void* action;              // (rows) int32 / int64, -1: none
-    float inv_temp;
+    double inv_temp;
+    float c_hi, c_lo;                // log2(e) / T as a sum of two floats: one alone, off by 2^-25, would tilt every sum the same way
     float* logp; float* stats;       // (rows), (rows, 3): m, S', 1 / S (0: a row that takes no part)
     const float* dlogp;              // gradient of log_prob
     const float* old_logp; const float* ref_logp; const float* adv; const float* weight;
@@ -75,7 +77,7 @@ __device__ __forceinline__ float cand_side(const CandArgs& a, long long row, int
 template <int MODE>
 __device__ __forceinline__ double cand_finish(const CandArgs& a, long long row, int act, float sa, float m, float rest, bool write,
                                               const RowSide& o, float* ga) {
-    const double x = act >= 0 ? (static_cast<double>(sa) - static_cast<double>(m)) * static_cast<double>(a.inv_temp) : 0.0;
+    const double x = act >= 0 ? (static_cast<double>(sa) - static_cast<double>(m)) * a.inv_temp : 0.0;
     const bool live = act >= 0 && !(sa == -INFINITY && rest == 0.f);
     const double S = static_cast<double>(expf(static_cast<float>(x))) + static_cast<double>(rest);
     const double lp = !live ? 0.0 : x == 0.0 && rest < 0.5f ? -static_cast<double>(log1pf(rest)) : x - cand_log_sum(S);
@@ -103,7 +105,7 @@ __device__ __forceinline__ double cand_finish(const CandArgs& a, long long row, 
     }
     if (write) a.kl[row] = kl;
     if (w == 0.f) return 0.0;                            // (a row of weight 0 may hold NaN)
-    const float g = w * dl * a.inv_temp;
+    const float g = w * dl * static_cast<float>(a.inv_temp);
     if (g != 0.f) *ga = g * inv;
     return static_cast<double>(w) * static_cast<double>(l);
 }
@@ -155,12 +157,15 @@ __device__ __forceinline__ float warp_max(float v) {
     return v;
 }
 // exp((f - m) / T) of V scores, two at a time (packed fp32 pairs: half the instructions of the subtraction and the product)
+struct Scale2 { float hi, lo; };
+__device__ __forceinline__ float cand_exp(float x, Scale2 c) { return cand_ex2(fmaf(x, c.hi, x * c.lo)); }      // exp(x / T)
 template <int V>
-__device__ __forceinline__ void cand_exps(float (&f)[V], float m, float c) {
-    const float2 nm = make_float2(-m, -m), c2 = make_float2(c, c);
+__device__ __forceinline__ void cand_exps(float (&f)[V], float m, Scale2 c) {
+    const float2 nm = make_float2(-m, -m), hi = make_float2(c.hi, c.hi), lo = make_float2(c.lo, c.lo);
 #pragma unroll
     for (int k = 0; k < V; k += 2) {
-        const float2 p = __fmul2_rn(__fadd2_rn(make_float2(f[k], f[k + 1]), nm), c2);
+        const float2 d = __fadd2_rn(make_float2(f[k], f[k + 1]), nm);
+        const float2 p = __ffma2_rn(d, hi, __fmul2_rn(d, lo));
         f[k] = cand_ex2(p.x); f[k + 1] = cand_ex2(p.y);
     }
 }
@@ -196,9 +201,9 @@ __device__ __forceinline__ uint4 mask_past(uint4 r, int first, int cnt) {
     return Vec<T>::close(f);
 }
 // (m, rest) of two disjoint parts of a row
-__device__ __forceinline__ void merge_parts(float& m, float& rest, float m2, float r2, float c) {
+__device__ __forceinline__ void merge_parts(float& m, float& rest, float m2, float r2, Scale2 c) {
     const float top = finite_or_zero(fmaxf(m, m2));
-    rest = rest * cand_ex2((m - top) * c) + r2 * cand_ex2((m2 - top) * c);
+    rest = rest * cand_exp(m - top, c) + r2 * cand_exp(m2 - top, c);
     m = fmaxf(m, m2);
 }
 
@@ -251,7 +256,7 @@ struct RowPart {
             if (i * THREADS < left) r[i] = __ldcs(src + i * THREADS);
         }
     }
-    __device__ __forceinline__ float stats(const Slice& q, int n, int cnt, int act, int tid, float c) {
+    __device__ __forceinline__ float stats(const Slice& q, int n, int cnt, int act, int tid, Scale2 c) {
         const int used = (q.v1 - q.v0 + THREADS - 1) / THREADS;               // registers that hold anything, the same for all
         if (cnt < n) {
 #pragma unroll
@@ -270,7 +275,7 @@ struct RowPart {
             const int v = (act - q.head) / V - q.v0;
             if (v >= 0 && v % THREADS == tid && q.v0 + v < q.v1) own = v / THREADS;
         }
-        const float e = cand_ex2((xe - mz) * c);
+        const float e = cand_exp(xe - mz, c);
         float2 sum = make_float2(xi != act ? e : 0.f, 0.f);
         if (kKeepExp) xe = e;
 #pragma unroll
@@ -292,12 +297,12 @@ struct RowPart {
         }
         return warp_sum(sum.x + sum.y);
     }
-    __device__ __forceinline__ void write(T* d, const Slice& q, int n, int cnt, int act, int tid, float c, float m, float rest, float ga) const {
+    __device__ __forceinline__ void write(T* d, const Slice& q, int n, int cnt, int act, int tid, Scale2 c, float m, float rest, float ga) const {
         uint4* dv = reinterpret_cast<uint4*>(d + q.head) + q.v0 + tid;
         const int left = q.v1 - q.v0 - tid;
         const float mall = finite_or_zero(m);
         // (a warp without a finite score has only zeros to scale: mz = 0 stands for nothing there)
-        const float f0 = ga == 0.f || (kKeepExp && mw == -INFINITY) ? 0.f : kKeepExp ? -ga * cand_ex2((mz - mall) * c) : -ga;
+        const float f0 = ga == 0.f || (kKeepExp && mw == -INFINITY) ? 0.f : kKeepExp ? -ga * cand_exp(mz - mall, c) : -ga;
         const float fa = ga == 0.f ? 0.f : ga * rest;
         const bool plain = cnt == n && ga != 0.f;                 // no padding, and something to write
 #pragma unroll
@@ -318,7 +323,7 @@ struct RowPart {
         if (own >= 0) cand_put(d + act, fa);                      // over the vector just stored by this thread
         if (xi >= 0) {
             float v = 0.f;
-            if (xi < cnt && ga != 0.f) v = xi == act ? fa : f0 * (kKeepExp ? xe : cand_ex2((xe - mall) * c));
+            if (xi < cnt && ga != 0.f) v = xi == act ? fa : f0 * (kKeepExp ? xe : cand_exp(xe - mall, c));
             cand_put(d + xi, v);
         }
     }
@@ -329,7 +334,7 @@ template <typename T, int I, int MODE>
 __global__ void __launch_bounds__(256, 4) cand_warp_kernel(CandArgs a) {
     __shared__ double red[8];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const float c = a.inv_temp * 1.4426950408889634f;
+    const Scale2 c = {a.c_hi, a.c_lo};
     double total = 0.0;
     for (long long row = (long long)blockIdx.x * 8 + warp; row < a.rows; row += (long long)gridDim.x * 8) {
         const T* s = static_cast<const T*>(a.scores) + row * a.ld;
@@ -382,7 +387,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) cand_row_kernel(CandArgs a) {
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(csize));
     const long long row = blockIdx.x / csize;
-    const float c = a.inv_temp * 1.4426950408889634f;
+    const Scale2 c = {a.c_hi, a.c_lo};
     const T* s = static_cast<const T*>(a.scores) + row * a.ld;
     const int cnt = cand_count(a, row);
     const Slice q = cand_slice(s, a.n, rank, csize);
@@ -409,7 +414,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) cand_row_kernel(CandArgs a) {
     // this CTA's vector that holds the chosen candidate, and its place in it
     const int av = act >= q.head && act < q.head + q.nv * V ? (act - q.head) / V - q.v0 : -1, ak = (act - q.head) % V;
     float m = xe, rest = 0.f, mz = finite_or_zero(m);
-    float2 sum = make_float2(xi != act ? cand_ex2((xe - mz) * c) : 0.f, 0.f);
+    float2 sum = make_float2(xi != act ? cand_exp(xe - mz, c) : 0.f, 0.f);
     __syncthreads();                      // the barrier exists
     if (!umma::mbar_wait(&full, 0)) {     // (the row's outputs are invalid; its copy is waited for once more)
         atomicOr(a.err, KGE_ERR_WAIT_TIMEOUT);
@@ -424,7 +429,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) cand_row_kernel(CandArgs a) {
         const float vm = Vec<T>::max(r);
         if (vm > m) {                     // a new maximum of this thread: rescale what it has (rare after the first vectors)
             mz = finite_or_zero(vm);
-            const float by = cand_ex2((m - mz) * c);
+            const float by = cand_exp(m - mz, c);
             sum = __fmul2_rn(sum, make_float2(by, by));
             m = vm;
         }
@@ -441,7 +446,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) cand_row_kernel(CandArgs a) {
     {
         const float mine = m;
         m = warp_max(m);
-        rest = warp_sum(rest * cand_ex2((mine - finite_or_zero(m)) * c));
+        rest = warp_sum(rest * cand_exp(mine - finite_or_zero(m), c));
     }
     if (lane == 0) parts[warp] = make_float2(m, rest);
     if (MODE == CM_POLICY && tid < 4) sides[tid] = side;
@@ -467,7 +472,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) cand_row_kernel(CandArgs a) {
         const float mine = m;
         m = warp_max(m);
         mz = finite_or_zero(m);
-        rest = warp_sum(rest * cand_ex2((mine - mz) * c));
+        rest = warp_sum(rest * cand_exp(mine - mz, c));
     }
     if (tid == 0) {
         float ga = 0.f;
@@ -503,11 +508,11 @@ __global__ void __launch_bounds__(THREADS, CTAS) cand_row_kernel(CandArgs a) {
                 float g[V];
                 Vec<T>::open(sv[v], g);
 #pragma unroll
-                for (int k = 0; k < V; ++k) if (at + k < cnt) f[k] = at + k == act ? fa : -ga * cand_ex2((g[k] - mz) * c);
+                for (int k = 0; k < V; ++k) if (at + k < cnt) f[k] = at + k == act ? fa : -ga * cand_exp(g[k] - mz, c);
             }
             __stcs(dv + v, Vec<T>::close(f));
         }
-        if (xi >= 0) cand_put(d + xi, xi >= cnt || ga == 0.f ? 0.f : xi == act ? fa : -ga * cand_ex2((xe - mz) * c));
+        if (xi >= 0) cand_put(d + xi, xi >= cnt || ga == 0.f ? 0.f : xi == act ? fa : -ga * cand_exp(xe - mz, c));
     }
     if (csize > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -520,7 +525,7 @@ __global__ void __launch_bounds__(256) cand_stats_kernel(CandArgs a, float2* par
     constexpr int V = Vec<T>::V;
     __shared__ float2 red[8];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const float c = a.inv_temp * 1.4426950408889634f;
+    const Scale2 c = {a.c_hi, a.c_lo};
     for (long long u = blockIdx.x; u < a.rows * chunks; u += gridDim.x) {
         const long long row = u / chunks;
         const int k = static_cast<int>(u - row * chunks);
@@ -535,7 +540,7 @@ __global__ void __launch_bounds__(256) cand_stats_kernel(CandArgs a, float2* par
                 const int xi = tid < 8 ? (tid < head ? tid : -1) : (head + nv * V + tid - 8 < n ? head + nv * V + tid - 8 : -1);
                 if (xi >= 0) {
                     m = cand_get(s + xi);
-                    rest = xi == la ? 0.f : cand_ex2((m - finite_or_zero(m)) * c);
+                    rest = xi == la ? 0.f : cand_exp(m - finite_or_zero(m), c);
                 }
             }
             const int av = la >= head && la < head + nv * V ? (la - head) / V : -1;
@@ -550,7 +555,7 @@ __global__ void __launch_bounds__(256) cand_stats_kernel(CandArgs a, float2* par
                 const float bm = fmaxf(fmaxf(Vec<T>::max(r[0]), Vec<T>::max(r[1])), fmaxf(Vec<T>::max(r[2]), Vec<T>::max(r[3])));
                 const float top = fmaxf(m, bm), mz = finite_or_zero(top);
                 if (bm > m) {
-                    const float by = cand_ex2((m - mz) * c);
+                    const float by = cand_exp(m - mz, c);
                     sum = __fmul2_rn(sum, make_float2(by, by));
                     m = top;
                 }
@@ -587,7 +592,7 @@ template <typename T, int MODE>
 __global__ void __launch_bounds__(256) cand_join_kernel(CandArgs a, const float2* parts, int chunks, float* coef) {
     __shared__ double red[8];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const float c = a.inv_temp * 1.4426950408889634f;
+    const Scale2 c = {a.c_hi, a.c_lo};
     double total = 0.0;
     for (long long row = (long long)blockIdx.x * 8 + warp; row < a.rows; row += (long long)gridDim.x * 8) {
         float m = -INFINITY, rest = 0.f;
@@ -626,7 +631,7 @@ template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(256) cand_grad_kernel(CandArgs a, const float* coef, long long pieces) {
     constexpr int V = ALIGNED ? Vec<T>::V : 1;
     const int lane = threadIdx.x & 31;
-    const float c = a.inv_temp * 1.4426950408889634f;
+    const Scale2 c = {a.c_hi, a.c_lo};
     const long long units = a.rows * pieces;
     for (long long u = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); u < units; u += (long long)gridDim.x * 8) {
         const long long row = u / pieces;
@@ -636,9 +641,9 @@ __global__ void __launch_bounds__(256) cand_grad_kernel(CandArgs a, const float*
         const int cnt = cand_count(a, row), act = cand_action(a, row, cnt, false);
         const float m = __ldg(coef + 3 * row), rest = __ldg(coef + 3 * row + 1);
         float ga = __ldg(coef + 3 * row + 2);
-        if (a.dlogp) { const float g = __ldg(a.dlogp + row) * a.inv_temp; ga = g == 0.f || act < 0 ? 0.f : g * ga; }
+        if (a.dlogp) { const float g = __ldg(a.dlogp + row) * static_cast<float>(a.inv_temp); ga = g == 0.f || act < 0 ? 0.f : g * ga; }
         const float fa = ga == 0.f ? 0.f : ga * rest;
-        auto one = [&](int j, float x) { return j >= cnt || ga == 0.f ? 0.f : j == act ? fa : -ga * cand_ex2((x - m) * c); };
+        auto one = [&](int j, float x) { return j >= cnt || ga == 0.f ? 0.f : j == act ? fa : -ga * cand_exp(x - m, c); };
         if constexpr (ALIGNED) {
             const int head = head_of(s, a.n), nv = (a.n - head) / V;
             const uint4* sv = reinterpret_cast<const uint4*>(s + head);
@@ -816,10 +821,10 @@ static int cand_go(const CandArgs& a, void* ws, int* n_partial, cudaStream_t s) 
 using namespace kge;
 
 static int check_candidates(const char* fn, const void* scores, int32_t dtype, int64_t ld, int64_t rows, int64_t n, const int32_t* n_cand,
-                            const void* action, int32_t id_bits, float temperature, CandArgs* a) {
+                            const void* action, int32_t id_bits, double temperature, CandArgs* a) {
     if (dtype != KGE_F32 && dtype != KGE_BF16) { set_error("%s: unknown dtype %d", fn, dtype); return KGE_E_UNSUPPORTED; }
     if (id_bits != 32 && id_bits != 64) { set_error("%s: id_bits must be 32 or 64, got %d", fn, id_bits); return KGE_E_UNSUPPORTED; }
-    if (!(temperature > 0.f) || !(1.f / temperature > 0.f) || isinf(1.f / temperature)) { set_error("%s: temperature %g is not a positive number", fn, temperature); return KGE_E_RANGE; }
+    if (!(temperature >= 1e-30 && temperature <= 1e30)) { set_error("%s: temperature %g outside [1e-30, 1e30]", fn, temperature); return KGE_E_RANGE; }
     if (rows < 0 || n < 0) { set_error("%s: negative size", fn); return KGE_E_SHAPE; }
     if (n > (1LL << 30) || rows > (1LL << 40)) { set_error("%s: more than 2^30 candidates or 2^40 rows", fn); return KGE_E_RANGE; }
     if (n > 0 && rows > (1LL << 46) / n) { set_error("%s: more than 2^46 scores", fn); return KGE_E_RANGE; }
@@ -831,7 +836,11 @@ static int check_candidates(const char* fn, const void* scores, int32_t dtype, i
     if ((reinterpret_cast<uintptr_t>(scores) & (dtype == KGE_F32 ? 3 : 1)) || (reinterpret_cast<uintptr_t>(action) & (id_bits / 8 - 1)) ||
         (reinterpret_cast<uintptr_t>(n_cand) & 3)) { set_error("%s: a pointer is not aligned to its element size", fn); return KGE_E_ALIGN; }
     a->scores = scores; a->ld = ld; a->rows = rows; a->n = static_cast<int>(n); a->n_cand = n_cand; a->action = action; a->id64 = id_bits == 64;
-    a->inv_temp = 1.f / temperature;
+    a->inv_temp = 1.0 / temperature;
+    const double c = 1.4426950408889634073599 / temperature;
+    a->c_hi = static_cast<float>(c);
+    if (static_cast<double>(a->c_hi) >= c) a->c_hi = nextafterf(a->c_hi, 0.f);     // c_lo > 0: a score of -infinity stays one in both products
+    a->c_lo = static_cast<float>(c - static_cast<double>(a->c_hi));
     a->err = device_error_word();
     if (!a->err) { set_error("%s: no usable device", fn); return KGE_E_DEVICE; }
     return 0;
@@ -857,7 +866,7 @@ size_t kge_candidates_workspace_bytes(int64_t rows, int64_t n) {
 }
 
 int kge_log_prob(const void* scores, int32_t dtype, int64_t ld, int64_t rows, int64_t n, const int32_t* n_cand, const void* action,
-                 int32_t id_bits, float temperature, float* logp, float* stats, void* workspace, size_t workspace_bytes,
+                 int32_t id_bits, double temperature, float* logp, float* stats, void* workspace, size_t workspace_bytes,
                  kge_stream_t stream) {
     const char* fn = "kge_log_prob";
     CandArgs a = {};
@@ -874,7 +883,7 @@ int kge_log_prob(const void* scores, int32_t dtype, int64_t ld, int64_t rows, in
 }
 
 int kge_log_prob_backward(const void* scores, int32_t dtype, int64_t ld, int64_t rows, int64_t n, const int32_t* n_cand, const void* action,
-                          int32_t id_bits, float temperature, const float* stats, const float* dlogp, void* dscores, int64_t ldd,
+                          int32_t id_bits, double temperature, const float* stats, const float* dlogp, void* dscores, int64_t ldd,
                           kge_stream_t stream) {
     const char* fn = "kge_log_prob_backward";
     CandArgs a = {};
@@ -888,7 +897,7 @@ int kge_log_prob_backward(const void* scores, int32_t dtype, int64_t ld, int64_t
 }
 
 int kge_policy_loss(const void* scores, int32_t dtype, int64_t ld, int64_t rows, int64_t n, const int32_t* n_cand, const void* action,
-                    int32_t id_bits, float temperature, const float* old_logp, const float* ref_logp, const float* advantage,
+                    int32_t id_bits, double temperature, const float* old_logp, const float* ref_logp, const float* advantage,
                     const float* weight, float clip_low, float clip_high, float kl_coef, float scale, float* loss, float* logp,
                     float* kl, void* dscores, int64_t ldd, void* workspace, size_t workspace_bytes, kge_stream_t stream) {
     const char* fn = "kge_policy_loss";

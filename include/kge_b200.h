@@ -413,7 +413,7 @@ KGE_API int kge_preference_loss(const float* pos, const float* ref_pos, const fl
  *                              + kl_coef * kl,   kl = exp(ref_logp - logp) - (ref_logp - logp) - 1  (0 without ref_logp)
  *                          loss = scale * sum_r weight[r] l_r and dscores = d(loss) / d(scores), in one call; logp and kl
  *                          (rows) are written too.  weight NULL: 1.  A clipped row's policy part has zero gradient.
- * action[r] = -1: nothing was chosen; any other id outside [0, n_cand[r]) is reported as KGE_ERR_ID_RANGE (kge_check) and taken
+ * temperature in [1e-30, 1e30].  action[r] = -1: nothing was chosen; any other id outside [0, n_cand[r]) is reported as KGE_ERR_ID_RANGE (kge_check) and taken
  * as -1.  Such a row, a row without candidates and a row whose scores are all -infinity has logp = kl = 0, adds nothing and
  * gets zero gradients; a row of weight 0 adds nothing and gets zero gradients.  A score of -infinity has probability 0; NaN or
  * +infinity make the row's outputs NaN.  dscores has the dtype of scores, pitch ldd, may be scores itself (same pitch); columns
@@ -421,13 +421,13 @@ KGE_API int kge_preference_loss(const float* pos, const float* ref_pos, const fl
  * logp, kl are fp32 (rows), loss (1,).  n <= 2^30.  workspace from kge_candidates_workspace_bytes.  No reference counterpart. */
 KGE_API size_t kge_candidates_workspace_bytes(int64_t rows, int64_t n);
 KGE_API int kge_log_prob(const void* scores, int32_t dtype, int64_t ld, int64_t rows, int64_t n, const int32_t* n_cand,
-                         const void* action, int32_t id_bits, float temperature, float* logp, float* stats, void* workspace,
+                         const void* action, int32_t id_bits, double temperature, float* logp, float* stats, void* workspace,
                          size_t workspace_bytes, kge_stream_t stream);
 KGE_API int kge_log_prob_backward(const void* scores, int32_t dtype, int64_t ld, int64_t rows, int64_t n, const int32_t* n_cand,
-                         const void* action, int32_t id_bits, float temperature, const float* stats, const float* dlogp,
+                         const void* action, int32_t id_bits, double temperature, const float* stats, const float* dlogp,
                          void* dscores, int64_t ldd, kge_stream_t stream);
 KGE_API int kge_policy_loss(const void* scores, int32_t dtype, int64_t ld, int64_t rows, int64_t n, const int32_t* n_cand,
-                         const void* action, int32_t id_bits, float temperature, const float* old_logp, const float* ref_logp,
+                         const void* action, int32_t id_bits, double temperature, const float* old_logp, const float* ref_logp,
                          const float* advantage, const float* weight, float clip_low, float clip_high, float kl_coef, float scale,
                          float* loss, float* logp, float* kl, void* dscores, int64_t ldd, void* workspace,
                          size_t workspace_bytes, kge_stream_t stream);
