@@ -151,9 +151,17 @@ template <> struct Vec<__nv_bfloat16> {
         return make_uint4(w[0], w[1], w[2], w[3]);
     }
 };
+// over groups of G adjacent lanes
+template <int G = 32>
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
-    for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kFull, v, o));
+    for (int o = G / 2; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kFull, v, o));
+    return v;
+}
+template <int G>
+__device__ __forceinline__ float group_sum(float v) {
+#pragma unroll
+    for (int o = G / 2; o; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
     return v;
 }
 // exp((f - m) / T) of V scores, two at a time (packed fp32 pairs: half the instructions of the subtraction and the product)
@@ -234,50 +242,56 @@ __device__ __forceinline__ int extra_index(const Slice& q, int n, int tid) {
     return tid < 16 && j < n ? j : -1;
 }
 
-// A thread's part of one row between the loads and the gradient: register i holds vector v0 + tid + i THREADS.
-template <typename T, int THREADS, int I>
+// A thread's part of one row between the loads and the gradient: register i holds vector lane + i G of the row, threads below 8
+// also one element of the head and one of the tail.
+template <typename T, int G, int I>
 struct RowPart {
     static constexpr int V = Vec<T>::V;
     static constexpr bool kKeepExp = sizeof(T) == 4;
     uint4 r[I];
-    float xe;                     // the extra element
-    int xi, own;                  // its index; the register that holds the chosen candidate, or -1
-    float mw, mz;                 // maximum of this warp's part, and with 0 in the place of -infinity
+    float xe[2];                  // the head and tail elements
+    int xi[2], own;               // their indexes or -1; the register that holds the chosen candidate, or -1
+    float mw, mz;                 // maximum of the row, and with 0 in the place of -infinity
 
-    // first vector (in units of THREADS) past this thread's vectors that hold a candidate
-    __device__ __forceinline__ static int filled(const Slice& q, int cnt, int tid) {
-        const int nvc = cnt <= q.head ? 0 : (cnt - q.head + V - 1) / V;
-        return min(q.v1, nvc) - q.v0 - tid;
-    }
-    __device__ __forceinline__ void load(const uint4* src, int left) {        // src: vector v0 + tid
+    __device__ __forceinline__ void load(const T* s, const Slice& q, int n, int cnt, int lane) {
+        const uint4* src = reinterpret_cast<const uint4*>(s + q.head) + lane;
+        const int nvc = cnt <= q.head ? 0 : (cnt - q.head + V - 1) / V, left = min(q.nv, nvc) - lane;
 #pragma unroll
         for (int i = 0; i < I; ++i) {
             r[i] = make_uint4(Vec<T>::kLow, Vec<T>::kLow, Vec<T>::kLow, Vec<T>::kLow);
-            if (i * THREADS < left) r[i] = __ldcs(src + i * THREADS);
+            if (i * G < left) r[i] = __ldcs(src + i * G);
         }
+        xi[0] = lane < q.head ? lane : -1;
+        xi[1] = lane < 8 && q.head + q.nv * V + lane < n ? q.head + q.nv * V + lane : -1;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) xe[k] = xi[k] >= 0 && xi[k] < cnt ? cand_get(s + xi[k]) : -INFINITY;
     }
-    __device__ __forceinline__ float stats(const Slice& q, int n, int cnt, int act, int tid, Scale2 c) {
-        const int used = (q.v1 - q.v0 + THREADS - 1) / THREADS;               // registers that hold anything, the same for all
+    __device__ __forceinline__ float stats(const Slice& q, int n, int cnt, int act, int lane, Scale2 c) {
+        const int used = (q.nv + G - 1) / G;                                  // registers that hold anything, the same for all
         if (cnt < n) {
 #pragma unroll
             for (int i = 0; i < I; ++i) {
-                const int at = q.head + (q.v0 + tid + i * THREADS) * V;
+                const int at = q.head + (lane + i * G) * V;
                 if (at < cnt && at + V > cnt) r[i] = mask_past<T>(r[i], at, cnt);
             }
         }
-        mw = xe;
+        mw = fmaxf(xe[0], xe[1]);
 #pragma unroll
         for (int i = 0; i < I; ++i) if (i < used) mw = fmaxf(mw, Vec<T>::max(r[i]));
-        mw = warp_max(mw);
+        mw = warp_max<G>(mw);
         mz = finite_or_zero(mw);
         own = -1;
         if (act >= q.head && act < q.head + q.nv * V) {
-            const int v = (act - q.head) / V - q.v0;
-            if (v >= 0 && v % THREADS == tid && q.v0 + v < q.v1) own = v / THREADS;
+            const int v = (act - q.head) / V;
+            if (v % G == lane) own = v / G;
         }
-        const float e = cand_exp(xe - mz, c);
-        float2 sum = make_float2(xi != act ? e : 0.f, 0.f);
-        if (kKeepExp) xe = e;
+        float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const float e = cand_exp(xe[k] - mz, c);
+            if (xi[k] != act) sum.x += e;
+            if (kKeepExp) xe[k] = e;
+        }
 #pragma unroll
         for (int i = 0; i < I; ++i) {
             if (i >= used) continue;
@@ -295,70 +309,78 @@ struct RowPart {
 #pragma unroll
             for (int i = 0; i < I; ++i) asm volatile("" : "+r"(r[i].x), "+r"(r[i].y), "+r"(r[i].z), "+r"(r[i].w));
         }
-        return warp_sum(sum.x + sum.y);
+        return group_sum<G>(sum.x + sum.y);
     }
-    __device__ __forceinline__ void write(T* d, const Slice& q, int n, int cnt, int act, int tid, Scale2 c, float m, float rest, float ga) const {
-        uint4* dv = reinterpret_cast<uint4*>(d + q.head) + q.v0 + tid;
-        const int left = q.v1 - q.v0 - tid;
-        const float mall = finite_or_zero(m);
-        // (a warp without a finite score has only zeros to scale: mz = 0 stands for nothing there)
-        const float f0 = ga == 0.f || (kKeepExp && mw == -INFINITY) ? 0.f : kKeepExp ? -ga * cand_exp(mz - mall, c) : -ga;
-        const float fa = ga == 0.f ? 0.f : ga * rest;
+    __device__ __forceinline__ void write(T* d, const Slice& q, int n, int cnt, int act, int lane, Scale2 c, float rest, float ga) const {
+        uint4* dv = reinterpret_cast<uint4*>(d + q.head) + lane;
+        const int left = q.nv - lane;
+        const float f0 = ga == 0.f ? 0.f : -ga, fa = ga == 0.f ? 0.f : ga * rest;
         const bool plain = cnt == n && ga != 0.f;                 // no padding, and something to write
 #pragma unroll
         for (int i = 0; i < I; ++i) {
-            if (i * THREADS < left) {
+            if (i * G < left) {
                 float f[V];
                 Vec<T>::open(r[i], f);
-                if (!kKeepExp) cand_exps<V>(f, mall, c);
+                if (!kKeepExp) cand_exps<V>(f, mz, c);
                 cand_scale<V>(f, f0);
                 if (!plain) {
-                    const int at = q.head + (q.v0 + tid + i * THREADS) * V;
+                    const int at = q.head + (lane + i * G) * V;
 #pragma unroll
                     for (int k = 0; k < V; ++k) if (ga == 0.f || at + k >= cnt) f[k] = 0.f;
                 }
-                __stcs(dv + i * THREADS, Vec<T>::close(f));
+                __stcs(dv + i * G, Vec<T>::close(f));
             }
         }
         if (own >= 0) cand_put(d + act, fa);                      // over the vector just stored by this thread
-        if (xi >= 0) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            if (xi[k] < 0) continue;
             float v = 0.f;
-            if (xi < cnt && ga != 0.f) v = xi == act ? fa : f0 * (kKeepExp ? xe : cand_exp(xe - mall, c));
-            cand_put(d + xi, v);
+            if (xi[k] < cnt && ga != 0.f) v = xi[k] == act ? fa : f0 * (kKeepExp ? xe[k] : cand_exp(xe[k] - mz, c));
+            cand_put(d + xi[k], v);
         }
     }
 };
 
-// One warp per row: rows of up to 32 I vectors.
-template <typename T, int I, int MODE>
-__global__ void __launch_bounds__(256, 4) cand_warp_kernel(CandArgs a) {
+// Short rows: G lanes per row, up to G I vectors.  With one warp a row whatever its length, 10782 rows of 35 took three waves of
+// resident warps; four rows a warp also share the instructions of the rows' scalars.
+template <typename T, int G, int I, int MODE>
+__global__ void __launch_bounds__(256, 4) cand_group_kernel(CandArgs a) {
+    constexpr int R = 32 / G;                                     // rows of a warp
     __shared__ double red[8];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gl = lane % G;
     const Scale2 c = {a.c_hi, a.c_lo};
     double total = 0.0;
-    for (long long row = (long long)blockIdx.x * 8 + warp; row < a.rows; row += (long long)gridDim.x * 8) {
+    for (long long first = ((long long)blockIdx.x * 8 + warp) * R; first < a.rows; first += (long long)gridDim.x * (8 * R)) {
+        const bool live = first + lane / G < a.rows;              // (all lanes take part in the shuffles)
+        const long long row = live ? first + lane / G : a.rows - 1;
         const T* s = static_cast<const T*>(a.scores) + row * a.ld;
         const int cnt = cand_count(a, row);
-        const int act = cand_action(a, row, cnt, lane == 0);
-        const float sa = act >= 0 ? cand_get(s + act) : 0.f;
-        float side = 0.f;                 // lane k < 4 requests operand k now: the finish of the row must not wait for memory
-        if (MODE == CM_POLICY && lane < 4) side = cand_side(a, row, lane);
+        const int act = cand_action(a, row, cnt, live && gl == 0);
+        const float sa = act >= 0 && gl == 0 ? cand_get(s + act) : 0.f;
+        float side = 0.f;                 // lane k < 4 of a row requests operand k now: its finish must not wait for memory
+        if (MODE == CM_POLICY && gl < 4) side = cand_side(a, row, gl);
         const Slice q = cand_slice(s, a.n, 0, 1);
-        RowPart<T, 32, I> p;
-        p.load(reinterpret_cast<const uint4*>(s + q.head) + lane, RowPart<T, 32, I>::filled(q, cnt, lane));
-        p.xi = extra_index<T>(q, a.n, lane);
-        p.xe = p.xi >= 0 && p.xi < cnt ? cand_get(s + p.xi) : -INFINITY;
-        const float rest = p.stats(q, a.n, cnt, act, lane, c);
+        RowPart<T, G, I> p;
+        p.load(s, q, a.n, cnt, gl);
+        const float rest = p.stats(q, a.n, cnt, act, gl, c);
         RowSide o = {};
         if (MODE == CM_POLICY) {
-            o.w = __shfl_sync(kFull, side, 0); o.adv = __shfl_sync(kFull, side, 1);
-            o.old = __shfl_sync(kFull, side, 2); o.ref = __shfl_sync(kFull, side, 3);
+            const int l0 = lane - gl;
+            o.w = __shfl_sync(kFull, side, l0); o.adv = __shfl_sync(kFull, side, l0 + 1);
+            o.old = __shfl_sync(kFull, side, l0 + 2); o.ref = __shfl_sync(kFull, side, l0 + 3);
         }
         float ga = 0.f;
-        if (lane == 0) total += cand_finish<MODE>(a, row, act, sa, p.mz, rest, true, o, &ga);
-        if (MODE == CM_POLICY) p.write(static_cast<T*>(a.dscores) + row * a.ldd, q, a.n, cnt, act, lane, c, p.mw, rest, __shfl_sync(kFull, ga, 0));
+        __syncwarp();                     // (rows written over their scores: every lane of the row has read its own)
+        if (gl == 0 && live) total += cand_finish<MODE>(a, row, act, sa, p.mz, rest, true, o, &ga);
+        if (MODE == CM_POLICY) {
+            ga = __shfl_sync(kFull, ga, lane - gl);
+            if (live) p.write(static_cast<T*>(a.dscores) + row * a.ldd, q, a.n, cnt, act, gl, c, rest, ga);
+        }
     }
     if (MODE == CM_POLICY) {
+#pragma unroll
+        for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(kFull, total, o);
         if (lane == 0) red[warp] = total;
         __syncthreads();
         if (threadIdx.x == 0) {
@@ -730,12 +752,13 @@ static CandLayout cand_layout(long long rows, long long n) {
     return L;
 }
 
-template <typename T, int I, int MODE>
-static int cand_warps(const CandArgs& a, int* n_partial, cudaStream_t s) {
-    const long long want = (a.rows + 7) / 8;
+template <typename T, int G, int I, int MODE>
+static int cand_groups(const CandArgs& a, int* n_partial, cudaStream_t s) {
+    constexpr int per = 8 * (32 / G);
+    const long long want = (a.rows + per - 1) / per;
     *n_partial = static_cast<int>(want < kCandMaxBlocks ? want : kCandMaxBlocks);
-    cand_warp_kernel<T, I, MODE><<<*n_partial, 256, 0, s>>>(a);
-    KGE_LAUNCH_CHECK("cand_warp_kernel");
+    cand_group_kernel<T, G, I, MODE><<<*n_partial, 256, 0, s>>>(a);
+    KGE_LAUNCH_CHECK("cand_group_kernel");
     return 0;
 }
 
@@ -804,9 +827,11 @@ template <typename T, int MODE>
 static int cand_go(const CandArgs& a, void* ws, int* n_partial, cudaStream_t s) {
     const long long nv = a.n / Vec<T>::V;              // vectors of a row, at most
     if (MODE == CM_POLICY && !same_phase<T>(a)) return cand_passes<T, MODE>(a, ws, n_partial, s);
-    if (nv <= 32) return cand_warps<T, 1, MODE>(a, n_partial, s);
-    if (nv <= 64) return cand_warps<T, 2, MODE>(a, n_partial, s);
-    if (nv <= 128) return cand_warps<T, 4, MODE>(a, n_partial, s);
+    if (nv <= 8) return cand_groups<T, 8, 1, MODE>(a, n_partial, s);
+    if (nv <= 16) return cand_groups<T, 8, 2, MODE>(a, n_partial, s);
+    if (nv <= 32) return cand_groups<T, 8, 4, MODE>(a, n_partial, s);
+    if (nv <= 64) return cand_groups<T, 16, 4, MODE>(a, n_partial, s);
+    if (nv <= 128) return cand_groups<T, 32, 4, MODE>(a, n_partial, s);
     if (a.rows >= (1LL << 31) / kMaxCluster) return cand_passes<T, MODE>(a, ws, n_partial, s);      // (beyond a grid of one CTA a row)
     if (nv <= 512) return cand_rows<T, 64, 16, MODE>(a, 1, nv, n_partial, s);
     if (nv <= 1024) return cand_rows<T, 128, 10, MODE>(a, 1, nv, n_partial, s);

@@ -87,12 +87,21 @@ template <> struct DropVec<__nv_bfloat16> {
 // eight resident CTAs per SM and at 6.4 TB/s with the vectors of a thread a grid apart.
 constexpr int kDropU = 2;
 template <typename T, bool PACKED>
-__global__ void __launch_bounds__(256) dropout_vec_kernel(DropoutArgs a, RoundKeys keys, long long vectors, int per_row) {
+__global__ void __launch_bounds__(256) dropout_vec_kernel(DropoutArgs a, RoundKeys keys, long long vectors, int per_row, int tail) {
     constexpr int V = DropVec<T>::V, U = kDropU;
     const uint32_t step = 0x80000000u | (a.step_dev ? static_cast<uint32_t>(*a.step_dev) + a.step : a.step);
     const uint4* x = static_cast<const uint4*>(a.x);
     const uint4* res = static_cast<const uint4*>(a.res);
     uint4* out = static_cast<uint4*>(a.out);
+    if (PACKED && tail > 0 && blockIdx.x == gridDim.x - 1 && static_cast<int>(threadIdx.x) < tail) {
+        // the elements behind the last whole vector, one a thread
+        const long long e = vectors * V + threadIdx.x, q = e >> 2;
+        const Philox4 w = philox4x32_10(static_cast<uint32_t>(q), static_cast<uint32_t>(q >> 32), a.stream, step, a.k0, a.k1);
+        const uint32_t word = w.x[e & 3];
+        float f = word >= a.threshold ? drop_get(static_cast<const T*>(a.x) + e) * a.scale : 0.f;
+        if (res) f += drop_get(static_cast<const T*>(a.res) + e);
+        drop_put(static_cast<T*>(a.out) + e, f);
+    }
     {
         const long long v0 = (long long)blockIdx.x * (256 * U) + threadIdx.x;
         uint4 r[U], q[U];
@@ -148,7 +157,7 @@ static bool drop_vectors(const DropoutArgs& a, bool* packed) {
     constexpr int V = DropVec<T>::V;
     if (!aligned16(a.x) || !aligned16(a.res) || !aligned16(a.out)) return false;
     *packed = a.rows == 1 || (a.ldx == a.dim && a.ldo == a.dim && (!a.res || a.ldr == a.dim));
-    if (*packed) return (a.rows * a.dim) % V == 0;
+    if (*packed) return a.rows * a.dim >= V;
     return a.dim % V == 0 && a.ldx % V == 0 && a.ldo % V == 0 && a.ldr % V == 0;
 }
 
@@ -168,8 +177,9 @@ static int drop_go(const DropoutArgs& a, cudaStream_t s) {
     if (want >= (1LL << 31)) { set_error("kge_dropout: more than 2^40 vectors"); return KGE_E_RANGE; }
     const unsigned blocks = static_cast<unsigned>(want);
     const int per_row = a.dim / DropVec<T>::V;
-    if (packed) dropout_vec_kernel<T, true><<<blocks, 256, 0, s>>>(a, keys, vectors, per_row);
-    else dropout_vec_kernel<T, false><<<blocks, 256, 0, s>>>(a, keys, vectors, per_row);
+    const int tail = static_cast<int>(a.rows * a.dim - vectors * DropVec<T>::V);
+    if (packed) dropout_vec_kernel<T, true><<<blocks, 256, 0, s>>>(a, keys, vectors, per_row, tail);
+    else dropout_vec_kernel<T, false><<<blocks, 256, 0, s>>>(a, keys, vectors, per_row, 0);
     KGE_LAUNCH_CHECK("dropout_vec_kernel");
     return 0;
 }
