@@ -349,6 +349,7 @@ __global__ void __launch_bounds__(256, 4) cand_group_kernel(CandArgs a) {
     constexpr int R = 32 / G;                                     // rows of a warp
     __shared__ double red[8];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gl = lane % G;
+    let_next_start();
     const Scale2 c = {a.c_hi, a.c_lo};
     double total = 0.0;
     for (long long first = ((long long)blockIdx.x * 8 + warp) * R; first < a.rows; first += (long long)gridDim.x * (8 * R)) {
@@ -408,6 +409,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) cand_row_kernel(CandArgs a) {
     uint32_t rank, csize;
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(csize));
+    let_next_start();
     const long long row = blockIdx.x / csize;
     const Scale2 c = {a.c_hi, a.c_lo};
     const T* s = static_cast<const T*>(a.scores) + row * a.ld;
@@ -546,6 +548,7 @@ template <typename T>
 __global__ void __launch_bounds__(256) cand_stats_kernel(CandArgs a, float2* parts, int chunk, int chunks) {
     constexpr int V = Vec<T>::V;
     __shared__ float2 red[8];
+    let_next_start();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const Scale2 c = {a.c_hi, a.c_lo};
     for (long long u = blockIdx.x; u < a.rows * chunks; u += gridDim.x) {
@@ -613,6 +616,8 @@ __global__ void __launch_bounds__(256) cand_stats_kernel(CandArgs a, float2* par
 template <typename T, int MODE>
 __global__ void __launch_bounds__(256) cand_join_kernel(CandArgs a, const float2* parts, int chunks, float* coef) {
     __shared__ double red[8];
+    let_next_start();
+    after_previous();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const Scale2 c = {a.c_hi, a.c_lo};
     double total = 0.0;
@@ -653,6 +658,8 @@ template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(256) cand_grad_kernel(CandArgs a, const float* coef, long long pieces) {
     constexpr int V = ALIGNED ? Vec<T>::V : 1;
     const int lane = threadIdx.x & 31;
+    let_next_start();
+    after_previous();
     const Scale2 c = {a.c_hi, a.c_lo};
     const long long units = a.rows * pieces;
     for (long long u = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); u < units; u += (long long)gridDim.x * 8) {
@@ -712,6 +719,7 @@ __global__ void __launch_bounds__(256) cand_grad_kernel(CandArgs a, const float*
 
 __global__ void __launch_bounds__(1024) sum_partials_kernel(const double* partial, int n, float* out) {
     __shared__ double red[32];
+    after_previous();
     double v = 0.0;
 #pragma unroll 4
     for (int i = threadIdx.x; i < n; i += 1024) v += partial[i];
@@ -728,8 +736,12 @@ __global__ void __launch_bounds__(1024) sum_partials_kernel(const double* partia
 }
 
 int launch_sum_partials(const double* partial, int n, float* out, cudaStream_t s) {
-    sum_partials_kernel<<<1, 1024, 0, s>>>(partial, n, out);
-    KGE_LAUNCH_CHECK("sum_partials_kernel");
+    if (n == 0) {                    // the only kernel of its call
+        sum_partials_kernel<<<1, 1024, 0, s>>>(partial, n, out);
+        KGE_LAUNCH_CHECK("sum_partials_kernel");
+        return 0;
+    }
+    KGE_LAUNCH_AFTER("sum_partials_kernel", sum_partials_kernel, 1u, 1024u, s, partial, n, out);
     return 0;
 }
 
@@ -790,10 +802,15 @@ static int cand_rows(const CandArgs& a, int cluster, long long slot, int* n_part
 }
 
 template <typename T>
-static int cand_gradient(const CandArgs& a, const float* coef, bool aligned, cudaStream_t s) {
+static int cand_gradient(const CandArgs& a, const float* coef, bool aligned, bool first, cudaStream_t s) {
     const int per = 128 * (aligned ? Vec<T>::V : 1);
     const long long pieces = a.n > 0 ? (a.n + per - 1) / per : 1, want = (a.rows * pieces + 7) / 8;
     const unsigned blocks = static_cast<unsigned>(want < (1 << 30) ? want : (1 << 30));       // (short CTAs copy faster than a loop)
+    if (!first) {
+        if (aligned) KGE_LAUNCH_AFTER("cand_grad_kernel", cand_grad_kernel<T, true>, blocks, 256u, s, a, coef, pieces);
+        else KGE_LAUNCH_AFTER("cand_grad_kernel", cand_grad_kernel<T, false>, blocks, 256u, s, a, coef, pieces);
+        return 0;
+    }
     if (aligned) cand_grad_kernel<T, true><<<blocks, 256, 0, s>>>(a, coef, pieces);
     else cand_grad_kernel<T, false><<<blocks, 256, 0, s>>>(a, coef, pieces);
     KGE_LAUNCH_CHECK("cand_grad_kernel");
@@ -816,9 +833,8 @@ static int cand_passes(const CandArgs& a, void* ws, int* n_partial, cudaStream_t
     KGE_LAUNCH_CHECK("cand_stats_kernel");
     const long long jb = (a.rows + 7) / 8;
     *n_partial = static_cast<int>(jb < kCandMaxBlocks ? jb : kCandMaxBlocks);
-    cand_join_kernel<T, MODE><<<*n_partial, 256, 0, s>>>(a, parts, L.chunks, coef);
-    KGE_LAUNCH_CHECK("cand_join_kernel");
-    return MODE == CM_POLICY ? cand_gradient<T>(a, coef, same_phase<T>(a), s) : 0;
+    KGE_LAUNCH_AFTER("cand_join_kernel", cand_join_kernel<T, MODE>, static_cast<unsigned>(*n_partial), 256u, s, a, parts, L.chunks, coef);
+    return MODE == CM_POLICY ? cand_gradient<T>(a, coef, same_phase<T>(a), false, s) : 0;
 }
 
 // Which form: the smallest group that holds a row in registers; passes where the rows are too long for a cluster, where the
@@ -918,7 +934,8 @@ int kge_log_prob_backward(const void* scores, int32_t dtype, int64_t ld, int64_t
         (rc = check_gradient(fn, dscores, dtype, ldd, rows, n))) return rc;
     a.stats = const_cast<float*>(stats); a.dlogp = dlogp; a.dscores = dscores; a.ldd = ldd;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    return dtype == KGE_F32 ? cand_gradient<float>(a, stats, same_phase<float>(a), s) : cand_gradient<__nv_bfloat16>(a, stats, same_phase<__nv_bfloat16>(a), s);
+    return dtype == KGE_F32 ? cand_gradient<float>(a, stats, same_phase<float>(a), true, s)
+                            : cand_gradient<__nv_bfloat16>(a, stats, same_phase<__nv_bfloat16>(a), true, s);
 }
 
 int kge_policy_loss(const void* scores, int32_t dtype, int64_t ld, int64_t rows, int64_t n, const int32_t* n_cand, const void* action,

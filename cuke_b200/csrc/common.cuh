@@ -24,6 +24,34 @@ void note_launch();                            // counts kernel launches issued 
         kge::note_launch();                                      \
     } while (0)
 
+// ---- kernels of one call that follow one another ------------------------------------------------------------------
+// A kernel launched by launch_after may start before the kernel ahead of it in the stream has ended (programmatic stream
+// serialization): its launch and prologue overlap that kernel's tail.  It calls after_previous() before it reads or writes
+// anything in global memory, which waits until the kernel ahead has completed; since every kernel of a chain does so, all
+// earlier ones have completed too.  The kernel ahead calls let_next_start() once; without that the next starts at its end.
+// Only the second and later kernels of a call are launched this way: the first is ordered after the caller's work as usual.
+__device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+template <typename... Params, typename... Args>
+inline cudaError_t launch_after(void (*kernel)(Params...), unsigned blocks, unsigned threads, cudaStream_t s, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(blocks);
+    cfg.blockDim = dim3(threads);
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+}
+#define KGE_LAUNCH_AFTER(what, ...)                                   \
+    do {                                                              \
+        cudaError_t e__ = kge::launch_after(__VA_ARGS__);             \
+        if (e__ != cudaSuccess) return kge::cuda_status(e__, what);   \
+        KGE_LAUNCH_CHECK(what);                                       \
+    } while (0)
+
 // ---- element access --------------------------------------------------------------------------------
 // A "quad" is 4 consecutive elements of a row; every row-wise kernel gives lane L the quads
 // L, L+32, L+64, ... so that a warp reads 512 B (fp32) / 256 B (bf16) contiguous per pass.

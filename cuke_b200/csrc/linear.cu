@@ -236,6 +236,8 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
     umma::cluster_sync();
     umma::tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
+    let_next_start();
+    after_previous();
 
     const uint32_t smem0 = umma::smem_u32(smem), full0 = umma::smem_u32(full), empty0 = umma::smem_u32(empty);
     const uint32_t acc_full0 = umma::smem_u32(acc_full), acc_empty0 = umma::smem_u32(acc_empty);
@@ -468,6 +470,8 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
 // Sum of the shares of a split contraction in share order, then the epilogue; one thread per 8 columns.
 template <int EPI>
 __global__ void __launch_bounds__(256) linear_join_kernel(LinEpilogue e, long long m, int n, int splits) {
+    let_next_start();
+    after_previous();
     const int per_row = n / 8;
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < m * per_row; i += (long long)gridDim.x * 256) {
         const long long row = i / per_row;
@@ -621,6 +625,7 @@ __global__ void __launch_bounds__(512) linear_dz_kernel(const __nv_bfloat16* __r
                                                         __nv_bfloat16* __restrict__ dz, float* __restrict__ colpart, long long m, int n,
                                                         unsigned strips) {
     constexpr int W = 16, R = LZ_ROWS / W;
+    let_next_start();
     __shared__ __align__(16) float red[W][256];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const long long block = blockIdx.x / strips;
@@ -669,6 +674,8 @@ __global__ void __launch_bounds__(512) linear_dz_kernel(const __nv_bfloat16* __r
 // db[c] = sum over row blocks, in fp32 and in a fixed order (32 interleaved partial sums per column)
 __global__ void __launch_bounds__(1024) linear_db_kernel(const float* colpart, long long blocks, int n, __nv_bfloat16* db) {
     __shared__ float red[32][33];
+    let_next_start();
+    after_previous();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int c = blockIdx.x * 32 + lane;
     float t = 0.f;
@@ -714,7 +721,7 @@ static int lin_splits(long long m, long long n, long long k, int sms) {
 }
 
 template <int EPI, int ACT, bool SLOPE>
-static int lin_launch(const CUtensorMap (&maps)[5], const LinGemm& p, unsigned ctas, size_t smem, cudaStream_t s) {
+static int lin_launch(const CUtensorMap (&maps)[5], const LinGemm& p, unsigned ctas, size_t smem, bool first, cudaStream_t s) {
     static std::atomic<bool> attr_set[128];          // the shared-memory opt-in is per device and kernel
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return cuda_status(cudaGetLastError(), "cudaGetDevice");
@@ -723,19 +730,31 @@ static int lin_launch(const CUtensorMap (&maps)[5], const LinGemm& p, unsigned c
         if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(linear_pair_kernel)");
         if (dev >= 0 && dev < 128) attr_set[dev].store(true, std::memory_order_release);
     }
-    linear_pair_kernel<EPI, ACT, SLOPE><<<ctas, LG_THREADS, smem, s>>>(maps[0], maps[1], maps[2], maps[3], maps[4], p);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(ctas);
+    cfg.blockDim = dim3(LG_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = first ? 0 : 1;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, linear_pair_kernel<EPI, ACT, SLOPE>, maps[0], maps[1], maps[2], maps[3], maps[4], p);
+    if (e != cudaSuccess) return cuda_status(e, "linear_pair_kernel");
     KGE_LAUNCH_CHECK("linear_pair_kernel");
     return 0;
 }
 
 template <int ACT>
-static int lin_launch_forward(const CUtensorMap (&maps)[5], const LinGemm& p, unsigned ctas, size_t smem, cudaStream_t s) {
-    return p.e.slope ? lin_launch<LE_FORWARD, ACT, true>(maps, p, ctas, smem, s) : lin_launch<LE_FORWARD, ACT, false>(maps, p, ctas, smem, s);
+static int lin_launch_forward(const CUtensorMap (&maps)[5], const LinGemm& p, unsigned ctas, size_t smem, bool first, cudaStream_t s) {
+    return p.e.slope ? lin_launch<LE_FORWARD, ACT, true>(maps, p, ctas, smem, first, s)
+                     : lin_launch<LE_FORWARD, ACT, false>(maps, p, ctas, smem, first, s);
 }
 
 // out[m][n] (+ epilogue) = sum_k A[m][k] B[n][k].  a_mn / b_mn: the operand lies as (k rows, m or n columns).
 static int lin_gemm(const void* a, long long lda, int a_mn, const void* b, long long ldb, int b_mn, long long m, long long n, long long k,
-                    LinEpilogue e, bool forward, float* part, size_t part_bytes, cudaStream_t s) {
+                    LinEpilogue e, bool forward, bool first, float* part, size_t part_bytes, cudaStream_t s) {
     const int sms = lin_sms();
     LinGemm p;
     memset(&p, 0, sizeof(p));
@@ -773,20 +792,19 @@ static int lin_gemm(const void* a, long long lda, int a_mn, const void* b, long 
     if (items >= (1LL << 30)) { set_error("linear: %lld tiles exceed the tile index", items); return KGE_E_RANGE; }
     const unsigned ctas = 2u * static_cast<unsigned>(items < sms / 2 ? items : sms / 2);
     if (p.splits == 1) {
-        if (!forward) return lin_launch<LE_STORE, ACT_NONE, false>(maps, p, ctas, smem, s);
+        if (!forward) return lin_launch<LE_STORE, ACT_NONE, false>(maps, p, ctas, smem, first, s);
         switch (e.act) {
-            case ACT_NONE: return lin_launch<LE_FORWARD, ACT_NONE, false>(maps, p, ctas, smem, s);
-            case ACT_RELU: return lin_launch_forward<ACT_RELU>(maps, p, ctas, smem, s);
-            case ACT_SILU: return lin_launch_forward<ACT_SILU>(maps, p, ctas, smem, s);
-            default: return lin_launch_forward<ACT_GELU>(maps, p, ctas, smem, s);
+            case ACT_NONE: return lin_launch<LE_FORWARD, ACT_NONE, false>(maps, p, ctas, smem, first, s);
+            case ACT_RELU: return lin_launch_forward<ACT_RELU>(maps, p, ctas, smem, first, s);
+            case ACT_SILU: return lin_launch_forward<ACT_SILU>(maps, p, ctas, smem, first, s);
+            default: return lin_launch_forward<ACT_GELU>(maps, p, ctas, smem, first, s);
         }
     }
-    if ((rc = lin_launch<LE_PARTIAL, ACT_NONE, false>(maps, p, ctas, smem, s))) return rc;
+    if ((rc = lin_launch<LE_PARTIAL, ACT_NONE, false>(maps, p, ctas, smem, first, s))) return rc;
     const long long groups = (m * (n / 8) + 255) / 256;
     const unsigned blocks = static_cast<unsigned>(groups < 148 * 8 ? groups : 148 * 8);
-    if (forward) linear_join_kernel<LE_FORWARD><<<blocks, 256, 0, s>>>(e, m, p.n, p.splits);
-    else linear_join_kernel<LE_STORE><<<blocks, 256, 0, s>>>(e, m, p.n, p.splits);
-    KGE_LAUNCH_CHECK("linear_join_kernel");
+    if (forward) KGE_LAUNCH_AFTER("linear_join_kernel", linear_join_kernel<LE_FORWARD>, blocks, 256u, s, e, m, p.n, p.splits);
+    else KGE_LAUNCH_AFTER("linear_join_kernel", linear_join_kernel<LE_STORE>, blocks, 256u, s, e, m, p.n, p.splits);
     return 0;
 }
 
@@ -882,7 +900,7 @@ int kge_linear_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, c
         if (m <= 4) return lin_few<4>(x, ldx, w, ldw, m, k, n, e, s);
         return lin_few<8>(x, ldx, w, ldw, m, k, n, e, s);
     }
-    return lin_gemm(x, pitch_of(ldx, m, k), 0, w, pitch_of(ldw, k, n), 1, m, n, k, e, true, static_cast<float*>(workspace), workspace_bytes,
+    return lin_gemm(x, pitch_of(ldx, m, k), 0, w, pitch_of(ldw, k, n), 1, m, n, k, e, true, true, static_cast<float*>(workspace), workspace_bytes,
                     reinterpret_cast<cudaStream_t>(stream));
 }
 
@@ -922,20 +940,22 @@ int kge_linear_backward(const void* dout, int64_t ldd, const void* x, int64_t ld
         KGE_LAUNCH_CHECK("linear_dz_kernel");
     }
     if (dbias) {
-        linear_db_kernel<<<static_cast<unsigned>((n + 31) / 32), 1024, 0, s>>>(colpart, blocks, static_cast<int>(n), static_cast<__nv_bfloat16*>(dbias));
-        KGE_LAUNCH_CHECK("linear_db_kernel");
+        KGE_LAUNCH_AFTER("linear_db_kernel", linear_db_kernel, static_cast<unsigned>((n + 31) / 32), 1024u, s, colpart, blocks, static_cast<int>(n),
+                         static_cast<__nv_bfloat16*>(dbias));
     }
+    bool first = !dz && !dbias;                   // nothing of this call is ahead of the first product
     const void* g = dz ? static_cast<const void*>(dz) : dout;
     const long long ldg = dz ? n : ldd;
     LinEpilogue e;
     memset(&e, 0, sizeof(e));
     if (dx) {
         e.out = static_cast<__nv_bfloat16*>(dx); e.ldo = pitch_of(lddx, m, k);
-        if ((rc = lin_gemm(g, ldg, 0, w, pitch_of(ldw, k, n), 0, m, k, n, e, false, reinterpret_cast<float*>(ws), part_bytes, s))) return rc;
+        if ((rc = lin_gemm(g, ldg, 0, w, pitch_of(ldw, k, n), 0, m, k, n, e, false, first, reinterpret_cast<float*>(ws), part_bytes, s))) return rc;
+        first = false;
     }
     if (dw) {
         e.out = static_cast<__nv_bfloat16*>(dw); e.ldo = n;
-        if ((rc = lin_gemm(x, pitch_of(ldx, m, k), 1, g, ldg, 1, k, n, m, e, false, reinterpret_cast<float*>(ws), part_bytes, s))) return rc;
+        if ((rc = lin_gemm(x, pitch_of(ldx, m, k), 1, g, ldg, 1, k, n, m, e, false, first, reinterpret_cast<float*>(ws), part_bytes, s))) return rc;
     }
     return 0;
 }

@@ -84,6 +84,7 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) pref_kernel(PrefArgs a) {
     __shared__ int rc[32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int gl = threadIdx.x % G;
+    let_next_start();
     double total = 0.0;
     const long long step = (long long)gridDim.x * (BLOCK / G);
     // every lane of a warp makes the same number of turns: the shuffles below need all of them
