@@ -1,13 +1,13 @@
 // Rows from features: out = act(x w + b) (+ residual) and its gradient, bf16 with fp32 accumulation.
 //
 //   forward   z = x w + b        x (M, K), w (K, N) in the framework's matrix orientation out[j] = sum_i x[i] w[i][j]
-//             out = act(z) + residual, and for training slope = act'(z) in fp16 (2^-12 relative: an eighth of a bf16 rounding)
+//             out = act(z) + residual, and for training slope = act'(z) in fp16 (2^-11 relative: an eighth of a bf16 rounding)
 //   backward  dz = dout * slope (bf16),  dx = dz w^T,  dw = x^T dz,  db = sum over rows of dz,  d(residual) = dout
 //
 // The three products run on one persistent tcgen05 kernel over CTA pairs (256-row tiles, cta_group::2): operands are
 // used as they lie in memory, K-major or MN-major, so nothing is transposed; two accumulators in tensor memory let a
 // tile's epilogue overlap the next tile's main loop.  Bias, activation, residual and slope are applied to the fp32
-// accumulator in the epilogue, with one rounding to bf16.
+// accumulator in the epilogue, with one rounding to bf16.  dx and dw are one launch: their tiles share one list of work.
 #include <string.h>
 #include <atomic>
 #include <cuda_fp16.h>
@@ -16,7 +16,7 @@
 namespace kge {
 
 enum { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3 };
-enum { LE_FORWARD = 0, LE_STORE = 1, LE_PARTIAL = 2 };
+enum { LE_FORWARD = 0, LE_PLAIN = 1 };            // the whole forward epilogue; rounding to bf16, or fp32 shares of a split sum
 
 constexpr int LG_BM = 128;                        // rows of a tile per CTA (a pair: 256)
 constexpr int LG_BK = 64;                         // contraction per stage: one 128-byte swizzle row of bf16
@@ -36,7 +36,7 @@ constexpr int LG_BLOCK = 32 * 64;
 constexpr int LG_STRIP = 32 * 4;                  // a block's bias in fp32, read by broadcast
 __host__ __device__ constexpr int lin_warp_stage(bool slope) { return (slope ? 3 : 2) * LG_BLOCK; }
 __host__ __device__ constexpr int lin_staging(int epi, bool slope) {
-    return epi == LE_PARTIAL ? 0 : LG_EPI_WARPS * (lin_warp_stage(slope) + (epi == LE_FORWARD ? LG_STRIP : 0));
+    return LG_EPI_WARPS * (lin_warp_stage(slope) + (epi == LE_FORWARD ? LG_STRIP : 0));
 }
 constexpr int LG_TAIL = 512;                      // barriers and the tensor-memory slot
 
@@ -44,16 +44,25 @@ struct LinEpilogue {
     const __nv_bfloat16* bias; const __nv_bfloat16* res; long long ldr;
     __nv_bfloat16* out; long long ldo;
     __half* slope;                                // (M, N) packed, or NULL
-    float* part;                                  // LE_PARTIAL: (splits, M, N)
     int act;
 };
-struct LinGemm {
+// One product: work items are (output tile, share of the contraction), all tiles of a share before the next share.
+struct LinShape {
     int m, n;                                     // output rows and columns
     int kb;                                       // stages of the whole contraction
-    int bn, a_mn, b_mn, stages, splits, tiles_m, tiles_n;
-    LinEpilogue e;
+    int bn, a_mn, b_mn, splits, tiles_m, tiles_n;
+    int items;                                    // tiles x splits
+    float* part;                                  // (splits, M, N) fp32 shares, where splits > 1
+};
+struct LinGemm {
+    LinShape q[2];                                // the second one may have no items
+    int items, stages, stage_bytes;
+    LinEpilogue e;                                // LE_FORWARD (of q[0])
+    const float* colpart; long long colblocks; __nv_bfloat16* db; int db_n;      // LE_PLAIN: db = column sums of colpart, if db
     int32_t* err;
 };
+struct LinMaps { CUtensorMap a[2], b[2], out[2], slope, res; };
+struct LinJoin { const float* part; LinEpilogue e; long long m, groups; int n, splits; };       // groups of 8 columns; 0: nothing
 
 // ---- elementwise pieces -------------------------------------------------------------------------------------------
 __device__ __forceinline__ float lin_ex2(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
@@ -157,6 +166,7 @@ __device__ __forceinline__ void lin_commit_both(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
                  ::"r"(bar), "h"(static_cast<uint16_t>(3)) : "memory");
 }
+__device__ __forceinline__ void lin_epilogue_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(32 * LG_EPI_WARPS) : "memory"); }
 // One lane of the (converged) warp.
 __device__ __forceinline__ bool lin_elect() {
     uint32_t is;
@@ -194,22 +204,17 @@ __device__ __forceinline__ void lin_tma_pair(uint32_t dst, const CUtensorMap* ma
                  ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(0), "r"(leader_bar) : "memory");
 }
 // ---- the product ----------------------------------------------------------------------------------------------------
-// Work item = (output tile, share of the contraction); items of the same share run over the column tiles first, so the
-// pairs working at one time read the same rows of A.  Pair p takes items p, p + pairs, ...
+// Items run over the column tiles first, so the pairs working at one time read the same rows of A.  Pair p takes items p,
+// p + pairs, ... of q[0] and then q[1].
 template <int EPI, int ACT, bool SLOPE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LG_THREADS, 1)
-linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_out,
-                   const __grid_constant__ CUtensorMap map_slope, const __grid_constant__ CUtensorMap map_res, LinGemm p) {
+linear_pair_kernel(const __grid_constant__ LinMaps maps, const __grid_constant__ LinGemm p) {
     extern __shared__ __align__(1024) uint8_t smem[];              // swizzle atoms start on 1024-byte boundaries; no room to round up
     if ((umma::smem_u32(smem) & 1023u) != 0) {                     // (every thread of both CTAs leaves: the launch reports itself)
         if (threadIdx.x == 0) atomicOr(p.err, KGE_ERR_WAIT_TIMEOUT);
         return;
     }
-    const int half_n = p.bn / 2;                                   // B columns staged by each CTA
-    const int b_slabs = (half_n + 63) / 64;
-    const int b_bytes = p.b_mn ? b_slabs * LG_SLAB : half_n * 128;
-    const int b_room = (b_bytes + 1023) & ~1023;                   // swizzle atoms start on 1024-byte boundaries
-    const int stage_bytes = LG_A_BYTES + b_room;
+    const int stage_bytes = p.stage_bytes;
     uint8_t* staging = smem + p.stages * stage_bytes;
     uint64_t* full = reinterpret_cast<uint64_t*>(staging + lin_staging(EPI, SLOPE));
     uint64_t* empty = full + p.stages;
@@ -222,7 +227,8 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
     const int warp = __shfl_sync(kFull, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const uint32_t rank = umma::cluster_ctarank();
     const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
-    const int tiles = p.tiles_m * p.tiles_n, items = tiles * p.splits;
+    const int items = p.items;
+    auto which = [&](int item) { return EPI == LE_PLAIN && item >= p.q[0].items ? 1 : 0; };
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < p.stages; ++s) { umma::mbar_init(&full[s], 1); umma::mbar_init(&empty[s], 1); }
@@ -246,18 +252,25 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
         // uniform registers, every copy and MMA gets its operands through moves, and a stage took its threads 650 cycles where
         // the MMAs take 512.
         const bool elected = lin_elect();
-        if (elected) { umma::prefetch_tensormap(&map_a); umma::prefetch_tensormap(&map_b); }
+        if (elected) { umma::prefetch_tensormap(&maps.a[0]); umma::prefetch_tensormap(&maps.b[0]); }
         const uint32_t lead0 = umma::map_to_cta(full0, 0);          // the leader's `full` barriers count the bytes of both CTAs
-        const uint32_t tx_pair = 2u * (LG_A_BYTES + b_bytes);
         int s = 0; uint32_t ph = 0;
         bool ok = true;
         for (int item = pair; item < items && ok; item += n_pairs) {
-            const int split = item / tiles, tile = item - split * tiles;
-            const int tm = tile / p.tiles_n;
+            const int w = which(item);
+            const LinShape& q = p.q[w];
+            const int half_n = q.bn / 2;                            // B columns staged by each CTA
+            const int b_slabs = (half_n + 63) / 64;
+            const uint32_t tx_pair = 2u * (LG_A_BYTES + (q.b_mn ? b_slabs * LG_SLAB : half_n * 128));
+            const CUtensorMap *map_a = &maps.a[w], *map_b = &maps.b[w];
+            const int mine = item - (w ? p.q[0].items : 0), tiles = q.tiles_m * q.tiles_n;
+            const int split = mine / tiles, tile = mine - split * tiles;
+            const int tm = tile / q.tiles_n;
             const int m0 = tm * 2 * LG_BM + static_cast<int>(rank) * LG_BM;
-            const int nb0 = (tile - tm * p.tiles_n) * p.bn + static_cast<int>(rank) * half_n;
-            const int kb0 = static_cast<int>(static_cast<long long>(p.kb) * split / p.splits);
-            const int kb1 = static_cast<int>(static_cast<long long>(p.kb) * (split + 1) / p.splits);
+            const int nb0 = (tile - tm * q.tiles_n) * q.bn + static_cast<int>(rank) * half_n;
+            const int kb0 = static_cast<int>(static_cast<long long>(q.kb) * split / q.splits);
+            const int kb1 = static_cast<int>(static_cast<long long>(q.kb) * (split + 1) / q.splits);
+            const bool a_mn = q.a_mn != 0, b_mn = q.b_mn != 0;
             for (int kb = kb0; kb < kb1; ++kb) {
                 ok = lin_wait(empty0 + 8 * s, ph ^ 1);
                 if (!ok) break;
@@ -265,17 +278,17 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
                     const uint32_t a = smem0 + s * stage_bytes, b = a + LG_A_BYTES, lead = lead0 + 8 * s;
                     if (rank == 0) lin_expect_tx(full0 + 8 * s, tx_pair);
                     const int k0 = kb * LG_BK;
-                    if (!p.a_mn) {
-                        lin_tma_pair(a, &map_a, k0, m0, lead);
+                    if (!a_mn) {
+                        lin_tma_pair(a, map_a, k0, m0, lead);
                     } else {
-                        lin_tma_pair(a, &map_a, m0, k0, lead);
-                        lin_tma_pair(a + LG_SLAB, &map_a, m0 + 64, k0, lead);
+                        lin_tma_pair(a, map_a, m0, k0, lead);
+                        lin_tma_pair(a + LG_SLAB, map_a, m0 + 64, k0, lead);
                     }
-                    if (!p.b_mn) {
-                        lin_tma_pair(b, &map_b, k0, nb0, lead);
+                    if (!b_mn) {
+                        lin_tma_pair(b, map_b, k0, nb0, lead);
                     } else {
-                        lin_tma_pair(b, &map_b, nb0, k0, lead);
-                        if (b_slabs > 1) lin_tma_pair(b + LG_SLAB, &map_b, nb0 + 64, k0, lead);
+                        lin_tma_pair(b, map_b, nb0, k0, lead);
+                        if (b_slabs > 1) lin_tma_pair(b + LG_SLAB, map_b, nb0 + 64, k0, lead);
                     }
                 }
                 __syncwarp();
@@ -290,16 +303,18 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
     } else if (warp == 1) {
         if (rank == 0) {
             const bool elected = lin_elect();
-            const uint64_t a_tmpl = p.a_mn ? umma::smem_desc_mn(0, LG_SLAB, 1024u, 2u) : umma::smem_desc_k_sw128(0);
-            const uint64_t b_tmpl = p.b_mn ? umma::smem_desc_mn(0, LG_SLAB, 1024u, 2u) : umma::smem_desc_k_sw128(0);
-            const uint32_t a_step = (p.a_mn ? 2048u : 32u) >> 4, b_step = (p.b_mn ? 2048u : 32u) >> 4;
-            const uint32_t idesc = umma::instr_desc(1u, 2 * LG_BM, static_cast<uint32_t>(p.bn), static_cast<uint32_t>(p.a_mn), static_cast<uint32_t>(p.b_mn));
             int s = 0, lt = 0; uint32_t ph = 0;
             bool ok = true;
             for (int item = pair; item < items && ok; item += n_pairs, ++lt) {
-                const int split = item / tiles;
-                const int nkb = static_cast<int>(static_cast<long long>(p.kb) * (split + 1) / p.splits) -
-                                static_cast<int>(static_cast<long long>(p.kb) * split / p.splits);
+                const int w = which(item);
+                const LinShape& q = p.q[w];
+                const uint64_t a_tmpl = q.a_mn ? umma::smem_desc_mn(0, LG_SLAB, 1024u, 2u) : umma::smem_desc_k_sw128(0);
+                const uint64_t b_tmpl = q.b_mn ? umma::smem_desc_mn(0, LG_SLAB, 1024u, 2u) : umma::smem_desc_k_sw128(0);
+                const uint32_t a_step = (q.a_mn ? 2048u : 32u) >> 4, b_step = (q.b_mn ? 2048u : 32u) >> 4;
+                const uint32_t idesc = umma::instr_desc(1u, 2 * LG_BM, static_cast<uint32_t>(q.bn), static_cast<uint32_t>(q.a_mn), static_cast<uint32_t>(q.b_mn));
+                const int split = (item - (w ? p.q[0].items : 0)) / (q.tiles_m * q.tiles_n);
+                const int nkb = static_cast<int>(static_cast<long long>(q.kb) * (split + 1) / q.splits) -
+                                static_cast<int>(static_cast<long long>(q.kb) * split / q.splits);
                 const int buf = lt & 1;
                 ok = lin_wait(acc_empty0 + 8 * buf, (static_cast<uint32_t>(lt >> 1) & 1) ^ 1);
                 if (!ok) break;
@@ -327,41 +342,70 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
         }
     } else {
         // thread = row of a block; the four warps of a lane quarter take the 32-column blocks of their rows in turn
-        const int q = warp & 3, part = (warp - 2) >> 2;
-        const int blocks = (p.bn + 31) / 32;
+        const int sub = warp & 3, part = (warp - 2) >> 2;
         uint8_t* mine = staging + (warp - 2) * lin_warp_stage(SLOPE);
         uint64_t* res_bar = res_full + 2 * (warp - 2);
         const bool has_res = EPI == LE_FORWARD && p.e.res != nullptr;
         const uint32_t swz = static_cast<uint32_t>(lane >> 1) & 3u;               // 64-byte swizzle: 16-byte piece c of row `lane` lies at c ^ swz
         float* strip = reinterpret_cast<float*>(staging + LG_EPI_WARPS * lin_warp_stage(SLOPE)) + 32 * (warp - 2);
         const uint32_t out_addr = umma::smem_u32(mine);
-        // tile coordinates of this item and the next, kept by addition (items of a split product: the tile within its share)
-        const int step_m = n_pairs / p.tiles_n, step_n = n_pairs - step_m * p.tiles_n;
-        int tm = pair / p.tiles_n, tn = pair - tm * p.tiles_n;                    // (in units of tiles over all shares)
-        const int row_in = static_cast<int>(rank) * LG_BM + q * 32;
+        const int row_in = static_cast<int>(rank) * LG_BM + sub * 32;
+        if (EPI == LE_PLAIN && p.db != nullptr) {
+            // db[c] = sum of its partial sums in fp32 and in a fixed order (16 interleaved sums a column), while the first tiles are
+            // multiplied: a kernel of its own took 3 us of the 8191 x 1024 x 400 backward pass
+            float* red = reinterpret_cast<float*>(staging);                       // 16 x 33: nothing is staged yet
+            for (int c0 = blockIdx.x * 32; c0 < p.db_n; c0 += gridDim.x * 32) {
+                const int c = c0 + lane;
+                float t = 0.f;
+                if (c < p.db_n) {
+#pragma unroll 8
+                    for (long long b = warp - 2; b < p.colblocks; b += LG_EPI_WARPS) t += p.colpart[b * p.db_n + c];
+                }
+                red[(warp - 2) * 33 + lane] = t;
+                lin_epilogue_barrier();
+                if (warp == 2 && c < p.db_n) {
+                    for (int w = 1; w < LG_EPI_WARPS; ++w) t += red[w * 33 + lane];
+                    p.db[c] = __float2bfloat16_rn(t);
+                }
+                lin_epilogue_barrier();
+            }
+        }
         int lt = 0, b = 0;
         uint32_t res_phase = 0, pending = 0;                                      // bit b: parity of buffer b's next load; a load is under way
         float bias_next = 0.f;
         // what the block at (row, col) needs from memory: its residual into buffer b, its bias into a register (whole warp calls)
         auto fetch = [&](bool exists, int row, int col, int b) {
             if (EPI != LE_FORWARD) return;
-            bias_next = exists && p.e.bias != nullptr && col + lane < p.n ? __bfloat162float(p.e.bias[col + lane]) : 0.f;
-            if (!has_res || !exists || row >= p.m || col >= p.n) return;
+            bias_next = exists && p.e.bias != nullptr && col + lane < p.q[0].n ? __bfloat162float(p.e.bias[col + lane]) : 0.f;
+            if (!has_res || !exists || row >= p.q[0].m || col >= p.q[0].n) return;
             pending |= 1u << b;
             if (lane == 0) {
                 umma::mbar_expect_tx(&res_bar[b], LG_BLOCK);
-                umma::tma_load_2d(mine + b * LG_BLOCK, &map_res, col, row, &res_bar[b]);
+                umma::tma_load_2d(mine + b * LG_BLOCK, &maps.res, col, row, &res_bar[b]);
             }
             __syncwarp();
         };
-        fetch(pair < items && part < blocks, tm * 2 * LG_BM + row_in, tn * p.bn + part * 32, 0);
+        // LE_FORWARD: coordinates of this tile and the next, kept by addition
+        const int step_m = n_pairs / p.q[0].tiles_n, step_n = n_pairs - step_m * p.q[0].tiles_n;
+        int tm = pair / p.q[0].tiles_n, tn = pair - tm * p.q[0].tiles_n;
+        fetch(pair < items && part < (p.q[0].bn + 31) / 32, tm * 2 * LG_BM + row_in, tn * p.q[0].bn + part * 32, 0);
         for (int item = pair; item < items; item += n_pairs, ++lt) {
-            int tm_next = tm + step_m, tn_next = tn + step_n;
-            if (tn_next >= p.tiles_n) { tn_next -= p.tiles_n; ++tm_next; }
-            const int split = EPI == LE_PARTIAL ? item / tiles : 0;
-            const int row = (tm - split * p.tiles_m) * 2 * LG_BM + row_in;
+            const int w = which(item);
+            const LinShape& q = p.q[w];
+            const int qm = q.m, qn = q.n, bn = q.bn, blocks = (bn + 31) / 32;
+            int tm_next = tm + step_m, tn_next = tn + step_n, split = 0;
+            if (EPI == LE_FORWARD) {
+                if (tn_next >= q.tiles_n) { tn_next -= q.tiles_n; ++tm_next; }
+            } else {
+                const int at = item - (w ? p.q[0].items : 0), tiles = q.tiles_m * q.tiles_n;
+                split = at / tiles;
+                tm = (at - split * tiles) / q.tiles_n;
+                tn = at - split * tiles - tm * q.tiles_n;
+            }
+            const bool shares = EPI == LE_PLAIN && q.splits > 1;
+            const int row = tm * 2 * LG_BM + row_in;
             const int buf = lt & 1;
-            const uint32_t taddr = tmem_base + buf * LG_ACC_COLS + (static_cast<uint32_t>(q * 32) << 16);
+            const uint32_t taddr = tmem_base + buf * LG_ACC_COLS + (static_cast<uint32_t>(sub * 32) << 16);
             bool ready = false;
             auto wait_full = [&]() { return lin_wait(acc_full0 + 8 * buf, static_cast<uint32_t>(lt >> 1) & 1); };
             auto drained = [&]() {                                                // this warp is done with the accumulator
@@ -372,8 +416,8 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
             bool ok = true;
 #pragma unroll 1
             for (int blk = part; blk < blocks; blk += 4, b ^= 1) {
-                const int col = tn * p.bn + blk * 32;
-                const bool live = row < p.m && col < p.n;                         // something of the block exists
+                const int col = tn * bn + blk * 32;
+                const bool live = row < qm && col < qn;                         // something of the block exists
                 const bool last = blk + 4 >= blocks;
                 if (EPI == LE_FORWARD) {
                     strip[lane] = bias_next;
@@ -397,9 +441,9 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
                     float v[16];
                     lin_tmem16(taddr + blk * 32 + h * 16, v);
                     if (last && h == 1) drained();
-                    if (EPI == LE_PARTIAL) {
-                        const int lim = live && row + lane < p.m && blk * 32 + h * 16 < p.bn ? p.n - (col + h * 16) : 0;
-                        float* d = p.e.part + (static_cast<long long>(split) * p.m + row + lane) * p.n + col + h * 16;
+                    if (shares) {
+                        const int lim = live && row + lane < qm && blk * 32 + h * 16 < bn ? qn - (col + h * 16) : 0;
+                        float* d = q.part + (static_cast<long long>(split) * qm + row + lane) * qn + col + h * 16;
                         if (lim > 0) lin_st8(d, reinterpret_cast<const uint32_t*>(v));
                         if (lim > 8) lin_st8(d + 8, reinterpret_cast<const uint32_t*>(v) + 8);
                         __syncwarp();
@@ -418,7 +462,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
                         if (h == 0) {             // the last block's copies have been read by now: its buffers take the next block
                             if (lane == 0) lin_wait_read();
                             __syncwarp();
-                            if (last) fetch(item + n_pairs < items, tm_next * 2 * LG_BM + row_in, tn_next * p.bn + part * 32, b ^ 1);
+                            if (last) fetch(item + n_pairs < items, tm_next * 2 * LG_BM + row_in, tn_next * bn + part * 32, b ^ 1);
                             else fetch(true, row, col + 128, b ^ 1);
                         }
                         if (SLOPE) {
@@ -436,12 +480,12 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
                     *p0 = make_uint4(w[0], w[1], w[2], w[3]);
                     *p1 = make_uint4(w[4], w[5], w[6], w[7]);
                 }
-                if (EPI != LE_PARTIAL) {
+                if (!shares) {
                     umma::fence_proxy_async();                                    // the staged block is visible to the copy engine
                     __syncwarp();
                     if (lane == 0 && live) {                                      // (rows and columns past the end are not written)
-                        lin_store_block(&map_out, out_addr + b * LG_BLOCK, col, row);
-                        if (SLOPE) lin_store_block(&map_slope, out_addr + 2 * LG_BLOCK, col, row);
+                        lin_store_block(&maps.out[w], out_addr + b * LG_BLOCK, col, row);
+                        if (SLOPE) lin_store_block(&maps.slope, out_addr + 2 * LG_BLOCK, col, row);
                         lin_commit();
                     }
                 }
@@ -459,7 +503,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
         }
         for (int i = 0; i < 2; ++i)                                               // only after a wait ran out: copies still under way
             if ((pending >> i) & 1u) umma::mbar_wait(&res_bar[i], (res_phase >> i) & 1u);
-        if (EPI != LE_PARTIAL && lane == 0) lin_wait_all();
+        if (lane == 0) lin_wait_all();
     }
     umma::tc_fence_before();
     __syncthreads();
@@ -467,18 +511,21 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
     if (warp == 1) { umma::tc_fence_after(); umma::tmem_dealloc_pair(tmem_base, 2 * LG_ACC_COLS); }
 }
 
-// Sum of the shares of a split contraction in share order, then the epilogue; one thread per 8 columns.
+// Sums of the shares of up to two split products in share order, then the epilogue; one thread per 8 columns.
 template <int EPI>
-__global__ void __launch_bounds__(256) linear_join_kernel(LinEpilogue e, long long m, int n, int splits) {
+__global__ void __launch_bounds__(256) linear_join_kernel(const __grid_constant__ LinJoin j0, const __grid_constant__ LinJoin j1) {
     let_next_start();
     after_previous();
-    const int per_row = n / 8;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < m * per_row; i += (long long)gridDim.x * 256) {
-        const long long row = i / per_row;
-        const int col = static_cast<int>(i - row * per_row) * 8;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < j0.groups + j1.groups; i += (long long)gridDim.x * 256) {
+        const LinJoin& j = EPI == LE_PLAIN && i >= j0.groups ? j1 : j0;
+        const long long at = &j == &j1 ? i - j0.groups : i, m = j.m;
+        const LinEpilogue& e = j.e;
+        const int n = j.n, per_row = n / 8, splits = j.splits;
+        const long long row = at / per_row;
+        const int col = static_cast<int>(at - row * per_row) * 8;
         float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
         for (int s = 0; s < splits; ++s) {
-            const float4* d = reinterpret_cast<const float4*>(e.part + (static_cast<long long>(s) * m + row) * n + col);
+            const float4* d = reinterpret_cast<const float4*>(j.part + (static_cast<long long>(s) * m + row) * n + col);
             const float4 a = __ldcs(d), b = __ldcs(d + 1);
             v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w; v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
         }
@@ -671,26 +718,6 @@ __global__ void __launch_bounds__(512) linear_dz_kernel(const __nv_bfloat16* __r
         colpart[block * n + c] = t;
     }
 }
-// db[c] = sum over row blocks, in fp32 and in a fixed order (32 interleaved partial sums per column)
-__global__ void __launch_bounds__(1024) linear_db_kernel(const float* colpart, long long blocks, int n, __nv_bfloat16* db) {
-    __shared__ float red[32][33];
-    let_next_start();
-    after_previous();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int c = blockIdx.x * 32 + lane;
-    float t = 0.f;
-    if (c < n) {
-#pragma unroll 8
-        for (long long b = warp; b < blocks; b += 32) t += colpart[b * n + c];
-    }
-    red[warp][lane] = t;
-    __syncthreads();
-    if (warp == 0 && c < n) {
-        for (int w = 1; w < 32; ++w) t += red[w][lane];
-        db[c] = __float2bfloat16_rn(t);
-    }
-}
-
 // ---- host -----------------------------------------------------------------------------------------------------------
 static int lin_sms() {
     int dev = 0, sms = 0;
@@ -704,24 +731,66 @@ static int lin_bn(long long n) {          // equal tiles of at most 256 columns:
     const long long tiles = (n + 255) / 256, unit = tiles > 1 ? 32 : 16;
     return static_cast<int>(((n + tiles - 1) / tiles + unit - 1) / unit * unit);
 }
-// Shares of the contraction: the count with the least (rounds of work items x stages per item + cost of the join).
-static int lin_splits(long long m, long long n, long long k, int sms) {
-    const int bn = lin_bn(n);
-    const long long tiles = ((m + 255) / 256) * ((n + bn - 1) / bn), kb = (k + 63) / 64, slots = sms / 2;
-    if (tiles >= slots) return 1;
-    double best = 0.0;
-    int pick = 1;
-    for (int s = 1; s <= 32 && s <= kb; ++s) {
-        const double rounds = static_cast<double>((tiles * s + slots - 1) / slots);
-        double t = rounds * (0.3 * bn / 256 * ((kb + s - 1) / s) + 1.0);             // us
-        if (s > 1) t += 2.5 + 8.0 * s * m * n / 6.0e6;
-        if (s == 1 || t < best) { best = t; pick = s; }
+struct LinDim { long long m, n, k; };       // out (m, n), contraction k
+// Shares of the contractions of the products of one launch (one, or dx and dw): the counts with the least estimated time.  The
+// first pair of each kind of load is followed through its items (longest items first); a pair takes about 0.4 us for a stage of
+// 256 columns and 1 us more for an item, the join 2.5 us and its traffic at 6 TB/s.
+static void lin_plan(const LinDim* d, int count, int sms, int* splits) {
+    const int slots = sms / 2;
+    long long tiles[2] = {0, 0}, kb[2] = {1, 1};
+    double stage[2] = {0, 0};
+    int cand[2][32], n_cand[2] = {1, 1};
+    cand[0][0] = cand[1][0] = 1;
+    for (int i = 0; i < count; ++i) {
+        const int bn = lin_bn(d[i].n);
+        tiles[i] = ((d[i].m + 255) / 256) * ((d[i].n + bn - 1) / bn);
+        kb[i] = (d[i].k + 63) / 64;
+        stage[i] = 0.4 * bn / 256;
+        if (tiles[i] >= slots) continue;
+        if (count == 1) {
+            for (int s = 2; s <= 32 && s <= kb[i]; ++s) cand[i][n_cand[i]++] = s;
+        } else {                              // half a round of pairs, one, two
+            for (int half = 1; half <= 4; half *= 2) {
+                const long long s = slots * half / (2 * tiles[i]);
+                if (s > cand[i][n_cand[i] - 1] && s <= 32 && s <= kb[i]) cand[i][n_cand[i]++] = static_cast<int>(s);
+            }
+        }
     }
-    return pick;
+    double best = 0.0;
+    splits[0] = splits[1] = 1;
+    for (int a = 0; a < n_cand[0]; ++a)
+        for (int b = 0; b < n_cand[1]; ++b) {
+            const int s[2] = {cand[0][a], cand[1][b]};
+            double item[2], join = 0.0;
+            long long items[2];
+            for (int i = 0; i < 2; ++i) {
+                item[i] = stage[i] * static_cast<double>((kb[i] + s[i] - 1) / s[i]) + 1.0;
+                items[i] = tiles[i] * s[i];
+                if (s[i] > 1) join += 8.0 * s[i] * d[i].m * d[i].n / 6.0e6;
+            }
+            const int l = item[1] > item[0] ? 1 : 0;
+            double t = 0.0;
+            for (long long p : {0LL, items[l] % slots}) {
+                const long long all = (items[0] + items[1] - p + slots - 1) / slots, longer = (items[l] - p + slots - 1) / slots;
+                const double mine = longer * item[l] + (all - longer) * item[1 - l];
+                if (mine > t) t = mine;
+            }
+            if (join > 0.0) t += join + 2.5;
+            if ((a == 0 && b == 0) || t < best) { best = t; splits[0] = s[0]; splits[1] = s[1]; }
+        }
+}
+static size_t lin_up(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
+static size_t lin_part_bytes(const LinDim* d, int count, int sms) {
+    int splits[2];
+    lin_plan(d, count, sms, splits);
+    size_t bytes = 0;
+    for (int i = 0; i < count; ++i)
+        if (splits[i] > 1) bytes += lin_up(sizeof(float) * static_cast<size_t>(splits[i]) * d[i].m * d[i].n);
+    return bytes;
 }
 
 template <int EPI, int ACT, bool SLOPE>
-static int lin_launch(const CUtensorMap (&maps)[5], const LinGemm& p, unsigned ctas, size_t smem, bool first, cudaStream_t s) {
+static int lin_launch(const LinMaps& maps, const LinGemm& p, unsigned ctas, size_t smem, bool first, cudaStream_t s) {
     static std::atomic<bool> attr_set[128];          // the shared-memory opt-in is per device and kernel
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return cuda_status(cudaGetLastError(), "cudaGetDevice");
@@ -740,71 +809,111 @@ static int lin_launch(const CUtensorMap (&maps)[5], const LinGemm& p, unsigned c
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = first ? 0 : 1;
-    cudaError_t e = cudaLaunchKernelEx(&cfg, linear_pair_kernel<EPI, ACT, SLOPE>, maps[0], maps[1], maps[2], maps[3], maps[4], p);
+    cudaError_t e = cudaLaunchKernelEx(&cfg, linear_pair_kernel<EPI, ACT, SLOPE>, maps, p);
     if (e != cudaSuccess) return cuda_status(e, "linear_pair_kernel");
     KGE_LAUNCH_CHECK("linear_pair_kernel");
     return 0;
 }
 
 template <int ACT>
-static int lin_launch_forward(const CUtensorMap (&maps)[5], const LinGemm& p, unsigned ctas, size_t smem, bool first, cudaStream_t s) {
-    return p.e.slope ? lin_launch<LE_FORWARD, ACT, true>(maps, p, ctas, smem, first, s)
-                     : lin_launch<LE_FORWARD, ACT, false>(maps, p, ctas, smem, first, s);
+static int lin_launch_forward(const LinMaps& maps, const LinGemm& p, unsigned ctas, size_t smem, cudaStream_t s) {
+    return p.e.slope ? lin_launch<LE_FORWARD, ACT, true>(maps, p, ctas, smem, true, s)
+                     : lin_launch<LE_FORWARD, ACT, false>(maps, p, ctas, smem, true, s);
 }
 
-// out[m][n] (+ epilogue) = sum_k A[m][k] B[n][k].  a_mn / b_mn: the operand lies as (k rows, m or n columns).
-static int lin_gemm(const void* a, long long lda, int a_mn, const void* b, long long ldb, int b_mn, long long m, long long n, long long k,
-                    LinEpilogue e, bool forward, bool first, float* part, size_t part_bytes, cudaStream_t s) {
+// out[m][n] = sum_k A[m][k] B[n][k].  a_mn / b_mn: the operand lies as (k rows, m or n columns).
+struct LinTask {
+    const void* a; long long lda; int a_mn;
+    const void* b; long long ldb; int b_mn;
+    LinDim d;
+    LinEpilogue e;
+};
+struct LinColumns { const float* colpart; long long blocks; int n; __nv_bfloat16* db; };
+// One product with the forward epilogue, or up to two plain ones and the column sums.  `first`: nothing of the call is ahead.
+static int lin_gemm(const LinTask* t, int count, bool forward, const LinColumns* cols, bool first, void* part, size_t part_bytes, cudaStream_t s) {
     const int sms = lin_sms();
+    LinDim d[2];
+    for (int i = 0; i < count; ++i) d[i] = t[i].d;
+    int splits[2] = {1, 1};
+    if (count > 0) lin_plan(d, count, sms, splits);
     LinGemm p;
     memset(&p, 0, sizeof(p));
-    p.m = static_cast<int>(m); p.n = static_cast<int>(n); p.kb = static_cast<int>((k + LG_BK - 1) / LG_BK);
-    p.bn = lin_bn(n); p.a_mn = a_mn; p.b_mn = b_mn;
-    p.tiles_m = static_cast<int>((m + 2 * LG_BM - 1) / (2 * LG_BM));
-    p.tiles_n = static_cast<int>((n + p.bn - 1) / p.bn);
-    p.splits = lin_splits(m, n, k, sms);
-    if (p.splits > 1 && (!part || part_bytes < sizeof(float) * static_cast<size_t>(p.splits) * m * n)) p.splits = 1;
-    e.part = part;
-    p.e = e;
+    p.q[0].tiles_m = p.q[0].tiles_n = p.q[1].tiles_m = p.q[1].tiles_n = p.q[0].bn = p.q[1].bn = 1;
     p.err = device_error_word();
     if (!p.err) { set_error("linear: no usable device"); return KGE_E_DEVICE; }
-    CUtensorMap maps[5];                        // A, B, out, slope, residual (the last three: one that exists stands in for one that does not)
-    CUtensorMap &ma = maps[0], &mb = maps[1];
-    int rc;
-    if ((rc = make_tensor_map_64b(&maps[2], e.out, m, n, static_cast<uint64_t>(e.ldo) * 2, 32))) return rc;
-    maps[3] = maps[4] = maps[2];
-    if (e.slope && (rc = make_tensor_map_64b(&maps[3], e.slope, m, n, static_cast<uint64_t>(n) * 2, 32))) return rc;
-    if (e.res && (rc = make_tensor_map_64b(&maps[4], e.res, m, n, static_cast<uint64_t>(e.ldr) * 2, 32))) return rc;
-    if (a_mn) rc = make_tensor_map_2d(&ma, a, 2, k, m, lda * 2, LG_BK, 64);
-    else rc = make_tensor_map_2d(&ma, a, 2, m, k, lda * 2, LG_BM, LG_BK);
-    if (rc) return rc;
-    if (b_mn) rc = make_tensor_map_2d(&mb, b, 2, k, n, ldb * 2, LG_BK, 64);
-    else rc = make_tensor_map_2d(&mb, b, 2, n, k, ldb * 2, static_cast<uint32_t>(p.bn / 2), LG_BK);
-    if (rc) return rc;
-    const int half_n = p.bn / 2;
-    const int b_room = ((b_mn ? (half_n + 63) / 64 * LG_SLAB : half_n * 128) + 1023) & ~1023;
-    const int stage = LG_A_BYTES + b_room;
-    const int staging = lin_staging(p.splits > 1 ? LE_PARTIAL : forward ? LE_FORWARD : LE_STORE, forward && e.slope != nullptr);
-    p.stages = (LG_MAX_SMEM - LG_TAIL - staging) / stage;          // 4 or 5 at 256 columns; 3 cost 6 %
+    if (cols) { p.colpart = cols->colpart; p.colblocks = cols->blocks; p.db_n = cols->n; p.db = cols->db; }
+    LinMaps maps;
+    LinJoin join[2];
+    memset(join, 0, sizeof(join));
+    memset(&maps, 0, sizeof(maps));
+    const bool fused = forward && splits[0] == 1;        // a split product gets its epilogue in the join
+    const bool slope = fused && t[0].e.slope != nullptr;
+    size_t used = 0;
+    long long items = 0, groups = 0;
+    // longest items first: what is short evens out the end
+    const int lead = count == 2 && (d[1].k + 63) / 64 / splits[1] * lin_bn(d[1].n) > (d[0].k + 63) / 64 / splits[0] * lin_bn(d[0].n) ? 1 : 0;
+    for (int at = 0; at < count; ++at) {
+        const int i = at ^ lead;
+        const LinTask& c = t[i];
+        const long long m = d[i].m, n = d[i].n, k = d[i].k;
+        LinShape& q = p.q[at];
+        q.m = static_cast<int>(m); q.n = static_cast<int>(n); q.kb = static_cast<int>((k + LG_BK - 1) / LG_BK);
+        q.bn = lin_bn(n); q.a_mn = c.a_mn; q.b_mn = c.b_mn;
+        q.tiles_m = static_cast<int>((m + 2 * LG_BM - 1) / (2 * LG_BM));
+        q.tiles_n = static_cast<int>((n + q.bn - 1) / q.bn);
+        q.splits = splits[i];
+        const long long mine = static_cast<long long>(q.tiles_m) * q.tiles_n * q.splits;
+        items += mine;
+        if (items >= (1LL << 30)) { set_error("linear: %lld tiles exceed the tile index", items); return KGE_E_RANGE; }
+        q.items = static_cast<int>(mine);
+        int rc;
+        if (q.splits > 1) {
+            const size_t need = lin_up(sizeof(float) * static_cast<size_t>(q.splits) * m * n);
+            if (used + need > part_bytes) { set_error("linear: the shares need %zu bytes of workspace, %zu are left", used + need, part_bytes); return KGE_E_WORKSPACE; }
+            q.part = reinterpret_cast<float*>(static_cast<char*>(part) + used);
+            used += need;
+            join[at].part = q.part; join[at].e = c.e; join[at].m = m; join[at].n = q.n; join[at].splits = q.splits;
+            join[at].groups = m * (n / 8);
+            groups += join[at].groups;
+        } else {
+            if ((rc = make_tensor_map_64b(&maps.out[at], c.e.out, m, n, static_cast<uint64_t>(c.e.ldo) * 2, 32))) return rc;
+            if (slope && (rc = make_tensor_map_64b(&maps.slope, c.e.slope, m, n, static_cast<uint64_t>(n) * 2, 32))) return rc;
+            if (fused && c.e.res && (rc = make_tensor_map_64b(&maps.res, c.e.res, m, n, static_cast<uint64_t>(c.e.ldr) * 2, 32))) return rc;
+        }
+        if (c.a_mn) rc = make_tensor_map_2d(&maps.a[at], c.a, 2, k, m, c.lda * 2, LG_BK, 64);
+        else rc = make_tensor_map_2d(&maps.a[at], c.a, 2, m, k, c.lda * 2, LG_BM, LG_BK);
+        if (rc) return rc;
+        const int half_n = q.bn / 2;
+        if (c.b_mn) rc = make_tensor_map_2d(&maps.b[at], c.b, 2, k, n, c.ldb * 2, LG_BK, 64);
+        else rc = make_tensor_map_2d(&maps.b[at], c.b, 2, n, k, c.ldb * 2, static_cast<uint32_t>(half_n), LG_BK);
+        if (rc) return rc;
+        const int b_room = ((c.b_mn ? (half_n + 63) / 64 * LG_SLAB : half_n * 128) + 1023) & ~1023;      // atoms start on 1024-byte boundaries
+        if (LG_A_BYTES + b_room > p.stage_bytes) p.stage_bytes = LG_A_BYTES + b_room;
+    }
+    if (fused) p.e = t[0].e;
+    if (p.stage_bytes == 0) p.stage_bytes = LG_A_BYTES;
+    p.items = static_cast<int>(items);
+    const int staging = lin_staging(fused ? LE_FORWARD : LE_PLAIN, slope);
+    p.stages = (LG_MAX_SMEM - LG_TAIL - staging) / p.stage_bytes;          // 4 or 5 at 256 columns; 3 cost 6 %
     if (p.stages > 8) p.stages = 8;
-    const size_t smem = static_cast<size_t>(p.stages) * stage + staging + LG_TAIL;
-    const long long items = static_cast<long long>(p.tiles_m) * p.tiles_n * p.splits;
-    if (items >= (1LL << 30)) { set_error("linear: %lld tiles exceed the tile index", items); return KGE_E_RANGE; }
-    const unsigned ctas = 2u * static_cast<unsigned>(items < sms / 2 ? items : sms / 2);
-    if (p.splits == 1) {
-        if (!forward) return lin_launch<LE_STORE, ACT_NONE, false>(maps, p, ctas, smem, first, s);
-        switch (e.act) {
-            case ACT_NONE: return lin_launch<LE_FORWARD, ACT_NONE, false>(maps, p, ctas, smem, first, s);
-            case ACT_RELU: return lin_launch_forward<ACT_RELU>(maps, p, ctas, smem, first, s);
-            case ACT_SILU: return lin_launch_forward<ACT_SILU>(maps, p, ctas, smem, first, s);
-            default: return lin_launch_forward<ACT_GELU>(maps, p, ctas, smem, first, s);
+    const size_t smem = static_cast<size_t>(p.stages) * p.stage_bytes + staging + LG_TAIL;
+    long long pairs = items;
+    if (p.db && pairs < (p.db_n + 63) / 64) pairs = (p.db_n + 63) / 64;    // a CTA sums 32 columns at a time
+    const unsigned ctas = 2u * static_cast<unsigned>(pairs < sms / 2 ? pairs : sms / 2);
+    if (fused) {
+        switch (t[0].e.act) {
+            case ACT_NONE: return lin_launch<LE_FORWARD, ACT_NONE, false>(maps, p, ctas, smem, true, s);
+            case ACT_RELU: return lin_launch_forward<ACT_RELU>(maps, p, ctas, smem, s);
+            case ACT_SILU: return lin_launch_forward<ACT_SILU>(maps, p, ctas, smem, s);
+            default: return lin_launch_forward<ACT_GELU>(maps, p, ctas, smem, s);
         }
     }
-    if ((rc = lin_launch<LE_PARTIAL, ACT_NONE, false>(maps, p, ctas, smem, first, s))) return rc;
-    const long long groups = (m * (n / 8) + 255) / 256;
-    const unsigned blocks = static_cast<unsigned>(groups < 148 * 8 ? groups : 148 * 8);
-    if (forward) KGE_LAUNCH_AFTER("linear_join_kernel", linear_join_kernel<LE_FORWARD>, blocks, 256u, s, e, m, p.n, p.splits);
-    else KGE_LAUNCH_AFTER("linear_join_kernel", linear_join_kernel<LE_STORE>, blocks, 256u, s, e, m, p.n, p.splits);
+    int rc = lin_launch<LE_PLAIN, ACT_NONE, false>(maps, p, ctas, smem, first, s);
+    if (rc || groups == 0) return rc;
+    const long long want = (groups + 255) / 256;
+    const unsigned blocks = static_cast<unsigned>(want < 148 * 8 ? want : 148 * 8);
+    if (forward) KGE_LAUNCH_AFTER("linear_join_kernel", linear_join_kernel<LE_FORWARD>, blocks, 256u, s, join[0], join[1]);
+    else KGE_LAUNCH_AFTER("linear_join_kernel", linear_join_kernel<LE_PLAIN>, blocks, 256u, s, join[0], join[1]);
     return 0;
 }
 
@@ -825,12 +934,6 @@ static int lin_few(const void* x, long long ldx, const void* w, long long ldw, l
     if (err != cudaSuccess) return cuda_status(err, "linear_few_kernel");
     KGE_LAUNCH_CHECK("linear_few_kernel");
     return 0;
-}
-
-static size_t lin_up(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
-static size_t lin_part_bytes(long long m, long long n, long long k, int sms) {
-    const int s = lin_splits(m, n, k, sms);
-    return s > 1 ? lin_up(sizeof(float) * static_cast<size_t>(s) * m * n) : 0;
 }
 
 }  // namespace kge
@@ -868,9 +971,14 @@ extern "C" {
 size_t kge_linear_workspace_bytes(int64_t m, int64_t k, int64_t n, int32_t act, int32_t backward) {
     if (m <= 0 || k <= 0 || n <= 0 || check_linear("kge_linear_workspace_bytes", m, k, n, act)) return 0;
     const int sms = lin_sms();
-    if (!backward) return m <= LF_ROWS ? 0 : lin_part_bytes(m, n, k, sms);
-    const size_t dx = lin_part_bytes(m, k, n, sms), dw = lin_part_bytes(k, n, m, sms);
-    return (act != ACT_NONE ? lin_up(2 * static_cast<size_t>(m) * n) : 0) + lin_up(sizeof(float) * ((m + LZ_ROWS - 1) / LZ_ROWS) * n) + (dx > dw ? dx : dw);
+    const LinDim fwd = {m, n, k}, both[2] = {{m, k, n}, {k, n, m}};
+    if (!backward) return m <= LF_ROWS ? 0 : lin_part_bytes(&fwd, 1, sms);
+    size_t part = lin_part_bytes(both, 2, sms);                              // both gradients, or either alone
+    for (int i = 0; i < 2; ++i) {
+        const size_t one = lin_part_bytes(&both[i], 1, sms);
+        if (one > part) part = one;
+    }
+    return (act != ACT_NONE ? lin_up(2 * static_cast<size_t>(m) * n) : 0) + lin_up(sizeof(float) * ((m + LZ_ROWS - 1) / LZ_ROWS) * n) + part;
 }
 
 int kge_linear_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* residual, int64_t ldr,
@@ -900,8 +1008,8 @@ int kge_linear_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, c
         if (m <= 4) return lin_few<4>(x, ldx, w, ldw, m, k, n, e, s);
         return lin_few<8>(x, ldx, w, ldw, m, k, n, e, s);
     }
-    return lin_gemm(x, pitch_of(ldx, m, k), 0, w, pitch_of(ldw, k, n), 1, m, n, k, e, true, true, static_cast<float*>(workspace), workspace_bytes,
-                    reinterpret_cast<cudaStream_t>(stream));
+    const LinTask t = {x, pitch_of(ldx, m, k), 0, w, pitch_of(ldw, k, n), 1, {m, n, k}, e};
+    return lin_gemm(&t, 1, true, nullptr, true, workspace, workspace_bytes, reinterpret_cast<cudaStream_t>(stream));
 }
 
 int kge_linear_backward(const void* dout, int64_t ldd, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* slope,
@@ -939,24 +1047,23 @@ int kge_linear_backward(const void* dout, int64_t ldd, const void* x, int64_t ld
             static_cast<int>(n), static_cast<unsigned>(strips));
         KGE_LAUNCH_CHECK("linear_dz_kernel");
     }
-    if (dbias) {
-        KGE_LAUNCH_AFTER("linear_db_kernel", linear_db_kernel, static_cast<unsigned>((n + 31) / 32), 1024u, s, colpart, blocks, static_cast<int>(n),
-                         static_cast<__nv_bfloat16*>(dbias));
-    }
-    bool first = !dz && !dbias;                   // nothing of this call is ahead of the first product
     const void* g = dz ? static_cast<const void*>(dz) : dout;
     const long long ldg = dz ? n : ldd;
-    LinEpilogue e;
-    memset(&e, 0, sizeof(e));
+    LinTask t[2];
+    memset(t, 0, sizeof(t));
+    int count = 0;
     if (dx) {
-        e.out = static_cast<__nv_bfloat16*>(dx); e.ldo = pitch_of(lddx, m, k);
-        if ((rc = lin_gemm(g, ldg, 0, w, pitch_of(ldw, k, n), 0, m, k, n, e, false, first, reinterpret_cast<float*>(ws), part_bytes, s))) return rc;
-        first = false;
+        t[count] = {g, ldg, 0, w, pitch_of(ldw, k, n), 0, {m, k, n}, {}};
+        t[count].e.out = static_cast<__nv_bfloat16*>(dx); t[count].e.ldo = pitch_of(lddx, m, k);
+        ++count;
     }
     if (dw) {
-        e.out = static_cast<__nv_bfloat16*>(dw); e.ldo = n;
-        if ((rc = lin_gemm(x, pitch_of(ldx, m, k), 1, g, ldg, 1, k, n, m, e, false, first, reinterpret_cast<float*>(ws), part_bytes, s))) return rc;
+        t[count] = {x, pitch_of(ldx, m, k), 1, g, ldg, 1, {k, n, m}, {}};
+        t[count].e.out = static_cast<__nv_bfloat16*>(dw); t[count].e.ldo = n;
+        ++count;
     }
+    const LinColumns cols = {colpart, blocks, static_cast<int>(n), static_cast<__nv_bfloat16*>(dbias)};
+    if (count > 0 || dbias) return lin_gemm(t, count, false, dbias ? &cols : nullptr, !dz && !dbias, ws, part_bytes, s);
     return 0;
 }
 
