@@ -345,7 +345,7 @@ struct RowPart {
 // Short rows: G lanes per row, up to G I vectors.  With one warp a row whatever its length, 10782 rows of 35 took three waves of
 // resident warps; four rows a warp also share the instructions of the rows' scalars.
 template <typename T, int G, int I, int MODE>
-__global__ void __launch_bounds__(256, 4) cand_group_kernel(CandArgs a) {
+__global__ void __launch_bounds__(256, I <= 4 ? 4 : 3) cand_group_kernel(CandArgs a) {
     constexpr int R = 32 / G;                                     // rows of a warp
     __shared__ double red[8];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gl = lane % G;
@@ -395,7 +395,8 @@ __global__ void __launch_bounds__(256, 4) cand_group_kernel(CandArgs a) {
 // A CTA, or a cluster, with one row each.  Its part of the row arrives by one bulk copy (in flight before anything else is
 // known about the row), is read twice from shared memory - online maximum and sum, then the gradient - and leaves by 16-byte
 // stores.  As many CTAs as shared memory holds (3 at 60 KB) share an SM, so that copies, arithmetic and stores of different
-// rows overlap.  Measured against rows in registers (4096 x 15000 fp32 / 1024 x 100000 bf16, us): see the launch code.
+// rows overlap.  Policy loss over 4096 x 15000 fp32 / 1024 x 100000 bf16: 77 / 87 us; a row in the registers of 512 threads
+// 95 / 136 us, of 256 threads 93 / 132 us; one CTA per SM with a ring of row slots 122 / 150 us.
 constexpr int kMaxCluster = 8;
 constexpr int kRowSlot = 4608, kRowSmem = 216 * 1024;          // vectors of a row per CTA, at most (72 KB: three CTAs per SM)
 template <typename T, int THREADS, int CTAS, int MODE>
@@ -837,8 +838,15 @@ static int cand_passes(const CandArgs& a, void* ws, int* n_partial, cudaStream_t
     return MODE == CM_POLICY ? cand_gradient<T>(a, coef, same_phase<T>(a), false, s) : 0;
 }
 
-// Which form: the smallest group that holds a row in registers; passes where the rows are too long for a cluster, where the
-// groups of all rows would leave most SMs idle, or where the gradient's alignment differs.
+// Which form: the smallest group of lanes that holds a row in registers, then a CTA a row, the smaller the shorter the row;
+// passes where the rows are too long for a cluster, where the groups of all rows would leave most SMs idle, or where the gradient's
+// alignment differs.  A row's own scalars cost a warp some 600 issue slots whatever its length, so few lanes a row win while the
+// lanes are busy (us, log_prob / policy loss):
+//   20000 x 420 fp32   16 lanes 11.4 / 19.0   32 lanes 12.4 / 22.3        but 800 x 900 bf16   16 lanes 4.2 / 7.3   32 lanes 3.7 / 6.3
+//   30000 x 300 bf16    8 lanes 11.4 / 18.5   16 lanes 12.4 / 21.1
+//   11237 x 2703 bf16  32 threads 18.1 / 33.0   64 threads 22.7 / 42.0     40000 x 1100 bf16   32 threads 43.6 / 66   64 threads 52 / 94
+//   12995 x 3297 fp32  64 threads 31.1 / 59.7   128 threads 33.5 / 62.0    32 threads 37.0 / 67.9
+//   8000 x 5600 fp32  128 threads 30.3 / 59.1   256 threads 37.5 / 67.0    4000 x 9200 fp32   128 threads 26.9 / 50.7   256 threads 26.0 / 49.8
 template <typename T, int MODE>
 static int cand_go(const CandArgs& a, void* ws, int* n_partial, cudaStream_t s) {
     const long long nv = a.n / Vec<T>::V;              // vectors of a row, at most
@@ -846,11 +854,12 @@ static int cand_go(const CandArgs& a, void* ws, int* n_partial, cudaStream_t s) 
     if (nv <= 8) return cand_groups<T, 8, 1, MODE>(a, n_partial, s);
     if (nv <= 16) return cand_groups<T, 8, 2, MODE>(a, n_partial, s);
     if (nv <= 32) return cand_groups<T, 8, 4, MODE>(a, n_partial, s);
-    if (nv <= 64) return cand_groups<T, 16, 4, MODE>(a, n_partial, s);
-    if (nv <= 128) return cand_groups<T, 32, 4, MODE>(a, n_partial, s);
+    if (nv <= 64) return cand_groups<T, 8, 8, MODE>(a, n_partial, s);
+    if (nv <= 128) return a.rows <= 148 * 16 ? cand_groups<T, 32, 4, MODE>(a, n_partial, s) : cand_groups<T, 16, 8, MODE>(a, n_partial, s);
     if (a.rows >= (1LL << 31) / kMaxCluster) return cand_passes<T, MODE>(a, ws, n_partial, s);      // (beyond a grid of one CTA a row)
-    if (nv <= 512) return cand_rows<T, 64, 16, MODE>(a, 1, nv, n_partial, s);
-    if (nv <= 1024) return cand_rows<T, 128, 10, MODE>(a, 1, nv, n_partial, s);
+    if (nv <= 512) return cand_rows<T, 32, 24, MODE>(a, 1, nv, n_partial, s);
+    if (nv <= 1024) return cand_rows<T, 64, 16, MODE>(a, 1, nv, n_partial, s);
+    if (nv <= 2048) return cand_rows<T, 128, 10, MODE>(a, 1, nv, n_partial, s);
     int cluster = 1;
     while (cluster <= kMaxCluster && nv > cluster * static_cast<long long>(kRowSlot)) cluster *= 2;
     if (cluster > kMaxCluster || a.rows * cluster < 32) return cand_passes<T, MODE>(a, ws, n_partial, s);
