@@ -69,14 +69,14 @@ __device__ __forceinline__ int pref_group_sum(int v) {
     return v;
 }
 
-// A group of G threads per row: one thread for a handful of negatives, a quarter warp, a warp, or a whole CTA.  VEC: four
+// A group of G threads per row: one thread for a handful of negatives, part of a warp, a warp, or a whole CTA.  VEC: four
 // negatives per access (all rows of neg, ref_neg, dneg on 16-byte and of mask on 4-byte boundaries).  The valid negatives of
 // a row are counted first - the mask is a thirteenth of the traffic and comes from L1 the second time - so that the main pass
 // writes final gradients; it requests U accesses of each array before it uses the first.  Without VEC a thread has the same four
 // negatives, read one by one: the order of the additions, and so every bit of the result, does not depend on alignment.
 template <int G, bool VEC, bool SQUARE, bool MASK>
-__global__ void __launch_bounds__(G > 256 ? G : 256) pref_kernel(PrefArgs a) {
-    constexpr int BLOCK = G > 256 ? G : 256;
+__global__ void __launch_bounds__(G > 32 ? G : 256) pref_kernel(PrefArgs a) {
+    constexpr int BLOCK = G > 32 ? G : 256;
     constexpr int W = 4;                           // consecutive negatives of a thread
     constexpr int U = G == 1 ? 1 : 2;
     __shared__ double red[32];
@@ -217,9 +217,9 @@ static long long pref_blocks(long long rows, int per) {
 
 template <int G, bool VEC, bool SQUARE, bool MASK>
 static int pref_go2(const PrefArgs& a, float* loss, cudaStream_t s) {
-    constexpr int per = G > 256 ? 1 : 256 / G;
+    constexpr int per = G > 32 ? 1 : 256 / G;
     const unsigned blocks = static_cast<unsigned>(pref_blocks(a.rows, per));
-    pref_kernel<G, VEC, SQUARE, MASK><<<blocks, G > 256 ? G : 256, 0, s>>>(a);
+    pref_kernel<G, VEC, SQUARE, MASK><<<blocks, G > 32 ? G : 256, 0, s>>>(a);
     KGE_LAUNCH_CHECK("pref_kernel");
     return launch_sum_partials(a.partial, static_cast<int>(blocks), loss, s);
 }
@@ -227,13 +227,23 @@ template <int G, bool VEC, bool SQUARE>
 static int pref_go(const PrefArgs& a, float* loss, cudaStream_t s) {
     return a.mask ? pref_go2<G, VEC, SQUARE, true>(a, loss, s) : pref_go2<G, VEC, SQUARE, false>(a, loss, s);
 }
+// Threads per row: the fewest that still fill the GPU, so that a thread has some eight negatives at once and few share a row's own
+// scalars and reductions.  us with reference and mask:
+//   400000 x 8      2 threads 16.2   4 threads 27.8   8 threads 51.4          100000 x 48   4 threads 15.0   8 threads 20.6
+//   60000 x 132     8 threads 24.2   32 threads 47.0        but 2000 x 100    8 threads 5.7    32 threads 4.2
+//   40000 x 512    32 threads 51.1    8 threads 54.8
+//   1336 x 3356   128 threads 11.9   32 threads 19.0   1024 threads 29.3      500 x 512   128 threads 4.7   32 threads 5.7
+//   5000 x 10000  256 threads 111   128 threads 115    32 threads 156         20 x 200000   1024 threads 42   256 threads 82
 template <bool VEC, bool SQUARE>
 static int pref_pick(const PrefArgs& a, float* loss, cudaStream_t s) {
     if (a.n <= 4) return pref_go<1, false, SQUARE>(a, loss, s);
-    if (a.n <= 64) return pref_go<8, VEC, SQUARE>(a, loss, s);
-    // a CTA per row where a warp per row would leave SMs without work
-    if (a.n > 2048 && a.rows < 148 * 16) return pref_go<1024, VEC, SQUARE>(a, loss, s);
-    return pref_go<32, VEC, SQUARE>(a, loss, s);
+    if (a.n <= 24) return pref_go<2, VEC, SQUARE>(a, loss, s);
+    if (a.n <= 64) return pref_go<4, VEC, SQUARE>(a, loss, s);
+    if (a.n <= 384 && a.rows >= 148 * 32) return pref_go<8, VEC, SQUARE>(a, loss, s);
+    if (a.n <= 2048 && a.rows >= 148 * 8) return pref_go<32, VEC, SQUARE>(a, loss, s);
+    if (a.n <= 8192) return pref_go<128, VEC, SQUARE>(a, loss, s);
+    if (a.n <= 65536 || a.rows >= 148 * 2) return pref_go<256, VEC, SQUARE>(a, loss, s);
+    return pref_go<1024, VEC, SQUARE>(a, loss, s);
 }
 
 static int launch_preference(const PrefArgs& a, float* loss, cudaStream_t s) {

@@ -162,6 +162,14 @@ def test_preference_logistic(rows, n, ref, mask, weight):
 
 
 @gpu
+@pytest.mark.parametrize("rows,n", [(300, 8), (301, 24), (130, 25), (100, 61), (4800, 68), (4740, 131), (1200, 200), (1190, 333), (40, 2044), (7, 9001), (5, 8200)])
+@pytest.mark.parametrize("mask", [False, True])
+def test_preference_every_group_of_threads(rows, n, mask):
+    pref_check(pref_case(rows, n, True, mask, True), beta=0.7, margin=0.2, smoothing=0.1)
+    pref_check(pref_case(rows, n, False, mask, False), kind="square", beta=0.3)
+
+
+@gpu
 @pytest.mark.parametrize("rows,n,mask", [(7, 1, False), (64, 20, True), (3, 1111, True)])
 def test_preference_square(rows, n, mask):
     pref_check(pref_case(rows, n, True, mask, True), kind="square", beta=0.3, margin=0.5)
@@ -307,6 +315,18 @@ def test_log_prob(rows, n, ragged, dtype):
     check_gradient(d, s, act, p, live, coef, 4 * EPS * coef.abs(), E, n)
     again, stats2 = losses.log_prob(ds, da, n_cand=dn, temperature=temp)
     assert torch.equal(logp, again) and torch.equal(d, losses.log_prob_backward(ds, da, stats2, dl.cuda(), n_cand=dn, temperature=temp))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,n", [(2400, 300), (2400, 700), (2369, 513)])
+def test_candidates_of_many_rows(rows, n, dtype):
+    """More rows than the GPU holds warps."""
+    s, act, n_cand, cnt, g = cand_case(rows, n, dtype, True)
+    policy_check(s, act, n_cand, cnt, g)
+    logp, stats = losses.log_prob(s.cuda(), act.cuda(), n_cand=n_cand.cuda(), temperature=0.8)
+    live, lp, p = cand_ref(s, act, cnt, 0.8)
+    assert ((logp.cpu().double() - lp).abs() <= rel_bound(s, cnt, 0.8) + 2 * EPS * lp.abs()).all()
 
 
 def policy64(lp, live, old, adv, ref, w, lo, hi, beta, scale):
