@@ -395,8 +395,44 @@ __global__ void __launch_bounds__(256, I <= 4 ? 4 : 3) cand_group_kernel(CandArg
 // A CTA, or a cluster, with one row each.  Its part of the row arrives by one bulk copy (in flight before anything else is
 // known about the row), is read twice from shared memory - online maximum and sum, then the gradient - and leaves by 16-byte
 // stores.  As many CTAs as shared memory holds (3 at 60 KB) share an SM, so that copies, arithmetic and stores of different
-// rows overlap.  Policy loss over 4096 x 15000 fp32 / 1024 x 100000 bf16: 77 / 87 us; a row in the registers of 512 threads
+// rows overlap.  Policy loss over 4096 x 15000 fp32 / 1024 x 100000 bf16: 78 / 86 us; a row in the registers of 512 threads
 // 95 / 136 us, of 256 threads 93 / 132 us; one CTA per SM with a ring of row slots 122 / 150 us.
+// The chosen candidate's place in shared memory reads as -infinity from here on, so that it adds nothing to S'; its score is the
+// caller's first maximum.  The thread that works on its vector calls this (one test for each vector instead cost an eighth of the
+// instructions).
+template <typename T>
+__device__ __forceinline__ float take_chosen(T* p) {
+    const float x = cand_get(p);
+    cand_put(p, -INFINITY);
+    return x;
+}
+// Maximum and sum over the vectors first, first + step, ... below nv; m comes in as the maximum so far.  Two vectors share a test for
+// a new maximum (rare after the first ones).
+template <typename T>
+__device__ __forceinline__ float2 online_sum(const uint4* sv, int first, int nv, int step, float& m, Scale2 c) {
+    constexpr int V = Vec<T>::V;
+    float2 sum = make_float2(0.f, 0.f);
+    float mz = finite_or_zero(m);
+    const uint4 low = make_uint4(Vec<T>::kLow, Vec<T>::kLow, Vec<T>::kLow, Vec<T>::kLow);
+    for (int v = first; v < nv; v += 2 * step) {
+        const uint4 r0 = sv[v], r1 = v + step < nv ? sv[v + step] : low;
+        const float vm = fmaxf(Vec<T>::max(r0), Vec<T>::max(r1));
+        if (vm > m) {                     // rescale what there is
+            mz = finite_or_zero(vm);
+            const float by = cand_exp(m - mz, c);
+            sum = __fmul2_rn(sum, make_float2(by, by));
+            m = vm;
+        }
+        float f[V], g[V];
+        Vec<T>::open(r0, f);
+        Vec<T>::open(r1, g);
+        cand_exps<V>(f, mz, c);
+        cand_exps<V>(g, mz, c);
+        cand_add<V>(sum, f);
+        cand_add<V>(sum, g);
+    }
+    return sum;
+}
 constexpr int kMaxCluster = 8;
 constexpr int kRowSlot = 4608, kRowSmem = 216 * 1024;          // vectors of a row per CTA, at most (72 KB: three CTAs per SM)
 template <typename T, int THREADS, int CTAS, int MODE>
@@ -436,10 +472,10 @@ __global__ void __launch_bounds__(THREADS, CTAS) cand_row_kernel(CandArgs a) {
     if (MODE == CM_POLICY && tid < 4) side = cand_side(a, row, tid);
     const int xi = rank == 0 ? extra_index<T>(q, a.n, tid) : -1;
     const float xe = xi >= 0 && xi < cnt ? cand_get(s + xi) : -INFINITY;
-    // this CTA's vector that holds the chosen candidate, and its place in it
-    const int av = act >= q.head && act < q.head + q.nv * V ? (act - q.head) / V - q.v0 : -1, ak = (act - q.head) % V;
-    float m = xe, rest = 0.f, mz = finite_or_zero(m);
-    float2 sum = make_float2(xi != act ? cand_exp(xe - mz, c) : 0.f, 0.f);
+    // this CTA's vector that holds the chosen candidate
+    const int av = act >= q.head && act < q.head + q.nv * V ? (act - q.head) / V - q.v0 : -1;
+    const bool mine_chosen = av >= 0 && av < have && av % THREADS == tid;
+    float m = -INFINITY, rest = 0.f, mz;
     __syncthreads();                      // the barrier exists
     if (!umma::mbar_wait(&full, 0)) {     // (the row's outputs are invalid; its copy is waited for once more)
         atomicOr(a.err, KGE_ERR_WAIT_TIMEOUT);
@@ -447,31 +483,15 @@ __global__ void __launch_bounds__(THREADS, CTAS) cand_row_kernel(CandArgs a) {
     }
     const uint4* sv = reinterpret_cast<const uint4*>(row_smem);
     const int whole = cnt >= a.n ? have : min(have, max(0, (cnt - q.head) / V - q.v0));      // vectors without padding in them
-#pragma unroll 2
-    for (int v = tid; v < have; v += THREADS) {
-        uint4 r = sv[v];
-        if (v >= whole) r = mask_past<T>(r, q.head + (q.v0 + v) * V, cnt);
-        const float vm = Vec<T>::max(r);
-        if (vm > m) {                     // a new maximum of this thread: rescale what it has (rare after the first vectors)
-            mz = finite_or_zero(vm);
-            const float by = cand_exp(m - mz, c);
-            sum = __fmul2_rn(sum, make_float2(by, by));
-            m = vm;
-        }
-        float f[V];
-        Vec<T>::open(r, f);
-        cand_exps<V>(f, mz, c);
-        if (v == av) {
-#pragma unroll
-            for (int k = 0; k < V; ++k) if (k == ak) f[k] = 0.f;
-        }
-        cand_add<V>(sum, f);
-    }
-    rest = sum.x + sum.y;
+    if (mine_chosen) m = take_chosen(reinterpret_cast<T*>(row_smem) + (act - q.head - q.v0 * V));
+    if (whole < have && whole % THREADS == tid)             // the vector that the count cuts: padding reads as -infinity
+        reinterpret_cast<uint4*>(row_smem)[whole] = mask_past<T>(sv[whole], q.head + (q.v0 + whole) * V, cnt);
+    const float2 sum = online_sum<T>(sv, tid, have, THREADS, m, c);
     {
         const float mine = m;
-        m = warp_max(m);
-        rest = warp_sum(rest * cand_exp(mine - finite_or_zero(m), c));
+        m = warp_max(fmaxf(m, xe));
+        mz = finite_or_zero(m);
+        rest = warp_sum((sum.x + sum.y) * cand_exp(mine - mz, c) + (xi != act ? cand_exp(xe - mz, c) : 0.f));
     }
     if (lane == 0) parts[warp] = make_float2(m, rest);
     if (MODE == CM_POLICY && tid < 4) sides[tid] = side;
@@ -518,13 +538,10 @@ __global__ void __launch_bounds__(THREADS, CTAS) cand_row_kernel(CandArgs a) {
             Vec<T>::open(sv[v], f);
             cand_exps<V>(f, mz, c);
             cand_scale<V>(f, -ga);
-            if (v == av) {
-#pragma unroll
-                for (int k = 0; k < V; ++k) if (k == ak) f[k] = fa;
-            }
             __stcs(dv + v, Vec<T>::close(f));
         }
-        for (int v = full_to + tid; v < mine; v += THREADS) {               // the vector that the count cuts, padding, dead rows
+        const int from = full_to <= tid ? tid : tid + (full_to - tid + THREADS - 1) / THREADS * THREADS;      // (a vector keeps its thread)
+        for (int v = from; v < mine; v += THREADS) {                        // the vector that the count cuts, padding, dead rows
             float f[V];
 #pragma unroll
             for (int k = 0; k < V; ++k) f[k] = 0.f;
@@ -533,10 +550,11 @@ __global__ void __launch_bounds__(THREADS, CTAS) cand_row_kernel(CandArgs a) {
                 float g[V];
                 Vec<T>::open(sv[v], g);
 #pragma unroll
-                for (int k = 0; k < V; ++k) if (at + k < cnt) f[k] = at + k == act ? fa : -ga * cand_exp(g[k] - mz, c);
+                for (int k = 0; k < V; ++k) if (at + k < cnt) f[k] = -ga * cand_exp(g[k] - mz, c);
             }
             __stcs(dv + v, Vec<T>::close(f));
         }
+        if (mine_chosen) cand_put(d + act, fa);             // over the vector just stored by this thread
         if (xi >= 0) cand_put(d + xi, xi >= cnt || ga == 0.f ? 0.f : xi == act ? fa : -ga * cand_exp(xe - mz, c));
     }
     if (csize > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -545,95 +563,103 @@ __global__ void __launch_bounds__(THREADS, CTAS) cand_row_kernel(CandArgs a) {
 // ---- rows cut over several CTAs, in passes ----------------------------------------------------------------------------
 // For a few long rows (every SM reads), rows that no cluster can hold, and rows whose gradient lies at another alignment.
 // Pass 1: (m, rest) of every chunk of a row; pass 2: a warp per row joins them; pass 3 (policy): the gradient, elementwise.
+// A chunk arrives in shared memory by one bulk copy, under way before anything else is known about its row: 16 rows of 4,000,000
+// fp32 scores 42 us (6.1 TB/s), with loads into registers instead 66 us; 1024 x 100000 bf16 45 us; CTAs that stay, with two slots each,
+// 52 us and 66 us.
+constexpr int kChunk = 8192;                                            // fp32 scores of a chunk, at most; bf16: twice as many
 template <typename T>
 __global__ void __launch_bounds__(256) cand_stats_kernel(CandArgs a, float2* parts, int chunk, int chunks) {
     constexpr int V = Vec<T>::V;
+    extern __shared__ __align__(128) uint8_t chunk_smem[];
+    __shared__ __align__(8) uint64_t full;
     __shared__ float2 red[8];
     let_next_start();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const Scale2 c = {a.c_hi, a.c_lo};
-    for (long long u = blockIdx.x; u < a.rows * chunks; u += gridDim.x) {
+    const uint4* sv = reinterpret_cast<const uint4*>(chunk_smem);
+    if (tid == 0) {
+        umma::mbar_init(&full, 1);
+        umma::fence_barrier_init();
+    }
+    uint32_t phase = 0;
+    for (long long u = blockIdx.x; u < a.rows * chunks; u += gridDim.x, phase ^= 1) {
         const long long row = u / chunks;
-        const int k = static_cast<int>(u - row * chunks);
-        const int cnt = cand_count(a, row), act = cand_action(a, row, cnt, tid == 0 && k == 0);
-        const int j0 = k * chunk, n = min(chunk, cnt - j0);                // (may be <= 0)
-        float m = -INFINITY, rest = 0.f;
-        if (n > 0) {
-            const T* s = static_cast<const T*>(a.scores) + row * a.ld + j0;
-            const int head = head_of(s, n), nv = (n - head) / V, la = act - j0;
-            const uint4* sv = reinterpret_cast<const uint4*>(s + head);
-            if (tid < 16) {
-                const int xi = tid < 8 ? (tid < head ? tid : -1) : (head + nv * V + tid - 8 < n ? head + nv * V + tid - 8 : -1);
-                if (xi >= 0) {
-                    m = cand_get(s + xi);
-                    rest = xi == la ? 0.f : cand_exp(m - finite_or_zero(m), c);
-                }
-            }
-            const int av = la >= head && la < head + nv * V ? (la - head) / V : -1;
-            float2 sum = make_float2(rest, 0.f);
-            for (int base = tid; base < nv; base += 4 * 256) {
-                uint4 r[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    r[i] = make_uint4(Vec<T>::kLow, Vec<T>::kLow, Vec<T>::kLow, Vec<T>::kLow);
-                    if (base + i * 256 < nv) r[i] = __ldcs(sv + base + i * 256);
-                }
-                const float bm = fmaxf(fmaxf(Vec<T>::max(r[0]), Vec<T>::max(r[1])), fmaxf(Vec<T>::max(r[2]), Vec<T>::max(r[3])));
-                const float top = fmaxf(m, bm), mz = finite_or_zero(top);
-                if (bm > m) {
-                    const float by = cand_exp(m - mz, c);
-                    sum = __fmul2_rn(sum, make_float2(by, by));
-                    m = top;
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float f[V];
-                    Vec<T>::open(r[i], f);
-                    cand_exps<V>(f, mz, c);
-                    if (base + i * 256 == av) {
-#pragma unroll
-                        for (int q = 0; q < V; ++q) if ((la - head) % V == q) f[q] = 0.f;
-                    }
-                    cand_add<V>(sum, f);
-                }
-            }
-            rest = sum.x + sum.y;
-        }
-#pragma unroll
-        for (int o = 16; o; o >>= 1) {
-            const float m2 = __shfl_xor_sync(kFull, m, o), r2 = __shfl_xor_sync(kFull, rest, o);
-            merge_parts(m, rest, m2, r2, c);
-        }
-        if (lane == 0) red[warp] = make_float2(m, rest);
-        __syncthreads();
+        const int k = static_cast<int>(u - row * chunks), j0 = k * chunk;
+        const int cnt = cand_count(a, row), n = max(0, min(chunk, cnt - j0));
+        const T* s = static_cast<const T*>(a.scores) + row * a.ld + j0;
+        const int head = head_of(s, n), nv = (n - head) / V;
         if (tid == 0) {
-            for (int w = 1; w < 8; ++w) merge_parts(m, rest, red[w].x, red[w].y, c);
-            parts[u] = make_float2(m, rest);
+            if (nv > 0) {
+                umma::mbar_expect_tx(&full, static_cast<uint32_t>(nv) * 16u);
+                asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                             ::"r"(umma::smem_u32(chunk_smem)), "l"(s + head), "r"(static_cast<uint32_t>(nv) * 16u), "r"(umma::smem_u32(&full)) : "memory");
+            } else {
+                umma::mbar_arrive(&full);
+            }
         }
-        __syncthreads();
+        const int act = cand_action(a, row, cnt, tid == 0 && k == 0), la = act - j0;
+        const int xi = tid < 8 ? (tid < head ? tid : -1) : tid < 16 && head + nv * V + tid - 8 < n ? head + nv * V + tid - 8 : -1;
+        const float xe = xi >= 0 ? cand_get(s + xi) : -INFINITY;
+        const int av = act >= 0 && la >= head && la < head + nv * V ? (la - head) / V : -1;
+        __syncthreads();                  // the barrier exists
+        if (!umma::mbar_wait(&full, phase)) {     // (the call's outputs are invalid; the copy is waited for once more)
+            atomicOr(a.err, KGE_ERR_WAIT_TIMEOUT);
+            umma::mbar_wait(&full, phase);
+        }
+        float m = -INFINITY;
+        if (av >= 0 && tid == (av & 255)) {
+            m = take_chosen(reinterpret_cast<T*>(chunk_smem) + (la - head));
+            umma::fence_proxy_async();    // (before the next chunk's copy)
+        }
+        float2 sum = online_sum<T>(sv, tid, nv, 256, m, c);
+        const float mine = m;
+        m = warp_max(fmaxf(m, xe));
+        const float mz = finite_or_zero(m);
+        float rest = warp_sum((sum.x + sum.y) * cand_exp(mine - mz, c) + (act < 0 || xi != la ? cand_exp(xe - mz, c) : 0.f));
+        if (lane == 0) red[warp] = make_float2(m, rest);
+        __syncthreads();                  // (also: the chunk has been read, the next one may arrive)
+        if (warp == 0) {
+            m = lane < 8 ? red[lane].x : -INFINITY;
+            rest = lane < 8 ? red[lane].y : 0.f;
+            const float own = m;
+            m = warp_max(m);
+            rest = warp_sum(rest * cand_exp(own - finite_or_zero(m), c));
+            if (lane == 0) parts[u] = make_float2(m, rest);
+        }
     }
 }
 
-template <typename T, int MODE>
+// WARPS warps per row: one, or the whole CTA for rows of many chunks
+template <typename T, int MODE, int WARPS>
 __global__ void __launch_bounds__(256) cand_join_kernel(CandArgs a, const float2* parts, int chunks, float* coef) {
     __shared__ double red[8];
+    __shared__ float2 merged[8];
     let_next_start();
     after_previous();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tid = threadIdx.x % (32 * WARPS);
     const Scale2 c = {a.c_hi, a.c_lo};
     double total = 0.0;
-    for (long long row = (long long)blockIdx.x * 8 + warp; row < a.rows; row += (long long)gridDim.x * 8) {
+    for (long long row = WARPS == 1 ? (long long)blockIdx.x * 8 + warp : blockIdx.x; row < a.rows; row += (long long)gridDim.x * (8 / WARPS)) {
         float m = -INFINITY, rest = 0.f;
-        for (int k = lane; k < chunks; k += 32) {
+#pragma unroll 4
+        for (int k = tid; k < chunks; k += 32 * WARPS) {
             const float2 q = parts[row * chunks + k];
             merge_parts(m, rest, q.x, q.y, c);
         }
-#pragma unroll
-        for (int o = 16; o; o >>= 1) {
-            const float m2 = __shfl_xor_sync(kFull, m, o), r2 = __shfl_xor_sync(kFull, rest, o);
-            merge_parts(m, rest, m2, r2, c);
+        float mine = m;
+        m = warp_max(m);
+        rest = warp_sum(rest * cand_exp(mine - finite_or_zero(m), c));
+        if (WARPS > 1) {
+            if (lane == 0) merged[warp] = make_float2(m, rest);
+            __syncthreads();
+            m = lane < WARPS ? merged[lane].x : -INFINITY;
+            rest = lane < WARPS ? merged[lane].y : 0.f;
+            mine = m;
+            m = warp_max(m);
+            rest = warp_sum(rest * cand_exp(mine - finite_or_zero(m), c));
+            __syncthreads();
         }
-        if (lane == 0) {
+        if (tid == 0) {
             const int act = cand_action(a, row, cand_count(a, row), false);
             const float sa = act >= 0 ? cand_get(static_cast<const T*>(a.scores) + row * a.ld + act) : 0.f;
             float ga;
@@ -752,10 +778,9 @@ constexpr int kCandMaxBlocks = 148 * 16;           // groups that take rows in t
 struct CandLayout { int chunk, chunks; size_t off_parts, off_coef, total; };
 static CandLayout cand_layout(long long rows, long long n) {
     CandLayout L;
-    // chunks of at least 8192 scores (32 KB of fp32: enough loads in flight per CTA), about 16 CTAs' worth of them per SM
-    long long per = (rows * n + 148 * 16 - 1) / (148 * 16);
-    per = per < 8192 ? 8192 : (per + 1023) / 1024 * 1024;
-    if (per > n) per = n > 0 ? n : 1;
+    // about eight chunks per SM, of 1024 to 8192 scores
+    long long per = (rows * n / (148 * 8) + 1023) / 1024 * 1024;
+    per = per < 1024 ? 1024 : per > kChunk ? kChunk : per;
     L.chunk = static_cast<int>(per);
     L.chunks = static_cast<int>((n + per - 1) / per);
     if (L.chunks < 1) L.chunks = 1;
@@ -829,12 +854,15 @@ static int cand_passes(const CandArgs& a, void* ws, int* n_partial, cudaStream_t
     const CandLayout L = cand_layout(a.rows, a.n);
     float2* parts = reinterpret_cast<float2*>(static_cast<char*>(ws) + L.off_parts);
     float* coef = reinterpret_cast<float*>(static_cast<char*>(ws) + L.off_coef);
-    const long long units = a.rows * L.chunks;
-    cand_stats_kernel<T><<<static_cast<unsigned>(units < 148 * 64 ? units : 148 * 64), 256, 0, s>>>(a, parts, L.chunk, L.chunks);
+    const int chunk = L.chunk * (4 / static_cast<int>(sizeof(T))), chunks = a.n > 0 ? (a.n - 1) / chunk + 1 : 1;      // the same bytes of either type
+    const long long units = a.rows * chunks;
+    cand_stats_kernel<T><<<static_cast<unsigned>(units < (1 << 30) ? units : (1 << 30)), 256, chunk * sizeof(T), s>>>(a, parts, chunk, chunks);
     KGE_LAUNCH_CHECK("cand_stats_kernel");
-    const long long jb = (a.rows + 7) / 8;
+    const bool wide = chunks > 64;
+    const long long jb = wide ? a.rows : (a.rows + 7) / 8;
     *n_partial = static_cast<int>(jb < kCandMaxBlocks ? jb : kCandMaxBlocks);
-    KGE_LAUNCH_AFTER("cand_join_kernel", cand_join_kernel<T, MODE>, static_cast<unsigned>(*n_partial), 256u, s, a, parts, L.chunks, coef);
+    if (wide) KGE_LAUNCH_AFTER("cand_join_kernel", (cand_join_kernel<T, MODE, 8>), static_cast<unsigned>(*n_partial), 256u, s, a, parts, chunks, coef);
+    else KGE_LAUNCH_AFTER("cand_join_kernel", (cand_join_kernel<T, MODE, 1>), static_cast<unsigned>(*n_partial), 256u, s, a, parts, chunks, coef);
     return MODE == CM_POLICY ? cand_gradient<T>(a, coef, same_phase<T>(a), false, s) : 0;
 }
 
@@ -863,6 +891,9 @@ static int cand_go(const CandArgs& a, void* ws, int* n_partial, cudaStream_t s) 
     int cluster = 1;
     while (cluster <= kMaxCluster && nv > cluster * static_cast<long long>(kRowSlot)) cluster *= 2;
     if (cluster > kMaxCluster || a.rows * cluster < 32) return cand_passes<T, MODE>(a, ws, n_partial, s);
+    // without a gradient nothing is read twice, and clusters only cost their barriers: 1000 x 100000 fp32 61 us in passes, 84 us in
+    // clusters; but 40 x 100000, with its second launch, 7.3 us and 6.7 us
+    if (MODE == CM_LOGP && cluster > 1 && a.rows * cluster >= 148 * 3) return cand_passes<T, MODE>(a, ws, n_partial, s);
     return cand_rows<T, 256, 5, MODE>(a, cluster, (nv + cluster - 1) / cluster, n_partial, s);
 }
 
