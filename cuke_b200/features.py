@@ -20,12 +20,16 @@ _CODES = {torch.float32: DTYPES["f32"], torch.bfloat16: DTYPES["bf16"]}
 
 def need_here(*ts) -> None:
     """The tensors are on the current CUDA device (the library launches on its current stream)."""
-    here = torch.cuda.current_device() if torch.cuda.is_available() else -2
+    here = -1
     for t in ts:
-        if t is not None and t.get_device() != here:
-            if not t.is_cuda:
-                raise ValueError("expected CUDA tensors")
-            raise ValueError(f"a tensor is on {t.device}, the current device is cuda:{here}; use torch.cuda.device(...)")
+        if t is not None:
+            at = t.get_device()
+            if at != here:
+                if at < 0:
+                    raise ValueError("expected CUDA tensors")
+                here = torch.cuda.current_device()
+                if at != here:
+                    raise ValueError(f"a tensor is on {t.device}, the current device is cuda:{here}; use torch.cuda.device(...)")
 
 
 def dtype_code(t: torch.Tensor) -> int:
