@@ -20,7 +20,7 @@ _CODES = {torch.float32: DTYPES["f32"], torch.bfloat16: DTYPES["bf16"]}
 
 def need_here(*ts) -> None:
     """The tensors are on the current CUDA device (the library launches on its current stream)."""
-    here = -1
+    here = None
     for t in ts:
         if t is not None:
             at = t.get_device()
