@@ -511,24 +511,38 @@ linear_pair_kernel(const __grid_constant__ LinMaps maps, const __grid_constant__
     if (warp == 1) { umma::tc_fence_after(); umma::tmem_dealloc_pair(tmem_base, 2 * LG_ACC_COLS); }
 }
 
-// Sums of the shares of up to two split products in share order, then the epilogue; one thread per 8 columns.
-template <int EPI>
+// Sums of the shares of up to two split products in a fixed order, then the epilogue.  8 columns per group of LANES threads, which
+// take the shares in turn: with one thread a group, 64 shares of a 128 x 128 gradient were a chain of 64 loads (11 us).
+template <int EPI, int LANES>
 __global__ void __launch_bounds__(256) linear_join_kernel(const __grid_constant__ LinJoin j0, const __grid_constant__ LinJoin j1) {
     let_next_start();
     after_previous();
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < j0.groups + j1.groups; i += (long long)gridDim.x * 256) {
-        const LinJoin& j = EPI == LE_PLAIN && i >= j0.groups ? j1 : j0;
-        const long long at = &j == &j1 ? i - j0.groups : i, m = j.m;
+    const long long total = j0.groups + j1.groups;
+    const int sub = threadIdx.x % LANES;
+    for (long long first = (long long)blockIdx.x * (256 / LANES); first < total; first += (long long)gridDim.x * (256 / LANES)) {
+        const bool live = first + threadIdx.x / LANES < total;                  // (all lanes take part in the shuffles)
+        const long long i = live ? first + threadIdx.x / LANES : total - 1;
+        const bool second = EPI == LE_PLAIN && i >= j0.groups;
+        const LinJoin& j = second ? j1 : j0;
+        const long long at = second ? i - j0.groups : i, m = j.m;
         const LinEpilogue& e = j.e;
         const int n = j.n, per_row = n / 8, splits = j.splits;
         const long long row = at / per_row;
         const int col = static_cast<int>(at - row * per_row) * 8;
         float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        for (int s = 0; s < splits; ++s) {
+#pragma unroll 4
+        for (int s = sub; s < splits; s += LANES) {
             const float4* d = reinterpret_cast<const float4*>(j.part + (static_cast<long long>(s) * m + row) * n + col);
             const float4 a = __ldcs(d), b = __ldcs(d + 1);
             v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w; v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
         }
+        if (LANES > 1) {
+#pragma unroll
+            for (int o = 1; o < LANES; o <<= 1)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) v[k] += __shfl_xor_sync(kFull, v[k], o);
+        }
+        if (!live || sub != 0) continue;
         if (EPI == LE_FORWARD) {
             uint4 bias = make_uint4(0u, 0u, 0u, 0u), res = bias;
             if (e.bias) bias = __ldg(reinterpret_cast<const uint4*>(e.bias + col));
@@ -727,65 +741,70 @@ static int lin_sms() {
     }
     return sms;
 }
-static int lin_bn(long long n) {          // equal tiles of at most 256 columns: whole 32-column blocks, or one tile in units of 16
-    const long long tiles = (n + 255) / 256, unit = tiles > 1 ? 32 : 16;
+// Columns of a tile when n columns are cut into so many: whole 32-column blocks, or one tile in units of 16.
+static int lin_bn(long long n, long long tiles) {
+    const long long unit = tiles > 1 ? 32 : 16;
     return static_cast<int>(((n + tiles - 1) / tiles + unit - 1) / unit * unit);
 }
+constexpr int LIN_MAX_SPLITS = 64;
 struct LinDim { long long m, n, k; };       // out (m, n), contraction k
-// Shares of the contractions of the products of one launch (one, or dx and dw): the counts with the least estimated time.  The
-// first pair of each kind of load is followed through its items (longest items first); a pair takes about 0.4 us for a stage of
-// 256 columns and 1 us more for an item, the join 2.5 us and its traffic at 6 TB/s.
-static void lin_plan(const LinDim* d, int count, int sms, int* splits) {
+struct LinPlan { int bn[2], splits[2]; };
+// Tile widths and shares of the contractions of the products of one launch (one, or dx and dw): the choice with the least estimated
+// time.  Widths: the fewest tiles of at most 256 columns, or two or four times as many (64 columns and more) while pairs would be idle.
+// Shares: 1, and what fills the pairs half, once or twice.  The first pair of each kind of load is followed through its items
+// (longest items first): 0.2 us + 0.2 us per 256 columns for a stage, 1 us for an item; the join 2.5 us and its traffic at 6 TB/s.
+// 4000 x 1024 x 512 with gelu, residual and slope: 10.9 us in tiles of 128 columns, 14.0 us of 256; backward 16.5 us of 256,
+// 19.6 us of 64.  16 x 2048 x 2048: 9.8 us in 9 shares of 256 columns, 12.9 us in tiles of 64.
+static LinPlan lin_plan(const LinDim* d, int count, int sms) {
     const int slots = sms / 2;
-    long long tiles[2] = {0, 0}, kb[2] = {1, 1};
-    double stage[2] = {0, 0};
-    int cand[2][32], n_cand[2] = {1, 1};
-    cand[0][0] = cand[1][0] = 1;
+    struct Option { double item, join; long long items; int bn, splits; } opt[2][16];
+    int n_opt[2] = {0, 0};
     for (int i = 0; i < count; ++i) {
-        const int bn = lin_bn(d[i].n);
-        tiles[i] = ((d[i].m + 255) / 256) * ((d[i].n + bn - 1) / bn);
-        kb[i] = (d[i].k + 63) / 64;
-        stage[i] = 0.4 * bn / 256;
-        if (tiles[i] >= slots) continue;
-        if (count == 1) {
-            for (int s = 2; s <= 32 && s <= kb[i]; ++s) cand[i][n_cand[i]++] = s;
-        } else {                              // half a round of pairs, one, two
-            for (int half = 1; half <= 4; half *= 2) {
-                const long long s = slots * half / (2 * tiles[i]);
-                if (s > cand[i][n_cand[i] - 1] && s <= 32 && s <= kb[i]) cand[i][n_cand[i]++] = static_cast<int>(s);
+        const long long rows = (d[i].m + 255) / 256, kb = (d[i].k + 63) / 64, least = (d[i].n + 255) / 256;
+        for (int times = 1; times <= 4; times *= 2) {
+            const long long cols = least * times, tiles = rows * cols;
+            if (times > 1 && (cols * 64 > d[i].n + 63 || tiles > slots)) break;
+            const int bn = lin_bn(d[i].n, cols);
+            long long last = 0;
+            for (int half = 0; half <= 4; half = half ? 2 * half : 1) {
+                long long s = half ? slots * half / (2 * tiles) : 1;
+                s = s < LIN_MAX_SPLITS ? s : LIN_MAX_SPLITS;
+                s = s < kb ? s : kb;
+                if (s <= last) continue;
+                last = s;
+                Option& o = opt[i][n_opt[i]++];
+                o.bn = bn;
+                o.splits = static_cast<int>(s);
+                o.item = (0.2 + 0.2 / 256 * bn) * static_cast<double>((kb + s - 1) / s) + 1.0;
+                o.join = s > 1 ? 8.0 / 6.0e6 * static_cast<double>(s * d[i].m * d[i].n) : 0.0;
+                o.items = tiles * s;
             }
         }
     }
-    double best = 0.0;
-    splits[0] = splits[1] = 1;
-    for (int a = 0; a < n_cand[0]; ++a)
-        for (int b = 0; b < n_cand[1]; ++b) {
-            const int s[2] = {cand[0][a], cand[1][b]};
-            double item[2], join = 0.0;
-            long long items[2];
-            for (int i = 0; i < 2; ++i) {
-                item[i] = stage[i] * static_cast<double>((kb[i] + s[i] - 1) / s[i]) + 1.0;
-                items[i] = tiles[i] * s[i];
-                if (s[i] > 1) join += 8.0 * s[i] * d[i].m * d[i].n / 6.0e6;
-            }
-            const int l = item[1] > item[0] ? 1 : 0;
+    if (count < 2) opt[1][n_opt[1]++] = {1.0, 0.0, 0, 0, 1};
+    LinPlan best = {};
+    double least = -1.0;
+    for (int a = 0; a < n_opt[0]; ++a)
+        for (int b = 0; b < n_opt[1]; ++b) {
+            const Option &x = opt[0][a], &y = opt[1][b];
+            const Option &lead = y.item > x.item ? y : x, &rest = y.item > x.item ? x : y;
             double t = 0.0;
-            for (long long p : {0LL, items[l] % slots}) {
-                const long long all = (items[0] + items[1] - p + slots - 1) / slots, longer = (items[l] - p + slots - 1) / slots;
-                const double mine = longer * item[l] + (all - longer) * item[1 - l];
+            for (long long p : {0LL, lead.items % slots}) {
+                const long long all = (lead.items + rest.items - p + slots - 1) / slots, longer = (lead.items - p + slots - 1) / slots;
+                const double mine = longer * lead.item + (all - longer) * rest.item;
                 if (mine > t) t = mine;
             }
-            if (join > 0.0) t += join + 2.5;
-            if ((a == 0 && b == 0) || t < best) { best = t; splits[0] = s[0]; splits[1] = s[1]; }
+            if (x.join + y.join > 0.0) t += x.join + y.join + 2.5;
+            if (least < 0.0 || t < least) { least = t; best = {{x.bn, y.bn}, {x.splits, y.splits}}; }
         }
+    return best;
 }
 static size_t lin_up(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
 static size_t lin_part_bytes(const LinDim* d, int count, int sms) {
-    int splits[2];
-    lin_plan(d, count, sms, splits);
+    const LinPlan plan = lin_plan(d, count, sms);
     size_t bytes = 0;
     for (int i = 0; i < count; ++i)
-        if (splits[i] > 1) bytes += lin_up(sizeof(float) * static_cast<size_t>(splits[i]) * d[i].m * d[i].n);
+        if (plan.splits[i] > 1) bytes += lin_up(sizeof(float) * static_cast<size_t>(plan.splits[i]) * d[i].m * d[i].n);
     return bytes;
 }
 
@@ -834,8 +853,8 @@ static int lin_gemm(const LinTask* t, int count, bool forward, const LinColumns*
     const int sms = lin_sms();
     LinDim d[2];
     for (int i = 0; i < count; ++i) d[i] = t[i].d;
-    int splits[2] = {1, 1};
-    if (count > 0) lin_plan(d, count, sms, splits);
+    const LinPlan plan = count > 0 ? lin_plan(d, count, sms) : LinPlan{{0, 0}, {1, 1}};
+    const int (&splits)[2] = plan.splits, (&bn)[2] = plan.bn;
     LinGemm p;
     memset(&p, 0, sizeof(p));
     p.q[0].tiles_m = p.q[0].tiles_n = p.q[1].tiles_m = p.q[1].tiles_n = p.q[0].bn = p.q[1].bn = 1;
@@ -851,14 +870,14 @@ static int lin_gemm(const LinTask* t, int count, bool forward, const LinColumns*
     size_t used = 0;
     long long items = 0, groups = 0;
     // longest items first: what is short evens out the end
-    const int lead = count == 2 && (d[1].k + 63) / 64 / splits[1] * lin_bn(d[1].n) > (d[0].k + 63) / 64 / splits[0] * lin_bn(d[0].n) ? 1 : 0;
+    const int lead = count == 2 && (d[1].k + 63) / 64 / splits[1] * bn[1] > (d[0].k + 63) / 64 / splits[0] * bn[0] ? 1 : 0;
     for (int at = 0; at < count; ++at) {
         const int i = at ^ lead;
         const LinTask& c = t[i];
         const long long m = d[i].m, n = d[i].n, k = d[i].k;
         LinShape& q = p.q[at];
         q.m = static_cast<int>(m); q.n = static_cast<int>(n); q.kb = static_cast<int>((k + LG_BK - 1) / LG_BK);
-        q.bn = lin_bn(n); q.a_mn = c.a_mn; q.b_mn = c.b_mn;
+        q.bn = bn[i]; q.a_mn = c.a_mn; q.b_mn = c.b_mn;
         q.tiles_m = static_cast<int>((m + 2 * LG_BM - 1) / (2 * LG_BM));
         q.tiles_n = static_cast<int>((n + q.bn - 1) / q.bn);
         q.splits = splits[i];
@@ -910,10 +929,15 @@ static int lin_gemm(const LinTask* t, int count, bool forward, const LinColumns*
     }
     int rc = lin_launch<LE_PLAIN, ACT_NONE, false>(maps, p, ctas, smem, first, s);
     if (rc || groups == 0) return rc;
-    const long long want = (groups + 255) / 256;
+    // (8191 x 1024 x 400, 9 shares of 51200 groups: one thread a group 20.6 us for the backward pass, eight 24.7 us; 39866 x 72 x 440,
+    // 37 shares of 3960: 27.3 and 22.8 us)
+    const bool many = (splits[0] >= 8 || splits[1] >= 8) && groups <= 148 * 64;
+    const long long want = many ? (groups + 31) / 32 : (groups + 255) / 256;
     const unsigned blocks = static_cast<unsigned>(want < 148 * 8 ? want : 148 * 8);
-    if (forward) KGE_LAUNCH_AFTER("linear_join_kernel", linear_join_kernel<LE_FORWARD>, blocks, 256u, s, join[0], join[1]);
-    else KGE_LAUNCH_AFTER("linear_join_kernel", linear_join_kernel<LE_PLAIN>, blocks, 256u, s, join[0], join[1]);
+    if (forward && many) KGE_LAUNCH_AFTER("linear_join_kernel", (linear_join_kernel<LE_FORWARD, 8>), blocks, 256u, s, join[0], join[1]);
+    else if (forward) KGE_LAUNCH_AFTER("linear_join_kernel", (linear_join_kernel<LE_FORWARD, 1>), blocks, 256u, s, join[0], join[1]);
+    else if (many) KGE_LAUNCH_AFTER("linear_join_kernel", (linear_join_kernel<LE_PLAIN, 8>), blocks, 256u, s, join[0], join[1]);
+    else KGE_LAUNCH_AFTER("linear_join_kernel", (linear_join_kernel<LE_PLAIN, 1>), blocks, 256u, s, join[0], join[1]);
     return 0;
 }
 
