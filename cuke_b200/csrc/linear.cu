@@ -1019,6 +1019,8 @@ int kge_linear_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, c
     const size_t need = kge_linear_workspace_bytes(m, k, n, act, 0);
     if (workspace_bytes < need) { set_error("%s: workspace needs %zu bytes, got %zu", fn, need, workspace_bytes); return KGE_E_WORKSPACE; }
     if (need && (rc = check_workspace(fn, workspace))) return rc;
+    if (out == x || out == w) { set_error("%s: out lies over an operand of the product", fn); return KGE_E_UNSUPPORTED; }
+    if (residual == out && m > 1 && ldr != ldo) { set_error("%s: out may be residual only with the same row pitch", fn); return KGE_E_SHAPE; }
     LinEpilogue e;
     memset(&e, 0, sizeof(e));
     e.bias = static_cast<const __nv_bfloat16*>(bias);
@@ -1057,6 +1059,8 @@ int kge_linear_backward(const void* dout, int64_t ldd, const void* x, int64_t ld
     const size_t need = kge_linear_workspace_bytes(m, k, n, act, 1);
     if (workspace_bytes < need) { set_error("%s: workspace needs %zu bytes, got %zu", fn, need, workspace_bytes); return KGE_E_WORKSPACE; }
     if ((rc = check_workspace(fn, workspace))) return rc;
+    for (const void* p : {dout, x, w, slope})
+        if (p && (p == dx || p == dw)) { set_error("%s: a gradient lies over an input", fn); return KGE_E_UNSUPPORTED; }
     char* ws = static_cast<char*>(workspace);
     __nv_bfloat16* dz = nullptr;
     if (act != ACT_NONE) { dz = reinterpret_cast<__nv_bfloat16*>(ws); ws += lin_up(2 * static_cast<size_t>(m) * lin_dz_pitch(n)); }

@@ -437,10 +437,11 @@ KGE_API int kge_policy_loss(const void* scores, int32_t dtype, int64_t ld, int64
  * entity rows computed from feature vectors instead of being read from a table.  w (k, n) has the orientation of the relation
  * matrices: out[j] = sum_i x[i] w[i][j].  act: none, relu, silu z s(z), gelu (tanh form) z s(2 sqrt(2/pi) (z + 0.044715 z^3)),
  * s the logistic function.  bias (n), residual (m, n) may be NULL.  slope: NULL, or (m, n) fp16 packed, receives act'(z) for the
- * backward call (not written for KGE_ACT_NONE).  residual may be out itself (same pitch).
+ * backward call (not written for KGE_ACT_NONE).  residual may be out itself (same pitch); outputs overlap nothing else.
  *   kge_linear_backward  dz = dout * slope (bf16);  dx = dz w^T (m, k);  dw = x^T dz (k, n) packed;  dbias = sum of dz over the rows
  *   (fp32 sums of the unrounded dz).  dx, dw, dbias may each be NULL (not computed); the gradient of residual is dout itself.
  * All operands are bf16 with 16-byte aligned bases and row pitches that are multiples of 8 elements; k, n multiples of 8; any m.
+ * (Row pitches that are multiples of 64 elements are read fastest.)
  * workspace (kge_linear_workspace_bytes; may be 0 bytes for the forward call) is 256-byte aligned.  The sums are taken in a fixed
  * order: the same call gives the same bits.  No reference counterpart. */
 #define KGE_ACT_NONE 0

@@ -44,6 +44,15 @@ def test_backward_refusals(kw, code):
 
 
 @needs_lib
+def test_outputs_over_inputs_are_refused():
+    x, w, out, res, dy, ws = (4096 * i for i in range(1, 7))
+    assert fwd(x=x, w=w, out=x, ws=ws) == -3 and fwd(x=x, w=w, out=w, ws=ws) == -3
+    assert fwd(x=x, w=w, out=out, res=out, ldr=32, ldo=24, ws=ws) == -4
+    for kw in (dict(dx=dy, dw=out), dict(dx=x, dw=out), dict(dx=w, dw=out), dict(dx=out, dw=res), dict(dx=NULL, dw=x)):
+        assert bwd(dout=dy, x=x, w=w, slope=res, ws=ws, db=NULL, **kw) == -3
+
+
+@needs_lib
 def test_workspace_sizes():
     W = _lib.lib().kge_linear_workspace_bytes
     assert W(0, 16, 16, 1, 1) == 0 and W(8, 12, 16, 1, 1) == 0 and fwd(m=0, x=NULL, out=NULL) == 0
