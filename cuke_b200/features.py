@@ -12,14 +12,14 @@ import torch
 
 from . import _lib
 from ._lib import ACTIVATIONS, DTYPES, check
-from .scoring import _ptr, _stream
+from .scoring import _ptr, _raw_stream
 
 
 _CODES = {torch.float32: DTYPES["f32"], torch.bfloat16: DTYPES["bf16"]}
 
 
-def need_here(*ts) -> None:
-    """The tensors are on the current CUDA device (the library launches on its current stream)."""
+def need_here(*ts) -> int:
+    """The number of the current CUDA device, which all the tensors are on (the library launches on its current stream)."""
     here = None
     for t in ts:
         if t is not None:
@@ -30,6 +30,12 @@ def need_here(*ts) -> None:
                 here = torch.cuda.current_device()
                 if at != here:
                     raise ValueError(f"a tensor is on {t.device}, the current device is cuda:{here}; use torch.cuda.device(...)")
+    return here
+
+
+def stream_on(here: int) -> int:
+    """Handle of the current stream of device `here`, as need_here returned it."""
+    return torch.cuda.current_stream(here).cuda_stream if _raw_stream is None else _raw_stream(here)
 
 
 def dtype_code(t: torch.Tensor) -> int:
@@ -42,6 +48,8 @@ def dtype_code(t: torch.Tensor) -> int:
 def pitch(t: torch.Tensor, name: str) -> int:
     """Row pitch in elements of a 2-D tensor whose columns are adjacent."""
     rows, cols = t.shape
+    if t.is_contiguous():
+        return cols or 1
     by_row, by_col = t.stride()
     if cols > 1 and by_col != 1:
         raise ValueError(f"{name}: the last dimension must be contiguous")
@@ -61,14 +69,17 @@ def dropout(x: torch.Tensor, p: float, seed: int, stream_id: int = 0, step: Unio
     dropout(d_out, p, seed, stream_id, step), the gradient of `residual` is d_out itself.  step may be a one-element int64
     CUDA tensor: it is read when the kernel runs, so a captured graph draws a new mask whenever that tensor is advanced
     between replays.  out may be x or residual itself."""
-    need_here(x, residual, out)
+    here = need_here(x, residual, out)
     dt = dtype_code(x)
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
         raise ValueError("residual must have the shape and dtype of x")
+    packed = x.is_contiguous() and (residual is None or residual.is_contiguous())
     if out is None:
-        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+        out = torch.empty_like(x) if packed else torch.empty_like(x, memory_format=torch.contiguous_format)
     elif out.shape != x.shape or out.dtype != x.dtype:
         raise ValueError("out must have the shape and dtype of x")
+    else:
+        packed = packed and out.is_contiguous()
     step_dev = None
     if isinstance(step, torch.Tensor):
         if step.dtype != torch.int64 or step.numel() != 1:
@@ -76,7 +87,7 @@ def dropout(x: torch.Tensor, p: float, seed: int, stream_id: int = 0, step: Unio
         need_here(step)
         step_dev, step = step.data_ptr(), 0
     ldr = 0
-    if x.is_contiguous() and out.is_contiguous() and (residual is None or residual.is_contiguous()):
+    if packed:
         n = x.numel()                                     # one run of elements, whatever the shape
         rows, dim = (1, n) if n < 1 << 31 else (n, 1)
         ldx = ldo = dim
@@ -92,8 +103,8 @@ def dropout(x: torch.Tensor, p: float, seed: int, stream_id: int = 0, step: Unio
         for other, ld in ((x, ldx), (residual, ldr)):
             if other is not None and other.data_ptr() == out.data_ptr() and rows > 1 and ld != ldo:
                 raise ValueError("out may be x or residual only with the same row pitch")
-    check(_lib.lib().kge_dropout(x.data_ptr(), dt, rows, dim, ldx, _ptr(residual), ldr, out.data_ptr(), ldo, p, int(seed) & 0xFFFFFFFFFFFFFFFF,
-                                 int(stream_id) & 0xFFFFFFFF, int(step) & 0x7FFFFFFF, step_dev, _stream()))
+    check(_lib.lib().kge_dropout(x.data_ptr(), dt, rows, dim, ldx, None if residual is None else residual.data_ptr(), ldr, out.data_ptr(), ldo, p,
+                                 int(seed) & 0xFFFFFFFFFFFFFFFF, int(stream_id) & 0xFFFFFFFF, int(step) & 0x7FFFFFFF, step_dev, stream_on(here)))
     return out
 
 
@@ -120,10 +131,10 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None
     bfloat16, accumulation is fp32 with one rounding at the end; K and N are multiples of 8, rows start on 16-byte
     boundaries.  act: "none", "relu", "silu" or "gelu" (tanh form).  With save_preact=True returns (out, preact), preact
     being what linear_backward needs of the pre-activation: act'(x w + bias) in float16, or None for act="none"."""
-    need_here(x, w, bias, residual, out)
+    here = need_here(x, w, bias, residual, out)
     if x.dim() != 2 or w.dim() != 2:
         raise ValueError("x and w must be matrices")
-    m, k, n = x.shape[0], x.shape[1], w.shape[1]
+    (m, k), n = x.shape, w.shape[1]
     code = _act(act)
     ldx, ldw = _matrix(x, "x", m, k), _matrix(w, "w", k, n)
     ldr = 0 if residual is None else _matrix(residual, "residual", m, n)
@@ -139,8 +150,8 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None
     L = _lib.lib()
     need = L.kge_linear_workspace_bytes(m, k, n, code, 0)
     ws = x.new_empty(need, dtype=torch.uint8) if need else None
-    check(L.kge_linear_forward(_ptr(x), ldx, _ptr(w), ldw, _ptr(bias), _ptr(residual), ldr, m, k, n, code, _ptr(out), ldo, _ptr(preact),
-                               _ptr(ws), need, _stream()))
+    check(L.kge_linear_forward(x.data_ptr(), ldx, w.data_ptr(), ldw, _ptr(bias), _ptr(residual), ldr, m, k, n, code, out.data_ptr(), ldo,
+                               _ptr(preact), _ptr(ws), need, stream_on(here)))
     return (out, preact) if save_preact else out
 
 
@@ -149,10 +160,10 @@ def linear_backward(dout: torch.Tensor, x: torch.Tensor, w: torch.Tensor, preact
                     need_dbias: bool = True) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor], Optional[torch.Tensor]]:
     """(dx, dw, dbias) of linear, bfloat16, from d(out) (M, N) and the preact it saved; None where not needed.  The gradient
     of `residual` is dout itself."""
-    need_here(dout, x, w, preact)
+    here = need_here(dout, x, w, preact)
     if x.dim() != 2 or w.dim() != 2:
         raise ValueError("x and w must be matrices")
-    m, k, n = x.shape[0], x.shape[1], w.shape[1]
+    (m, k), n = x.shape, w.shape[1]
     code = _act(act)
     ldd, ldx, ldw = _matrix(dout, "dout", m, n), _matrix(x, "x", m, k), _matrix(w, "w", k, n)
     if code and (preact is None or preact.dtype != torch.float16 or preact.shape != (m, n) or not preact.is_contiguous()):
@@ -163,6 +174,6 @@ def linear_backward(dout: torch.Tensor, x: torch.Tensor, w: torch.Tensor, preact
     L = _lib.lib()
     need = L.kge_linear_workspace_bytes(m, k, n, code, 1)
     ws = x.new_empty(need, dtype=torch.uint8) if need else None
-    check(L.kge_linear_backward(_ptr(dout), ldd, _ptr(x), ldx, _ptr(w), ldw, _ptr(preact) if code else None, m, k, n, code, _ptr(dx), k, _ptr(dw),
-                                _ptr(db), _ptr(ws), need, _stream()))
+    check(L.kge_linear_backward(dout.data_ptr(), ldd, x.data_ptr(), ldx, w.data_ptr(), ldw, preact.data_ptr() if code else None, m, k, n, code,
+                                _ptr(dx), k, _ptr(dw), _ptr(db), _ptr(ws), need, stream_on(here)))
     return dx, dw, db

@@ -13,8 +13,8 @@ import torch
 
 from . import _lib
 from ._lib import PREFERENCE_KINDS, check
-from .features import dtype_code, need_here, pitch
-from .scoring import _id_bits, _ptr, _stream
+from .features import dtype_code, need_here, pitch, stream_on
+from .scoring import _id_bits, _ptr
 
 
 def _floats(t: Optional[torch.Tensor], rows: int, name: str) -> Optional[torch.Tensor]:
@@ -40,7 +40,7 @@ def preference_loss(pos: torch.Tensor, neg: torch.Tensor, ref_pos: Optional[torc
     kind "logistic": (1 - smoothing) softplus(-z) + smoothing softplus(z); "square": z^2.  A positive's pairs are averaged
     over its valid negatives (mask True = valid; a row without any adds nothing), positives are weighted by `weight` (B,)
     and summed, or averaged over B with reduction="mean"."""
-    need_here(pos, neg, ref_pos, ref_neg, mask, weight)
+    here = need_here(pos, neg, ref_pos, ref_neg, mask, weight)
     rows = pos.numel()
     n = neg.shape[-1] if neg.dim() else 0
     if neg.dim() < 2 or neg.numel() != rows * n:
@@ -50,42 +50,45 @@ def preference_loss(pos: torch.Tensor, neg: torch.Tensor, ref_pos: Optional[torc
     if (ref_pos is None) != (ref_neg is None):
         raise ValueError("ref_pos and ref_neg come together")
 
-    def flat(t, name, dtype):
-        if t is None:
-            return None, 0
+    def row_pitch(t, name, dtype):
         if t.dtype != dtype or t.shape != neg.shape:
             raise ValueError(f"{name} must be {dtype} of the shape of neg")
+        if t.is_contiguous():
+            return n
         if t.dim() != 2:
-            if not t.is_contiguous():
-                raise ValueError(f"{name}: tensors that are not 2-D must be contiguous")
-            return t, n
-        return t, pitch(t, name)
+            raise ValueError(f"{name}: tensors that are not 2-D must be contiguous")
+        return pitch(t, name)
 
-    neg, ldn = flat(neg, "neg", torch.float32)
-    ref_neg, ldr = flat(ref_neg, "ref_neg", torch.float32)
-    mask, ldm = flat(mask, "mask", torch.bool)
-    _floats(pos, rows, "pos"), _floats(ref_pos, rows, "ref_pos"), _floats(weight, rows, "weight")
+    ldn, ldr, ldm = row_pitch(neg, "neg", torch.float32), 0, 0
+    _floats(pos, rows, "pos")
+    if ref_neg is not None:
+        ldr = row_pitch(ref_neg, "ref_neg", torch.float32)
+        _floats(ref_pos, rows, "ref_pos")
+    if mask is not None:
+        ldm = row_pitch(mask, "mask", torch.bool)
+    if weight is not None:
+        _floats(weight, rows, "weight")
     loss = pos.new_empty(1)
     dpos, dneg = torch.empty_like(pos), torch.empty_like(neg, memory_format=torch.contiguous_format)
     L = _lib.lib()
     need = L.kge_preference_workspace_bytes(rows, n)
     ws = pos.new_empty(need, dtype=torch.uint8)
-    check(L.kge_preference_loss(_ptr(pos), _ptr(ref_pos), _ptr(neg), ldn, _ptr(ref_neg), ldr, _ptr(mask), ldm, _ptr(weight), rows, n,
-                                PREFERENCE_KINDS[kind], float(beta), float(margin), float(smoothing), _scale(reduction, rows),
-                                _ptr(loss), _ptr(dpos), _ptr(dneg), max(n, 1), _ptr(ws), need, _stream()))
+    check(L.kge_preference_loss(pos.data_ptr(), _ptr(ref_pos), neg.data_ptr(), ldn, _ptr(ref_neg), ldr, _ptr(mask), ldm, _ptr(weight), rows, n,
+                                PREFERENCE_KINDS[kind], beta, margin, smoothing, _scale(reduction, rows),
+                                loss.data_ptr(), dpos.data_ptr(), dneg.data_ptr(), n or 1, ws.data_ptr(), need, stream_on(here)))
     return loss, dpos, dneg
 
 
 def _candidates(scores, action, n_cand):
-    need_here(scores, action, n_cand)
+    """What every call over candidates passes on first; the tensors' device has been checked."""
     if scores.dim() != 2:
         raise ValueError("scores must be (rows, candidates)")
-    rows = scores.shape[0]
+    rows, n = scores.shape
     if action.numel() != rows or not action.is_contiguous():
         raise ValueError("action must hold one id per row of scores")
     if n_cand is not None and (n_cand.dtype != torch.int32 or n_cand.numel() != rows or not n_cand.is_contiguous()):
         raise ValueError("n_cand must be a contiguous int32 tensor with one count per row of scores")
-    return _ptr(scores), dtype_code(scores), pitch(scores, "scores"), rows, scores.shape[1], _ptr(n_cand), _ptr(action), _id_bits(action)
+    return scores.data_ptr(), dtype_code(scores), pitch(scores, "scores"), rows, n, _ptr(n_cand), action.data_ptr(), _id_bits(action)
 
 
 def log_prob(scores: torch.Tensor, action: torch.Tensor, n_cand: Optional[torch.Tensor] = None,
@@ -94,6 +97,7 @@ def log_prob(scores: torch.Tensor, action: torch.Tensor, n_cand: Optional[torch.
 
     scores (rows, n) float32 or bfloat16, n_cand (rows,) int32: row r has its first n_cand[r] columns only; action (rows,)
     int32 / int64, -1 where nothing was chosen (logp 0, zero gradient).  stats is what log_prob_backward needs."""
+    here = need_here(scores, action, n_cand)
     how = _candidates(scores, action, n_cand)
     rows, n = how[3], how[4]
     logp = scores.new_empty(rows, dtype=torch.float32)
@@ -101,18 +105,18 @@ def log_prob(scores: torch.Tensor, action: torch.Tensor, n_cand: Optional[torch.
     L = _lib.lib()
     need = L.kge_candidates_workspace_bytes(rows, n)
     ws = scores.new_empty(need, dtype=torch.uint8)
-    check(L.kge_log_prob(*how, float(temperature), _ptr(logp), _ptr(stats), _ptr(ws), need, _stream()))
+    check(L.kge_log_prob(*how, temperature, logp.data_ptr(), stats.data_ptr(), ws.data_ptr(), need, stream_on(here)))
     return logp, stats
 
 
 def log_prob_backward(scores: torch.Tensor, action: torch.Tensor, stats: torch.Tensor, dlogp: torch.Tensor,
                       n_cand: Optional[torch.Tensor] = None, temperature: float = 1.0) -> torch.Tensor:
     """d(scores), in the dtype of scores, from d(logp) (rows,) and the stats of log_prob over the same arguments."""
+    here = need_here(scores, action, n_cand, stats, dlogp)
     how = _candidates(scores, action, n_cand)
-    need_here(stats, dlogp)
     _floats(stats, 3 * how[3], "stats"), _floats(dlogp, how[3], "dlogp")
     dscores = torch.empty_like(scores, memory_format=torch.contiguous_format)
-    check(_lib.lib().kge_log_prob_backward(*how, float(temperature), _ptr(stats), _ptr(dlogp), _ptr(dscores), max(how[4], 1), _stream()))
+    check(_lib.lib().kge_log_prob_backward(*how, temperature, stats.data_ptr(), dlogp.data_ptr(), dscores.data_ptr(), how[4] or 1, stream_on(here)))
     return dscores
 
 
@@ -126,20 +130,23 @@ def policy_loss(scores: torch.Tensor, action: torch.Tensor, old_logp: torch.Tens
     kl = exp(ref_logp - logp) - (ref_logp - logp) - 1 (needs ref_logp); rows are weighted by `weight` (0: the row adds nothing)
     and averaged over their number, or summed with reduction="sum".  scores, action, n_cand, temperature as in log_prob;
     dscores has the dtype of scores."""
+    here = need_here(scores, action, n_cand, old_logp, advantage, ref_logp, weight)
     how = _candidates(scores, action, n_cand)
     rows, n = how[3], how[4]
-    need_here(old_logp, advantage, ref_logp, weight)
     _floats(old_logp, rows, "old_logp"), _floats(advantage, rows, "advantage")
-    _floats(ref_logp, rows, "ref_logp"), _floats(weight, rows, "weight")
-    if kl_coef and ref_logp is None:
+    if ref_logp is not None:
+        _floats(ref_logp, rows, "ref_logp")
+    elif kl_coef:
         raise ValueError("kl_coef needs ref_logp")
+    if weight is not None:
+        _floats(weight, rows, "weight")
     loss = old_logp.new_empty(1)
     logp, kl = old_logp.new_empty(rows), old_logp.new_empty(rows)
     dscores = torch.empty_like(scores, memory_format=torch.contiguous_format)
     L = _lib.lib()
     need = L.kge_candidates_workspace_bytes(rows, n)
     ws = old_logp.new_empty(need, dtype=torch.uint8)
-    check(L.kge_policy_loss(*how, float(temperature), _ptr(old_logp), _ptr(ref_logp), _ptr(advantage), _ptr(weight), float(clip_low),
-                            float(clip_high), float(kl_coef), _scale(reduction, rows), _ptr(loss), _ptr(logp), _ptr(kl), _ptr(dscores),
-                            max(n, 1), _ptr(ws), need, _stream()))
+    check(L.kge_policy_loss(*how, temperature, old_logp.data_ptr(), _ptr(ref_logp), advantage.data_ptr(), _ptr(weight), clip_low, clip_high,
+                            kl_coef, _scale(reduction, rows), loss.data_ptr(), logp.data_ptr(), kl.data_ptr(), dscores.data_ptr(), n or 1,
+                            ws.data_ptr(), need, stream_on(here)))
     return loss, logp, kl, dscores
