@@ -802,8 +802,9 @@ static LinPlan lin_plan(const LinDim* d, int count, int sms) {
 // dz rows start on 128-byte lines, as the tiled loads read them: backward of 53333 x 520 x 696 123 us, with packed rows 145 us.
 static long long lin_dz_pitch(long long n) { return (n + 63) & ~63LL; }
 static size_t lin_up(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
-static size_t lin_part_bytes(const LinDim* d, int count, int sms) {
-    const LinPlan plan = lin_plan(d, count, sms);
+static size_t lin_dz_bytes(long long m, long long n, int act) { return act != ACT_NONE ? lin_up(2 * static_cast<size_t>(m) * lin_dz_pitch(n)) : 0; }
+static size_t lin_col_bytes(long long m, long long n) { return lin_up(sizeof(float) * ((m + LZ_ROWS - 1) / LZ_ROWS) * n); }
+static size_t lin_part_bytes(const LinDim* d, int count, const LinPlan& plan) {
     size_t bytes = 0;
     for (int i = 0; i < count; ++i)
         if (plan.splits[i] > 1) bytes += lin_up(sizeof(float) * static_cast<size_t>(plan.splits[i]) * d[i].m * d[i].n);
@@ -851,11 +852,10 @@ struct LinTask {
 };
 struct LinColumns { const float* colpart; long long blocks; int n; __nv_bfloat16* db; };
 // One product with the forward epilogue, or up to two plain ones and the column sums.  `first`: nothing of the call is ahead.
-static int lin_gemm(const LinTask* t, int count, bool forward, const LinColumns* cols, bool first, void* part, size_t part_bytes, cudaStream_t s) {
-    const int sms = lin_sms();
+static int lin_gemm(const LinTask* t, int count, const LinPlan& plan, int sms, bool forward, const LinColumns* cols, bool first, void* part,
+                    cudaStream_t s) {
     LinDim d[2];
     for (int i = 0; i < count; ++i) d[i] = t[i].d;
-    const LinPlan plan = count > 0 ? lin_plan(d, count, sms) : LinPlan{{0, 0}, {1, 1}};
     const int (&splits)[2] = plan.splits, (&bn)[2] = plan.bn;
     LinGemm p;
     memset(&p, 0, sizeof(p));
@@ -889,10 +889,8 @@ static int lin_gemm(const LinTask* t, int count, bool forward, const LinColumns*
         q.items = static_cast<int>(mine);
         int rc;
         if (q.splits > 1) {
-            const size_t need = lin_up(sizeof(float) * static_cast<size_t>(q.splits) * m * n);
-            if (used + need > part_bytes) { set_error("linear: the shares need %zu bytes of workspace, %zu are left", used + need, part_bytes); return KGE_E_WORKSPACE; }
             q.part = reinterpret_cast<float*>(static_cast<char*>(part) + used);
-            used += need;
+            used += lin_up(sizeof(float) * static_cast<size_t>(q.splits) * m * n);
             join[at].part = q.part; join[at].e = c.e; join[at].m = m; join[at].n = q.n; join[at].splits = q.splits;
             join[at].groups = m * (n / 8);
             groups += join[at].groups;
@@ -998,13 +996,13 @@ size_t kge_linear_workspace_bytes(int64_t m, int64_t k, int64_t n, int32_t act, 
     if (m <= 0 || k <= 0 || n <= 0 || check_linear("kge_linear_workspace_bytes", m, k, n, act)) return 0;
     const int sms = lin_sms();
     const LinDim fwd = {m, n, k}, both[2] = {{m, k, n}, {k, n, m}};
-    if (!backward) return m <= LF_ROWS ? 0 : lin_part_bytes(&fwd, 1, sms);
-    size_t part = lin_part_bytes(both, 2, sms);                              // both gradients, or either alone
+    if (!backward) return m <= LF_ROWS ? 0 : lin_part_bytes(&fwd, 1, lin_plan(&fwd, 1, sms));
+    size_t part = lin_part_bytes(both, 2, lin_plan(both, 2, sms));           // both gradients, or either alone
     for (int i = 0; i < 2; ++i) {
-        const size_t one = lin_part_bytes(&both[i], 1, sms);
+        const size_t one = lin_part_bytes(&both[i], 1, lin_plan(&both[i], 1, sms));
         if (one > part) part = one;
     }
-    return (act != ACT_NONE ? lin_up(2 * static_cast<size_t>(m) * lin_dz_pitch(n)) : 0) + lin_up(sizeof(float) * ((m + LZ_ROWS - 1) / LZ_ROWS) * n) + part;
+    return lin_dz_bytes(m, n, act) + lin_col_bytes(m, n) + part;
 }
 
 int kge_linear_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* residual, int64_t ldr,
@@ -1016,7 +1014,10 @@ int kge_linear_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, c
     if ((rc = check_rows(fn, "x", x, ldx, m, k, true)) || (rc = check_rows(fn, "w", w, ldw, k, n, true)) ||
         (rc = check_rows(fn, "bias", bias, n, 1, n, false)) || (rc = check_rows(fn, "residual", residual, ldr, m, n, false)) ||
         (rc = check_rows(fn, "out", out, ldo, m, n, true)) || (rc = check_rows(fn, "slope", slope, n, m, n, false))) return rc;
-    const size_t need = kge_linear_workspace_bytes(m, k, n, act, 0);
+    const int sms = lin_sms();
+    const LinDim dim = {m, n, k};
+    const LinPlan plan = m <= LF_ROWS ? LinPlan{{0, 0}, {1, 1}} : lin_plan(&dim, 1, sms);
+    const size_t need = lin_part_bytes(&dim, 1, plan);
     if (workspace_bytes < need) { set_error("%s: workspace needs %zu bytes, got %zu", fn, need, workspace_bytes); return KGE_E_WORKSPACE; }
     if (need && (rc = check_workspace(fn, workspace))) return rc;
     if (out == x || out == w) { set_error("%s: out lies over an operand of the product", fn); return KGE_E_UNSUPPORTED; }
@@ -1037,7 +1038,7 @@ int kge_linear_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, c
         return lin_few<8>(x, ldx, w, ldw, m, k, n, e, s);
     }
     const LinTask t = {x, pitch_of(ldx, m, k), 0, w, pitch_of(ldw, k, n), 1, {m, n, k}, e};
-    return lin_gemm(&t, 1, true, nullptr, true, workspace, workspace_bytes, reinterpret_cast<cudaStream_t>(stream));
+    return lin_gemm(&t, 1, plan, sms, true, nullptr, true, workspace, reinterpret_cast<cudaStream_t>(stream));
 }
 
 int kge_linear_backward(const void* dout, int64_t ldd, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* slope,
@@ -1056,18 +1057,21 @@ int kge_linear_backward(const void* dout, int64_t ldd, const void* x, int64_t ld
     if ((rc = check_rows(fn, "dout", dout, ldd, m, n, true)) || (rc = check_rows(fn, "x", x, ldx, m, k, dw != nullptr)) ||
         (rc = check_rows(fn, "w", w, ldw, k, n, dx != nullptr)) || (rc = check_rows(fn, "slope", slope, n, m, n, act != ACT_NONE)) ||
         (rc = check_rows(fn, "dx", dx, lddx, m, k, false))) return rc;
-    const size_t need = kge_linear_workspace_bytes(m, k, n, act, 1);
+    const int sms = lin_sms(), count = (dx != nullptr) + (dw != nullptr);
+    const LinDim both[2] = {{m, k, n}, {k, n, m}}, *dim = dx ? both : both + 1;          // dx and dw, or the one that is wanted
+    const LinPlan plan = count > 0 ? lin_plan(dim, count, sms) : LinPlan{{0, 0}, {1, 1}};
+    const size_t need = lin_dz_bytes(m, n, act) + lin_col_bytes(m, n) + lin_part_bytes(dim, count, plan);
     if (workspace_bytes < need) { set_error("%s: workspace needs %zu bytes, got %zu", fn, need, workspace_bytes); return KGE_E_WORKSPACE; }
     if ((rc = check_workspace(fn, workspace))) return rc;
     for (const void* p : {dout, x, w, slope})
         if (p && (p == dx || p == dw)) { set_error("%s: a gradient lies over an input", fn); return KGE_E_UNSUPPORTED; }
     char* ws = static_cast<char*>(workspace);
     __nv_bfloat16* dz = nullptr;
-    if (act != ACT_NONE) { dz = reinterpret_cast<__nv_bfloat16*>(ws); ws += lin_up(2 * static_cast<size_t>(m) * lin_dz_pitch(n)); }
+    if (act != ACT_NONE) dz = reinterpret_cast<__nv_bfloat16*>(ws);
+    ws += lin_dz_bytes(m, n, act);
     const long long blocks = (m + LZ_ROWS - 1) / LZ_ROWS;
     float* colpart = reinterpret_cast<float*>(ws);
-    ws += lin_up(sizeof(float) * blocks * n);
-    const size_t part_bytes = workspace_bytes - static_cast<size_t>(ws - static_cast<char*>(workspace));
+    ws += lin_col_bytes(m, n);
     ldd = pitch_of(ldd, m, n);
     if (dz || dbias) {
         const long long strips = (n + 255) / 256;
@@ -1081,19 +1085,18 @@ int kge_linear_backward(const void* dout, int64_t ldd, const void* x, int64_t ld
     const long long ldg = dz ? lin_dz_pitch(n) : ldd;
     LinTask t[2];
     memset(t, 0, sizeof(t));
-    int count = 0;
+    int at = 0;
     if (dx) {
-        t[count] = {g, ldg, 0, w, pitch_of(ldw, k, n), 0, {m, k, n}, {}};
-        t[count].e.out = static_cast<__nv_bfloat16*>(dx); t[count].e.ldo = pitch_of(lddx, m, k);
-        ++count;
+        t[at] = {g, ldg, 0, w, pitch_of(ldw, k, n), 0, both[0], {}};
+        t[at].e.out = static_cast<__nv_bfloat16*>(dx); t[at].e.ldo = pitch_of(lddx, m, k);
+        ++at;
     }
     if (dw) {
-        t[count] = {x, pitch_of(ldx, m, k), 1, g, ldg, 1, {k, n, m}, {}};
-        t[count].e.out = static_cast<__nv_bfloat16*>(dw); t[count].e.ldo = n;
-        ++count;
+        t[at] = {x, pitch_of(ldx, m, k), 1, g, ldg, 1, both[1], {}};
+        t[at].e.out = static_cast<__nv_bfloat16*>(dw); t[at].e.ldo = n;
     }
     const LinColumns cols = {colpart, blocks, static_cast<int>(n), static_cast<__nv_bfloat16*>(dbias)};
-    if (count > 0 || dbias) return lin_gemm(t, count, false, dbias ? &cols : nullptr, !dz && !dbias, ws, part_bytes, s);
+    if (count > 0 || dbias) return lin_gemm(t, count, plan, sms, false, dbias ? &cols : nullptr, !dz && !dbias, ws, s);
     return 0;
 }
 
