@@ -493,6 +493,13 @@ __global__ void __launch_bounds__(THREADS, CTAS) cand_row_kernel(CandArgs a) {
         mz = finite_or_zero(m);
         rest = warp_sum((sum.x + sum.y) * cand_exp(mine - mz, c) + (xi != act ? cand_exp(xe - mz, c) : 0.f));
     }
+    RowSide o = {};
+    if (kWarps == 1) {                    // (one warp: always a row of its own)
+        if (MODE == CM_POLICY) {
+            o.w = __shfl_sync(kFull, side, 0); o.adv = __shfl_sync(kFull, side, 1);
+            o.old = __shfl_sync(kFull, side, 2); o.ref = __shfl_sync(kFull, side, 3);
+        }
+    } else {
     if (lane == 0) parts[warp] = make_float2(m, rest);
     if (MODE == CM_POLICY && tid < 4) sides[tid] = side;
     if (csize == 1) __syncthreads();
@@ -519,16 +526,22 @@ __global__ void __launch_bounds__(THREADS, CTAS) cand_row_kernel(CandArgs a) {
         mz = finite_or_zero(m);
         rest = warp_sum(rest * cand_exp(mine - mz, c));
     }
+    if (MODE == CM_POLICY && tid == 0) o = RowSide{sides[0], sides[1], sides[2], sides[3]};
+    }
+    float ga = 0.f;
     if (tid == 0) {
-        float ga = 0.f;
-        const RowSide o = {sides[0], sides[1], sides[2], sides[3]};
         const double l = cand_finish<MODE>(a, row, act, sa, mz, rest, rank == 0, o, &ga);
-        bcast = ga;
+        if (kWarps > 1) bcast = ga;
         if (MODE == CM_POLICY && rank == 0) a.partial[row] = l;
     }
     if (MODE == CM_POLICY) {
-        __syncthreads();
-        const float ga = bcast, fa = ga == 0.f ? 0.f : ga * rest;
+        if (kWarps > 1) {
+            __syncthreads();
+            ga = bcast;
+        } else {
+            ga = __shfl_sync(kFull, ga, 0);
+        }
+        const float fa = ga == 0.f ? 0.f : ga * rest;
         T* d = static_cast<T*>(a.dscores) + row * a.ldd;
         uint4* dv = reinterpret_cast<uint4*>(d + q.head) + q.v0;
         const int mine = q.v1 - q.v0, full_to = ga == 0.f ? 0 : whole;
