@@ -435,19 +435,23 @@ __device__ __forceinline__ float2 online_sum(const uint4* sv, int first, int nv,
 }
 constexpr int kMaxCluster = 8;
 constexpr int kRowSlot = 4608, kRowSmem = 216 * 1024;          // vectors of a row per CTA, at most (72 KB: three CTAs per SM)
-template <typename T, int THREADS, int CTAS, int MODE>
-__global__ void __launch_bounds__(THREADS, CTAS) cand_row_kernel(CandArgs a) {
+template <typename T, int THREADS, int ROWS, int CTAS, int MODE>
+__global__ void __launch_bounds__(THREADS * ROWS, CTAS) cand_row_kernel(CandArgs a, int slot) {
     constexpr int kWarps = THREADS / 32, V = Vec<T>::V;
-    extern __shared__ __align__(128) uint8_t row_smem[];
-    __shared__ __align__(8) uint64_t full;
+    static_assert(ROWS == 1 || THREADS == 32, "rows that share a CTA have a warp each");
+    extern __shared__ __align__(128) uint8_t cta_smem[];
+    __shared__ __align__(8) uint64_t fulls[ROWS];
     __shared__ float2 parts[kWarps];
     __shared__ float bcast, sides[4];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int tid = threadIdx.x % THREADS, lane = tid & 31, warp = tid >> 5, mine_of = threadIdx.x / THREADS;
+    uint8_t* row_smem = cta_smem + mine_of * slot * 16;
+    uint64_t& full = fulls[mine_of];
     uint32_t rank, csize;
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(csize));
     let_next_start();
-    const long long row = blockIdx.x / csize;
+    const long long row = ROWS > 1 ? (long long)blockIdx.x * ROWS + mine_of : blockIdx.x / csize;
+    if (ROWS > 1 && row >= a.rows) return;
     const Scale2 c = {a.c_hi, a.c_lo};
     const T* s = static_cast<const T*>(a.scores) + row * a.ld;
     const int cnt = cand_count(a, row);
@@ -476,7 +480,8 @@ __global__ void __launch_bounds__(THREADS, CTAS) cand_row_kernel(CandArgs a) {
     const int av = act >= q.head && act < q.head + q.nv * V ? (act - q.head) / V - q.v0 : -1;
     const bool mine_chosen = av >= 0 && av < have && av % THREADS == tid;
     float m = -INFINITY, rest = 0.f, mz;
-    __syncthreads();                      // the barrier exists
+    if (ROWS > 1) __syncwarp();           // the barrier exists
+    else __syncthreads();
     if (!umma::mbar_wait(&full, 0)) {     // (the row's outputs are invalid; its copy is waited for once more)
         atomicOr(a.err, KGE_ERR_WAIT_TIMEOUT);
         umma::mbar_wait(&full, 0);
@@ -500,33 +505,33 @@ __global__ void __launch_bounds__(THREADS, CTAS) cand_row_kernel(CandArgs a) {
             o.old = __shfl_sync(kFull, side, 2); o.ref = __shfl_sync(kFull, side, 3);
         }
     } else {
-    if (lane == 0) parts[warp] = make_float2(m, rest);
-    if (MODE == CM_POLICY && tid < 4) sides[tid] = side;
-    if (csize == 1) __syncthreads();
-    else asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-    // every warp merges all parts of the row, in the same order
-    m = -INFINITY;
-    rest = 0.f;
-    if (csize == 1) {
-        if (lane < kWarps) { m = parts[lane].x; rest = parts[lane].y; }
-    } else {
-        for (int j = lane; j < kWarps * static_cast<int>(csize); j += 32) {
-            float2 o;
-            uint32_t remote;
-            asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(umma::smem_u32(&parts[j % kWarps])), "r"(static_cast<uint32_t>(j / kWarps)));
-            asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(o.x), "=f"(o.y) : "r"(remote) : "memory");
-            merge_parts(m, rest, o.x, o.y, c);
+        if (lane == 0) parts[warp] = make_float2(m, rest);
+        if (MODE == CM_POLICY && tid < 4) sides[tid] = side;
+        if (csize == 1) __syncthreads();
+        else asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        // every warp merges all parts of the row, in the same order
+        m = -INFINITY;
+        rest = 0.f;
+        if (csize == 1) {
+            if (lane < kWarps) { m = parts[lane].x; rest = parts[lane].y; }
+        } else {
+            for (int j = lane; j < kWarps * static_cast<int>(csize); j += 32) {
+                float2 o;
+                uint32_t remote;
+                asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(umma::smem_u32(&parts[j % kWarps])), "r"(static_cast<uint32_t>(j / kWarps)));
+                asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(o.x), "=f"(o.y) : "r"(remote) : "memory");
+                merge_parts(m, rest, o.x, o.y, c);
+            }
+            // the parts have been read: no CTA of the cluster leaves before the others have got here (nothing is handed over)
+            asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
         }
-        // the parts have been read: no CTA of the cluster leaves before the others have got here (nothing is handed over)
-        asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
-    }
-    {
-        const float mine = m;
-        m = warp_max(m);
-        mz = finite_or_zero(m);
-        rest = warp_sum(rest * cand_exp(mine - mz, c));
-    }
-    if (MODE == CM_POLICY && tid == 0) o = RowSide{sides[0], sides[1], sides[2], sides[3]};
+        {
+            const float mine = m;
+            m = warp_max(m);
+            mz = finite_or_zero(m);
+            rest = warp_sum(rest * cand_exp(mine - mz, c));
+        }
+        if (MODE == CM_POLICY && tid == 0) o = RowSide{sides[0], sides[1], sides[2], sides[3]};
     }
     float ga = 0.f;
     if (tid == 0) {
@@ -814,27 +819,27 @@ static int cand_groups(const CandArgs& a, int* n_partial, cudaStream_t s) {
 }
 
 // slot: vectors of a row that one CTA holds
-template <typename T, int THREADS, int CTAS, int MODE>
+template <typename T, int THREADS, int ROWS, int CTAS, int MODE>
 static int cand_rows(const CandArgs& a, int cluster, long long slot, int* n_partial, cudaStream_t s) {
     static std::atomic<bool> attr_set[128];          // the shared-memory opt-in is per device and kernel
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return cuda_status(cudaGetLastError(), "cudaGetDevice");
     if (dev < 0 || dev >= 128 || !attr_set[dev].load(std::memory_order_acquire)) {
-        cudaError_t e = cudaFuncSetAttribute(cand_row_kernel<T, THREADS, CTAS, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowSmem);
+        cudaError_t e = cudaFuncSetAttribute(cand_row_kernel<T, THREADS, ROWS, CTAS, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowSmem);
         if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(cand_row_kernel)");
         if (dev >= 0 && dev < 128) attr_set[dev].store(true, std::memory_order_release);
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(a.rows * cluster));
-    cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = static_cast<size_t>(slot) * 16;
+    cfg.gridDim = dim3(static_cast<unsigned>((a.rows + ROWS - 1) / ROWS * cluster));
+    cfg.blockDim = dim3(THREADS * ROWS);
+    cfg.dynamicSmemBytes = static_cast<size_t>(slot) * ROWS * 16;
     cfg.stream = s;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = cluster; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
     cfg.attrs = at; cfg.numAttrs = cluster > 1 ? 1 : 0;
     *n_partial = static_cast<int>(a.rows);
-    cudaError_t e = cudaLaunchKernelEx(&cfg, cand_row_kernel<T, THREADS, CTAS, MODE>, a);
+    cudaError_t e = cudaLaunchKernelEx(&cfg, cand_row_kernel<T, THREADS, ROWS, CTAS, MODE>, a, static_cast<int>(slot));
     if (e != cudaSuccess) return cuda_status(e, "cand_row_kernel");
     KGE_LAUNCH_CHECK("cand_row_kernel");
     return 0;
@@ -879,13 +884,14 @@ static int cand_passes(const CandArgs& a, void* ws, int* n_partial, cudaStream_t
     return MODE == CM_POLICY ? cand_gradient<T>(a, coef, same_phase<T>(a), false, s) : 0;
 }
 
-// Which form: the smallest group of lanes that holds a row in registers, then a CTA a row, the smaller the shorter the row;
-// passes where the rows are too long for a cluster, where the groups of all rows would leave most SMs idle, or where the gradient's
-// alignment differs.  A row's own scalars cost a warp some 600 issue slots whatever its length, so few lanes a row win while the
-// lanes are busy (us, log_prob / policy loss):
+// Which form: the smallest group of lanes that holds a row in registers, then a warp or a CTA a row, the smaller the shorter the
+// row; passes where the rows are too long for a cluster, where the groups of all rows would leave most SMs idle, or where the
+// gradient's alignment differs.  A row's own scalars cost a warp some 500 issue slots whatever its length, so few lanes a row win
+// while the lanes are busy (us, log_prob / policy loss):
 //   20000 x 420 fp32   16 lanes 11.4 / 19.0   32 lanes 12.4 / 22.3        but 800 x 900 bf16   16 lanes 4.2 / 7.3   32 lanes 3.7 / 6.3
 //   30000 x 300 bf16    8 lanes 11.4 / 18.5   16 lanes 12.4 / 21.1
-//   11237 x 2703 bf16  32 threads 18.1 / 33.0   64 threads 22.7 / 42.0     40000 x 1100 bf16   32 threads 43.6 / 66   64 threads 52 / 94
+//   8350 x 923 bf16   a warp, shared memory 7.8 / 14.1   16 lanes 9.3 / 15.1       20000 x 420 fp32   a warp 11.9 / 22.1
+//   40000 x 1100 bf16   four warps a CTA, a row each 29.8 / 57.5   CTAs of one warp 42.7 / 59.5   two warps a row 52 / 94
 //   12995 x 3297 fp32  64 threads 31.1 / 59.7   128 threads 33.5 / 62.0    32 threads 37.0 / 67.9
 //   8000 x 5600 fp32  128 threads 30.3 / 59.1   256 threads 37.5 / 67.0    4000 x 9200 fp32   128 threads 26.9 / 50.7   256 threads 26.0 / 49.8
 template <typename T, int MODE>
@@ -896,18 +902,19 @@ static int cand_go(const CandArgs& a, void* ws, int* n_partial, cudaStream_t s) 
     if (nv <= 16) return cand_groups<T, 8, 2, MODE>(a, n_partial, s);
     if (nv <= 32) return cand_groups<T, 8, 4, MODE>(a, n_partial, s);
     if (nv <= 64) return cand_groups<T, 8, 8, MODE>(a, n_partial, s);
-    if (nv <= 128) return a.rows <= 148 * 16 ? cand_groups<T, 32, 4, MODE>(a, n_partial, s) : cand_groups<T, 16, 8, MODE>(a, n_partial, s);
+    if (nv <= 128 && a.rows <= 148 * 16) return cand_groups<T, 32, 4, MODE>(a, n_partial, s);
+    if (nv <= (sizeof(T) == 4 ? 128 : 96)) return cand_groups<T, 16, 8, MODE>(a, n_partial, s);
     if (a.rows >= (1LL << 31) / kMaxCluster) return cand_passes<T, MODE>(a, ws, n_partial, s);      // (beyond a grid of one CTA a row)
-    if (nv <= 512) return cand_rows<T, 32, 24, MODE>(a, 1, nv, n_partial, s);
-    if (nv <= 1024) return cand_rows<T, 64, 16, MODE>(a, 1, nv, n_partial, s);
-    if (nv <= 2048) return cand_rows<T, 128, 10, MODE>(a, 1, nv, n_partial, s);
+    if (nv <= 512) return cand_rows<T, 32, 4, 8, MODE>(a, 1, nv, n_partial, s);
+    if (nv <= 1024) return cand_rows<T, 64, 1, 16, MODE>(a, 1, nv, n_partial, s);
+    if (nv <= 2048) return cand_rows<T, 128, 1, 10, MODE>(a, 1, nv, n_partial, s);
     int cluster = 1;
     while (cluster <= kMaxCluster && nv > cluster * static_cast<long long>(kRowSlot)) cluster *= 2;
     if (cluster > kMaxCluster || a.rows * cluster < 32) return cand_passes<T, MODE>(a, ws, n_partial, s);
     // without a gradient nothing is read twice, and clusters only cost their barriers: 1000 x 100000 fp32 61 us in passes, 84 us in
     // clusters; but 40 x 100000, with its second launch, 7.3 us and 6.7 us
     if (MODE == CM_LOGP && cluster > 1 && a.rows * cluster >= 148 * 3) return cand_passes<T, MODE>(a, ws, n_partial, s);
-    return cand_rows<T, 256, 5, MODE>(a, cluster, (nv + cluster - 1) / cluster, n_partial, s);
+    return cand_rows<T, 256, 1, 5, MODE>(a, cluster, (nv + cluster - 1) / cluster, n_partial, s);
 }
 
 }  // namespace kge
