@@ -697,24 +697,25 @@ __global__ void __launch_bounds__(256) cand_join_kernel(CandArgs a, const float2
     }
 }
 
-// ds from (m, rest, ga) per row, or, with dlogp, from the stats of log_prob: ga = dlogp / T / S.  A warp takes pieces of
-// 32 x 4 vectors (ALIGNED: scores and gradient rows at the same 16-byte phase) or of 32 x 4 elements.
+// ds from (m, rest, ga) per row, or, with dlogp, from the stats of log_prob: ga = dlogp / T / S.  ALIGNED (scores and gradient rows
+// at the same 16-byte phase): eight lanes take pieces of 32 vectors, so that a warp's scalars serve four of them (100000 x 40 fp32 11.8 us,
+// 40000 x 1100 bf16 38.5 us; with a warp a piece of 128 vectors 32.9 and 50.2 us); otherwise a warp takes pieces of 128 elements.
 template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(256) cand_grad_kernel(CandArgs a, const float* coef, long long pieces) {
-    constexpr int V = ALIGNED ? Vec<T>::V : 1;
-    const int lane = threadIdx.x & 31;
+    constexpr int V = ALIGNED ? Vec<T>::V : 1, G = ALIGNED ? 8 : 32;
+    const int lane = threadIdx.x % G;
     let_next_start();
     after_previous();
     const Scale2 c = {a.c_hi, a.c_lo};
-    const long long units = a.rows * pieces;
-    for (long long u = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); u < units; u += (long long)gridDim.x * 8) {
-        const long long row = u / pieces;
+    const long long units = a.rows * pieces, step = (long long)gridDim.x * (256 / G);
+    for (long long u = (long long)blockIdx.x * (256 / G) + threadIdx.x / G; u < units; u += step) {
+        const long long row = units < (1LL << 32) ? static_cast<uint32_t>(u) / static_cast<uint32_t>(pieces) : u / pieces;
         const int piece = static_cast<int>(u - row * pieces);
         const T* s = static_cast<const T*>(a.scores) + row * a.ld;
         T* d = static_cast<T*>(a.dscores) + row * a.ldd;
         const int cnt = cand_count(a, row), act = cand_action(a, row, cnt, false);
-        const float m = __ldg(coef + 3 * row), rest = __ldg(coef + 3 * row + 1);
-        float ga = __ldg(coef + 3 * row + 2);
+        const float m = coef[3 * row], rest = coef[3 * row + 1];       // (plain loads: the kernel ahead wrote them)
+        float ga = coef[3 * row + 2];
         if (a.dlogp) { const float g = __ldg(a.dlogp + row) * static_cast<float>(a.inv_temp); ga = g == 0.f || act < 0 ? 0.f : g * ga; }
         const float fa = ga == 0.f ? 0.f : ga * rest;
         auto one = [&](int j, float x) { return j >= cnt || ga == 0.f ? 0.f : j == act ? fa : -ga * cand_exp(x - m, c); };
@@ -725,12 +726,12 @@ __global__ void __launch_bounds__(256) cand_grad_kernel(CandArgs a, const float*
             uint4 r[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int v = piece * 128 + i * 32 + lane;
+                const int v = piece * (4 * G) + i * G + lane;
                 if (v < nv && head + v * V < cnt) r[i] = __ldcs(sv + v);
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int v = piece * 128 + i * 32 + lane, at = head + v * V;
+                const int v = piece * (4 * G) + i * G + lane, at = head + v * V;
                 if (v >= nv) continue;
                 float f[V];
                 if (at >= cnt || ga == 0.f) {
@@ -748,9 +749,10 @@ __global__ void __launch_bounds__(256) cand_grad_kernel(CandArgs a, const float*
                 }
                 __stcs(dv + v, Vec<T>::close(f));
             }
-            if (piece == 0 && lane < 16) {
-                const int xi = lane < 8 ? (lane < head ? lane : -1) : (head + nv * V + lane - 8 < a.n ? head + nv * V + lane - 8 : -1);
-                if (xi >= 0) cand_put(d + xi, one(xi, xi < cnt ? cand_get(s + xi) : 0.f));
+            if (piece == 0) {             // fewer than 8 elements before the first vector, and behind the last one
+                const int tail = head + nv * V + lane;
+                if (lane < head) cand_put(d + lane, one(lane, lane < cnt ? cand_get(s + lane) : 0.f));
+                if (tail < a.n) cand_put(d + tail, one(tail, tail < cnt ? cand_get(s + tail) : 0.f));
             }
         } else {
 #pragma unroll
@@ -847,8 +849,8 @@ static int cand_rows(const CandArgs& a, int cluster, long long slot, int* n_part
 
 template <typename T>
 static int cand_gradient(const CandArgs& a, const float* coef, bool aligned, bool first, cudaStream_t s) {
-    const int per = 128 * (aligned ? Vec<T>::V : 1);
-    const long long pieces = a.n > 0 ? (a.n + per - 1) / per : 1, want = (a.rows * pieces + 7) / 8;
+    const int per = aligned ? 32 * Vec<T>::V : 128, groups = aligned ? 32 : 8;          // elements of a piece, pieces of a CTA
+    const long long pieces = a.n > 0 ? (a.n + per - 1) / per : 1, want = (a.rows * pieces + groups - 1) / groups;
     const unsigned blocks = static_cast<unsigned>(want < (1 << 30) ? want : (1 << 30));       // (short CTAs copy faster than a loop)
     if (!first) {
         if (aligned) KGE_LAUNCH_AFTER("cand_grad_kernel", cand_grad_kernel<T, true>, blocks, 256u, s, a, coef, pieces);
