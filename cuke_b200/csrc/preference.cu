@@ -233,7 +233,8 @@ static int pref_go(const PrefArgs& a, float* loss, cudaStream_t s) {
 //   60000 x 132     8 threads 24.2   32 threads 47.0        but 2000 x 100    8 threads 5.7    32 threads 4.2
 //   40000 x 512    32 threads 51.1    8 threads 54.8
 //   1336 x 3356   128 threads 11.9   32 threads 19.0   1024 threads 29.3      500 x 512   128 threads 4.7   32 threads 5.7
-//   5000 x 10000  256 threads 111   128 threads 115    32 threads 156         20 x 200000   1024 threads 42   256 threads 82
+//   5000 x 10000  256 threads 111   128 threads 115    32 threads 156         100 x 3000   256 threads 5.2   128 threads 6.3
+//   140 x 60000  1024 threads 20.8   256 threads 40    but 300 x 20000  1024 threads 21.7   256 threads 19.1
 template <bool VEC, bool SQUARE>
 static int pref_pick(const PrefArgs& a, float* loss, cudaStream_t s) {
     if (a.n <= 4) return pref_go<1, false, SQUARE>(a, loss, s);
@@ -241,9 +242,9 @@ static int pref_pick(const PrefArgs& a, float* loss, cudaStream_t s) {
     if (a.n <= 64) return pref_go<4, VEC, SQUARE>(a, loss, s);
     if (a.n <= 384 && a.rows >= 148 * 32) return pref_go<8, VEC, SQUARE>(a, loss, s);
     if (a.n <= 2048 && a.rows >= 148 * 8) return pref_go<32, VEC, SQUARE>(a, loss, s);
-    if (a.n <= 8192) return pref_go<128, VEC, SQUARE>(a, loss, s);
-    if (a.n <= 65536 || a.rows >= 148 * 2) return pref_go<256, VEC, SQUARE>(a, loss, s);
-    return pref_go<1024, VEC, SQUARE>(a, loss, s);
+    if ((a.n > 4096 && a.rows <= 148) || (a.n > 32768 && a.rows <= 148 * 2)) return pref_go<1024, VEC, SQUARE>(a, loss, s);
+    if (a.n <= 512 || (a.n <= 8192 && a.rows >= 148 * 5)) return pref_go<128, VEC, SQUARE>(a, loss, s);
+    return pref_go<256, VEC, SQUARE>(a, loss, s);
 }
 
 static int launch_preference(const PrefArgs& a, float* loss, cudaStream_t s) {
