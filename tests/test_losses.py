@@ -162,7 +162,8 @@ def test_preference_logistic(rows, n, ref, mask, weight):
 
 
 @gpu
-@pytest.mark.parametrize("rows,n", [(300, 8), (301, 24), (130, 25), (100, 61), (4800, 68), (4740, 131), (1200, 200), (1190, 333), (40, 2044), (7, 9001), (5, 8200)])
+@pytest.mark.parametrize("rows,n", [(300, 8), (301, 24), (130, 25), (100, 61), (4800, 68), (4740, 131), (1200, 200), (1190, 333), (40, 300), (800, 701),
+                                    (40, 2044), (7, 9001), (5, 8200), (160, 4100)])
 @pytest.mark.parametrize("mask", [False, True])
 def test_preference_every_group_of_threads(rows, n, mask):
     pref_check(pref_case(rows, n, True, mask, True), beta=0.7, margin=0.2, smoothing=0.1)
