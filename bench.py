@@ -782,6 +782,7 @@ def main():
             cpu = {k: res[k] for k in ("value", "unit", "cores", "kind", "sample")}
         except Exception as e:          # the baseline is reported, never required
             cpu = {"value": None, "unit": "triples/s", "cores": 0, "kind": "port", "sample": f"failed: {e}"}
+    staging = staging_note(stepper, world)
     if rank == 0 and world == 1 and not args.no_side:
         # the parity configurations c1-c4, after the timed c5 regions: one record per scorer (cold- and warm-L2 figures,
         # HBM view of the roofline, the reference's OpenMP C++ on a bounded sample)
@@ -798,7 +799,7 @@ def main():
         line = {"metric": METRIC, "value": value, "unit": "triples/s", "n_gpus": world, "steps": args.steps,
                 "warmup": max(args.warmup, 3), "ms_per_step": ms_step, "higher_is_better": True, "scaling": "weak",
                 "vs_baseline": None, "dtype": "f32", "data": "synthetic", "config": dict(workload_config(cfg, models, world), micro_batches=micro,
-                                                                                         staging=staging_note(stepper, world),
+                                                                                         staging=staging,
                                                                                          arithmetic=(
                     "fp32 storage and accumulation; contractions on the tensor cores over a two-term bf16 split of each fp32 "
                     "operand (three MMAs per product, error-compensated; see the parity block for the measured error)"
