@@ -141,15 +141,15 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None
     if bias is not None and (bias.dtype != torch.bfloat16 or bias.shape != (n,) or not bias.is_contiguous()):
         raise ValueError(f"bias must be a contiguous bfloat16 vector of {n}")
     if out is None:
-        out, ldo = x.new_empty((m, n)), n
+        out, ldo = x.new_empty(m, n), n
     else:
         ldo = _matrix(out, "out", m, n)
     if residual is not None and residual.data_ptr() == out.data_ptr() and ldr != ldo:
         raise ValueError("out may be residual only with the same row pitch")
-    preact = x.new_empty((m, n), dtype=torch.float16) if save_preact and code else None
+    preact = x.new_empty(m, n, dtype=torch.float16) if save_preact and code else None
     L = _lib.lib()
     need = L.kge_linear_workspace_bytes(m, k, n, code, 0)
-    ws = x.new_empty(need, dtype=torch.uint8) if need else None
+    ws = x.new_empty((need + 1) // 2) if need else None            # (of two-byte elements: the quickest allocation)
     check(L.kge_linear_forward(x.data_ptr(), ldx, w.data_ptr(), ldw, _ptr(bias), _ptr(residual), ldr, m, k, n, code, out.data_ptr(), ldo,
                                _ptr(preact), _ptr(ws), need, stream_on(here)))
     return (out, preact) if save_preact else out
@@ -168,12 +168,12 @@ def linear_backward(dout: torch.Tensor, x: torch.Tensor, w: torch.Tensor, preact
     ldd, ldx, ldw = _matrix(dout, "dout", m, n), _matrix(x, "x", m, k), _matrix(w, "w", k, n)
     if code and (preact is None or preact.dtype != torch.float16 or preact.shape != (m, n) or not preact.is_contiguous()):
         raise ValueError("preact must be what linear(..., save_preact=True) returned")
-    dx = x.new_empty((m, k)) if need_dx else None
-    dw = x.new_empty((k, n)) if need_dw else None
+    dx = x.new_empty(m, k) if need_dx else None
+    dw = x.new_empty(k, n) if need_dw else None
     db = x.new_empty(n) if need_dbias else None
     L = _lib.lib()
     need = L.kge_linear_workspace_bytes(m, k, n, code, 1)
-    ws = x.new_empty(need, dtype=torch.uint8) if need else None
+    ws = x.new_empty((need + 1) // 2) if need else None            # (of two-byte elements: the quickest allocation)
     check(L.kge_linear_backward(dout.data_ptr(), ldd, x.data_ptr(), ldx, w.data_ptr(), ldw, preact.data_ptr() if code else None, m, k, n, code,
                                 _ptr(dx), k, _ptr(dw), _ptr(db), _ptr(ws), need, stream_on(here)))
     return dx, dw, db

@@ -72,7 +72,7 @@ def preference_loss(pos: torch.Tensor, neg: torch.Tensor, ref_pos: Optional[torc
     dpos, dneg = torch.empty_like(pos), torch.empty_like(neg, memory_format=torch.contiguous_format)
     L = _lib.lib()
     need = L.kge_preference_workspace_bytes(rows, n)
-    ws = pos.new_empty(need, dtype=torch.uint8)
+    ws = pos.new_empty((need + 3) // 4)
     check(L.kge_preference_loss(pos.data_ptr(), _ptr(ref_pos), neg.data_ptr(), ldn, _ptr(ref_neg), ldr, _ptr(mask), ldm, _ptr(weight), rows, n,
                                 PREFERENCE_KINDS[kind], beta, margin, smoothing, _scale(reduction, rows),
                                 loss.data_ptr(), dpos.data_ptr(), dneg.data_ptr(), n or 1, ws.data_ptr(), need, stream_on(here)))
@@ -101,10 +101,10 @@ def log_prob(scores: torch.Tensor, action: torch.Tensor, n_cand: Optional[torch.
     how = _candidates(scores, action, n_cand)
     rows, n = how[3], how[4]
     logp = scores.new_empty(rows, dtype=torch.float32)
-    stats = scores.new_empty((rows, 3), dtype=torch.float32)
+    stats = logp.new_empty(rows, 3)
     L = _lib.lib()
     need = L.kge_candidates_workspace_bytes(rows, n)
-    ws = scores.new_empty(need, dtype=torch.uint8)
+    ws = logp.new_empty((need + 3) // 4)
     check(L.kge_log_prob(*how, temperature, logp.data_ptr(), stats.data_ptr(), ws.data_ptr(), need, stream_on(here)))
     return logp, stats
 
@@ -145,7 +145,7 @@ def policy_loss(scores: torch.Tensor, action: torch.Tensor, old_logp: torch.Tens
     dscores = torch.empty_like(scores, memory_format=torch.contiguous_format)
     L = _lib.lib()
     need = L.kge_candidates_workspace_bytes(rows, n)
-    ws = old_logp.new_empty(need, dtype=torch.uint8)
+    ws = old_logp.new_empty((need + 3) // 4)
     check(L.kge_policy_loss(*how, temperature, old_logp.data_ptr(), _ptr(ref_logp), advantage.data_ptr(), _ptr(weight), clip_low, clip_high,
                             kl_coef, _scale(reduction, rows), loss.data_ptr(), logp.data_ptr(), kl.data_ptr(), dscores.data_ptr(), n or 1,
                             ws.data_ptr(), need, stream_on(here)))
