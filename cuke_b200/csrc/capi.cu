@@ -27,8 +27,13 @@ void note_launch() { g_launches.fetch_add(1, std::memory_order_relaxed); }
 
 __device__ int32_t g_error_word = 0;
 int32_t* device_error_word() {
-    int32_t* p = nullptr;
+    static std::atomic<int32_t*> known[128];         // by device: the runtime's lookup takes longer than a launch's checks
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return nullptr;
+    int32_t* p = dev >= 0 && dev < 128 ? known[dev].load(std::memory_order_acquire) : nullptr;
+    if (p) return p;
     if (cudaGetSymbolAddress(reinterpret_cast<void**>(&p), g_error_word) != cudaSuccess) return nullptr;
+    if (dev >= 0 && dev < 128) known[dev].store(p, std::memory_order_release);
     return p;
 }
 

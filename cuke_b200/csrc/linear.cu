@@ -734,11 +734,14 @@ __global__ void __launch_bounds__(512) linear_dz_kernel(const __nv_bfloat16* __r
 }
 // ---- host -----------------------------------------------------------------------------------------------------------
 static int lin_sms() {
+    static std::atomic<int> known[128];              // by device
     int dev = 0, sms = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms < 2) {
+    if (cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 128 && (sms = known[dev].load(std::memory_order_relaxed)) > 0) return sms;
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms < 2) {
         cudaGetLastError();
         return 148;
     }
+    if (dev >= 0 && dev < 128) known[dev].store(sms, std::memory_order_relaxed);
     return sms;
 }
 // Columns of a tile when n columns are cut into so many: whole 32-column blocks, or one tile in units of 16.
