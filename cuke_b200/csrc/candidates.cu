@@ -26,7 +26,7 @@ struct CandArgs {
     const float* dlogp;              // gradient of log_prob
     const float* old_logp; const float* ref_logp; const float* adv; const float* weight;
     float clip_lo, clip_hi, kl_coef, scale;
-    float* kl; double* partial;
+    float* kl; float* loss; double* partial;     // loss: written by the only CTA of a launch, else summed from partial
     int32_t* err;
 };
 
@@ -386,7 +386,8 @@ __global__ void __launch_bounds__(256, I <= 4 ? 4 : 3) cand_group_kernel(CandArg
         __syncthreads();
         if (threadIdx.x == 0) {
             for (int w = 1; w < 8; ++w) total += red[w];
-            a.partial[blockIdx.x] = total;
+            if (gridDim.x == 1) *a.loss = static_cast<float>(total);
+            else a.partial[blockIdx.x] = total;
         }
     }
 }
@@ -817,6 +818,7 @@ static int cand_groups(const CandArgs& a, int* n_partial, cudaStream_t s) {
     *n_partial = static_cast<int>(want < kCandMaxBlocks ? want : kCandMaxBlocks);
     cand_group_kernel<T, G, I, MODE><<<*n_partial, 256, 0, s>>>(a);
     KGE_LAUNCH_CHECK("cand_group_kernel");
+    if (*n_partial == 1) *n_partial = 0;               // (nothing left to sum)
     return 0;
 }
 
@@ -1022,10 +1024,11 @@ int kge_policy_loss(const void* scores, int32_t dtype, int64_t ld, int64_t rows,
     a.logp = logp; a.kl = kl; a.dscores = dscores; a.ldd = ldd;
     a.old_logp = old_logp; a.ref_logp = ref_logp; a.adv = advantage; a.weight = weight;
     a.clip_lo = clip_low; a.clip_hi = clip_high; a.kl_coef = kl_coef; a.scale = scale;
+    a.loss = loss;
     a.partial = static_cast<double*>(workspace);
     int parts = 0;
     rc = dtype == KGE_F32 ? cand_go<float, CM_POLICY>(a, workspace, &parts, s) : cand_go<__nv_bfloat16, CM_POLICY>(a, workspace, &parts, s);
-    return rc ? rc : launch_sum_partials(a.partial, parts, loss, s);
+    return rc || parts == 0 ? rc : launch_sum_partials(a.partial, parts, loss, s);
 }
 
 }  // extern "C"

@@ -17,7 +17,7 @@ int launch_sum_partials(const double* partial, int n, float* out, cudaStream_t s
 struct PrefArgs {
     const float* pos; const float* rpos; const float* neg; const float* rneg;
     const unsigned char* mask; const float* weight;
-    float* dpos; float* dneg; double* partial;
+    float* dpos; float* dneg; float* loss; double* partial;     // loss: written by the only CTA of a launch, else summed from partial
     long long rows, ldn, ldr, ldm, ldd;
     int n, kind;
     float beta, margin, smooth, scale;
@@ -194,7 +194,10 @@ __global__ void __launch_bounds__(G > 32 ? G : 256) pref_kernel(PrefArgs a) {
         if (G > 32) __syncthreads();               // rc, rl, rd are free for the next row
     }
     if (G > 32) {
-        if (threadIdx.x == 0) a.partial[blockIdx.x] = total;
+        if (threadIdx.x == 0) {
+            if (gridDim.x == 1) *a.loss = static_cast<float>(total);
+            else a.partial[blockIdx.x] = total;
+        }
     } else {
 #pragma unroll
         for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(kFull, total, o);
@@ -202,7 +205,8 @@ __global__ void __launch_bounds__(G > 32 ? G : 256) pref_kernel(PrefArgs a) {
         __syncthreads();
         if (threadIdx.x == 0) {
             for (int w = 1; w < 8; ++w) total += red[w];
-            a.partial[blockIdx.x] = total;
+            if (gridDim.x == 1) *a.loss = static_cast<float>(total);
+            else a.partial[blockIdx.x] = total;
         }
     }
 }
@@ -221,7 +225,9 @@ static int pref_go2(const PrefArgs& a, float* loss, cudaStream_t s) {
     const unsigned blocks = static_cast<unsigned>(pref_blocks(a.rows, per));
     pref_kernel<G, VEC, SQUARE, MASK><<<blocks, G > 32 ? G : 256, 0, s>>>(a);
     KGE_LAUNCH_CHECK("pref_kernel");
-    return launch_sum_partials(a.partial, static_cast<int>(blocks), loss, s);
+    // one CTA has written the loss itself (200 x 3: 2.7 us, with a sum 3.7 us; one CTA of 1024 threads for more rows is slower: 500 x 20
+    // 5.7 us against 4.2 us)
+    return blocks > 1 ? launch_sum_partials(a.partial, static_cast<int>(blocks), loss, s) : 0;
 }
 template <int G, bool VEC, bool SQUARE>
 static int pref_go(const PrefArgs& a, float* loss, cudaStream_t s) {
@@ -231,7 +237,7 @@ static int pref_go(const PrefArgs& a, float* loss, cudaStream_t s) {
 // scalars and reductions.  us with reference and mask:
 //   400000 x 8      2 threads 16.2   4 threads 27.8   8 threads 51.4          100000 x 48   4 threads 15.0   8 threads 20.6
 //   60000 x 132     8 threads 24.2   32 threads 47.0        but 2000 x 100    8 threads 5.7    32 threads 4.2
-//   40000 x 512    32 threads 51.1    8 threads 54.8
+//   40000 x 512    32 threads 51.1    8 threads 54.8        but 25915 x 412   8 threads 28.0   32 threads 35.4
 //   1336 x 3356   128 threads 11.9   32 threads 19.0   1024 threads 29.3      500 x 512   128 threads 4.7   32 threads 5.7
 //   5000 x 10000  256 threads 111   128 threads 115    32 threads 156         100 x 3000   256 threads 5.2   128 threads 6.3
 //   140 x 60000  1024 threads 20.8   256 threads 40    but 300 x 20000  1024 threads 21.7   256 threads 19.1
@@ -240,7 +246,7 @@ static int pref_pick(const PrefArgs& a, float* loss, cudaStream_t s) {
     if (a.n <= 4) return pref_go<1, false, SQUARE>(a, loss, s);
     if (a.n <= 24) return pref_go<2, VEC, SQUARE>(a, loss, s);
     if (a.n <= 64) return pref_go<4, VEC, SQUARE>(a, loss, s);
-    if (a.n <= 384 && a.rows >= 148 * 32) return pref_go<8, VEC, SQUARE>(a, loss, s);
+    if (a.n <= 448 && a.rows >= 148 * 32) return pref_go<8, VEC, SQUARE>(a, loss, s);
     if (a.n <= 2048 && a.rows >= 148 * 8) return pref_go<32, VEC, SQUARE>(a, loss, s);
     if ((a.n > 4096 && a.rows <= 148) || (a.n > 32768 && a.rows <= 148 * 2)) return pref_go<1024, VEC, SQUARE>(a, loss, s);
     if (a.n <= 512 || (a.n <= 8192 && a.rows >= 148 * 5)) return pref_go<128, VEC, SQUARE>(a, loss, s);
@@ -288,7 +294,7 @@ int kge_preference_loss(const float* pos, const float* ref_pos, const float* neg
     if (workspace_bytes < kge_preference_workspace_bytes(rows, n)) { set_error("%s: workspace too small", fn); return KGE_E_WORKSPACE; }
     if (!workspace) { set_error("%s: workspace is NULL", fn); return KGE_E_NULL; }
     if (!aligned16(workspace)) { set_error("%s: workspace is not 16-byte aligned", fn); return KGE_E_ALIGN; }
-    PrefArgs a = {pos, ref_pos, neg, ref_neg, mask, weight, dpos, dneg, static_cast<double*>(workspace), rows, ld_neg, ld_ref, ld_mask, ld_dneg,
+    PrefArgs a = {pos, ref_pos, neg, ref_neg, mask, weight, dpos, dneg, loss, static_cast<double*>(workspace), rows, ld_neg, ld_ref, ld_mask, ld_dneg,
                   static_cast<int>(n), kind, beta, margin, smoothing, scale};
     return launch_preference(a, loss, s);
 }
