@@ -57,14 +57,20 @@ __device__ __forceinline__ double cand_log_sum(double S) {
     const float r = fmaf(s, expf(-y), -1.f) + static_cast<float>(S - static_cast<double>(s)) / s;
     return static_cast<double>(y) + static_cast<double>(r);
 }
-// e^d - 1 - d: its power series near 0, where the three terms cancel (next term below 2^-24 of the sum for |d| <= 1)
-__device__ __forceinline__ float exp_minus_line(float d) {
-    if (fabsf(d) > 1.f) return expm1f(d) - d;
+// e^d - 1 - d: its power series near 0, where the three terms cancel (next term below 2^-24 of the sum for |d| <= 1); e^d - 1 in
+// *em1: farther out it cannot be had back as the difference of the two (d = -1e8 has a step of 8)
+__device__ __forceinline__ float exp_minus_line(float d, float* em1) {
+    if (fabsf(d) > 1.f) {
+        *em1 = expm1f(d);
+        return *em1 - d;
+    }
     float t = 1.f / 479001600.f;
     t = fmaf(t, d, 1.f / 39916800.f); t = fmaf(t, d, 1.f / 3628800.f); t = fmaf(t, d, 1.f / 362880.f); t = fmaf(t, d, 1.f / 40320.f);
     t = fmaf(t, d, 1.f / 5040.f); t = fmaf(t, d, 1.f / 720.f); t = fmaf(t, d, 1.f / 120.f); t = fmaf(t, d, 1.f / 24.f);
     t = fmaf(t, d, 1.f / 6.f); t = fmaf(t, d, 0.5f);
-    return d * d * t;
+    const float kl = d * d * t;
+    *em1 = kl + d;
+    return kl;
 }
 
 // What follows from a row's statistics: logp, kl, loss term (returned), and the factor ga of the gradient,
@@ -99,9 +105,10 @@ __device__ __forceinline__ double cand_finish(const CandArgs& a, long long row, 
     float l = -(held ? (A > 0.f ? hi : lo) : ratio) * A, dl = held ? 0.f : -ratio * A, kl = 0.f;
     if (a.ref_logp) {
         const float d = static_cast<float>(static_cast<double>(o.ref) - lp);
-        kl = exp_minus_line(d);
+        float em1;
+        kl = exp_minus_line(d, &em1);
         l = fmaf(a.kl_coef, kl, l);
-        dl = fmaf(-a.kl_coef, kl + d, dl);               // e^d - 1 = kl + d
+        dl = fmaf(-a.kl_coef, em1, dl);
     }
     if (write) a.kl[row] = kl;
     if (w == 0.f) return 0.0;                            // (a row of weight 0 may hold NaN)

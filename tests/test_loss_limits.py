@@ -1,0 +1,46 @@
+"""Losses over scores at the limits of their terms: coefficients of zero beside infinities, rows that take no part."""
+import pytest
+import torch
+
+from cuke_b200 import losses
+
+pytestmark = pytest.mark.gpu
+EPS = 2.0 ** -24                            # half a step of fp32, relative
+INF = float("inf")
+
+
+def policy_case(rows=6, n=50, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    s = torch.randn(rows, n, generator=g)
+    act = torch.randint(0, n, (rows,), generator=g)
+    lp = torch.log_softmax(s.double(), 1).gather(1, act[:, None])[:, 0]
+    return s.cuda(), act.cuda(), lp, torch.log_softmax(s.double(), 1)
+
+
+def test_kl_gradient_far_below_the_reference():
+    """d = ref - logp far below zero: the slope kl_coef (e^d - 1) tends to -kl_coef, down to ref = -infinity.
+
+    Relative error of the gradient: 128 half-steps (argument of the exponentials 6 A with A = 8, sums of 50 terms, the factors)."""
+    temp, kl_coef = 0.8, 0.5
+    g = torch.Generator().manual_seed(2)
+    gap = torch.tensor([2.0, 50.0, 1e4, 1e7, 1e30, 3e38, INF])
+    rows, n = len(gap), 50
+    s = torch.randn(rows, n, generator=g)
+    act = torch.randint(0, n, (rows,), generator=g)
+    x = torch.log_softmax(s.double() / temp, 1)
+    lp = x.gather(1, act[:, None])[:, 0]
+    ref = (lp - gap.double()).float()
+    d = ref.double() - lp
+    zero, old = torch.zeros(rows, device="cuda"), lp.float().cuda()
+    for upto, finite in ((rows, False), (rows - 1, True)):
+        c = lambda t: t[:upto].cuda()  # noqa: E731
+        loss, _, kl, grad = losses.policy_loss(c(s), c(act), old[:upto], zero[:upto], ref_logp=c(ref), temperature=temp, kl_coef=kl_coef, reduction="sum")
+        slope = kl_coef * -torch.expm1(d[:upto])
+        onehot = torch.zeros(upto, n, dtype=torch.float64).scatter_(1, act[:upto, None], 1.0)
+        want = slope[:, None] / temp * (onehot - torch.exp(x[:upto]))
+        assert ((grad.cpu().double() - want).abs() <= 128 * EPS * want.abs()).all()
+        kl64 = torch.expm1(d[:upto]) - d[:upto]
+        near = torch.where(torch.isinf(kl64), torch.zeros_like(kl64), kl64)
+        assert torch.equal(torch.isinf(kl.cpu()), torch.isinf(kl64)) and (kl.cpu().double()[~torch.isinf(kl64)] - near[~torch.isinf(kl64)]).abs().le(
+            16 * EPS * near[~torch.isinf(kl64)] + 16 * EPS).all()
+        assert torch.isinf(loss).item() is not finite and not torch.isnan(loss).item()
