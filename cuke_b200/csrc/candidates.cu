@@ -62,7 +62,7 @@ __device__ __forceinline__ double cand_log_sum(double S) {
 __device__ __forceinline__ float exp_minus_line(float d, float* em1) {
     if (fabsf(d) > 1.f) {
         *em1 = expm1f(d);
-        return *em1 - d;
+        return d == INFINITY ? d : *em1 - d;             // (a chosen candidate of probability 0)
     }
     float t = 1.f / 479001600.f;
     t = fmaf(t, d, 1.f / 39916800.f); t = fmaf(t, d, 1.f / 3628800.f); t = fmaf(t, d, 1.f / 362880.f); t = fmaf(t, d, 1.f / 40320.f);

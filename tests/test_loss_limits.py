@@ -44,3 +44,16 @@ def test_kl_gradient_far_below_the_reference():
         assert torch.equal(torch.isinf(kl.cpu()), torch.isinf(kl64)) and (kl.cpu().double()[~torch.isinf(kl64)] - near[~torch.isinf(kl64)]).abs().le(
             16 * EPS * near[~torch.isinf(kl64)] + 16 * EPS).all()
         assert torch.isinf(loss).item() is not finite and not torch.isnan(loss).item()
+
+
+def chosen_of_probability_zero():
+    s, act, lp, _ = policy_case(seed=3)
+    s[torch.arange(6, device="cuda"), act] = -INF
+    return s, act, lp.float().cuda(), (lp + 0.1).float().cuda(), torch.ones(6, device="cuda")
+
+
+def test_kl_of_a_chosen_candidate_of_probability_zero():
+    """logp = -infinity: infinitely far from any reference (kl = +infinity, not NaN)."""
+    s, act, old, ref, adv = chosen_of_probability_zero()
+    loss, logp, kl, d = losses.policy_loss(s, act, old, adv, ref_logp=ref, kl_coef=0.1)
+    assert (logp == -INF).all() and (kl == INF).all() and loss.item() == INF
