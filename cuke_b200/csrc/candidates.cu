@@ -107,8 +107,10 @@ __device__ __forceinline__ double cand_finish(const CandArgs& a, long long row, 
         const float d = static_cast<float>(static_cast<double>(o.ref) - lp);
         float em1;
         kl = exp_minus_line(d, &em1);
-        l = fmaf(a.kl_coef, kl, l);
-        dl = fmaf(-a.kl_coef, em1, dl);
+        if (a.kl_coef > 0.f) {                           // (0 x infinity without the test: kl is only reported then)
+            l = fmaf(a.kl_coef, kl, l);
+            dl = fmaf(-a.kl_coef, em1, dl);
+        }
     }
     if (write) a.kl[row] = kl;
     if (w == 0.f) return 0.0;                            // (a row of weight 0 may hold NaN)

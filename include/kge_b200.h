@@ -410,7 +410,8 @@ KGE_API int kge_preference_loss(const float* pos, const float* ref_pos, const fl
  *   kge_log_prob_backward  dscores[r][j] = dlogp[r] / temperature * (1[j = action[r]] - softmax_j), zeros at [n_cand[r], n)
  *   kge_policy_loss        ratio = exp(logp - old_logp);
  *                          l = -min(ratio A, clip(ratio, 1 - clip_low, 1 + clip_high) A)
- *                              + kl_coef * kl,   kl = exp(ref_logp - logp) - (ref_logp - logp) - 1  (0 without ref_logp)
+ *                              + kl_coef * kl,   kl = exp(ref_logp - logp) - (ref_logp - logp) - 1  (0 without ref_logp;
+ *                              with kl_coef = 0 it is only reported, an infinite one too)
  *                          loss = scale * sum_r weight[r] l_r and dscores = d(loss) / d(scores), in one call; logp and kl
  *                          (rows) are written too.  weight NULL: 1.  A clipped row's policy part has zero gradient.
  * temperature in [1e-30, 1e30].  action[r] = -1: nothing was chosen; any other id outside [0, n_cand[r]) is reported as KGE_ERR_ID_RANGE (kge_check) and taken

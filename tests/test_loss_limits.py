@@ -17,6 +17,19 @@ def policy_case(rows=6, n=50, seed=0):
     return s.cuda(), act.cuda(), lp, torch.log_softmax(s.double(), 1)
 
 
+def test_kl_of_coefficient_zero_is_only_reported():
+    """ref - logp of 100, +-infinity and beyond fp32's exponential: the call without a reference, bit for bit, and kl beside it."""
+    s, act, lp, _ = policy_case()
+    gap = torch.tensor([0.1, 100.0, INF, -INF, -1e30, 88.0])
+    ref = (lp + gap.double()).float()
+    old, adv = (lp - 0.05).float().cuda(), torch.tensor([1.0, -1.0, 0.5, -0.5, 2.0, 0.0]).cuda()
+    loss, logp, kl, d = losses.policy_loss(s, act, old, adv, ref_logp=ref.cuda(), kl_coef=0.0)
+    want = losses.policy_loss(s, act, old, adv)
+    assert torch.isfinite(loss).all() and torch.isfinite(d).all()
+    assert torch.equal(loss, want[0]) and torch.equal(logp, want[1]) and torch.equal(d, want[3])
+    assert kl[1] == INF and kl[2] == INF and kl[3] == INF and (kl[[0, 4, 5]] > 0).all() and torch.isfinite(kl[[0, 4, 5]]).all()
+
+
 def test_kl_gradient_far_below_the_reference():
     """d = ref - logp far below zero: the slope kl_coef (e^d - 1) tends to -kl_coef, down to ref = -infinity.
 
@@ -57,3 +70,9 @@ def test_kl_of_a_chosen_candidate_of_probability_zero():
     s, act, old, ref, adv = chosen_of_probability_zero()
     loss, logp, kl, d = losses.policy_loss(s, act, old, adv, ref_logp=ref, kl_coef=0.1)
     assert (logp == -INF).all() and (kl == INF).all() and loss.item() == INF
+
+
+def test_kl_of_coefficient_zero_beside_a_probability_of_zero():
+    s, act, old, ref, adv = chosen_of_probability_zero()
+    loss, logp, kl, d = losses.policy_loss(s, act, old, adv, ref_logp=ref)
+    assert (logp == -INF).all() and (kl == INF).all() and loss.item() == 0 and (d == 0).all()
