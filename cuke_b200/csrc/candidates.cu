@@ -102,7 +102,8 @@ __device__ __forceinline__ double cand_finish(const CandArgs& a, long long row, 
     const float ratio = expf(static_cast<float>(lp - static_cast<double>(o.old)));
     const float lo = 1.f - a.clip_lo, hi = 1.f + a.clip_hi;
     const bool held = (A > 0.f && ratio > hi) || (A < 0.f && ratio < lo);
-    float l = -(held ? (A > 0.f ? hi : lo) : ratio) * A, dl = held ? 0.f : -ratio * A, kl = 0.f;
+    const float gain = A == 0.f && ratio == INFINITY ? 0.f : ratio * A;      // (exp(89) is past fp32; 0 times it is 0)
+    float l = held ? -(A > 0.f ? hi : lo) * A : -gain, dl = held ? 0.f : -gain, kl = 0.f;
     if (a.ref_logp) {
         const float d = static_cast<float>(static_cast<double>(o.ref) - lp);
         float em1;

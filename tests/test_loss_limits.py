@@ -30,6 +30,19 @@ def test_kl_of_coefficient_zero_is_only_reported():
     assert kl[1] == INF and kl[2] == INF and kl[3] == INF and (kl[[0, 4, 5]] > 0).all() and torch.isfinite(kl[[0, 4, 5]]).all()
 
 
+def test_advantage_of_zero_beside_a_ratio_past_fp32():
+    """exp(100) times an advantage of 0 is 0: the row gives what it gives at a ratio of 1."""
+    s, act, lp, _ = policy_case(seed=1)
+    ref, zero = (lp + 0.2).float().cuda(), torch.zeros(6, device="cuda")
+    for kl_coef in (0.0, 0.3):
+        want = losses.policy_loss(s, act, lp.float().cuda(), zero, ref_logp=ref, kl_coef=kl_coef)
+        got = losses.policy_loss(s, act, (lp - 100).float().cuda(), zero, ref_logp=ref, kl_coef=kl_coef)
+        assert torch.isfinite(got[0]).all() and all(torch.equal(a, b) for a, b in zip(got, want))
+    s[2, 3] = float("nan")                  # a row of NaN stays one
+    loss, logp, kl, d = losses.policy_loss(s, act, (lp - 100).float().cuda(), zero)
+    assert torch.isnan(loss).all() and torch.isnan(logp[2]) and torch.isnan(d[2]).all() and (d[[0, 1, 3, 4, 5]] == 0).all()
+
+
 def test_kl_gradient_far_below_the_reference():
     """d = ref - logp far below zero: the slope kl_coef (e^d - 1) tends to -kl_coef, down to ref = -infinity.
 
