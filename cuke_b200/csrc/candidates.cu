@@ -727,7 +727,10 @@ __global__ void __launch_bounds__(256) cand_grad_kernel(CandArgs a, const float*
         const int cnt = cand_count(a, row), act = cand_action(a, row, cnt, false);
         const float m = coef[3 * row], rest = coef[3 * row + 1];       // (plain loads: the kernel ahead wrote them)
         float ga = coef[3 * row + 2];
-        if (a.dlogp) { const float g = __ldg(a.dlogp + row) * static_cast<float>(a.inv_temp); ga = g == 0.f || act < 0 ? 0.f : g * ga; }
+        if (a.dlogp) {                    // 1 / S of 0: a row that takes no part, whatever dlogp holds there
+            const float g = __ldg(a.dlogp + row) * static_cast<float>(a.inv_temp);
+            ga = g == 0.f || act < 0 || ga == 0.f ? 0.f : g * ga;
+        }
         const float fa = ga == 0.f ? 0.f : ga * rest;
         auto one = [&](int j, float x) { return j >= cnt || ga == 0.f ? 0.f : j == act ? fa : -ga * cand_exp(x - m, c); };
         if constexpr (ALIGNED) {

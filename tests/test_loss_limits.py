@@ -89,3 +89,18 @@ def test_kl_of_coefficient_zero_beside_a_probability_of_zero():
     s, act, old, ref, adv = chosen_of_probability_zero()
     loss, logp, kl, d = losses.policy_loss(s, act, old, adv, ref_logp=ref)
     assert (logp == -INF).all() and (kl == INF).all() and loss.item() == 0 and (d == 0).all()
+
+
+@pytest.mark.parametrize("n", [50, 700, 20000])
+@pytest.mark.parametrize("bad", [float("nan"), INF, -INF])
+def test_log_prob_gradient_of_rows_without_a_distribution(n, bad):
+    """A row that takes no part has a zero gradient whatever d(logp) holds there."""
+    s = torch.randn(5, n, generator=torch.Generator().manual_seed(4)).cuda()
+    s[1] = -INF
+    act = torch.tensor([0, 1, -1, 0, 2], device="cuda")
+    cnt = torch.tensor([n, n, n, 0, n], dtype=torch.int32, device="cuda")
+    act[3] = -1
+    logp, stats = losses.log_prob(s, act, n_cand=cnt)
+    dlogp = torch.tensor([1.0, bad, bad, bad, 1.0], device="cuda")
+    d = losses.log_prob_backward(s, act, stats, dlogp, n_cand=cnt)
+    assert (logp[1:4] == 0).all() and (d[1:4] == 0).all() and torch.isfinite(d).all() and (d[[0, 4]] != 0).any()
