@@ -48,8 +48,10 @@ __device__ __forceinline__ void pref_pairs(const PrefArgs& a, float keep, float2
     const bool ux = z.x >= 0.f, uy = z.y >= 0.f;
     const float2 hi = make_float2(ux ? a.smooth : -keep, uy ? a.smooth : -keep), lo = make_float2(ux ? -keep : a.smooth, uy ? -keep : a.smooth);
     d = __ffma2_rn(hi, inv, __fmul2_rn(lo, small));
-    l = __ffma2_rn(f2(keep), make_float2(fmaxf(-z.x, 0.f), fmaxf(-z.y, 0.f)), __fmul2_rn(w, q));
-    if (a.smooth > 0.f)                                                                    // (0 x inf without the test)
+    l = __fmul2_rn(w, q);
+    if (keep > 0.f)                                                                        // (0 x inf without the tests)
+        l = __ffma2_rn(f2(keep), make_float2(fmaxf(-z.x, 0.f), fmaxf(-z.y, 0.f)), l);
+    if (a.smooth > 0.f)
         l = __ffma2_rn(f2(a.smooth), make_float2(fmaxf(z.x, 0.f), fmaxf(z.y, 0.f)), l);
 }
 

@@ -104,3 +104,15 @@ def test_log_prob_gradient_of_rows_without_a_distribution(n, bad):
     dlogp = torch.tensor([1.0, bad, bad, bad, 1.0], device="cuda")
     d = losses.log_prob_backward(s, act, stats, dlogp, n_cand=cnt)
     assert (logp[1:4] == 0).all() and (d[1:4] == 0).all() and torch.isfinite(d).all() and (d[[0, 4]] != 0).any()
+
+
+@pytest.mark.parametrize("n", [1, 3, 40])
+def test_preference_smoothing_of_one_beside_infinities(n):
+    """smoothing = 1 leaves softplus(z): z = -infinity costs nothing, as z = +infinity does without smoothing."""
+    pos = torch.zeros(2, device="cuda")
+    for value, smoothing in ((INF, 1.0), (3e38, 1.0), (-INF, 0.0), (-3e38, 0.0)):
+        neg = torch.full((2, n), value, device="cuda")
+        loss, dpos, dneg = losses.preference_loss(pos, neg, smoothing=smoothing, beta=2.0)         # (2 x 3e38 overflows)
+        assert loss.item() == 0 and (dpos == 0).all() and (dneg == 0).all()
+    loss, dpos, dneg = losses.preference_loss(pos, torch.full((2, n), -INF, device="cuda"), smoothing=1.0)
+    assert loss.item() == INF and (dneg != 0).all()
