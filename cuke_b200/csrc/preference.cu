@@ -6,8 +6,9 @@
 //   loss = scale sum_b w_b / c_b sum_{j valid} l,  dpos_b = scale beta w_b / c_b sum_j l',  dneg_bj = -scale beta w_b / c_b l'
 //
 // c_b is the number of valid negatives of row b; a row without any contributes nothing and gets zero gradients.
-// fp32 per pair (both sigmoids from one exponential of -|z|, so neither side loses its small values), a row's sum in
-// fp32, the sum over rows in fp64 and in a fixed order.
+// fp32 per pair (both sigmoids from one exponential of -|z|, so neither side loses its small values).  Sums are taken in a fixed
+// order: a row's in fp32 with at most 64 additions behind one another in a thread, longer ones continued in fp64; the sum over
+// rows in fp64.
 #include "common.cuh"
 
 namespace kge {
@@ -69,19 +70,29 @@ __device__ __forceinline__ int pref_group_sum(int v) {
     return v;
 }
 
+// Turns of a long row after which a thread's fp32 sums, of four terms a turn, go to its 64-bit ones and start again.
+constexpr int kPrefFold = 16;
+__device__ __forceinline__ void pref_fold(double2& wide, bool more, float2& ls, float2& ds) {
+    const double l = static_cast<double>(ls.x) + static_cast<double>(ls.y), d = static_cast<double>(ds.x) + static_cast<double>(ds.y);
+    wide = more ? make_double2(wide.x + l, wide.y + d) : make_double2(l, d);
+    ls = ds = f2(0.f);
+}
+
 // A group of G threads per row: one thread for a handful of negatives, part of a warp, a warp, or a whole CTA.  VEC: four
 // negatives per access (all rows of neg, ref_neg, dneg on 16-byte and of mask on 4-byte boundaries).  The valid negatives of
 // a row are counted first - the mask is a thirteenth of the traffic and comes from L1 the second time - so that the main pass
 // writes final gradients; it requests U accesses of each array before it uses the first.  Without VEC a thread has the same four
 // negatives, read one by one: the order of the additions, and so every bit of the result, does not depend on alignment.
-template <int G, bool VEC, bool SQUARE, bool MASK>
+template <int G, bool VEC, bool SQUARE, bool MASK, bool LONG>
 __global__ void __launch_bounds__(G > 32 ? G : 256) pref_kernel(PrefArgs a) {
     constexpr int BLOCK = G > 32 ? G : 256;
     constexpr int W = 4;                           // consecutive negatives of a thread
     constexpr int U = G == 1 ? 1 : 2;
+    constexpr int FOLD = G * W * U * kPrefFold;    // LONG: negatives after which the threads' sums go to 64 bits
     __shared__ double red[32];
     __shared__ float rl[32], rd[32];
     __shared__ int rc[32];
+    __shared__ double2 wide[LONG ? G : 1];         // a thread's own
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int gl = threadIdx.x % G;
     let_next_start();
@@ -123,62 +134,71 @@ __global__ void __launch_bounds__(G > 32 ? G : 256) pref_kernel(PrefArgs a) {
         const float dscale = -cw * a.beta, keep = 1.f - a.smooth;
         const bool off = cw == 0.f;                    // nothing valid, or weight 0: zeros, whatever the scores hold
         float2 ls = f2(0.f), ds = f2(0.f);
-        for (int j0 = gl * W; j0 < n; j0 += G * W * U) {
-            float x[U][W], y[U][W];
-            uint32_t m[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int j = j0 + u * G * W;
-                m[u] = 0;
-                if (j < n) {
-                    if (VEC) {
-                        const float4 f = __ldcs(reinterpret_cast<const float4*>(neg + j));
-                        float4 g = make_float4(0.f, 0.f, 0.f, 0.f);
-                        if (rneg) g = __ldcs(reinterpret_cast<const float4*>(rneg + j));
-                        if (MASK) m[u] = *reinterpret_cast<const uint32_t*>(mask + j);
-                        x[u][0] = f.x; x[u][1] = f.y; x[u][2] = f.z; x[u][3] = f.w;
-                        y[u][0] = g.x; y[u][1] = g.y; y[u][2] = g.z; y[u][3] = g.w;
-                    } else {
-#pragma unroll
-                        for (int k = 0; k < W; ++k) {
-                            x[u][k] = y[u][k] = 0.f;
-                            if (j + k < n) {
-                                x[u][k] = neg[j + k];
-                                if (rneg) y[u][k] = rneg[j + k];
-                                if (!MASK || mask[j + k]) m[u] |= 0xFFu << (8 * k);
+        for (int s0 = 0; s0 < n; s0 += LONG ? FOLD : n) {
+            const int s1 = LONG ? s0 + min(n - s0, FOLD) : n;
+            if (LONG && s0 > 0) pref_fold(wide[threadIdx.x], s0 > FOLD, ls, ds);
+            for (int j0 = s0 + gl * W; j0 < s1; j0 += G * W * U) {
+                float x[U][W], y[U][W];
+                uint32_t m[U];
+    #pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int j = j0 + u * G * W;
+                    m[u] = 0;
+                    if (j < n) {
+                        if (VEC) {
+                            const float4 f = __ldcs(reinterpret_cast<const float4*>(neg + j));
+                            float4 g = make_float4(0.f, 0.f, 0.f, 0.f);
+                            if (rneg) g = __ldcs(reinterpret_cast<const float4*>(rneg + j));
+                            if (MASK) m[u] = *reinterpret_cast<const uint32_t*>(mask + j);
+                            x[u][0] = f.x; x[u][1] = f.y; x[u][2] = f.z; x[u][3] = f.w;
+                            y[u][0] = g.x; y[u][1] = g.y; y[u][2] = g.z; y[u][3] = g.w;
+                        } else {
+    #pragma unroll
+                            for (int k = 0; k < W; ++k) {
+                                x[u][k] = y[u][k] = 0.f;
+                                if (j + k < n) {
+                                    x[u][k] = neg[j + k];
+                                    if (rneg) y[u][k] = rneg[j + k];
+                                    if (!MASK || mask[j + k]) m[u] |= 0xFFu << (8 * k);
+                                }
                             }
                         }
                     }
                 }
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int j = j0 + u * G * W;
-                if (j < n) {
-                    float o[W];
-#pragma unroll
-                    for (int k = 0; k < W; k += 2) {
-                        float2 l, d;
-                        const float2 gap = __ffma2_rn(make_float2(x[u][k], x[u][k + 1]), f2(-1.f), make_float2(y[u][k], y[u][k + 1]));
-                        pref_pairs<SQUARE>(a, keep, __ffma2_rn(f2(a.beta), __fadd2_rn(f2(base), gap), f2(-a.margin)), l, d);
-                        if (MASK || !VEC) {
-                            if (!(m[u] & (0xFFu << (8 * k)))) { l.x = 0.f; d.x = 0.f; }
-                            if (!(m[u] & (0xFFu << (8 * k + 8)))) { l.y = 0.f; d.y = 0.f; }
+    #pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int j = j0 + u * G * W;
+                    if (j < n) {
+                        float o[W];
+    #pragma unroll
+                        for (int k = 0; k < W; k += 2) {
+                            float2 l, d;
+                            const float2 gap = __ffma2_rn(make_float2(x[u][k], x[u][k + 1]), f2(-1.f), make_float2(y[u][k], y[u][k + 1]));
+                            pref_pairs<SQUARE>(a, keep, __ffma2_rn(f2(a.beta), __fadd2_rn(f2(base), gap), f2(-a.margin)), l, d);
+                            if (MASK || !VEC) {
+                                if (!(m[u] & (0xFFu << (8 * k)))) { l.x = 0.f; d.x = 0.f; }
+                                if (!(m[u] & (0xFFu << (8 * k + 8)))) { l.y = 0.f; d.y = 0.f; }
+                            }
+                            ls = __fadd2_rn(ls, l);
+                            ds = __fadd2_rn(ds, d);
+                            const float2 g = __fmul2_rn(f2(dscale), d);
+                            o[k] = g.x; o[k + 1] = g.y;
                         }
-                        ls = __fadd2_rn(ls, l);
-                        ds = __fadd2_rn(ds, d);
-                        const float2 g = __fmul2_rn(f2(dscale), d);
-                        o[k] = g.x; o[k + 1] = g.y;
-                    }
-                    if (off) o[0] = o[1] = o[2] = o[3] = 0.f;
-                    if (VEC) {
-                        __stcs(reinterpret_cast<float4*>(dneg + j), make_float4(o[0], o[1], o[2], o[3]));
-                    } else {
-#pragma unroll
-                        for (int k = 0; k < W; ++k) if (j + k < n) dneg[j + k] = o[k];
+                        if (off) o[0] = o[1] = o[2] = o[3] = 0.f;
+                        if (VEC) {
+                            __stcs(reinterpret_cast<float4*>(dneg + j), make_float4(o[0], o[1], o[2], o[3]));
+                        } else {
+    #pragma unroll
+                            for (int k = 0; k < W; ++k) if (j + k < n) dneg[j + k] = o[k];
+                        }
                     }
                 }
             }
+        }
+        if (LONG) {
+            pref_fold(wide[threadIdx.x], n > FOLD, ls, ds);
+            ls.x = static_cast<float>(wide[threadIdx.x].x);
+            ds.x = static_cast<float>(wide[threadIdx.x].y);
         }
         float lsum = pref_group_sum<G>(ls.x + ls.y), dsum = pref_group_sum<G>(ds.x + ds.y);
         if (G > 32) {
@@ -219,11 +239,11 @@ static long long pref_blocks(long long rows, int per) {
     return want < kPrefMaxBlocks ? want : kPrefMaxBlocks;
 }
 
-template <int G, bool VEC, bool SQUARE, bool MASK>
+template <int G, bool VEC, bool SQUARE, bool MASK, bool LONG>
 static int pref_go2(const PrefArgs& a, float* loss, cudaStream_t s) {
     constexpr int per = G > 32 ? 1 : 256 / G;
     const unsigned blocks = static_cast<unsigned>(pref_blocks(a.rows, per));
-    pref_kernel<G, VEC, SQUARE, MASK><<<blocks, G > 32 ? G : 256, 0, s>>>(a);
+    pref_kernel<G, VEC, SQUARE, MASK, LONG><<<blocks, G > 32 ? G : 256, 0, s>>>(a);
     KGE_LAUNCH_CHECK("pref_kernel");
     // one CTA has written the loss itself (200 x 3: 2.7 us, with a sum 3.7 us; one CTA of 1024 threads for more rows is slower: 500 x 20
     // 5.7 us against 4.2 us)
@@ -231,7 +251,14 @@ static int pref_go2(const PrefArgs& a, float* loss, cudaStream_t s) {
 }
 template <int G, bool VEC, bool SQUARE>
 static int pref_go(const PrefArgs& a, float* loss, cudaStream_t s) {
-    return a.mask ? pref_go2<G, VEC, SQUARE, true>(a, loss, s) : pref_go2<G, VEC, SQUARE, false>(a, loss, s);
+    // More than kPrefFold turns of eight negatives a thread (fewer than 256 threads never have such rows).  16 x 4000000 with reference
+    // 661 us, with mask too 904 us; without the folds 733 and 839 us, and a loss off by 4e-5 of itself; rows of fewer turns, with the
+    // folds all the same: up to 7 % slower.
+    if (G >= 256 && a.n > G * 8 * kPrefFold) {
+        constexpr bool LONG = G >= 256;
+        return a.mask ? pref_go2<G, VEC, SQUARE, true, LONG>(a, loss, s) : pref_go2<G, VEC, SQUARE, false, LONG>(a, loss, s);
+    }
+    return a.mask ? pref_go2<G, VEC, SQUARE, true, false>(a, loss, s) : pref_go2<G, VEC, SQUARE, false, false>(a, loss, s);
 }
 // Threads per row: the fewest that still fill the GPU, so that a thread has some eight negatives at once and few share a row's own
 // scalars and reductions.  us with reference and mask:

@@ -1,4 +1,6 @@
 """Losses over scores at the limits of their terms: coefficients of zero beside infinities, rows that take no part."""
+import math
+
 import pytest
 import torch
 
@@ -116,3 +118,25 @@ def test_preference_smoothing_of_one_beside_infinities(n):
         assert loss.item() == 0 and (dpos == 0).all() and (dneg == 0).all()
     loss, dpos, dneg = losses.preference_loss(pos, torch.full((2, n), -INF, device="cuda"), smoothing=1.0)
     assert loss.item() == INF and (dneg != 0).all()
+
+
+@pytest.mark.parametrize("rows,n,mask", [(1, 1 << 24, False), (2, (1 << 24) + 3, True), (1, 40_000_001, False), (300, 1 << 18, True)])
+def test_preference_sums_over_long_rows(rows, n, mask):
+    """Equal pairs: the loss is that of one pair and d(pos) its slope, whatever the number of pairs.
+
+    At most 64 additions in fp32 follow one another in a thread before they go to 64 bits; 5 more add a warp and 31 a row's warps; the
+    pair itself is good to 16 half-steps (of 1): 120 half-steps of 1 cover all."""
+    z, beta = 0.3, 1.0
+    pos = torch.full((rows,), z, device="cuda")
+    neg = torch.zeros(rows, n, device="cuda")
+    m = None
+    if mask:
+        m = torch.rand(rows, n, device="cuda") > 0.3
+        neg = neg.masked_fill(~m, float("nan"))
+    loss, dpos, dneg = losses.preference_loss(pos, neg, mask=m, beta=beta, reduction="mean")
+    z64 = float(torch.tensor(z, dtype=torch.float32))
+    want, slope = math.log1p(math.exp(-z64)), -1 / (1 + math.exp(z64))
+    assert abs(loss.item() - want) <= 120 * EPS
+    assert ((dpos.double() * rows - slope).abs() <= 120 * EPS).all()
+    loss, dpos, _ = losses.preference_loss(pos, neg, mask=m, kind="square", reduction="mean")
+    assert abs(loss.item() - z64 * z64) <= 120 * EPS * z64 * z64 and ((dpos.double() * rows - 2 * z64).abs() <= 120 * EPS).all()
