@@ -354,16 +354,17 @@ linear_pair_kernel(const __grid_constant__ LinMaps maps, const __grid_constant__
         const uint32_t out_addr = umma::smem_u32(mine);
         const int row_in = static_cast<int>(rank) * LG_BM + sub * 32;
         if (EPI == LE_PLAIN && p.db != nullptr) {
-            // db[c] = sum of its partial sums in fp32 and in a fixed order (16 interleaved sums a column), while the first tiles are
-            // multiplied: a kernel of its own took 3 us of the 8191 x 1024 x 400 backward pass
+            // db[c] = sum of its partial sums in a fixed order (16 interleaved sums a column, in fp64: each has a million terms at 2^30
+            // rows), while the first tiles are multiplied: a kernel of its own took 3 us of the 8191 x 1024 x 400 backward pass
             float* red = reinterpret_cast<float*>(staging);                       // 16 x 33: nothing is staged yet
             for (int c0 = blockIdx.x * 32; c0 < p.db_n; c0 += gridDim.x * 32) {
                 const int c = c0 + lane;
-                float t = 0.f;
+                double wide = 0.0;
                 if (c < p.db_n) {
 #pragma unroll 8
-                    for (long long b = warp - 2; b < p.colblocks; b += LG_EPI_WARPS) t += p.colpart[b * p.db_n + c];
+                    for (long long b = warp - 2; b < p.colblocks; b += LG_EPI_WARPS) wide += static_cast<double>(p.colpart[b * p.db_n + c]);
                 }
+                float t = static_cast<float>(wide);
                 red[(warp - 2) * 33 + lane] = t;
                 lin_epilogue_barrier();
                 if (warp == 2 && c < p.db_n) {
