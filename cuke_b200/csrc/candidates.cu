@@ -838,13 +838,12 @@ static int cand_groups(const CandArgs& a, int* n_partial, cudaStream_t s) {
 // slot: vectors of a row that one CTA holds
 template <typename T, int THREADS, int ROWS, int CTAS, int MODE>
 static int cand_rows(const CandArgs& a, int cluster, long long slot, int* n_partial, cudaStream_t s) {
-    static std::atomic<bool> attr_set[128];          // the shared-memory opt-in is per device and kernel
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess) return cuda_status(cudaGetLastError(), "cudaGetDevice");
-    if (dev < 0 || dev >= 128 || !attr_set[dev].load(std::memory_order_acquire)) {
+    static thread_local unsigned long long opted_in = 0;      // the shared-memory opt-in is per context and kernel
+    const unsigned long long here = context_number();
+    if (here == 0 || here != opted_in) {
         cudaError_t e = cudaFuncSetAttribute(cand_row_kernel<T, THREADS, ROWS, CTAS, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowSmem);
         if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(cand_row_kernel)");
-        if (dev >= 0 && dev < 128) attr_set[dev].store(true, std::memory_order_release);
+        opted_in = context_number();
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>((a.rows + ROWS - 1) / ROWS * cluster));

@@ -3,6 +3,7 @@
 #include <stdarg.h>
 #include <string.h>
 #include <atomic>
+#include <cuda.h>
 #include "common.cuh"
 
 namespace kge {
@@ -25,15 +26,29 @@ int cuda_status(cudaError_t e, const char* what) {
 static std::atomic<long long> g_launches{0};
 void note_launch() { g_launches.fetch_add(1, std::memory_order_relaxed); }
 
+typedef CUresult (*CtxIdFn)(CUcontext, unsigned long long*);
+static CtxIdFn ctx_id_fn() {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    const bool ok = cudaGetDriverEntryPoint("cuCtxGetId", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess;
+    if (!ok) cudaGetLastError();
+    return ok ? reinterpret_cast<CtxIdFn>(p) : nullptr;
+}
+unsigned long long context_number() {
+    static const CtxIdFn fn = ctx_id_fn();
+    unsigned long long id = 0;
+    return fn && fn(nullptr, &id) == CUDA_SUCCESS ? id : 0;
+}
+
 __device__ int32_t g_error_word = 0;
 int32_t* device_error_word() {
-    static std::atomic<int32_t*> known[128];         // by device: the runtime's lookup takes longer than a launch's checks
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess) return nullptr;
-    int32_t* p = dev >= 0 && dev < 128 ? known[dev].load(std::memory_order_acquire) : nullptr;
-    if (p) return p;
+    // of the thread's last context: the runtime's lookup takes longer than a launch's checks
+    static thread_local struct { unsigned long long context; int32_t* word; } known = {0, nullptr};
+    const unsigned long long here = context_number();
+    if (here && here == known.context) return known.word;
+    int32_t* p = nullptr;
     if (cudaGetSymbolAddress(reinterpret_cast<void**>(&p), g_error_word) != cudaSuccess) return nullptr;
-    if (dev >= 0 && dev < 128) known[dev].store(p, std::memory_order_release);
+    known = {context_number(), p};                   // (the lookup makes the context, if there was none)
     return p;
 }
 

@@ -15,6 +15,9 @@ constexpr unsigned kFull = 0xffffffffu;
 void set_error(const char* fmt, ...);          // thread-local message (capi.cu)
 int cuda_status(cudaError_t e, const char* what);  // 0 or positive cudaError_t, records message
 int32_t* device_error_word();                  // per-device error word (capi.cu)
+// Number of the calling thread's CUDA context, unique in the process, or 0 where there is none yet.  What is remembered of a device
+// between calls (an address, a kernel's shared-memory opt-in) holds for one context: cudaDeviceReset ends it.
+unsigned long long context_number();           // (capi.cu)
 void note_launch();                            // counts kernel launches issued by this library (capi.cu)
 
 #define KGE_LAUNCH_CHECK(what)                                   \

@@ -820,13 +820,12 @@ static size_t lin_part_bytes(const LinDim* d, int count, const LinPlan& plan) {
 
 template <int EPI, int ACT, bool SLOPE>
 static int lin_launch(const LinMaps& maps, const LinGemm& p, unsigned ctas, size_t smem, bool first, cudaStream_t s) {
-    static std::atomic<bool> attr_set[128];          // the shared-memory opt-in is per device and kernel
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess) return cuda_status(cudaGetLastError(), "cudaGetDevice");
-    if (dev < 0 || dev >= 128 || !attr_set[dev].load(std::memory_order_acquire)) {
+    static thread_local unsigned long long opted_in = 0;      // the shared-memory opt-in is per context and kernel
+    const unsigned long long here = context_number();
+    if (here == 0 || here != opted_in) {
         cudaError_t e = cudaFuncSetAttribute(linear_pair_kernel<EPI, ACT, SLOPE>, cudaFuncAttributeMaxDynamicSharedMemorySize, LG_MAX_SMEM);
         if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(linear_pair_kernel)");
-        if (dev >= 0 && dev < 128) attr_set[dev].store(true, std::memory_order_release);
+        opted_in = context_number();
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas);
