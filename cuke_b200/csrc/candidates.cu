@@ -9,7 +9,6 @@
 // logp = -log1p(S') then keep their digits when the chosen candidate has nearly all the mass.
 // Row statistics are fp32, the loss is summed over rows in 64 bits.
 #include <math.h>
-#include <atomic>
 #include "umma.cuh"
 
 namespace kge {

@@ -252,8 +252,8 @@ static int pref_go2(const PrefArgs& a, float* loss, cudaStream_t s) {
 template <int G, bool VEC, bool SQUARE>
 static int pref_go(const PrefArgs& a, float* loss, cudaStream_t s) {
     // More than kPrefFold turns of eight negatives a thread (fewer than 256 threads never have such rows).  16 x 4000000 with reference
-    // 661 us, with mask too 904 us; without the folds 733 and 839 us, and a loss off by 4e-5 of itself; rows of fewer turns, with the
-    // folds all the same: up to 7 % slower.
+    // 661 us, with mask too 904 us; without the folds 733 and 839 us, but 40,000,001 equal pairs were then off by 7e-5 of their loss;
+    // rows of fewer turns, with the folds all the same: up to 7 % slower.
     if (G >= 256 && a.n > G * 8 * kPrefFold) {
         constexpr bool LONG = G >= 256;
         return a.mask ? pref_go2<G, VEC, SQUARE, true, LONG>(a, loss, s) : pref_go2<G, VEC, SQUARE, false, LONG>(a, loss, s);

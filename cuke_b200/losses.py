@@ -127,7 +127,8 @@ def policy_loss(scores: torch.Tensor, action: torch.Tensor, old_logp: torch.Tens
     """(loss (1,), logp (rows,), kl (rows,), dscores) of a clipped policy step with a KL term (kge_policy_loss).
 
     ratio = exp(logp - old_logp); per row -min(ratio A, clip(ratio, 1 - clip_low, 1 + clip_high) A) + kl_coef * kl with
-    kl = exp(ref_logp - logp) - (ref_logp - logp) - 1 (needs ref_logp); rows are weighted by `weight` (0: the row adds nothing)
+    kl = exp(ref_logp - logp) - (ref_logp - logp) - 1 (needs ref_logp; with kl_coef = 0 it is only reported); rows are weighted by
+    `weight` (0: the row adds nothing)
     and averaged over their number, or summed with reduction="sum".  scores, action, n_cand, temperature as in log_prob;
     dscores has the dtype of scores."""
     here = need_here(scores, action, n_cand, old_logp, advantage, ref_logp, weight)

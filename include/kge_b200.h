@@ -394,7 +394,8 @@ KGE_API int kge_apply_adagrad(void* table, int32_t dtype, float* state, int32_t 
  * read into the result (it may hold infinities or NaN), its dneg is 0; a row without valid negatives, or of weight 0, adds
  * nothing and gets zero gradients.  pos, ref_pos, weight, dpos (rows); neg, ref_neg, mask, dneg (rows, n) with row pitches in
  * elements; ref_pos and ref_neg are both given or both NULL; mask, weight may be NULL (all valid, weight 1).  All fp32 (the
- * scorers' output type), aligned to 4 bytes; sums in a fixed order.  dneg may be neg itself (same pitch).  loss (1,).
+ * scorers' output type), aligned to 4 bytes; sums in a fixed order, fp32 over at most 64 terms of a thread and fp64 beyond.  dneg
+ * may be neg itself (same pitch).  loss (1,).
  * Chunk-shared scores (batch/chunk, chunk, n) are the same rows.  n <= 2^30.  No reference counterpart. */
 #define KGE_PREF_LOGISTIC 0
 #define KGE_PREF_SQUARE 1
@@ -407,7 +408,8 @@ KGE_API int kge_preference_loss(const float* pos, const float* ref_pos, const fl
 /* Score rows as distributions over candidates: scores (rows, n) fp32 or bf16 with row pitch ld in elements; row r has the
  * candidates [0, n_cand[r]) (n_cand clamped to [0, n]; NULL: all n); action[r] is the chosen one (id_bits wide).
  *   kge_log_prob           logp[r] = log softmax(scores[r] / temperature)[action[r]];  stats (rows, 3): what the gradient needs
- *   kge_log_prob_backward  dscores[r][j] = dlogp[r] / temperature * (1[j = action[r]] - softmax_j), zeros at [n_cand[r], n)
+ *   kge_log_prob_backward  dscores[r][j] = dlogp[r] / temperature * (1[j = action[r]] - softmax_j), zeros at [n_cand[r], n); a row
+ *                          whose dlogp is 0 gets zeros
  *   kge_policy_loss        ratio = exp(logp - old_logp);
  *                          l = -min(ratio A, clip(ratio, 1 - clip_low, 1 + clip_high) A)
  *                              + kl_coef * kl,   kl = exp(ref_logp - logp) - (ref_logp - logp) - 1  (0 without ref_logp;
@@ -440,7 +442,8 @@ KGE_API int kge_policy_loss(const void* scores, int32_t dtype, int64_t ld, int64
  * s the logistic function.  bias (n), residual (m, n) may be NULL.  slope: NULL, or (m, n) fp16 packed, receives act'(z) for the
  * backward call (not written for KGE_ACT_NONE).  residual may be out itself (same pitch); outputs overlap nothing else.
  *   kge_linear_backward  dz = dout * slope (bf16);  dx = dz w^T (m, k);  dw = x^T dz (k, n) packed;  dbias = sum of dz over the rows
- *   (fp32 sums of the unrounded dz).  dx, dw, dbias may each be NULL (not computed); the gradient of residual is dout itself.
+ *   (of the unrounded dz: fp32 within 64 rows, fp64 over those).  dx, dw, dbias may each be NULL (not computed); the gradient of
+ *   residual is dout itself.
  * All operands are bf16 with 16-byte aligned bases and row pitches that are multiples of 8 elements; k, n multiples of 8; any m.
  * (Row pitches that are multiples of 64 elements are read fastest.)
  * workspace (kge_linear_workspace_bytes; may be 0 bytes for the forward call) is 256-byte aligned.  The sums are taken in a fixed
