@@ -966,10 +966,11 @@ static int check_floats(const char* fn, const char* name, const float* p, bool r
     if (reinterpret_cast<uintptr_t>(p) & 3) { set_error("%s: %s is not aligned to its element size", fn, name); return KGE_E_ALIGN; }
     return 0;
 }
-static int check_gradient(const char* fn, void* dscores, int32_t dtype, int64_t ldd, int64_t rows, int64_t n) {
+static int check_gradient(const char* fn, const void* scores, int64_t ld, void* dscores, int32_t dtype, int64_t ldd, int64_t rows, int64_t n) {
     if (rows > 1 && ldd < n) { set_error("%s: row pitch %lld of dscores is below n", fn, (long long)ldd); return KGE_E_SHAPE; }
     if (ldd > (1LL << 40)) { set_error("%s: row pitch above 2^40", fn); return KGE_E_RANGE; }
     if (!dscores && n > 0) { set_error("%s: dscores is NULL", fn); return KGE_E_NULL; }
+    if (dscores == scores && rows > 1 && n > 0 && ldd != ld) { set_error("%s: dscores may be scores only with the same row pitch", fn); return KGE_E_SHAPE; }
     if (reinterpret_cast<uintptr_t>(dscores) & (dtype == KGE_F32 ? 3 : 1)) { set_error("%s: dscores is not aligned to its element size", fn); return KGE_E_ALIGN; }
     return 0;
 }
@@ -1006,7 +1007,7 @@ int kge_log_prob_backward(const void* scores, int32_t dtype, int64_t ld, int64_t
     int rc = check_candidates(fn, scores, dtype, ld, rows, n, n_cand, action, id_bits, temperature, &a);
     if (rc || rows == 0) return rc;
     if ((rc = check_floats(fn, "stats", stats, true)) || (rc = check_floats(fn, "dlogp", dlogp, true)) ||
-        (rc = check_gradient(fn, dscores, dtype, ldd, rows, n))) return rc;
+        (rc = check_gradient(fn, scores, ld, dscores, dtype, ldd, rows, n))) return rc;
     a.stats = const_cast<float*>(stats); a.dlogp = dlogp; a.dscores = dscores; a.ldd = ldd;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     return dtype == KGE_F32 ? cand_gradient<float>(a, stats, same_phase<float>(a), true, s)
@@ -1028,7 +1029,7 @@ int kge_policy_loss(const void* scores, int32_t dtype, int64_t ld, int64_t rows,
     if ((rc = check_floats(fn, "old_logp", old_logp, true)) || (rc = check_floats(fn, "ref_logp", ref_logp, false)) ||
         (rc = check_floats(fn, "advantage", advantage, true)) || (rc = check_floats(fn, "weight", weight, false)) ||
         (rc = check_floats(fn, "logp", logp, true)) || (rc = check_floats(fn, "kl", kl, true)) ||
-        (rc = check_gradient(fn, dscores, dtype, ldd, rows, n))) return rc;
+        (rc = check_gradient(fn, scores, ld, dscores, dtype, ldd, rows, n))) return rc;
     if (workspace_bytes < kge_candidates_workspace_bytes(rows, n)) { set_error("%s: workspace too small", fn); return KGE_E_WORKSPACE; }
     if (!workspace) { set_error("%s: workspace is NULL", fn); return KGE_E_NULL; }
     if (!aligned16(workspace)) { set_error("%s: workspace is not 16-byte aligned", fn); return KGE_E_ALIGN; }

@@ -202,6 +202,8 @@ extern "C" int kge_dropout(const void* x, int32_t dtype, int64_t rows, int32_t d
     if (rows > (1LL << 60) / dim) { set_error("%s: rows x dim above 2^60", fn); return KGE_E_RANGE; }
     if (rows > 1 && (ldx < dim || ldo < dim || (residual && ldr < dim))) { set_error("%s: a row pitch is below dim", fn); return KGE_E_SHAPE; }
     if (!x || !out) { set_error("%s: x / out is NULL", fn); return KGE_E_NULL; }
+    if (rows > 1 && ((out == x && ldo != ldx) || (out == residual && ldo != ldr))) {
+        set_error("%s: out may be x or residual only with the same row pitch", fn); return KGE_E_SHAPE; }
     const uintptr_t m = dtype == KGE_F32 ? 3 : 1;
     if ((reinterpret_cast<uintptr_t>(x) & m) || (reinterpret_cast<uintptr_t>(out) & m) || (reinterpret_cast<uintptr_t>(residual) & m) ||
         (reinterpret_cast<uintptr_t>(step_dev) & 7)) { set_error("%s: a pointer is not aligned to its element size", fn); return KGE_E_ALIGN; }

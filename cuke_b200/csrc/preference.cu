@@ -314,6 +314,7 @@ int kge_preference_loss(const float* pos, const float* ref_pos, const float* neg
     if (!loss) { set_error("%s: loss is NULL", fn); return KGE_E_NULL; }
     if (rows > 0 && (!pos || !dpos || (n > 0 && (!neg || !dneg)))) { set_error("%s: pos / neg / dpos / dneg is NULL", fn); return KGE_E_NULL; }
     if (rows > 0 && n > 0 && (ref_pos == nullptr) != (ref_neg == nullptr)) { set_error("%s: ref_pos and ref_neg come together", fn); return KGE_E_NULL; }
+    if (rows > 1 && n > 0 && dneg == neg && ld_dneg != ld_neg) { set_error("%s: dneg may be neg only with the same row pitch", fn); return KGE_E_SHAPE; }
     const void* ptrs[] = {pos, ref_pos, neg, ref_neg, weight, loss, dpos, dneg};
     for (const void* p : ptrs)
         if (reinterpret_cast<uintptr_t>(p) & 3) { set_error("%s: a pointer is not aligned to its element size", fn); return KGE_E_ALIGN; }
