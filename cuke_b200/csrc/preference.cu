@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(G > 32 ? G : 256) pref_kernel(PrefArgs a) {
             for (int j0 = s0 + gl * W; j0 < s1; j0 += G * W * U) {
                 float x[U][W], y[U][W];
                 uint32_t m[U];
-    #pragma unroll
+#pragma unroll
                 for (int u = 0; u < U; ++u) {
                     const int j = j0 + u * G * W;
                     m[u] = 0;
@@ -153,7 +153,7 @@ __global__ void __launch_bounds__(G > 32 ? G : 256) pref_kernel(PrefArgs a) {
                             x[u][0] = f.x; x[u][1] = f.y; x[u][2] = f.z; x[u][3] = f.w;
                             y[u][0] = g.x; y[u][1] = g.y; y[u][2] = g.z; y[u][3] = g.w;
                         } else {
-    #pragma unroll
+#pragma unroll
                             for (int k = 0; k < W; ++k) {
                                 x[u][k] = y[u][k] = 0.f;
                                 if (j + k < n) {
@@ -165,12 +165,12 @@ __global__ void __launch_bounds__(G > 32 ? G : 256) pref_kernel(PrefArgs a) {
                         }
                     }
                 }
-    #pragma unroll
+#pragma unroll
                 for (int u = 0; u < U; ++u) {
                     const int j = j0 + u * G * W;
                     if (j < n) {
                         float o[W];
-    #pragma unroll
+#pragma unroll
                         for (int k = 0; k < W; k += 2) {
                             float2 l, d;
                             const float2 gap = __ffma2_rn(make_float2(x[u][k], x[u][k + 1]), f2(-1.f), make_float2(y[u][k], y[u][k + 1]));
@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(G > 32 ? G : 256) pref_kernel(PrefArgs a) {
                         if (VEC) {
                             __stcs(reinterpret_cast<float4*>(dneg + j), make_float4(o[0], o[1], o[2], o[3]));
                         } else {
-    #pragma unroll
+#pragma unroll
                             for (int k = 0; k < W; ++k) if (j + k < n) dneg[j + k] = o[k];
                         }
                     }
